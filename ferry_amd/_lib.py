@@ -21,6 +21,12 @@ SIGNATURES = [
     ('ferry_abi_version', _i32, []),
     ('ferry_router_topk', ctypes.c_int,
      [_c_p, _i32, _i64, _i64, _i64, _i32, _f32, _i32, _c_p, _c_p, _c_p, _c_p, _c_p]),
+    ('ferry_route_experts', ctypes.c_int,
+     [_c_p, _i32, _i64, _i64, _i64, _i32, _c_p, _i64, _i64, _i32, _i32, _f32, _c_p, _c_p, _c_p]),
+    ('ferry_mxfp4_quantize', ctypes.c_int,
+     [_c_p, _i32, _i64, _i64, _i64, _c_p, _i64, _c_p, _i64, _c_p]),
+    ('ferry_mxfp4_dequantize', ctypes.c_int,
+     [_c_p, _i64, _c_p, _i64, _i64, _i64, _c_p, _i32, _i64, _c_p]),
     ('ferry_layout_workspace_bytes', _i64, [_i64, _i64, _i64]),
     ('ferry_layout', ctypes.c_int,
      [_c_p, _c_p, _i64, _i64, _i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _i64, _c_p]),

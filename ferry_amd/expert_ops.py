@@ -21,7 +21,8 @@ from .h2d import H2DEngine
 
 __all__ = ['execute_experts', 'pack_dispatch', 'unpack_dispatch', 'reduce_partials',
            'scatter_returned', 'H2DEngine', 'router_topk', 'layout', 'gate_logits', 'expert_ffn',
-           'combine', 'SharedExpert', 'history_update', 'history_ready_words', 'current_stream', 'PHASE_UP',
+           'combine', 'SharedExpert', 'route_experts', 'mxfp4_quantize', 'mxfp4_dequantize',
+           'mxfp4_expert_rows', 'history_update', 'history_ready_words', 'current_stream', 'PHASE_UP',
            'PHASE_DOWN', 'PHASE_BOTH']
 
 MAX_EXPERTS = 512
@@ -118,6 +119,145 @@ def router_topk(logits, topk, renorm=True, scale=1.0, sorted=True, return_probs=
         _dev(tie_counter, 'tie_counter', torch.int32) if tie_counter is not None else None,
         _stream_of(logits)), 'router_topk')
     return (w, idx, probs) if return_probs else (w, idx)
+
+
+_DTYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}   # FERRY_BF16, FERRY_F32, FERRY_F16
+
+
+def route_experts(logits, topk, scoring='softmax', bias=None, groups=1, topk_groups=None,
+                  group_score='max', renorm=True, scale=1.0):
+    """Expert selection of a general gate: ``scoring`` 'softmax' or 'sigmoid', an additive balance
+    ``bias`` on the scores that choose (not on the weights), ``groups`` of consecutive experts of which
+    the best ``topk_groups`` stay, scored by their largest choice score ('max') or by the sum of their two
+    largest ('top2'), then the ``topk`` experts with the largest choice scores.
+
+    ``logits`` is bf16, fp32 or fp16 [T, E], ``bias`` fp32 [E].  Returns (weights bf16 [T, topk], selected
+    int64 [T, topk], by descending choice score): the chosen experts' scores, divided by their sum with
+    ``renorm``, times ``scale``.  Ties go to the lowest index (``router_topk`` keeps torch's CPU order);
+    scores are compared in 64 bits.  A logit of -inf masks an expert (chosen last, weight 0); the IDs of a
+    row are distinct whatever the logits hold, and a softmax row with a NaN or +inf has NaN weights.
+    No counterpart in the reference; the results carry no gradient.
+    """
+    if logits.dim() != 2:
+        raise RuntimeError('logits must be [tokens, experts]')
+    dt = _DTYPES.get(logits.dtype)
+    if dt is None:
+        raise RuntimeError('logits must be bf16, fp32 or fp16')
+    if scoring not in ('softmax', 'sigmoid'):
+        raise ValueError("scoring must be 'softmax' or 'sigmoid'")
+    if group_score not in ('max', 'top2'):
+        raise ValueError("group_score must be 'max' or 'top2'")
+    T, E = logits.shape
+    if bias is not None:
+        if bias.shape != (E,):
+            raise RuntimeError('bias must be fp32 [experts]')
+        _on_device(bias, 'bias', logits)
+    at = _dev(logits, 'logits')
+    idx = torch.empty((T, topk), dtype=torch.int64, device=logits.device)
+    w = torch.empty((T, topk), dtype=torch.bfloat16, device=logits.device)
+    _native(logits, 'route_experts', lib().ferry_route_experts,
+            at, dt, T, E, topk, int(scoring == 'sigmoid'),
+            _dev(bias, 'bias', torch.float32) if bias is not None else None, groups,
+            groups if topk_groups is None else topk_groups, int(group_score == 'top2'),
+            int(bool(renorm)), float(scale), idx.data_ptr(), w.data_ptr())
+    return w, idx
+
+
+def _native(t, what, fn, *args):
+    """``fn(*args, stream)`` on the device of the CUDA tensor ``t`` and its current stream there."""
+    if t.get_device() == torch.cuda.current_device():
+        check(fn(*args, _stream_of(t)), what)
+    else:
+        with torch.cuda.device(t.device):
+            check(fn(*args, _stream_of(t)), what)
+
+
+def _on_device(t, name, like):
+    if not isinstance(t, torch.Tensor) or t.device != like.device:
+        raise RuntimeError(f'{name} must be on {like.device}')
+
+
+def _row_stride(t, name):
+    """Elements from one row of [rows, cols] to the next; the elements of a row follow each other."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise RuntimeError(f'{name} must be a CUDA tensor')
+    if t.dim() == 2 and (t.shape[1] <= 1 or t.stride(1) == 1) and (
+            t.shape[0] <= 1 or t.stride(0) >= t.shape[1]):
+        return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    if not t.is_contiguous():
+        raise RuntimeError(f'{name} must be contiguous, or a matrix of contiguous rows')
+    return t.shape[-1]
+
+
+def _mxfp4_quantize(x, codes, ldc, scales, lds):
+    cols = x.shape[-1]
+    stride = _row_stride(x, 'x')
+    _native(x, 'mxfp4_quantize', lib().ferry_mxfp4_quantize, x.data_ptr(), _DTYPES[x.dtype],
+            x.numel() // cols if cols else 0, cols, stride, codes, ldc, scales, lds)
+
+
+def mxfp4_quantize(x):
+    """(codes, scales) of the rows of ``x`` (bf16, fp32 or fp16 [..., cols]; a matrix may have a row
+    stride) in MXFP4: uint8 codes [..., 16 * blocks], two elements a byte, the first in the low half, and
+    uint8 scales [..., blocks], 2^(byte - 127), for ``blocks`` = ceil(cols / 32) blocks of 32 elements.
+
+    A block's scale is 2^(floor(log2(its largest magnitude)) - 2), elements round to the nearest of 0,
+    0.5, 1, 1.5, 2, 3, 4, 6 (ties to the even code) and saturate at 6; a block with an infinity or a NaN
+    reads back as NaN.  No counterpart in the reference, whose expert rows are bf16."""
+    if not isinstance(x, torch.Tensor) or x.dim() < 1:
+        raise RuntimeError('x must be a tensor of rows')
+    if x.dtype not in _DTYPES:
+        raise RuntimeError('x must be bf16, fp32 or fp16')
+    blocks = -(-x.shape[-1] // 32)
+    _row_stride(x, 'x')
+    codes = torch.empty((*x.shape[:-1], blocks * 16), dtype=torch.uint8, device=x.device)
+    scales = torch.empty((*x.shape[:-1], blocks), dtype=torch.uint8, device=x.device)
+    _mxfp4_quantize(x, codes.data_ptr(), blocks * 16, scales.data_ptr(), blocks)
+    return codes, scales
+
+
+def mxfp4_dequantize(codes, scales, columns=None, dtype=torch.bfloat16):
+    """The values of ``mxfp4_quantize``'s (codes, scales) rounded to ``dtype`` (bf16 holds them exactly),
+    [..., columns]; all 32 * blocks columns without ``columns``.  Both may be matrices with a row stride
+    (the two parts of ``mxfp4_expert_rows``)."""
+    if dtype not in _DTYPES:
+        raise RuntimeError('dtype must be bf16, fp32 or fp16')
+    ldc, lds = _row_stride(codes, 'codes'), _row_stride(scales, 'scales')
+    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        raise RuntimeError('codes and scales must be uint8')
+    blocks = scales.shape[-1]
+    if codes.shape != (*scales.shape[:-1], 16 * blocks):
+        raise RuntimeError('codes must have 16 bytes for every scale')
+    _on_device(scales, 'scales', codes)
+    cols = 32 * blocks if columns is None else int(columns)
+    if not 32 * blocks - 32 < cols <= 32 * blocks:
+        raise RuntimeError(f'columns must end in the last of the {blocks} blocks')
+    out = torch.empty((*scales.shape[:-1], cols), dtype=dtype, device=codes.device)
+    _native(codes, 'mxfp4_dequantize', lib().ferry_mxfp4_dequantize, codes.data_ptr(), ldc,
+            scales.data_ptr(), lds, out.numel() // cols if cols else 0, cols, out.data_ptr(),
+            _DTYPES[dtype], cols)
+    return out
+
+
+def mxfp4_expert_rows(rows, out=None):
+    """Expert rows ``[gate | up | down]`` (bf16, fp32 or fp16 [n, elements], the cache and pool row format)
+    as MXFP4 rows: uint8 [n, elements / 32 * 17], a row's codes and then its scales.  ``elements`` must be
+    a multiple of 128, as 3 * hidden * intermediate is.  ``out`` (optional) receives the rows."""
+    if not isinstance(rows, torch.Tensor) or rows.dim() != 2 or rows.dtype not in _DTYPES:
+        raise RuntimeError('rows must be bf16, fp32 or fp16 [experts, elements]')
+    n, elements = rows.shape
+    if elements % 128:
+        raise RuntimeError('a row must hold a multiple of 128 elements')
+    _row_stride(rows, 'rows')
+    width = elements // 32 * 17
+    if out is None:
+        out = torch.empty((n, width), dtype=torch.uint8, device=rows.device)
+    elif out.shape != (n, width):
+        raise RuntimeError(f'out must be uint8 [{n}, {width}]')
+    at = _dev(out, 'out', torch.uint8)
+    _on_device(out, 'out', rows)
+    _mxfp4_quantize(rows, at, width, at + elements // 2, width)
+    return out
 
 
 def _gate_kernel_takes(x, weight):

@@ -48,7 +48,7 @@ int ferry_timing_overlap(int64_t begin, int64_t end, void* t0, void* t1, double*
 int64_t ferry_hbm_read_sink_bytes(int64_t bytes);
 int ferry_hbm_read(const void* data, int64_t bytes, void* sink, int64_t sink_bytes, void* stream);
 
-enum { FERRY_BF16 = 0, FERRY_F32 = 1 };
+enum { FERRY_BF16 = 0, FERRY_F32 = 1, FERRY_F16 = 2 };
 
 /*
  * Router: fp32 softmax over each row of logits[T, E], top-k, optional renormalisation of the
@@ -66,6 +66,41 @@ int ferry_router_topk(const void* logits, int32_t logits_dtype, int64_t tokens, 
                       int64_t topk, int32_t renorm, float scale, int32_t sorted,
                       int64_t* idx_out, void* w_out_bf16, float* probs_out, int32_t* tie_rows,
                       void* stream);
+
+/*
+ * Expert selection of a general gate (no counterpart in the reference, whose gates are softmax + top-k).
+ * Over logits[T, E] (bf16, fp32 or fp16): scores s = 1 / (1 + e^-logit) with `sigmoid`, else the row's
+ * softmax; choice scores c = s + bias (fp32 [E], nullable).  With groups > 1 the E / groups consecutive
+ * experts of a group give it their largest c, or with group_top2 the sum of their two largest, and only
+ * the experts of the best topk_groups groups can be chosen.  The topk experts with the largest c, in
+ * descending order, go to idx_out[T, topk]; their s (divided by their sum with `renorm`, 0 where that is
+ * 0) times scale, rounded to bf16, to w_out_bf16.  Ties go to the lowest group and the lowest expert.
+ * Scores, sums and comparisons are 64-bit.  An expert with a logit of -infinity is masked: it is chosen
+ * last, with weight 0; a choice score that is a NaN counts as -infinity too.  A softmax row with a NaN
+ * or +infinity has NaN weights.  The IDs of a row are always distinct and in [0, E).
+ * E <= 512, topk <= 32.
+ */
+int ferry_route_experts(const void* logits, int32_t logits_dtype, int64_t tokens, int64_t experts,
+                        int64_t topk, int32_t sigmoid, const float* bias, int64_t groups,
+                        int64_t topk_groups, int32_t group_top2, int32_t renorm, float scale,
+                        int64_t* idx_out, void* w_out_bf16, void* stream);
+
+/*
+ * MXFP4 rows (no counterpart in the reference, whose rows are bf16): 4-bit elements (sign, two exponent
+ * bits, one mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6) with one scale byte, 2^(byte - 127), per 32
+ * consecutive elements of a row; element 2 i is the low half of its byte.  A row of `cols` elements has
+ * ceil(cols / 32) scales and 16 code bytes for each of them; elements past `cols` are 0.
+ * Quantisation: the scale of a block is 2^(floor(log2(largest magnitude)) - 2), at least 2^-127; an
+ * element is the nearest value, ties to the even code, saturating at 6.  A block with an infinity or
+ * a NaN has scale byte 255 and reads back as NaN.  Dequantisation rounds to the output type.
+ * Strides are those of rows: elements of x / out, bytes of codes (a multiple of 4) and scales.
+ */
+int ferry_mxfp4_quantize(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t x_stride,
+                         void* codes, int64_t codes_stride, void* scales, int64_t scales_stride,
+                         void* stream);
+int ferry_mxfp4_dequantize(const void* codes, int64_t codes_stride, const void* scales,
+                           int64_t scales_stride, int64_t rows, int64_t cols, void* out, int32_t dtype,
+                           int64_t out_stride, void* stream);
 
 /*
  * Dispatch layout at world = 1.  Replaces ferry/layout.py:12-94 (build_layout +

@@ -1,0 +1,539 @@
+// Grouped SwiGLU expert FFN over MXFP4 cache slots.
+//
+// For each expert e with rows p in [starts[e], starts[e+1]):
+//   x = in[rows[p]];  g = x Wg^T;  u = x Wu^T;  a = silu(g) * u;  y = a Wd^T;
+//   out = bf16(y * w[rows[p], cols[p]])
+// with cache[slot] = [codes of Wg (I x H) | Wu (I x H) | Wd (H x I), then their scales], the MXFP4 form
+// of the bf16 cache row (mxfp4.hip).  Sums are fp32.  Two kinds of activations:
+//  * bf16 (Q = false): x is bf16 and a is rounded to bf16, an operand of the bf16 matrix instruction.
+//    The 4-bit weights become bf16 in registers, which is exact.
+//  * MXFP4 (Q = true): x is codes and scales, and a is quantised from fp32 in the up epilogue, per 32
+//    columns, as mxfp4_quantize does; both products run on the scaled 4-bit matrix instruction.
+//
+// A lane's 16-byte load of weight codes is one block of 32 along K with one scale.  In a chunk of 128
+// along K, the lanes of row r take the blocks lane / 16 = 0..3: for the 4-bit instruction that is its
+// operand layout, and for the bf16 one the four steps s of a chunk multiply the elements 8 s .. 8 s + 7
+// of the blocks; the order along K inside a product is free as long as both operands share it.  So the
+// weights go from the plain row-major rows straight to registers, with no LDS, shuffle or repacking.
+#include "ffn_common.h"
+
+#include <type_traits>
+
+namespace ferry {
+namespace {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kSmallRows = 16;   // experts with at most this many rows run mx_small
+
+struct MxArgs {
+  const uint8_t* cache;
+  const uint8_t* x;         // bf16 [R, H], or codes [R, H / 2]
+  const uint8_t* x_scales;  // [R, H / 32] (Q)
+  const bf16_t* w;          // [R, k] routing weights in sorted-ID order
+  const int64_t* starts;    // [E+1]
+  const int64_t* rows;      // [R*k]
+  const int64_t* cols;      // [R*k]
+  uint8_t* act;             // bf16 [R*k, I], or codes [R*k, I / 2]
+  uint8_t* act_scales;      // [R*k, I / 32] (Q)
+  bf16_t* out;              // [R*k, H]
+  int64_t H, I, k;
+  int32_t out_mode;
+  ExpertList list;
+};
+
+// 8 elements of a code word as bf16, scaled (exact)
+__device__ __forceinline__ bf16x8 decode8(uint32_t c, float s) {
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 0);
+  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 1);
+  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 2);
+  const bf16x2 e = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 3);
+  return bf16x8{a[0], a[1], b[0], b[1], d[0], d[1], e[0], e[1]};
+}
+// the scale of a byte for the conversions, which read the exponent field (0: 2^-127, 255: NaN)
+__device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
+
+__device__ __forceinline__ floatx4 mma_fp4(u32x4 w, int sw, u32x4 x, int sx, floatx4 c) {
+  const i32x8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
+  const i32x8 b = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 4, 0, sw, 0, sx);
+}
+
+// The weight matrix of a projection in a cache row: codes and scales of `row`, K columns.
+struct Weights {
+  const uint8_t* codes;
+  const uint8_t* scales;
+};
+// MODE 0: gate (part 0) and up (part 1), rows of H; MODE 1: down, rows of I
+template <int MODE>
+__device__ __forceinline__ Weights weights_at(const MxArgs& a, int slot, int part, int64_t row) {
+  const int64_t n = a.H * a.I;   // elements of a matrix
+  const int64_t at = MODE == 0 ? part * n + row * a.H : 2 * n + row * a.I;
+  const uint8_t* base = a.cache + (int64_t)slot * (3 * n / 32 * 17);
+  return {base + at / 2, base + 3 * n / 2 + at / 32};
+}
+
+// a = silu(g) * u quantised: this lane's values v of a block that it shares with the lanes ^ 16, ^ 32
+// (each lane 8 of 32 columns); returns the scale byte
+__device__ __forceinline__ int block_scale(const float (&v)[8]) {
+  uint32_t amax = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(v[i]) & 0x7fffffffu);
+  amax = max(amax, (uint32_t)__shfl_xor((int)amax, 16, 64));
+  amax = max(amax, (uint32_t)__shfl_xor((int)amax, 32, 64));
+  const int ex = (int)(amax >> 23);
+  return ex == 255 ? 255 : (ex > 2 ? ex - 2 : 0);
+}
+__device__ __forceinline__ uint32_t block_codes(const float (&v)[8], int byte) {
+  const bool bad = byte == 255;
+  const float inv = __uint_as_float((uint32_t)(bad ? 0 : 254 - byte) << 23);   // 2^(127 - byte), exact
+  float y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = bad ? 0.0f : v[i] * inv;
+  uint32_t c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0, y[0], y[1], 1.0f, 0);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, y[2], y[3], 1.0f, 1);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, y[4], y[5], 1.0f, 2);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, y[6], y[7], 1.0f, 3);
+}
+
+// =============================================================================================
+// Experts with at most 16 rows (decode, and the smallest experts of a prefill)
+// =============================================================================================
+
+// One workgroup: NF tiles of 16 weight rows (MODE 0: 32 columns of gate and of up; MODE 1: 64 hidden rows)
+// x the expert's rows; its four wavefronts split K, their sums meet in LDS in wavefront order.  Bound by
+// the weight bytes.
+template <int MODE, bool Q>
+__global__ __launch_bounds__(256) void mx_small(MxArgs a) {
+  constexpr int NF = 4;
+  __shared__ floatx4 part[4][NF][64];
+  const int li = blockIdx.y, bx = blockIdx.x;
+  const int e = a.list.expert[li], slot = a.list.slot[li];
+  const int64_t start = a.starts[e];
+  const int64_t n = a.starts[e + 1] - start;
+  if (n < 1 || n > kSmallRows) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, q = lane >> 4;
+  const int64_t K = MODE == 0 ? a.H : a.I;
+  const int chunks = (int)(K / 128), c0 = wave * chunks / 4, c1 = (wave + 1) * chunks / 4;
+  const int64_t p = start + (r < n ? r : 0);   // lanes without a row of their own read the first one's
+  const int64_t src = MODE == 0 ? a.rows[p] : p;
+  const uint8_t* xp = MODE == 0 ? a.x : a.act;
+  const uint8_t* xs = MODE == 0 ? a.x_scales : a.act_scales;
+  xp += Q ? src * (K / 2) + q * 16 : src * K * 2 + q * 64;
+  if (Q) xs += src * (K / 32) + q;
+  Weights wp[NF];
+#pragma unroll
+  for (int f = 0; f < NF; ++f) {
+    wp[f] = MODE == 0 ? weights_at<0>(a, slot, f >> 1, bx * 32 + (f & 1) * 16 + r)
+                      : weights_at<1>(a, slot, 0, bx * 64 + f * 16 + r);
+    wp[f].codes += q * 16;
+    wp[f].scales += q;
+  }
+  floatx4 acc[NF];
+#pragma unroll
+  for (int f = 0; f < NF; ++f) acc[f] = floatx4{0, 0, 0, 0};
+  for (int c = c0; c < c1; ++c) {
+    u32x4 wc[NF];
+    uint32_t ws[NF];
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+      wc[f] = *(const u32x4*)(wp[f].codes + c * 64);
+      ws[f] = wp[f].scales[c * 4];
+    }
+    if constexpr (Q) {
+      const u32x4 xc = *(const u32x4*)(xp + c * 64);
+      const uint32_t xb = xs[c * 4];
+#pragma unroll
+      for (int f = 0; f < NF; ++f) acc[f] = mma_fp4(wc[f], (int)ws[f], xc, (int)xb, acc[f]);
+    } else {
+      bf16x8 xv[4];
+#pragma unroll
+      for (int s = 0; s < 4; ++s) xv[s] = *(const bf16x8*)(xp + c * 256 + s * 16);
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int f = 0; f < NF; ++f)
+          acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(decode8(wc[f][s], scale_of(ws[f])), xv[s], acc[f],
+                                                           0, 0, 0);
+    }
+  }
+#pragma unroll
+  for (int f = 0; f < NF; ++f) part[wave][f][lane] = acc[f];
+  __syncthreads();
+  // lane l of a tile holds the columns (l / 16) * 4 + i of row l % 16
+  auto sum = [&](int f) {
+    floatx4 v = part[0][f][lane];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) v += part[w][f][lane];
+    return v;
+  };
+  const bool live = r < n;
+  if constexpr (MODE == 0) {
+    if constexpr (Q) {
+      if (wave != 0) return;
+      float v[8];   // columns 16 (i / 4) + 4 q + i % 4
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const floatx4 g = sum(b), u = sum(2 + b);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[4 * b + i] = silu_mul(g[i], u[i]);
+      }
+      const int byte = block_scale(v);
+      const uint32_t c = block_codes(v, byte);
+      if (live) {
+        uint8_t* o = a.act + p * (a.I / 2) + bx * 16 + q * 2;
+        *(uint16_t*)o = (uint16_t)c;
+        *(uint16_t*)(o + 8) = (uint16_t)(c >> 16);
+        if (q == 0) a.act_scales[p * (a.I / 32) + bx] = (uint8_t)byte;
+      }
+    } else {
+      if (wave >= 2) return;
+      const floatx4 g = sum(wave), u = sum(2 + wave);
+      u32x2 y;
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) y[i / 2] = pk_bf16(silu_mul(g[i], u[i]), silu_mul(g[i + 1], u[i + 1]));
+      if (live) *(u32x2*)(a.act + (p * a.I + bx * 32 + wave * 16 + q * 4) * 2) = y;
+    }
+  } else {
+    const floatx4 y = sum(wave);
+    if (live) {
+      const int64_t t = a.rows[p] * a.k + a.cols[p];
+      const float wt = bf16_to_f32(a.w[t]);
+      const int64_t o = a.out_mode == 0 ? t : p;
+      *(u32x2*)(a.out + o * a.H + bx * 64 + wave * 16 + q * 4) =
+          u32x2{pk_bf16(y[0] * wt, y[1] * wt), pk_bf16(y[2] * wt, y[3] * wt)};
+    }
+  }
+}
+
+// =============================================================================================
+// Larger experts: tiles of TM rows x TN weight rows
+// =============================================================================================
+
+// WM x WN wavefronts, each MI x NI tiles of 16 rows x 16 weight rows.  The rows' activations of a chunk of
+// 128 along K are staged in LDS by direct loads, two chunks in turn; the weights go straight to
+// registers, one chunk ahead.  A row's 16-byte pieces are stored at slot piece ^ swizzle(row), so that
+// the 16 rows that a quarter of a wavefront reads lie on 16 different 16-byte bank groups (of the 256-byte
+// bank line: one bf16 row of a chunk, or four 4-bit rows).
+// MODE 0: of a wavefront's NI = 4 weight tiles, two are gate rows and two the up rows of the same 32 columns.
+// The weight rows of the two tiles c of 32 columns interleave in groups of four, 8 g + 4 c + [0, 4):
+// a lane then holds 8 consecutive output columns of one row.
+template <int MODE, bool Q, int WM, int WN, int MI>
+__global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM * WN / 4, WM * WN / 4)))
+void mx_tiled(MxArgs a) {
+  constexpr int NI = 4, W = WM * WN, TM = 16 * WM * MI;
+  constexpr int COLS = MODE == 0 ? 32 * WN : 64 * WN;   // output columns of a tile
+  constexpr int RB = Q ? 64 : 256;                      // a row's bytes of a chunk
+  constexpr int LA = TM * RB / (1024 * W);              // direct loads per wavefront and chunk
+  constexpr int kStage = TM * RB, kScales = Q ? TM * 4 : 0;
+  constexpr int kBatch = TM / 64;                       // wavefronts that load the scales
+  static_assert(LA >= 1 && kBatch <= W);
+  __shared__ TileTable tt;
+  __shared__ __attribute__((aligned(1024))) char smem[2 * (kStage + kScales)];
+  __shared__ int32_t src_s[MODE == 0 ? TM : 1], orow_s[MODE == 1 ? TM : 1];
+  __shared__ float wt_s[MODE == 1 ? TM : 1];
+  build_tile_table<TM, kSmallRows>(a, tt);
+  const int64_t K = MODE == 0 ? a.H : a.I;
+  const int ntn = (int)((MODE == 0 ? a.I : a.H) / COLS);
+  const int total = __builtin_amdgcn_readfirstlane(tt.total) * ntn;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  const int r = lane & 15, q = lane >> 4;
+  const int chunks = (int)(K / 128);
+  const uint32_t smem0 = lds_addr(smem);
+  const char* const abase = reinterpret_cast<const char*>(MODE == 0 ? a.x : a.act);
+  const char* const sbase = reinterpret_cast<const char*>(MODE == 0 ? a.x_scales : a.act_scales);
+  auto swz = [](int row) { return Q ? (row >> 2) & 3 : row & 15; };
+  const int wrow = 8 * (r >> 2) + (r & 3);   // this lane's weight row of a pair of tiles (c = 0)
+  const uint32_t wcode = (uint32_t)wrow * (uint32_t)(K / 2) + (uint32_t)(q * 16);
+  const uint32_t wscale = (uint32_t)wrow * (uint32_t)(K / 32) + (uint32_t)q;
+
+  const int per_xcd = gridDim.x % 8 == 0 ? (int)gridDim.x / 8 : 0;
+  const int first = per_xcd ? (int)(blockIdx.x % 8) * per_xcd + (int)(blockIdx.x / 8) : (int)blockIdx.x;
+  for (int tile = first; tile < total; tile += gridDim.x) {
+    const int mt = tile / ntn, nt = tile - mt * ntn;
+    const int li = __builtin_amdgcn_readfirstlane(find_entry(tt, mt));
+    const int64_t start = uniform64(tt.start[li]);
+    const int m0 = (mt - __builtin_amdgcn_readfirstlane(tt.cum[li])) * TM;
+    const int vrows = __builtin_amdgcn_readfirstlane(tt.rows[li]) - m0;   // > 0
+    const int64_t row0 = start + m0;
+    const int slot = a.list.slot[li];
+    // the rows' sources; rows past the last take the first one's (they are never stored)
+    for (int t = tid; t < TM; t += 64 * W) {
+      const int64_t p = row0 + (t < vrows ? t : 0);
+      const int64_t tok = a.rows[p];
+      if constexpr (MODE == 0) {
+        src_s[t] = (int32_t)tok;
+      } else {
+        const int64_t tj = tok * a.k + a.cols[p];
+        orow_s[t] = (int32_t)(a.out_mode == 0 ? tj : p);
+        wt_s[t] = bf16_to_f32(a.w[tj]);
+      }
+    }
+    __syncthreads();
+    uint32_t aoff[LA], soff = 0;
+    auto src_row = [&](int t) {
+      return MODE == 0 ? (uint32_t)src_s[t] : (uint32_t)(row0 + (t < vrows ? t : 0));
+    };
+#pragma unroll
+    for (int j = 0; j < LA; ++j) {
+      const int piece = (wave * LA + j) * 64 + lane, t = piece * 16 / RB, s = piece % (RB / 16);
+      aoff[j] = src_row(t) * (uint32_t)(Q ? K / 2 : K * 2) + (uint32_t)((s ^ swz(t)) * 16);
+    }
+    if (Q && wave < kBatch) soff = src_row(wave * 64 + lane) * (uint32_t)(K / 32);
+    auto stage = [&](int c) {
+      const uint32_t dst = smem0 + (uint32_t)((c & 1) * (kStage + kScales));
+#pragma unroll
+      for (int j = 0; j < LA; ++j)
+        dma16(abase + (int64_t)c * RB, aoff[j], dst + (uint32_t)((wave * LA + j) * 1024));
+      if (Q && wave < kBatch) dma4(sbase + (int64_t)c * 4, soff, dst + (uint32_t)(kStage + wave * 256));
+    };
+    const uint8_t *wc[2], *ws[2];   // per pair of tiles (MODE 0: gate, up; MODE 1: two groups of 32 rows)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const Weights m = MODE == 0 ? weights_at<0>(a, slot, h, nt * COLS + wn * 32)
+                                  : weights_at<1>(a, slot, 0, nt * COLS + wn * 64 + h * 32);
+      wc[h] = uniform_ptr(m.codes);
+      ws[h] = uniform_ptr(m.scales);
+    }
+    u32x4 wn_c[NI];
+    uint32_t wn_s[NI];
+    auto load_w = [&](int c) {
+#pragma unroll
+      for (int f = 0; f < NI; ++f) {
+        wn_c[f] = *(const u32x4*)(wc[f >> 1] + (f & 1) * (2 * K) + c * 64 + wcode);
+        wn_s[f] = *(ws[f >> 1] + (f & 1) * (K / 8) + c * 4 + wscale);
+      }
+    };
+    // tiles of 16 rows of this wavefront that hold rows of the expert: rows 16 (WM i + wm) ..
+    const int left = vrows - 16 * wm;
+    const int nf = __builtin_amdgcn_readfirstlane(left <= 0 ? 0 : min(MI, (left + 16 * WM - 1) / (16 * WM)));
+    floatx4 acc[MI][NI];
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int f = 0; f < NI; ++f) acc[i][f] = floatx4{0, 0, 0, 0};
+    stage(0);
+    load_w(0);
+    auto loop = [&](auto partial) {
+      constexpr bool PARTIAL = decltype(partial)::value;
+      for (int c = 0; c < chunks; ++c) {
+        u32x4 cw[NI];
+        uint32_t cs[NI];
+#pragma unroll
+        for (int f = 0; f < NI; ++f) cw[f] = wn_c[f], cs[f] = wn_s[f];
+        wait_cnt<0>();   // chunk c's activations have landed
+        wg_barrier();    // ... everybody's, and nobody reads the other buffer any more
+        if (c + 1 < chunks) {
+          stage(c + 1);
+          load_w(c + 1);
+        }
+        const uint32_t at = smem0 + (uint32_t)((c & 1) * (kStage + kScales));
+        if constexpr (Q) {
+#pragma unroll
+          for (int i = 0; i < MI; ++i) {
+            if (PARTIAL && i >= nf) continue;
+            const int t = 16 * (WM * i + wm) + r;
+            const u32x4 xv = *reinterpret_cast<__attribute__((address_space(3))) const u32x4*>(
+                (uintptr_t)(at + (uint32_t)(t * RB + ((q ^ swz(t)) << 4))));
+            const uint32_t sx = *reinterpret_cast<__attribute__((address_space(3))) const uint32_t*>(
+                                    (uintptr_t)(at + (uint32_t)(kStage + t * 4))) >> (8 * q);
+#pragma unroll
+            for (int f = 0; f < NI; ++f) acc[i][f] = mma_fp4(cw[f], (int)cs[f], xv, (int)sx, acc[i][f]);
+          }
+        } else {
+#pragma unroll
+          for (int s = 0; s < 4; ++s) {
+            bf16x8 wv[NI];
+#pragma unroll
+            for (int f = 0; f < NI; ++f) wv[f] = decode8(cw[f][s], scale_of(cs[f]));
+#pragma unroll
+            for (int i = 0; i < MI; ++i) {
+              if (PARTIAL && i >= nf) continue;
+              const int t = 16 * (WM * i + wm) + r;
+              const bf16x8 xv = lds_read16(at + (uint32_t)(t * RB + (((4 * q + s) ^ swz(t)) << 4)));
+#pragma unroll
+              for (int f = 0; f < NI; ++f)
+                acc[i][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv[f], xv, acc[i][f], 0, 0, 0);
+            }
+          }
+        }
+      }
+    };
+    if (vrows >= TM)
+      loop(std::false_type{});
+    else
+      loop(std::true_type{});
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const int t = 16 * (WM * i + wm) + r;
+      const bool live = t < vrows;
+      if constexpr (MODE == 0) {
+        float v[8];
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[4 * c + j] = silu_mul(acc[i][c][j], acc[i][2 + c][j]);
+        const int64_t col = nt * COLS + wn * 32;
+        if constexpr (Q) {
+          const int byte = block_scale(v);
+          const uint32_t c = block_codes(v, byte);
+          if (live) {
+            *(uint32_t*)(a.act + (row0 + t) * (a.I / 2) + col / 2 + q * 4) = c;
+            if (q == 0) a.act_scales[(row0 + t) * (a.I / 32) + col / 32] = (uint8_t)byte;
+          }
+        } else if (live) {
+          *(u32x4*)(a.act + ((row0 + t) * a.I + col + q * 8) * 2) =
+              u32x4{pk_bf16(v[0], v[1]), pk_bf16(v[2], v[3]), pk_bf16(v[4], v[5]), pk_bf16(v[6], v[7])};
+        }
+      } else if (live) {
+        const float wt = wt_s[t];
+        bf16_t* const o = a.out + (int64_t)orow_s[t] * a.H + nt * COLS + wn * 64 + q * 8;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          u32x4 y;
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int j = 0; j < 4; j += 2)
+              y[2 * c + j / 2] = pk_bf16(acc[i][2 * h + c][j] * wt, acc[i][2 * h + c][j + 1] * wt);
+          *(u32x4*)(o + 32 * h) = y;
+        }
+      }
+    }
+    __syncthreads();   // the next tile rewrites the row tables and the first buffer
+  }
+}
+
+int device_cus(int* cus) {
+  int dev = 0;
+  FERRY_HIP(hipGetDevice(&dev));
+  FERRY_HIP(hipDeviceGetAttribute(cus, hipDeviceAttributeMultiprocessorCount, dev));
+  if (*cus <= 0) *cus = 256;
+  return 0;
+}
+
+// The launches of one list in one kind of activations; tiles: row tiles of 256 rows of the experts with more
+// than kSmallRows rows (an upper bound).
+template <bool Q>
+int launch_list(const MxArgs& a, bool small, int64_t tiles, int32_t phases, int64_t cus, hipStream_t s) {
+  for (int mode = 0; mode < 2; ++mode) {
+    if (!(phases & (1 << mode))) continue;
+    if (small) {
+      const dim3 g((unsigned)(mode == 0 ? a.I / 32 : a.H / 64), (unsigned)a.list.n);
+      launch(mode == 0 ? "mx_small_up" : "mx_small_down", mode == 0 ? mx_small<0, Q> : mx_small<1, Q>, g,
+             dim3(256), 0, s, a);
+      FERRY_LAUNCHED("mx_small");
+    }
+    if (tiles) {
+      const int64_t t = tiles * (mode == 0 ? a.I / 128 : a.H / 256);
+      launch(mode == 0 ? "mx_tiled_up" : "mx_tiled_down", mode == 0 ? mx_tiled<0, Q, 2, 4, 8> : mx_tiled<1, Q, 2, 4, 8>,
+             dim3((unsigned)(t < cus ? t : cus)), dim3(512), 0, s, a);
+      FERRY_LAUNCHED("mx_tiled");
+    }
+  }
+  return 0;
+}
+
+}  // namespace
+}  // namespace ferry
+
+using namespace ferry;
+
+extern "C" int ferry_mxfp4_expert_ffn(const void* cache, int64_t cache_rows, int64_t hidden, int64_t inter,
+                                      const void* x, const void* x_scales, int64_t rows_in, int64_t topk,
+                                      const void* w_sorted, const int64_t* starts, const int64_t* rows,
+                                      const int64_t* cols, const int32_t* expert_list, int32_t n_list,
+                                      const int32_t* slot_of, int64_t experts, int64_t max_rows_per_expert,
+                                      int64_t min_rows_per_expert, const int32_t* list_rows, void* act,
+                                      void* out, int32_t out_mode, int32_t phases, int32_t spare_cus,
+                                      void* stream) {
+  clear_error();
+  FERRY_CHECK_ARG(phases >= 1 && phases <= 3, "phases must be 1 (up), 2 (down) or 3 (both)");
+  FERRY_CHECK_ARG(hidden > 0 && hidden % 128 == 0, "hidden must be a positive multiple of 128");
+  FERRY_CHECK_ARG(inter > 0 && inter % 128 == 0, "intermediate must be a positive multiple of 128");
+  FERRY_CHECK_ARG(hidden <= 1 << 20 && inter <= 1 << 20, "hidden and intermediate must be at most 2^20");
+  FERRY_CHECK_ARG(topk >= 1 && rows_in >= 0 && n_list >= 0 && max_rows_per_expert >= 0, "bad sizes");
+  FERRY_CHECK_ARG(min_rows_per_expert >= 0 && min_rows_per_expert <= max_rows_per_expert,
+                  "min_rows_per_expert must be in [0, max_rows_per_expert]");
+  FERRY_CHECK_ARG(experts >= 1 && experts <= FERRY_MAX_EXPERTS, "experts must be in [1, %d]",
+                  FERRY_MAX_EXPERTS);
+  FERRY_CHECK_ARG(out_mode == 0 || out_mode == 1, "out_mode must be 0 or 1");
+  FERRY_CHECK_ARG(spare_cus >= 0 && spare_cus <= 128, "spare_cus must be in [0, 128]");
+  FERRY_CHECK_ARG(hidden % 256 == 0 || max_rows_per_expert <= kSmallRows,
+                  "hidden must be a multiple of 256 when an expert has more than %d rows", kSmallRows);
+  FERRY_CHECK_ARG(rows_in < (int64_t)1 << 31 && topk < (int64_t)1 << 31 && rows_in * topk < (int64_t)1 << 31,
+                  "rows*topk must be < 2^31");
+  // the kernels address activations with 32-bit byte offsets
+  FERRY_CHECK_ARG(rows_in < ((int64_t)1 << 31) / hidden && rows_in * topk < ((int64_t)1 << 31) / inter,
+                  "x / act must hold fewer than 2^31 elements");
+  if (n_list == 0 || rows_in == 0) return 0;
+  FERRY_CHECK_ARG(cache && x && w_sorted && starts && rows && cols && expert_list && slot_of && act && out,
+                  "null pointer argument");
+  FERRY_CHECK_ARG(((uintptr_t)cache | (uintptr_t)x | (uintptr_t)act | (uintptr_t)out) % 16 == 0,
+                  "cache, x, act and out must be 16-byte aligned");
+  FERRY_CHECK_ARG((uintptr_t)x_scales % 4 == 0, "x_scales must be 4-byte aligned");
+  for (int32_t i = 0; i < n_list; ++i) {
+    const int32_t e = expert_list[i];
+    FERRY_CHECK_ARG(e >= 0 && e < experts, "expert_list[%d] = %d out of range", i, e);
+    const int32_t s = slot_of[e];
+    FERRY_CHECK_ARG(s >= 0 && s < cache_rows, "expert %d is not cached (slot %d)", e, s);
+    if (list_rows)
+      FERRY_CHECK_ARG(list_rows[i] >= min_rows_per_expert && list_rows[i] <= max_rows_per_expert,
+                      "list_rows[%d] = %d outside [min_rows_per_expert, max_rows_per_expert]", i,
+                      list_rows[i]);
+  }
+  int cus = 0;
+  if (const int rc = device_cus(&cus)) return rc;
+  if (cus > 2 * spare_cus) cus -= spare_cus;
+  const bool quantised = x_scales != nullptr;
+  const int64_t pairs = rows_in * topk;
+  MxArgs a;
+  a.cache = (const uint8_t*)cache;
+  a.x = (const uint8_t*)x;
+  a.x_scales = (const uint8_t*)x_scales;
+  a.w = (const bf16_t*)w_sorted;
+  a.starts = starts;
+  a.rows = rows;
+  a.cols = cols;
+  a.act = (uint8_t*)act;
+  a.act_scales = (uint8_t*)act + pairs * (inter / 2);
+  a.out = (bf16_t*)out;
+  a.H = hidden;
+  a.I = inter;
+  a.k = topk;
+  a.out_mode = out_mode;
+  a.list.n_mid = 0;
+  // one pass over the small experts, one over the others; without row counts every expert is in both, and
+  // the kernels pass over those of the other kind by the device's starts
+  for (int big = 0; big < 2; ++big) {
+    if (big ? max_rows_per_expert <= kSmallRows : min_rows_per_expert > kSmallRows) continue;
+    int64_t tiles = 0;
+    a.list.n = 0;
+    auto flush = [&]() {
+      if (a.list.n == 0) return 0;
+      // row counts unknown: sum ceil(n / 256) <= pairs / 256 + the experts with more than kSmallRows rows
+      if (big && !list_rows) tiles = pairs / 256 + (a.list.n < pairs / (kSmallRows + 1) + 1 ? a.list.n : pairs / (kSmallRows + 1) + 1);
+      const int rc = quantised ? launch_list<true>(a, !big, tiles, phases, cus, (hipStream_t)stream)
+                               : launch_list<false>(a, !big, tiles, phases, cus, (hipStream_t)stream);
+      a.list.n = 0;
+      tiles = 0;
+      return rc;
+    };
+    for (int32_t i = 0; i < n_list; ++i) {
+      if (list_rows) {
+        if (list_rows[i] < 1 || (list_rows[i] > kSmallRows) != (big != 0)) continue;
+        if (big) tiles += ceil_div(list_rows[i], 256);
+      }
+      a.list.expert[a.list.n] = (int16_t)expert_list[i];
+      a.list.slot[a.list.n++] = slot_of[expert_list[i]];
+      if (a.list.n == kListMax)
+        if (const int rc = flush()) return rc;
+    }
+    if (const int rc = flush()) return rc;
+  }
+  return 0;
+}

@@ -22,7 +22,7 @@ from .h2d import H2DEngine
 __all__ = ['execute_experts', 'pack_dispatch', 'unpack_dispatch', 'reduce_partials',
            'scatter_returned', 'H2DEngine', 'router_topk', 'layout', 'gate_logits', 'expert_ffn',
            'combine', 'SharedExpert', 'route_experts', 'mxfp4_quantize', 'mxfp4_dequantize',
-           'mxfp4_expert_rows', 'history_update', 'history_ready_words', 'current_stream', 'PHASE_UP',
+           'mxfp4_expert_rows', 'mxfp4_expert_ffn', 'history_update', 'history_ready_words', 'current_stream', 'PHASE_UP',
            'PHASE_DOWN', 'PHASE_BOTH']
 
 MAX_EXPERTS = 512
@@ -411,6 +411,68 @@ def expert_ffn(cache, x, w_sorted, starts, rows, cols, expert_list, slot_of, hid
         rows_of = c.tolist()
         check(lib().ferry_expert_ffn_spare(*args, el_at, n, so_at, E, max(rows_of), min(rows_of),
                                      c.tobytes(), *tail), 'expert_ffn')
+    return out
+
+
+def mxfp4_expert_ffn(cache, x, w_sorted, starts, rows, cols, expert_list, slot_of, hidden,
+                     intermediate, act, out, out_mode=0, max_rows=None, experts=None, phases=PHASE_BOTH,
+                     counts=None, spare_cus=0):
+    """``expert_ffn`` over cache slots of MXFP4 rows (``mxfp4_expert_rows``: uint8 [slots, 3 * hidden *
+    intermediate / 32 * 17]), read as they are: 4.25 bits a weight.
+
+    ``x`` is bf16 [R, hidden], with ``act`` bf16 scratch of R * topk * intermediate elements; or
+    ``mxfp4_quantize``'s (codes, scales) of the rows, with ``act`` uint8 scratch of R * topk *
+    intermediate / 32 * 17 bytes: both products then take 4-bit operands on either side, which is the
+    faster form for prompts, and silu(g) * u is quantised on the way.  Sums and SwiGLU are fp32; an
+    output row is rounded to bf16 once, after its routing weight.  The other arguments are
+    ``expert_ffn``'s; rows of ``out`` that belong to experts outside the list are left as they are.
+    No counterpart in the reference.
+    """
+    R, k = w_sorted.shape
+    H, I = int(hidden), int(intermediate)
+    quantised = isinstance(x, (tuple, list))
+    codes, scales = x if quantised else (x, None)
+    at = [_dev(cache, 'cache', torch.uint8)]
+    if cache.dim() != 2 or cache.shape[1] * 32 != 3 * H * I * 17:
+        raise RuntimeError('cache must be uint8 [slots, 3 * hidden * intermediate / 32 * 17]')
+    if quantised:
+        at += [_dev(codes, 'x codes', torch.uint8), _dev(scales, 'x scales', torch.uint8)]
+        if codes.shape != (R, H // 2) or scales.shape != (R, H // 32):
+            raise RuntimeError('x must be the codes [rows, hidden / 2] and scales [rows, hidden / 32]')
+    else:
+        at += [_dev(codes, 'x', torch.bfloat16), None]
+        if codes.shape != (R, H):
+            raise RuntimeError('x must be bf16 [rows, hidden]')
+    el = np.ascontiguousarray(expert_list, dtype=np.int32)
+    so = np.ascontiguousarray(slot_of, dtype=np.int32)
+    E = int(experts if experts is not None else len(so))
+    if E > len(so) or (counts is not None and E > len(counts)):
+        raise RuntimeError('slot_of and counts must have an entry for every expert')
+    if len(el) and not 0 <= int(el.min()) <= int(el.max()) < E:
+        raise RuntimeError(f'expert_list must name experts in [0, {E})')
+    idx = [v if isinstance(v, int) else _dev(v, name, torch.int64) for v, name in ((rows, 'rows'), (cols, 'cols'))]
+    weights, first = _dev(w_sorted, 'w_sorted', torch.bfloat16), _dev(starts, 'starts', torch.int64)
+    if starts.numel() < E + 1:
+        raise RuntimeError('starts must have an entry for every expert, and the end')
+    act_at = _dev(act, 'act', torch.uint8 if quantised else torch.bfloat16)
+    out_at = _dev(out, 'out', torch.bfloat16)
+    if act.numel() < R * k * (I // 32 * 17 if quantised else I) or out.numel() < R * k * H:
+        raise RuntimeError('act and out must hold the rows of rows * topk (token, expert) pairs')
+    for t, name in ((codes, 'x'), (scales, 'x scales'), (w_sorted, 'w_sorted'), (starts, 'starts'), (rows, 'rows'),
+                    (cols, 'cols'), (act, 'act'), (out, 'out')):
+        if isinstance(t, torch.Tensor):
+            _on_device(t, name, cache)
+    list_rows, most, least = None, int(max_rows if max_rows is not None else R), 0
+    if isinstance(rows, torch.Tensor) and not rows.numel():
+        return out   # no pairs
+    if counts is not None:
+        c = np.ascontiguousarray(np.asarray(counts, dtype=np.int64)[el], dtype=np.int32)
+        if not len(c):
+            return out
+        list_rows, most, least = c.tobytes(), int(c.max()), int(c.min())
+    _native(cache, 'mxfp4_expert_ffn', lib().ferry_mxfp4_expert_ffn, at[0], cache.shape[0], H, I, at[1], at[2],
+            R, k, weights, first, idx[0], idx[1], el.tobytes(), len(el), so.tobytes(), E, most, least,
+            list_rows, act_at, out_at, int(out_mode), int(phases), int(spare_cus))
     return out
 
 

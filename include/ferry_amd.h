@@ -205,6 +205,26 @@ int ferry_expert_ffn_spare(const void* cache, int64_t cache_rows, int64_t hidden
                      int64_t experts, int64_t max_rows_per_expert,
                      int64_t min_rows_per_expert, const int32_t* list_rows, void* act, void* out,
                      int32_t out_mode, int32_t phases, int32_t spare_cus, void* stream);
+
+/*
+ * ferry_expert_ffn on MXFP4 cache rows (no counterpart in the reference): cache[slot] holds the codes
+ * of [gate I*H | up I*H | down H*I] and then their scales, 3 * H * I / 32 * 17 bytes (ferry_mxfp4_quantize
+ * of the bf16 row, or of its three matrices' rows).  With x_scales null, x is bf16 [R, H] and act bf16
+ * scratch of R * k * I elements, rounded once from fp32; otherwise x holds the codes [R, H / 2] and
+ * x_scales the scales [R, H / 32] of MXFP4 rows, and act is R * k * I / 32 * 17 bytes: the codes
+ * [R * k, I / 2] and then the scales [R * k, I / 32] of silu(g) * u, quantised from fp32.  The sums and
+ * the SwiGLU are fp32 and an output is rounded once, after its routing weight.  All other arguments as
+ * ferry_expert_ffn_spare's; experts with at most 16 rows run the bandwidth-bound kernels.  Output rows of
+ * experts that are not listed stay as they were.  hidden and intermediate are multiples of 128,
+ * hidden one of 256 when an expert has more than 16 rows; cache, x, act and out 16-byte aligned.
+ */
+int ferry_mxfp4_expert_ffn(const void* cache, int64_t cache_rows, int64_t hidden, int64_t inter,
+                           const void* x, const void* x_scales, int64_t rows_in, int64_t topk,
+                           const void* w_sorted, const int64_t* starts, const int64_t* rows,
+                           const int64_t* cols, const int32_t* expert_list, int32_t n_list,
+                           const int32_t* slot_of, int64_t experts, int64_t max_rows_per_expert,
+                           int64_t min_rows_per_expert, const int32_t* list_rows, void* act, void* out,
+                           int32_t out_mode, int32_t phases, int32_t spare_cus, void* stream);
 int ferry_expert_ffn_sync_timeouts(int64_t* count);
 int ferry_expert_ffn_set_sync_spin_limit(int64_t limit);
 

@@ -212,26 +212,37 @@ __global__ __launch_bounds__(256) void mx_small(MxArgs a) {
 // Larger experts: tiles of TM rows x TN weight rows
 // =============================================================================================
 
-// WM x WN wavefronts, each MI x NI tiles of 16 rows x 16 weight rows.  The rows' activations of a chunk of
-// 128 along K are staged in LDS by direct loads, two chunks in turn; the weights go straight to
-// registers, one chunk ahead.  A row's 16-byte pieces are stored at slot piece ^ swizzle(row), so that
-// the 16 rows that a quarter of a wavefront reads lie on 16 different 16-byte bank groups (of the 256-byte
-// bank line: one bf16 row of a chunk, or four 4-bit rows).
-// MODE 0: of a wavefront's NI = 4 weight tiles, two are gate rows and two the up rows of the same 32 columns.
+// WM x WN wavefronts, each MI x 4 tiles of 16 rows x 16 weight rows.  Activations and weights are staged in
+// LDS by direct loads, in rows of 128 bytes (whole cache lines, eight lanes a row): 256 along K of 4-bit
+// values (a stage), 64 of bf16 (four steps to a stage).  Loading the weights to registers in operand order
+// instead takes no LDS, but its lanes touch 64 places of 16 bytes: address processing then bounds the kernel
+// (5 us for 128 along K, whatever the products).  Two buffers each, the loads one stage or step ahead of
+// the products.  A row's 16-byte pieces are stored at slot piece ^ swizzle(row), so that the 16 rows that a
+// quarter of a wavefront reads lie on 16 different 16-byte bank groups.
+// MODE 0: of a wavefront's four weight tiles, two are gate rows and two the up rows of the same 32 columns.
 // The weight rows of the two tiles c of 32 columns interleave in groups of four, 8 g + 4 c + [0, 4):
 // a lane then holds 8 consecutive output columns of one row.
+__device__ __forceinline__ int swz_x(int row) { return (row >> 1) & 7; }
+__device__ __forceinline__ int swz_w(int row) { return ((row >> 1) & 1) | (((row >> 3) & 3) << 1); }
+
+typedef __attribute__((address_space(3))) const u32x4 lds_u32x4;
+typedef __attribute__((address_space(3))) const u32x2 lds_u32x2;
+typedef __attribute__((address_space(3))) const uint32_t lds_u32;
+template <typename T>
+__device__ __forceinline__ auto lds_get(uint32_t at) { return *reinterpret_cast<T*>((uintptr_t)at); }
+
 template <int MODE, bool Q, int WM, int WN, int MI>
 __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM * WN / 4, WM * WN / 4)))
 void mx_tiled(MxArgs a) {
-  constexpr int NI = 4, W = WM * WN, TM = 16 * WM * MI;
-  constexpr int COLS = MODE == 0 ? 32 * WN : 64 * WN;   // output columns of a tile
-  constexpr int RB = Q ? 64 : 256;                      // a row's bytes of a chunk
-  constexpr int LA = TM * RB / (1024 * W);              // direct loads per wavefront and chunk
-  constexpr int kStage = TM * RB, kScales = Q ? TM * 4 : 0;
-  constexpr int kBatch = TM / 64;                       // wavefronts that load the scales
-  static_assert(LA >= 1 && kBatch <= W);
+  constexpr int NI = 4, W = WM * WN, TM = 16 * WM * MI, TN = 16 * NI * WN;
+  constexpr int COLS = MODE == 0 ? TN / 2 : TN;          // output columns of a tile
+  constexpr int kX = TM * 128, kW = TN * 128;            // bytes of a buffer
+  constexpr int LX = kX / (1024 * W), LW = kW / (1024 * W);   // direct loads of a wavefront for one
+  constexpr int kXS = Q ? TM * 8 : 0, kWS = TN * 8;      // scale bytes of a stage
+  constexpr int H = Q ? 1 : 4;                           // steps of activations in a stage
+  static_assert(LX >= 1 && LW >= 1 && TM + TN <= 64 * W * (Q ? 1 : 2));
   __shared__ TileTable tt;
-  __shared__ __attribute__((aligned(1024))) char smem[2 * (kStage + kScales)];
+  __shared__ __attribute__((aligned(1024))) char smem[2 * (kX + kW + kXS + kWS)];
   __shared__ int32_t src_s[MODE == 0 ? TM : 1], orow_s[MODE == 1 ? TM : 1];
   __shared__ float wt_s[MODE == 1 ? TM : 1];
   build_tile_table<TM, kSmallRows>(a, tt);
@@ -242,14 +253,21 @@ void mx_tiled(MxArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
   const int r = lane & 15, q = lane >> 4;
-  const int chunks = (int)(K / 128);
+  const int chunks = (int)(K / 128), stages = (chunks + 1) / 2;
   const uint32_t smem0 = lds_addr(smem);
-  const char* const abase = reinterpret_cast<const char*>(MODE == 0 ? a.x : a.act);
-  const char* const sbase = reinterpret_cast<const char*>(MODE == 0 ? a.x_scales : a.act_scales);
-  auto swz = [](int row) { return Q ? (row >> 2) & 3 : row & 15; };
-  const int wrow = 8 * (r >> 2) + (r & 3);   // this lane's weight row of a pair of tiles (c = 0)
-  const uint32_t wcode = (uint32_t)wrow * (uint32_t)(K / 2) + (uint32_t)(q * 16);
-  const uint32_t wscale = (uint32_t)wrow * (uint32_t)(K / 32) + (uint32_t)q;
+  const uint32_t wbuf = smem0 + 2 * kX, xsbuf = wbuf + 2 * kW, wsbuf = xsbuf + 2 * kXS;
+  const char* const xbase = reinterpret_cast<const char*>(MODE == 0 ? a.x : a.act);
+  const uint8_t* const xsbase = MODE == 0 ? a.x_scales : a.act_scales;
+
+  // fragment reads: addresses of tile 0, the others at constant offsets
+  const int xrow = 16 * wm + r;
+  const int wrow = (MODE == 0 ? wn * 32 : wn * 64) + 8 * (r >> 2) + (r & 3);
+  const uint32_t xa = smem0 + (uint32_t)(xrow * 128 + (((Q ? q : 2 * q) ^ swz_x(xrow)) << 4));
+  const uint32_t wa = wbuf + (uint32_t)(wrow * 128 + (((Q ? q : q >> 1) ^ swz_w(wrow)) << 4) + (Q ? 0 : (q & 1) * 8));
+  constexpr int kXTile = 16 * WM * 128;
+  auto wtile = [](int f) { return (f >> 1) * (MODE == 0 ? TN / 2 : 32) + (f & 1) * 4; };   // in rows
+  // direct loads: load j of a wavefront moves the rows 8 (wave L + j) + lane / 8
+  const int r8 = lane >> 3, slot8 = lane & 7;
 
   const int per_xcd = gridDim.x % 8 == 0 ? (int)gridDim.x / 8 : 0;
   const int first = per_xcd ? (int)(blockIdx.x % 8) * per_xcd + (int)(blockIdx.x / 8) : (int)blockIdx.x;
@@ -260,7 +278,6 @@ void mx_tiled(MxArgs a) {
     const int m0 = (mt - __builtin_amdgcn_readfirstlane(tt.cum[li])) * TM;
     const int vrows = __builtin_amdgcn_readfirstlane(tt.rows[li]) - m0;   // > 0
     const int64_t row0 = start + m0;
-    const int slot = a.list.slot[li];
     // the rows' sources; rows past the last take the first one's (they are never stored)
     for (int t = tid; t < TM; t += 64 * W) {
       const int64_t p = row0 + (t < vrows ? t : 0);
@@ -274,99 +291,214 @@ void mx_tiled(MxArgs a) {
       }
     }
     __syncthreads();
-    uint32_t aoff[LA], soff = 0;
     auto src_row = [&](int t) {
       return MODE == 0 ? (uint32_t)src_s[t] : (uint32_t)(row0 + (t < vrows ? t : 0));
     };
+    const Weights m0w = weights_at<MODE>(a, a.list.slot[li], 0, nt * COLS);
+    const Weights m1w = MODE == 0 ? weights_at<MODE>(a, a.list.slot[li], 1, nt * COLS) : m0w;
+    uint32_t xoff[LX], woff[LW];
+    const char* wbase[LW];
 #pragma unroll
-    for (int j = 0; j < LA; ++j) {
-      const int piece = (wave * LA + j) * 64 + lane, t = piece * 16 / RB, s = piece % (RB / 16);
-      aoff[j] = src_row(t) * (uint32_t)(Q ? K / 2 : K * 2) + (uint32_t)((s ^ swz(t)) * 16);
+    for (int j = 0; j < LX; ++j) {
+      const int t = 8 * (wave * LX + j) + r8;
+      xoff[j] = src_row(t) * (uint32_t)(Q ? K / 2 : K * 2) + (uint32_t)((slot8 ^ swz_x(t)) * 16);
     }
-    if (Q && wave < kBatch) soff = src_row(wave * 64 + lane) * (uint32_t)(K / 32);
-    auto stage = [&](int c) {
-      const uint32_t dst = smem0 + (uint32_t)((c & 1) * (kStage + kScales));
 #pragma unroll
-      for (int j = 0; j < LA; ++j)
-        dma16(abase + (int64_t)c * RB, aoff[j], dst + (uint32_t)((wave * LA + j) * 1024));
-      if (Q && wave < kBatch) dma4(sbase + (int64_t)c * 4, soff, dst + (uint32_t)(kStage + wave * 256));
-    };
-    const uint8_t *wc[2], *ws[2];   // per pair of tiles (MODE 0: gate, up; MODE 1: two groups of 32 rows)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const Weights m = MODE == 0 ? weights_at<0>(a, slot, h, nt * COLS + wn * 32)
-                                  : weights_at<1>(a, slot, 0, nt * COLS + wn * 64 + h * 32);
-      wc[h] = uniform_ptr(m.codes);
-      ws[h] = uniform_ptr(m.scales);
+    for (int j = 0; j < LW; ++j) {
+      const int t0 = 8 * (wave * LW + j), part = MODE == 0 ? t0 / (TN / 2) : 0;
+      wbase[j] = reinterpret_cast<const char*>(uniform_ptr(part ? m1w.codes : m0w.codes));
+      woff[j] = (uint32_t)(t0 - part * (TN / 2) + r8) * (uint32_t)(K / 2) + (uint32_t)((slot8 ^ swz_w(t0 + r8)) * 16);
     }
-    u32x4 wn_c[NI];
-    uint32_t wn_s[NI];
-    auto load_w = [&](int c) {
-#pragma unroll
-      for (int f = 0; f < NI; ++f) {
-        wn_c[f] = *(const u32x4*)(wc[f >> 1] + (f & 1) * (2 * K) + c * 64 + wcode);
-        wn_s[f] = *(ws[f >> 1] + (f & 1) * (K / 8) + c * 4 + wscale);
+    // this thread's row of scales: a weight row, or (Q) an activation row
+    constexpr int kScaleRows = TN + (Q ? TM : 0);
+    const uint8_t* sp = nullptr;
+    uint32_t sdst = 0;
+    if (tid < TN) {
+      const int part = MODE == 0 ? tid / (TN / 2) : 0;
+      sp = (part ? m1w.scales : m0w.scales) + (int64_t)(tid - part * (TN / 2)) * (K / 32);
+      sdst = wsbuf + (uint32_t)(tid * 8);
+    } else if (tid < kScaleRows) {
+      sp = xsbase + (int64_t)src_row(tid - TN) * (K / 32);
+      sdst = xsbuf + (uint32_t)((tid - TN) * 8);
+    }
+    u32x2 sv = {0, 0};
+    auto load_s = [&](int st) {
+      if (tid < kScaleRows) {
+        if (2 * st + 1 < chunks) __builtin_memcpy(&sv, sp + st * 8, 8);
+        else __builtin_memcpy(&sv, sp + st * 8, 4);
       }
     };
-    // tiles of 16 rows of this wavefront that hold rows of the expert: rows 16 (WM i + wm) ..
-    const int left = vrows - 16 * wm;
-    const int nf = __builtin_amdgcn_readfirstlane(left <= 0 ? 0 : min(MI, (left + 16 * WM - 1) / (16 * WM)));
+    auto store_s = [&](int st) {
+      if (tid < kScaleRows)
+        *reinterpret_cast<__attribute__((address_space(3))) u32x2*>((uintptr_t)(sdst + (uint32_t)((st & 1) * (tid < TN ? kWS : kXS)))) = sv;
+    };
+    // Where the number of chunks is odd, the last stage's rows of 4-bit values end in its middle: the lanes of
+    // the second half read the first half again (it is not multiplied).
+    auto back = [&](int piece) { return (uint32_t)((piece & 4) << 4); };
+    auto load_x = [&](int n) {   // Q: stage n; bf16: step n
+      const uint32_t dst = smem0 + (uint32_t)((n & 1) * kX);
+#pragma unroll
+      for (int j = 0; j < LX; ++j) {
+        const uint32_t tail = Q && 2 * n + 1 >= chunks ? back(slot8 ^ swz_x(8 * (wave * LX + j) + r8)) : 0u;
+        dma16(xbase + (int64_t)n * 128, xoff[j] - tail, dst + (uint32_t)((wave * LX + j) * 1024));
+      }
+    };
+    auto load_w = [&](int st, int j) {
+      const uint32_t tail = 2 * st + 1 >= chunks ? back(slot8 ^ swz_w(8 * (wave * LW + j) + r8)) : 0u;
+      dma16(wbase[j] + (int64_t)st * 128, woff[j] - tail, wbuf + (uint32_t)((st & 1) * kW + (wave * LW + j) * 1024));
+    };
     floatx4 acc[MI][NI];
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
       for (int f = 0; f < NI; ++f) acc[i][f] = floatx4{0, 0, 0, 0};
-    stage(0);
-    load_w(0);
-    auto loop = [&](auto partial) {
-      constexpr bool PARTIAL = decltype(partial)::value;
-      for (int c = 0; c < chunks; ++c) {
-        u32x4 cw[NI];
-        uint32_t cs[NI];
+    load_s(0);
 #pragma unroll
-        for (int f = 0; f < NI; ++f) cw[f] = wn_c[f], cs[f] = wn_s[f];
-        wait_cnt<0>();   // chunk c's activations have landed
-        wg_barrier();    // ... everybody's, and nobody reads the other buffer any more
-        if (c + 1 < chunks) {
-          stage(c + 1);
-          load_w(c + 1);
-        }
-        const uint32_t at = smem0 + (uint32_t)((c & 1) * (kStage + kScales));
-        if constexpr (Q) {
+    for (int j = 0; j < LW; ++j) load_w(0, j);
+    load_x(0);
+    store_s(0);
+    wait_cnt<0>();
+    wg_barrier();
+    // ROWS: tiles of 16 rows of a wavefront that are multiplied; the others hold no row of the expert
+    auto loop = [&](auto rows) {
+      constexpr int ROWS = decltype(rows)::value;
+      if constexpr (Q) {
+        for (int st = 0; st < stages; ++st) {
+          const uint32_t xb = xa + (uint32_t)((st & 1) * kX), wb = wa + (uint32_t)((st & 1) * kW);
+          const uint32_t xsb = xsbuf + (uint32_t)((st & 1) * kXS + xrow * 8), wsb = wsbuf + (uint32_t)((st & 1) * kWS + wrow * 8);
+          u32x4 xn[2], wv[NI];
+          uint32_t xsn[2], ws[NI];
+          auto read_x = [&](int j, int i) {
 #pragma unroll
-          for (int i = 0; i < MI; ++i) {
-            if (PARTIAL && i >= nf) continue;
-            const int t = 16 * (WM * i + wm) + r;
-            const u32x4 xv = *reinterpret_cast<__attribute__((address_space(3))) const u32x4*>(
-                (uintptr_t)(at + (uint32_t)(t * RB + ((q ^ swz(t)) << 4))));
-            const uint32_t sx = *reinterpret_cast<__attribute__((address_space(3))) const uint32_t*>(
-                                    (uintptr_t)(at + (uint32_t)(kStage + t * 4))) >> (8 * q);
+            for (int v = 0; v < 2; ++v) {
+              xn[v] = lds_get<lds_u32x4>((xb ^ (uint32_t)(j << 6)) + (uint32_t)(kXTile * (i + v)));
+              xsn[v] = lds_get<lds_u32>(xsb + (uint32_t)(16 * WM * 8 * (i + v) + 4 * j));
+            }
+          };
+          auto read_w = [&](int j) {
 #pragma unroll
-            for (int f = 0; f < NI; ++f) acc[i][f] = mma_fp4(cw[f], (int)cs[f], xv, (int)sx, acc[i][f]);
+            for (int f = 0; f < NI; ++f) {
+              wv[f] = lds_get<lds_u32x4>((wb ^ (uint32_t)(j << 6)) + (uint32_t)(wtile(f) * 128));
+              ws[f] = lds_get<lds_u32>(wsb + (uint32_t)(wtile(f) * 8 + 4 * j));
+            }
+          };
+          read_w(0);
+          read_x(0, 0);
+          if (st + 1 < stages) {
+            load_s(st + 1);
+#pragma unroll
+            for (int j = 0; j < LW; ++j) load_w(st + 1, j);
+            load_x(st + 1);
           }
-        } else {
+          const int two = 2 * st + 1 < chunks;
 #pragma unroll
-          for (int s = 0; s < 4; ++s) {
-            bf16x8 wv[NI];
+          for (int j = 0; j < 2; ++j) {
+            if (j == 1 && !two) break;
+            u32x4 cw[NI];
+            int cs[NI];
 #pragma unroll
-            for (int f = 0; f < NI; ++f) wv[f] = decode8(cw[f][s], scale_of(cs[f]));
+            for (int f = 0; f < NI; ++f) cw[f] = wv[f], cs[f] = (int)(ws[f] >> (8 * q));
 #pragma unroll
-            for (int i = 0; i < MI; ++i) {
-              if (PARTIAL && i >= nf) continue;
-              const int t = 16 * (WM * i + wm) + r;
-              const bf16x8 xv = lds_read16(at + (uint32_t)(t * RB + (((4 * q + s) ^ swz(t)) << 4)));
+            for (int i = 0; i < ROWS; i += 2) {
+              const u32x4 x0 = xn[0], x1 = xn[1];
+              const int s0 = (int)(xsn[0] >> (8 * q)), s1 = (int)(xsn[1] >> (8 * q));
+              if (i + 2 < ROWS) {
+                read_x(j, i + 2);
+              } else if (j == 0) {
+                read_x(1, 0);
+                read_w(1);
+              }
+#pragma unroll
+              for (int f = 0; f < NI; ++f) acc[i][f] = mma_fp4(cw[f], cs[f], x0, s0, acc[i][f]);
+#pragma unroll
+              for (int f = 0; f < NI; ++f) acc[i + 1][f] = mma_fp4(cw[f], cs[f], x1, s1, acc[i + 1][f]);
+              __builtin_amdgcn_sched_barrier(0);
+            }
+          }
+          if (st + 1 < stages) store_s(st + 1);
+          wait_cnt<0>();   // the next stage's loads have landed, this one's fragments are read
+          wg_barrier();
+        }
+      } else {
+        u32x2 wr[NI], ws[NI];   // the weights' codes of the next step; their scales of the stage
+        u32x4 wv[2][NI];
+        auto read_w = [&](int st, int h) {
+          const uint32_t at = (wa + (uint32_t)((st & 1) * kW)) ^ (uint32_t)(h << 5);
+#pragma unroll
+          for (int f = 0; f < NI; ++f) wr[f] = lds_get<lds_u32x2>(at + (uint32_t)(wtile(f) * 128));
+        };
+        auto read_s = [&](int st) {
+#pragma unroll
+          for (int f = 0; f < NI; ++f)
+            ws[f] = lds_get<lds_u32x2>(wsbuf + (uint32_t)((st & 1) * kWS + (wrow + wtile(f)) * 8));
+        };
+        for (int st = 0; st < stages; ++st) {
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            const int n = 4 * st + h;
+            if (h >= 2 && 2 * st + 1 >= chunks) break;
+            const uint32_t xb = xa + (uint32_t)((h & 1) * kX);
+            bf16x8 xr[3];
+            auto read = [&](int m) {
+              xr[m % 3] = lds_read16((xb ^ (uint32_t)((m / ROWS) << 4)) + (uint32_t)(kXTile * (m % ROWS)));
+            };
+            if (h == 0) read_s(st);
+            read_w(st, h);
+            read(0);
+            read(1);
+            if (n + 1 < 2 * chunks) load_x(n + 1);
+            if (st + 1 < stages) {
+              if (h == 0) {
+                load_s(st + 1);
+#pragma unroll
+                for (int j = 0; j < (LW + 1) / 2; ++j) load_w(st + 1, j);
+              } else if (h == 1) {
+#pragma unroll
+                for (int j = (LW + 1) / 2; j < LW; ++j) load_w(st + 1, j);
+              }
+            }
+            float sc[NI];
+#pragma unroll
+            for (int f = 0; f < NI; ++f)
+              sc[f] = scale_of(__builtin_amdgcn_ubfe(ws[f][h >> 1], 16 * (h & 1) + 8 * (q >> 1), 8));
+            auto decode = [&](int s, int part) {   // half a weight tile's 32 columns
+              const int f = part >> 1, half = part & 1;
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                const bf16x2 d = half ? (j ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(wr[f][s], sc[f], 3)
+                                           : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(wr[f][s], sc[f], 2))
+                                      : (j ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(wr[f][s], sc[f], 1)
+                                           : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(wr[f][s], sc[f], 0));
+                wv[s][f][2 * half + j] = __builtin_bit_cast(uint32_t, d);
+              }
+            };
+#pragma unroll
+            for (int part = 0; part < 2 * NI; ++part) decode(0, part);
+#pragma unroll
+            for (int m = 0; m < 2 * ROWS; ++m) {
+              const int s = m / ROWS, i = m % ROWS;
+              if (m + 2 < 2 * ROWS) read(m + 2);
+              if (s == 0)
+#pragma unroll
+                for (int part = i * 2 * NI / ROWS; part < (i + 1) * 2 * NI / ROWS; ++part) decode(1, part);
 #pragma unroll
               for (int f = 0; f < NI; ++f)
-                acc[i][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv[f], xv, acc[i][f], 0, 0, 0);
+                acc[i][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, wv[s][f]), xr[m % 3],
+                                                                   acc[i][f], 0, 0, 0);
+              __builtin_amdgcn_sched_barrier(0);
             }
+            if (h == 1 && st + 1 < stages) store_s(st + 1);
+            wait_cnt<0>();
+            wg_barrier();
           }
         }
       }
     };
-    if (vrows >= TM)
-      loop(std::false_type{});
-    else
-      loop(std::true_type{});
+    // rows 16 (WM i + wm) .. + 16 are tile i of wavefront row wm: the tile's rows in steps of a quarter
+    if (vrows > TM / 4 * 3) loop(std::integral_constant<int, MI>{});
+    else if (vrows > TM / 2) loop(std::integral_constant<int, MI / 4 * 3>{});
+    else if (vrows > TM / 4) loop(std::integral_constant<int, MI / 2>{});
+    else loop(std::integral_constant<int, MI / 4>{});
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
       const int t = 16 * (WM * i + wm) + r;
@@ -404,7 +536,7 @@ void mx_tiled(MxArgs a) {
         }
       }
     }
-    __syncthreads();   // the next tile rewrites the row tables and the first buffer
+    __syncthreads();   // the next tile rewrites the row tables and the buffers
   }
 }
 

@@ -40,6 +40,7 @@ struct MxArgs {
   bf16_t* out;              // [R*k, H]
   int64_t H, I, k;
   int32_t out_mode;
+  int32_t known;            // the listed experts' row counts were given
   ExpertList list;
 };
 
@@ -59,6 +60,12 @@ __device__ __forceinline__ floatx4 mma_fp4(u32x4 w, int sw, u32x4 x, int sx, flo
   const i32x8 b = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], 0, 0, 0, 0};
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 4, 0, sw, 0, sx);
 }
+
+typedef __attribute__((address_space(3))) const u32x4 lds_u32x4;
+typedef __attribute__((address_space(3))) const u32x2 lds_u32x2;
+typedef __attribute__((address_space(3))) const uint32_t lds_u32;
+template <typename T>
+__device__ __forceinline__ auto lds_get(uint32_t at) { return *reinterpret_cast<T*>((uintptr_t)at); }
 
 // The weight matrix of a projection in a cache row: codes and scales of `row`, K columns.
 struct Weights {
@@ -101,64 +108,123 @@ __device__ __forceinline__ uint32_t block_codes(const float (&v)[8], int byte) {
 // Experts with at most 16 rows (decode, and the smallest experts of a prefill)
 // =============================================================================================
 
-// One workgroup: NF tiles of 16 weight rows (MODE 0: 32 columns of gate and of up; MODE 1: 64 hidden rows)
-// x the expert's rows; its four wavefronts split K, their sums meet in LDS in wavefront order.  Bound by
-// the weight bytes.
-template <int MODE, bool Q>
+// One workgroup: 16 NF weight rows (MODE 0: 8 NF columns of gate and of up; MODE 1: 16 NF hidden rows) x the
+// expert's rows.  Its four wavefronts split K in units of 256, whose sums meet in LDS in wavefront order.
+// Bound by the weight bytes: a wavefront brings up to kUnits units of its weights at once, by direct loads
+// of whole cache lines (8 rows x 128 bytes) into LDS, from where it reads the operands (swizzled as in the
+// tiles below); straight to registers in operand order, the lanes' 64 places of 16 bytes a load bound the
+// kernel at 3 TB/s.  The rows' activations go to registers: only the lanes of rows that are there load.
+constexpr int kUnits = 2;
+__device__ __forceinline__ int swz_w16(int row) { return (row >> 1) & 7; }   // 16 consecutive rows
+
+template <int MODE, bool Q, int NF>
 __global__ __launch_bounds__(256) void mx_small(MxArgs a) {
-  constexpr int NF = 4;
-  __shared__ floatx4 part[4][NF][64];
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  constexpr int kRowsW = 16 * NF, kW = kRowsW * 128, kUnit = kW + kRowsW * 8;   // LDS of a unit: codes, scales
   const int li = blockIdx.y, bx = blockIdx.x;
   const int e = a.list.expert[li], slot = a.list.slot[li];
-  const int64_t start = a.starts[e];
-  const int64_t n = a.starts[e + 1] - start;
-  if (n < 1 || n > kSmallRows) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, q = lane >> 4;
   const int64_t K = MODE == 0 ? a.H : a.I;
-  const int chunks = (int)(K / 128), c0 = wave * chunks / 4, c1 = (wave + 1) * chunks / 4;
-  const int64_t p = start + (r < n ? r : 0);   // lanes without a row of their own read the first one's
+  const int chunks = (int)(K / 128), units = (chunks + 1) / 2;
+  const int u0 = wave * units / 4, u1 = (wave + 1) * units / 4;
+  const uint32_t lds0 = lds_addr(smem) + (uint32_t)(wave * min(kUnits, (units + 3) / 4) * kUnit);
+
+  const Weights wp0 = weights_at<MODE>(a, slot, 0, MODE == 0 ? bx * (8 * NF) : bx * (16 * NF));
+  const Weights wp1 = MODE == 0 ? weights_at<MODE>(a, slot, 1, bx * (8 * NF)) : wp0;
+  u32x2 sv[kUnits];
+  auto load_w = [&](int u, int b) {
+    const uint32_t dst = lds0 + (uint32_t)(b * kUnit);
+    const bool tail = 2 * u + 1 >= chunks;   // half a unit: its other half is read again, not multiplied
+#pragma unroll
+    for (int j = 0; j < 2 * NF; ++j) {
+      const int t = 8 * j + (lane >> 3), part = MODE == 0 ? j / NF : 0;
+      const int piece = (lane & 7) ^ swz_w16(t);
+      const uint32_t off = (uint32_t)(t - part * 8 * NF) * (uint32_t)(K / 2) + (uint32_t)((tail ? piece & 3 : piece) * 16);
+      dma16(reinterpret_cast<const char*>(uniform_ptr((part ? wp1.codes : wp0.codes) + u * 128)), off,
+            dst + (uint32_t)(j * 1024));
+    }
+    const int part = MODE == 0 && lane >= 8 * NF;
+    const uint8_t* sp = (part ? wp1.scales : wp0.scales) + (int64_t)(lane - part * 8 * NF) * (K / 32) + u * 8;
+    if (lane < kRowsW) {
+      if (tail) __builtin_memcpy(&sv[b], sp, 4);
+      else __builtin_memcpy(&sv[b], sp, 8);
+    }
+  };
+  // the first units' weights do not depend on the expert's rows: where those are known to be 1 to 16, their
+  // loads go first
+  if (a.known)
+#pragma unroll
+    for (int b = 0; b < kUnits; ++b)
+      if (u0 + b < u1) load_w(u0 + b, b);
+  const int64_t start = a.starts[e];
+  const int64_t n = a.starts[e + 1] - start;
+  if (n < 1 || n > kSmallRows) {
+    wait_cnt<0>();
+    return;
+  }
+  const bool live = r < n;
+  const int64_t p = start + (live ? r : 0);
   const int64_t src = MODE == 0 ? a.rows[p] : p;
   const uint8_t* xp = MODE == 0 ? a.x : a.act;
   const uint8_t* xs = MODE == 0 ? a.x_scales : a.act_scales;
   xp += Q ? src * (K / 2) + q * 16 : src * K * 2 + q * 64;
   if (Q) xs += src * (K / 32) + q;
-  Weights wp[NF];
-#pragma unroll
-  for (int f = 0; f < NF; ++f) {
-    wp[f] = MODE == 0 ? weights_at<0>(a, slot, f >> 1, bx * 32 + (f & 1) * 16 + r)
-                      : weights_at<1>(a, slot, 0, bx * 64 + f * 16 + r);
-    wp[f].codes += q * 16;
-    wp[f].scales += q;
-  }
   floatx4 acc[NF];
 #pragma unroll
   for (int f = 0; f < NF; ++f) acc[f] = floatx4{0, 0, 0, 0};
-  for (int c = c0; c < c1; ++c) {
-    u32x4 wc[NF];
-    uint32_t ws[NF];
+  for (int u = u0; u < u1; u += kUnits) {
+    if (u > u0 || !a.known)
 #pragma unroll
-    for (int f = 0; f < NF; ++f) {
-      wc[f] = *(const u32x4*)(wp[f].codes + c * 64);
-      ws[f] = wp[f].scales[c * 4];
-    }
-    if constexpr (Q) {
-      const u32x4 xc = *(const u32x4*)(xp + c * 64);
-      const uint32_t xb = xs[c * 4];
+      for (int b = 0; b < kUnits; ++b)
+        if (u + b < u1) load_w(u + b, b);
+    constexpr int XL = Q ? 1 : 4;   // 16-byte loads of a lane and chunk
+    u32x4 xv[kUnits][2][XL] = {};
+    uint32_t xb[kUnits][2] = {};
+    if (live)
 #pragma unroll
-      for (int f = 0; f < NF; ++f) acc[f] = mma_fp4(wc[f], (int)ws[f], xc, (int)xb, acc[f]);
-    } else {
-      bf16x8 xv[4];
+      for (int b = 0; b < kUnits; ++b)
 #pragma unroll
-      for (int s = 0; s < 4; ++s) xv[s] = *(const bf16x8*)(xp + c * 256 + s * 16);
+        for (int j = 0; j < 2; ++j) {
+          const int c = 2 * (u + b) + j;
+          if (u + b < u1 && c < chunks) {
 #pragma unroll
-      for (int s = 0; s < 4; ++s)
+            for (int s = 0; s < XL; ++s) xv[b][j][s] = *(const u32x4*)(xp + (int64_t)c * (Q ? 64 : 256) + s * 16);
+            if (Q) xb[b][j] = xs[c * 4];
+          }
+        }
 #pragma unroll
-        for (int f = 0; f < NF; ++f)
-          acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(decode8(wc[f][s], scale_of(ws[f])), xv[s], acc[f],
-                                                           0, 0, 0);
+    for (int b = 0; b < kUnits; ++b)
+      if (u + b < u1 && lane < kRowsW)
+        *reinterpret_cast<__attribute__((address_space(3))) u32x2*>(
+            (uintptr_t)(lds0 + (uint32_t)(b * kUnit + kW + lane * 8))) = sv[b];
+    wait_cnt<0>();   // the wavefront's own LDS: no barrier
+#pragma unroll
+    for (int b = 0; b < kUnits; ++b) {
+      if (u + b >= u1) break;
+      const uint32_t at = lds0 + (uint32_t)(b * kUnit);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (2 * (u + b) + j >= chunks) break;
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+          const u32x4 c = lds_get<lds_u32x4>(at + (uint32_t)(f * 2048 + r * 128 + (((4 * j + q) ^ swz_w16(r)) << 4)));
+          const uint32_t sw = lds_get<lds_u32>(at + (uint32_t)(kW + (f * 16 + r) * 8 + j * 4));
+          if constexpr (Q) {
+            acc[f] = mma_fp4(c, (int)(sw >> (8 * q)), xv[b][j][0], (int)xb[b][j], acc[f]);
+          } else {
+            const float sc = scale_of(__builtin_amdgcn_ubfe(sw, 8 * q, 8));
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+              acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(decode8(c[s], sc), __builtin_bit_cast(bf16x8, xv[b][j][s]),
+                                                               acc[f], 0, 0, 0);
+          }
+        }
+      }
     }
   }
+  __syncthreads();   // the weights' LDS becomes that of the sums
+  floatx4(*part)[NF][64] = reinterpret_cast<floatx4(*)[NF][64]>(smem);
 #pragma unroll
   for (int f = 0; f < NF; ++f) part[wave][f][lane] = acc[f];
   __syncthreads();
@@ -169,9 +235,9 @@ __global__ __launch_bounds__(256) void mx_small(MxArgs a) {
     for (int w = 1; w < 4; ++w) v += part[w][f][lane];
     return v;
   };
-  const bool live = r < n;
   if constexpr (MODE == 0) {
     if constexpr (Q) {
+      static_assert(NF == 4);   // a block of 32 columns
       if (wave != 0) return;
       float v[8];   // columns 16 (i / 4) + 4 q + i % 4
 #pragma unroll
@@ -189,23 +255,35 @@ __global__ __launch_bounds__(256) void mx_small(MxArgs a) {
         if (q == 0) a.act_scales[p * (a.I / 32) + bx] = (uint8_t)byte;
       }
     } else {
-      if (wave >= 2) return;
-      const floatx4 g = sum(wave), u = sum(2 + wave);
+      if (wave >= NF / 2) return;
+      const floatx4 g = sum(wave), u = sum(NF / 2 + wave);
       u32x2 y;
 #pragma unroll
       for (int i = 0; i < 4; i += 2) y[i / 2] = pk_bf16(silu_mul(g[i], u[i]), silu_mul(g[i + 1], u[i + 1]));
-      if (live) *(u32x2*)(a.act + (p * a.I + bx * 32 + wave * 16 + q * 4) * 2) = y;
+      if (live) *(u32x2*)(a.act + (p * a.I + bx * (8 * NF) + wave * 16 + q * 4) * 2) = y;
     }
   } else {
+    if (wave >= NF) return;
     const floatx4 y = sum(wave);
     if (live) {
       const int64_t t = a.rows[p] * a.k + a.cols[p];
       const float wt = bf16_to_f32(a.w[t]);
       const int64_t o = a.out_mode == 0 ? t : p;
-      *(u32x2*)(a.out + o * a.H + bx * 64 + wave * 16 + q * 4) =
+      *(u32x2*)(a.out + o * a.H + bx * (16 * NF) + wave * 16 + q * 4) =
           u32x2{pk_bf16(y[0] * wt, y[1] * wt), pk_bf16(y[2] * wt, y[3] * wt)};
     }
   }
+}
+
+template <int MODE, bool Q, int NF>
+int small_launch(const MxArgs& a, hipStream_t s) {
+  const int64_t K = MODE == 0 ? a.H : a.I, units = ceil_div(K, 256);
+  const dim3 g((unsigned)(MODE == 0 ? a.I / (8 * NF) : a.H / (16 * NF)), (unsigned)a.list.n);
+  const int64_t bytes = 4 * (units > 4 ? kUnits : 1) * (16 * NF * 136), sums = 4 * NF * 1024;
+  launch(MODE == 0 ? "mx_small_up" : "mx_small_down", mx_small<MODE, Q, NF>, g, dim3(256),
+         (uint32_t)(bytes > sums ? bytes : sums), s, a);
+  FERRY_LAUNCHED("mx_small");
+  return 0;
 }
 
 // =============================================================================================
@@ -224,12 +302,6 @@ __global__ __launch_bounds__(256) void mx_small(MxArgs a) {
 // a lane then holds 8 consecutive output columns of one row.
 __device__ __forceinline__ int swz_x(int row) { return (row >> 1) & 7; }
 __device__ __forceinline__ int swz_w(int row) { return ((row >> 1) & 1) | (((row >> 3) & 3) << 1); }
-
-typedef __attribute__((address_space(3))) const u32x4 lds_u32x4;
-typedef __attribute__((address_space(3))) const u32x2 lds_u32x2;
-typedef __attribute__((address_space(3))) const uint32_t lds_u32;
-template <typename T>
-__device__ __forceinline__ auto lds_get(uint32_t at) { return *reinterpret_cast<T*>((uintptr_t)at); }
 
 template <int MODE, bool Q, int WM, int WN, int MI>
 __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM * WN / 4, WM * WN / 4)))
@@ -554,12 +626,8 @@ template <bool Q>
 int launch_list(const MxArgs& a, bool small, int64_t tiles, int32_t phases, int64_t cus, hipStream_t s) {
   for (int mode = 0; mode < 2; ++mode) {
     if (!(phases & (1 << mode))) continue;
-    if (small) {
-      const dim3 g((unsigned)(mode == 0 ? a.I / 32 : a.H / 64), (unsigned)a.list.n);
-      launch(mode == 0 ? "mx_small_up" : "mx_small_down", mode == 0 ? mx_small<0, Q> : mx_small<1, Q>, g,
-             dim3(256), 0, s, a);
-      FERRY_LAUNCHED("mx_small");
-    }
+    if (small)
+      if (const int rc = mode == 0 ? small_launch<0, Q, Q ? 4 : 2>(a, s) : small_launch<1, Q, 4>(a, s)) return rc;
     if (tiles) {
       const int64_t t = tiles * (mode == 0 ? a.I / 128 : a.H / 256);
       launch(mode == 0 ? "mx_tiled_up" : "mx_tiled_down", mode == 0 ? mx_tiled<0, Q, 2, 4, 8> : mx_tiled<1, Q, 2, 4, 8>,
@@ -638,6 +706,7 @@ extern "C" int ferry_mxfp4_expert_ffn(const void* cache, int64_t cache_rows, int
   a.I = inter;
   a.k = topk;
   a.out_mode = out_mode;
+  a.known = list_rows != nullptr;
   a.list.n_mid = 0;
   // one pass over the small experts, one over the others; without row counts every expert is in both, and
   // the kernels pass over those of the other kind by the device's starts

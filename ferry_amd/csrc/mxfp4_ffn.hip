@@ -295,8 +295,11 @@ int small_launch(const MxArgs& a, hipStream_t s) {
 // values (a stage), 64 of bf16 (four steps to a stage).  Loading the weights to registers in operand order
 // instead takes no LDS, but its lanes touch 64 places of 16 bytes: address processing then bounds the kernel
 // (5 us for 128 along K, whatever the products).  Two buffers each, the loads one stage or step ahead of
-// the products.  A row's 16-byte pieces are stored at slot piece ^ swizzle(row), so that the 16 rows that a
+// the products, across tiles too: the last ones of a tile load the first of the next, whose rows are looked
+// up meanwhile.  A row's 16-byte pieces are stored at slot piece ^ swizzle(row), so that the 16 rows that a
 // quarter of a wavefront reads lie on 16 different 16-byte bank groups.
+// Rows of a tile that hold no row of the expert are neither loaded nor multiplied, in steps of a quarter.
+// (bf16) The weights of a step are read before the barrier that its rows wait for.
 // MODE 0: of a wavefront's four weight tiles, two are gate rows and two the up rows of the same 32 columns.
 // The weight rows of the two tiles c of 32 columns interleave in groups of four, 8 g + 4 c + [0, 4):
 // a lane then holds 8 consecutive output columns of one row.
@@ -311,12 +314,15 @@ void mx_tiled(MxArgs a) {
   constexpr int kX = TM * 128, kW = TN * 128;            // bytes of a buffer
   constexpr int LX = kX / (1024 * W), LW = kW / (1024 * W);   // direct loads of a wavefront for one
   constexpr int kXS = Q ? TM * 8 : 0, kWS = TN * 8;      // scale bytes of a stage
-  constexpr int H = Q ? 1 : 4;                           // steps of activations in a stage
-  static_assert(LX >= 1 && LW >= 1 && TM + TN <= 64 * W * (Q ? 1 : 2));
+  constexpr int kScaleRows = TN + (Q ? TM : 0);
+  static_assert(LX == 4 && TM == 32 * W && LW >= 1 && kScaleRows <= 64 * W && TM <= 64 * W && MI % 4 == 0);
   __shared__ TileTable tt;
   __shared__ __attribute__((aligned(1024))) char smem[2 * (kX + kW + kXS + kWS)];
-  __shared__ int32_t src_s[MODE == 0 ? TM : 1], orow_s[MODE == 1 ? TM : 1];
-  __shared__ float wt_s[MODE == 1 ? TM : 1];
+  // per tile row, two sets taken in turn: the token, and for MODE 1 the slot index, the output row and the
+  // routing weight (bf16 bits)
+  __shared__ __attribute__((aligned(256))) int32_t row_s[2][TM], col_s[MODE == 1 ? 2 : 1][MODE == 1 ? TM : 1];
+  __shared__ __attribute__((aligned(256))) int32_t orow_s[MODE == 1 ? 2 : 1][MODE == 1 ? TM : 1],
+      wt_s[MODE == 1 ? 2 : 1][MODE == 1 ? TM : 1];
   build_tile_table<TM, kSmallRows>(a, tt);
   const int64_t K = MODE == 0 ? a.H : a.I;
   const int ntn = (int)((MODE == 0 ? a.I : a.H) / COLS);
@@ -338,108 +344,171 @@ void mx_tiled(MxArgs a) {
   const uint32_t wa = wbuf + (uint32_t)(wrow * 128 + (((Q ? q : q >> 1) ^ swz_w(wrow)) << 4) + (Q ? 0 : (q & 1) * 8));
   constexpr int kXTile = 16 * WM * 128;
   auto wtile = [](int f) { return (f >> 1) * (MODE == 0 ? TN / 2 : 32) + (f & 1) * 4; };   // in rows
-  // direct loads: load j of a wavefront moves the rows 8 (wave L + j) + lane / 8
-  const int r8 = lane >> 3, slot8 = lane & 7;
 
-  const int per_xcd = gridDim.x % 8 == 0 ? (int)gridDim.x / 8 : 0;
-  const int first = per_xcd ? (int)(blockIdx.x % 8) * per_xcd + (int)(blockIdx.x / 8) : (int)blockIdx.x;
-  for (int tile = first; tile < total; tile += gridDim.x) {
-    const int mt = tile / ntn, nt = tile - mt * ntn;
+  struct Tile {
+    int64_t row0;        // grouped row of the tile's first row
+    int vrows, nt, slot;
+  };
+  auto locate = [&](int tile) {
+    Tile t;
+    const int mt = tile / ntn;
+    t.nt = tile - mt * ntn;
     const int li = __builtin_amdgcn_readfirstlane(find_entry(tt, mt));
-    const int64_t start = uniform64(tt.start[li]);
     const int m0 = (mt - __builtin_amdgcn_readfirstlane(tt.cum[li])) * TM;
-    const int vrows = __builtin_amdgcn_readfirstlane(tt.rows[li]) - m0;   // > 0
-    const int64_t row0 = start + m0;
-    // the rows' sources; rows past the last take the first one's (they are never stored)
-    for (int t = tid; t < TM; t += 64 * W) {
-      const int64_t p = row0 + (t < vrows ? t : 0);
-      const int64_t tok = a.rows[p];
-      if constexpr (MODE == 0) {
-        src_s[t] = (int32_t)tok;
-      } else {
-        const int64_t tj = tok * a.k + a.cols[p];
-        orow_s[t] = (int32_t)(a.out_mode == 0 ? tj : p);
-        wt_s[t] = bf16_to_f32(a.w[tj]);
-      }
+    t.row0 = uniform64(tt.start[li]) + m0;
+    t.vrows = __builtin_amdgcn_readfirstlane(tt.rows[li]) - m0;   // > 0
+    t.slot = a.list.slot[li];
+    return t;
+  };
+  // the tile rows' indices (low words; rows past the last: the first row's) into set p, direct loads
+  auto load_rows = [&](const Tile& t, int p) {
+    if (wave < TM / 64) {
+      const int v = 64 * wave + lane;
+      const uint32_t off = (uint32_t)((v < t.vrows ? v : 0) * 8);
+      dma4(reinterpret_cast<const char*>(uniform_ptr(a.rows + t.row0)), off, lds_addr(row_s[p]) + 256 * wave);
+      if constexpr (MODE == 1)
+        dma4(reinterpret_cast<const char*>(uniform_ptr(a.cols + t.row0)), off, lds_addr(col_s[p]) + 256 * wave);
     }
-    __syncthreads();
-    auto src_row = [&](int t) {
-      return MODE == 0 ? (uint32_t)src_s[t] : (uint32_t)(row0 + (t < vrows ? t : 0));
+  };
+
+  // The tiles whose activations and weights are being loaded.  Direct load j of a wavefront moves 8 rows, lane / 8 of them,
+  // its lane % 8 the piece (lane % 8) ^ swizzle: rows 64 j .. of the activations over all wavefronts (W = 8),
+  // so that a tile of few rows takes the first loads only.
+  const int r8 = lane >> 3, slot8 = lane & 7;
+  auto xload_row = [&](int j) { return 8 * (W * j + wave) + r8; };
+  uint32_t xoff[LX], woff[LW], sdst;
+  const char* wbase[LW];
+  const uint8_t* sp = nullptr;   // this thread's row of scales: a weight row, or (Q) an activation row
+  int xloads = LX;
+  if (tid < TN) sdst = wsbuf + (uint32_t)(tid * 8);
+  else sdst = xsbuf + (uint32_t)((tid - TN) * 8);
+  auto aim_x = [&](const Tile& t, int p) {
+    auto src_row = [&](int v) {
+      return MODE == 0 ? (uint32_t)row_s[p][v] : (uint32_t)(t.row0 + (v < t.vrows ? v : 0));
     };
-    const Weights m0w = weights_at<MODE>(a, a.list.slot[li], 0, nt * COLS);
-    const Weights m1w = MODE == 0 ? weights_at<MODE>(a, a.list.slot[li], 1, nt * COLS) : m0w;
-    uint32_t xoff[LX], woff[LW];
-    const char* wbase[LW];
+    xloads = t.vrows > TM / 4 * 3 ? 4 : (t.vrows > TM / 2 ? 3 : (t.vrows > TM / 4 ? 2 : 1));
 #pragma unroll
     for (int j = 0; j < LX; ++j) {
-      const int t = 8 * (wave * LX + j) + r8;
-      xoff[j] = src_row(t) * (uint32_t)(Q ? K / 2 : K * 2) + (uint32_t)((slot8 ^ swz_x(t)) * 16);
+      const int v = xload_row(j);
+      xoff[j] = src_row(v) * (uint32_t)(Q ? K / 2 : K * 2) + (uint32_t)((slot8 ^ swz_x(v)) * 16);
     }
+    if (Q && tid >= TN && tid < kScaleRows) sp = xsbase + (int64_t)src_row(tid - TN) * (K / 32);
+  };
+  auto aim_w = [&](const Tile& t) {
+    const Weights m0 = weights_at<MODE>(a, t.slot, 0, t.nt * COLS);
+    const Weights m1 = MODE == 0 ? weights_at<MODE>(a, t.slot, 1, t.nt * COLS) : m0;
 #pragma unroll
     for (int j = 0; j < LW; ++j) {
       const int t0 = 8 * (wave * LW + j), part = MODE == 0 ? t0 / (TN / 2) : 0;
-      wbase[j] = reinterpret_cast<const char*>(uniform_ptr(part ? m1w.codes : m0w.codes));
+      wbase[j] = reinterpret_cast<const char*>(uniform_ptr(part ? m1.codes : m0.codes));
       woff[j] = (uint32_t)(t0 - part * (TN / 2) + r8) * (uint32_t)(K / 2) + (uint32_t)((slot8 ^ swz_w(t0 + r8)) * 16);
     }
-    // this thread's row of scales: a weight row, or (Q) an activation row
-    constexpr int kScaleRows = TN + (Q ? TM : 0);
-    const uint8_t* sp = nullptr;
-    uint32_t sdst = 0;
     if (tid < TN) {
       const int part = MODE == 0 ? tid / (TN / 2) : 0;
-      sp = (part ? m1w.scales : m0w.scales) + (int64_t)(tid - part * (TN / 2)) * (K / 32);
-      sdst = wsbuf + (uint32_t)(tid * 8);
-    } else if (tid < kScaleRows) {
-      sp = xsbase + (int64_t)src_row(tid - TN) * (K / 32);
-      sdst = xsbuf + (uint32_t)((tid - TN) * 8);
+      sp = (part ? m1.scales : m0.scales) + (int64_t)(tid - part * (TN / 2)) * (K / 32);
     }
-    u32x2 sv = {0, 0};
-    auto load_s = [&](int st) {
-      if (tid < kScaleRows) {
-        if (2 * st + 1 < chunks) __builtin_memcpy(&sv, sp + st * 8, 8);
-        else __builtin_memcpy(&sv, sp + st * 8, 4);
-      }
-    };
-    auto store_s = [&](int st) {
-      if (tid < kScaleRows)
-        *reinterpret_cast<__attribute__((address_space(3))) u32x2*>((uintptr_t)(sdst + (uint32_t)((st & 1) * (tid < TN ? kWS : kXS)))) = sv;
-    };
-    // Where the number of chunks is odd, the last stage's rows of 4-bit values end in its middle: the lanes of
-    // the second half read the first half again (it is not multiplied).
-    auto back = [&](int piece) { return (uint32_t)((piece & 4) << 4); };
-    auto load_x = [&](int n) {   // Q: stage n; bf16: step n
-      const uint32_t dst = smem0 + (uint32_t)((n & 1) * kX);
+  };
+  u32x2 sv = {0, 0};
+  auto load_s = [&](int st) {
+    if (tid < kScaleRows) {
+      if (2 * st + 1 < chunks) __builtin_memcpy(&sv, sp + st * 8, 8);
+      else __builtin_memcpy(&sv, sp + st * 8, 4);
+    }
+  };
+  auto store_s = [&](int b) {
+    if (tid < kScaleRows)
+      *reinterpret_cast<__attribute__((address_space(3))) u32x2*>((uintptr_t)(sdst + (uint32_t)(b * (tid < TN ? kWS : kXS)))) = sv;
+  };
+  // Where the number of chunks is odd, the last stage's rows of 4-bit values end in its middle: the lanes of
+  // the second half read the first half again (it is not multiplied).
+  auto back = [&](int piece) { return (uint32_t)((piece & 4) << 4); };
+  auto load_x = [&](int n, int b) {   // Q: stage n; bf16: step n
+    const uint32_t dst = smem0 + (uint32_t)(b * kX + wave * 1024);
 #pragma unroll
-      for (int j = 0; j < LX; ++j) {
-        const uint32_t tail = Q && 2 * n + 1 >= chunks ? back(slot8 ^ swz_x(8 * (wave * LX + j) + r8)) : 0u;
-        dma16(xbase + (int64_t)n * 128, xoff[j] - tail, dst + (uint32_t)((wave * LX + j) * 1024));
+    for (int j = 0; j < LX; ++j)
+      if (j < xloads) {
+        const uint32_t tail = Q && 2 * n + 1 >= chunks ? back(slot8 ^ swz_x(xload_row(j))) : 0u;
+        dma16(xbase + (int64_t)n * 128, xoff[j] - tail, dst + (uint32_t)(W * j * 1024));
       }
-    };
-    auto load_w = [&](int st, int j) {
+  };
+  auto load_w = [&](int st, int b) {
+#pragma unroll
+    for (int j = 0; j < LW; ++j) {
       const uint32_t tail = 2 * st + 1 >= chunks ? back(slot8 ^ swz_w(8 * (wave * LW + j) + r8)) : 0u;
-      dma16(wbase[j] + (int64_t)st * 128, woff[j] - tail, wbuf + (uint32_t)((st & 1) * kW + (wave * LW + j) * 1024));
-    };
+      dma16(wbase[j] + (int64_t)st * 128, woff[j] - tail, wbuf + (uint32_t)(b * kW + (wave * LW + j) * 1024));
+    }
+  };
+
+  // XCD-aware order: workgroup b runs on XCD b % 8, whose workgroups take a contiguous run of tiles; tiles of
+  // one expert follow each other, columns fastest, and share their rows and weights in that XCD's L2.
+  const int per_xcd = gridDim.x % 8 == 0 ? (int)gridDim.x / 8 : 0;
+  const int first = per_xcd ? (int)(blockIdx.x % 8) * per_xcd + (int)(blockIdx.x / 8) : (int)blockIdx.x;
+  if (first >= total) return;
+  Tile cur = locate(first);
+  load_rows(cur, 0);
+  wait_cnt<0>();
+  wg_barrier();
+  aim_x(cur, 0);
+  aim_w(cur);
+  load_s(0);
+  load_w(0, 0);
+  load_x(0, 0);
+  store_s(0);
+  wait_cnt<0>();
+  wg_barrier();
+  int set = 0, wb = 0;   // set of row tables; buffer of the present stage (Q: of its activations too)
+
+  // bf16: the weights' codes of the next step, their scales of its chunk
+  u32x2 wr[NI];
+  uint32_t ws[NI];
+  auto read_w = [&](uint32_t at) {
+#pragma unroll
+    for (int f = 0; f < NI; ++f) wr[f] = lds_get<lds_u32x2>(at + (uint32_t)(wtile(f) * 128));
+  };
+  auto read_s = [&](uint32_t at) {
+#pragma unroll
+    for (int f = 0; f < NI; ++f) ws[f] = lds_get<lds_u32>(at + (uint32_t)((wrow + wtile(f)) * 8));
+  };
+  if constexpr (!Q) {
+    read_w(wa);
+    read_s(wsbuf);
+  }
+  for (int tile = first; tile < total; tile += gridDim.x, set ^= 1) {
+    // the tile after this one; after the last tile its own first stage is loaded again
+    const bool more = tile + (int)gridDim.x < total;
+    const Tile next = more ? locate(tile + gridDim.x) : cur;
+    load_rows(next, set ^ 1);
+    if constexpr (MODE == 1) {
+      // output row and routing weight of tile row tid, in LDS before the epilogue reads them
+      if (wave < TM / 64) {
+        const int64_t tj = (int64_t)row_s[set][tid] * a.k + col_s[set][tid];
+        dma2(reinterpret_cast<const char*>(a.w), (uint32_t)(tj * 2), lds_addr(wt_s[set]) + 256 * wave);
+        orow_s[set][tid] = a.out_mode == 0 ? (int32_t)tj : (int32_t)(cur.row0 + (tid < cur.vrows ? tid : 0));
+      }
+    }
     floatx4 acc[MI][NI];
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
       for (int f = 0; f < NI; ++f) acc[i][f] = floatx4{0, 0, 0, 0};
-    load_s(0);
-#pragma unroll
-    for (int j = 0; j < LW; ++j) load_w(0, j);
-    load_x(0);
-    store_s(0);
-    wait_cnt<0>();
-    wg_barrier();
+    // In the last stage (bf16 activations: step) the loads turn to the next tile, whose row indices may still
+    // be on their way where it is the only one.
+    auto turn_x = [&]() {
+      if (stages == 1) {
+        wait_cnt<0>();
+        wg_barrier();
+      }
+      aim_x(next, set ^ 1);
+    };
     // ROWS: tiles of 16 rows of a wavefront that are multiplied; the others hold no row of the expert
     auto loop = [&](auto rows) {
       constexpr int ROWS = decltype(rows)::value;
       if constexpr (Q) {
-        for (int st = 0; st < stages; ++st) {
-          const uint32_t xb = xa + (uint32_t)((st & 1) * kX), wb = wa + (uint32_t)((st & 1) * kW);
-          const uint32_t xsb = xsbuf + (uint32_t)((st & 1) * kXS + xrow * 8), wsb = wsbuf + (uint32_t)((st & 1) * kWS + wrow * 8);
-          u32x4 xn[2], wv[NI];
-          uint32_t xsn[2], ws[NI];
+        for (int st = 0; st < stages; ++st, wb ^= 1) {
+          const uint32_t xb = xa + (uint32_t)(wb * kX), wbb = wa + (uint32_t)(wb * kW);
+          const uint32_t xsb = xsbuf + (uint32_t)(wb * kXS + xrow * 8), wsb = wsbuf + (uint32_t)(wb * kWS + wrow * 8);
+          u32x4 xn[2], wf[NI];
+          uint32_t xsn[2], wsf[NI];
           auto read_x = [&](int j, int i) {
 #pragma unroll
             for (int v = 0; v < 2; ++v) {
@@ -447,29 +516,32 @@ void mx_tiled(MxArgs a) {
               xsn[v] = lds_get<lds_u32>(xsb + (uint32_t)(16 * WM * 8 * (i + v) + 4 * j));
             }
           };
-          auto read_w = [&](int j) {
+          auto read_wq = [&](int j) {
 #pragma unroll
             for (int f = 0; f < NI; ++f) {
-              wv[f] = lds_get<lds_u32x4>((wb ^ (uint32_t)(j << 6)) + (uint32_t)(wtile(f) * 128));
-              ws[f] = lds_get<lds_u32>(wsb + (uint32_t)(wtile(f) * 8 + 4 * j));
+              wf[f] = lds_get<lds_u32x4>((wbb ^ (uint32_t)(j << 6)) + (uint32_t)(wtile(f) * 128));
+              wsf[f] = lds_get<lds_u32>(wsb + (uint32_t)(wtile(f) * 8 + 4 * j));
             }
           };
-          read_w(0);
+          read_wq(0);
           read_x(0, 0);
-          if (st + 1 < stages) {
-            load_s(st + 1);
-#pragma unroll
-            for (int j = 0; j < LW; ++j) load_w(st + 1, j);
-            load_x(st + 1);
+          const bool last = st + 1 == stages;
+          if (last) {
+            turn_x();
+            aim_w(next);
           }
-          const int two = 2 * st + 1 < chunks;
+          const int ls = last ? 0 : st + 1;
+          load_s(ls);
+          load_w(ls, wb ^ 1);
+          load_x(ls, wb ^ 1);
+          const bool two = 2 * st + 1 < chunks;
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             if (j == 1 && !two) break;
             u32x4 cw[NI];
             int cs[NI];
 #pragma unroll
-            for (int f = 0; f < NI; ++f) cw[f] = wv[f], cs[f] = (int)(ws[f] >> (8 * q));
+            for (int f = 0; f < NI; ++f) cw[f] = wf[f], cs[f] = (int)(wsf[f] >> (8 * q));
 #pragma unroll
             for (int i = 0; i < ROWS; i += 2) {
               const u32x4 x0 = xn[0], x1 = xn[1];
@@ -478,7 +550,7 @@ void mx_tiled(MxArgs a) {
                 read_x(j, i + 2);
               } else if (j == 0) {
                 read_x(1, 0);
-                read_w(1);
+                read_wq(1);
               }
 #pragma unroll
               for (int f = 0; f < NI; ++f) acc[i][f] = mma_fp4(cw[f], cs[f], x0, s0, acc[i][f]);
@@ -487,79 +559,77 @@ void mx_tiled(MxArgs a) {
               __builtin_amdgcn_sched_barrier(0);
             }
           }
-          if (st + 1 < stages) store_s(st + 1);
+          store_s(wb ^ 1);
           wait_cnt<0>();   // the next stage's loads have landed, this one's fragments are read
           wg_barrier();
         }
       } else {
-        u32x2 wr[NI], ws[NI];   // the weights' codes of the next step; their scales of the stage
-        u32x4 wv[2][NI];
-        auto read_w = [&](int st, int h) {
-          const uint32_t at = (wa + (uint32_t)((st & 1) * kW)) ^ (uint32_t)(h << 5);
+        for (int c = 0; c < chunks; ++c) {
+          const bool first_half = (c & 1) == 0, last = c + 1 == chunks;
+          const bool stage_end = !first_half || last;   // the next chunk lies in the other buffer
 #pragma unroll
-          for (int f = 0; f < NI; ++f) wr[f] = lds_get<lds_u32x2>(at + (uint32_t)(wtile(f) * 128));
-        };
-        auto read_s = [&](int st) {
-#pragma unroll
-          for (int f = 0; f < NI; ++f)
-            ws[f] = lds_get<lds_u32x2>(wsbuf + (uint32_t)((st & 1) * kWS + (wrow + wtile(f)) * 8));
-        };
-        for (int st = 0; st < stages; ++st) {
-#pragma unroll
-          for (int h = 0; h < 4; ++h) {
-            const int n = 4 * st + h;
-            if (h >= 2 && 2 * st + 1 >= chunks) break;
-            const uint32_t xb = xa + (uint32_t)((h & 1) * kX);
+          for (int h = 0; h < 2; ++h) {
+            uint32_t xb = xa, wat = wa;   // computed here, not kept in registers through the loop
+            asm volatile("" : "+v"(xb), "+v"(wat));
+            xb += (uint32_t)(h * kX);
             bf16x8 xr[3];
             auto read = [&](int m) {
               xr[m % 3] = lds_read16((xb ^ (uint32_t)((m / ROWS) << 4)) + (uint32_t)(kXTile * (m % ROWS)));
             };
-            if (h == 0) read_s(st);
-            read_w(st, h);
             read(0);
             read(1);
-            if (n + 1 < 2 * chunks) load_x(n + 1);
-            if (st + 1 < stages) {
-              if (h == 0) {
-                load_s(st + 1);
-#pragma unroll
-                for (int j = 0; j < (LW + 1) / 2; ++j) load_w(st + 1, j);
-              } else if (h == 1) {
-#pragma unroll
-                for (int j = (LW + 1) / 2; j < LW; ++j) load_w(st + 1, j);
-              }
-            }
+            // the first 32 along K are decoded while the first fragments are on their way, the second 32
+            // between the products of the first
+            u32x4 wv[2][NI];
+            uint32_t c1[NI];
             float sc[NI];
-#pragma unroll
-            for (int f = 0; f < NI; ++f)
-              sc[f] = scale_of(__builtin_amdgcn_ubfe(ws[f][h >> 1], 16 * (h & 1) + 8 * (q >> 1), 8));
-            auto decode = [&](int s, int part) {   // half a weight tile's 32 columns
+            auto decode = [&](uint32_t v, int s, int part) {   // half of a weight tile's 8 elements a lane
               const int f = part >> 1, half = part & 1;
 #pragma unroll
               for (int j = 0; j < 2; ++j) {
-                const bf16x2 d = half ? (j ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(wr[f][s], sc[f], 3)
-                                           : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(wr[f][s], sc[f], 2))
-                                      : (j ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(wr[f][s], sc[f], 1)
-                                           : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(wr[f][s], sc[f], 0));
+                const bf16x2 d = half ? (j ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, sc[f], 3)
+                                           : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, sc[f], 2))
+                                      : (j ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, sc[f], 1)
+                                           : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, sc[f], 0));
                 wv[s][f][2 * half + j] = __builtin_bit_cast(uint32_t, d);
               }
             };
 #pragma unroll
-            for (int part = 0; part < 2 * NI; ++part) decode(0, part);
+            for (int f = 0; f < NI; ++f)
+              c1[f] = wr[f][1], sc[f] = scale_of(__builtin_amdgcn_ubfe(ws[f], 16 * h + 8 * (q >> 1), 8));
+#pragma unroll
+            for (int part = 0; part < 2 * NI; ++part) decode(wr[part >> 1][0], 0, part);
+            __builtin_amdgcn_sched_barrier(0);
+            if (h == 0) {
+              if (first_half) {   // the next stage's weights: there one step later
+                const bool final_stage = c + 2 >= chunks;
+                if (final_stage) aim_w(next);
+                load_s(final_stage ? 0 : c / 2 + 1);
+                load_w(final_stage ? 0 : c / 2 + 1, wb ^ 1);
+              }
+              load_x(2 * c + 1, 1);
+              read_w((wat + (uint32_t)(wb * kW)) ^ (uint32_t)((c & 1) << 6) ^ 32u);
+            } else {
+              if (last) turn_x();
+              load_x(last ? 0 : 2 * c + 2, 0);
+              if (stage_end) wb ^= 1;
+              read_w((wat + (uint32_t)(wb * kW)) ^ (uint32_t)(stage_end ? 0 : 64));
+              read_s(wsbuf + (uint32_t)(wb * kWS + (stage_end ? 0 : 4)));
+            }
 #pragma unroll
             for (int m = 0; m < 2 * ROWS; ++m) {
               const int s = m / ROWS, i = m % ROWS;
               if (m + 2 < 2 * ROWS) read(m + 2);
               if (s == 0)
 #pragma unroll
-                for (int part = i * 2 * NI / ROWS; part < (i + 1) * 2 * NI / ROWS; ++part) decode(1, part);
+                for (int part = i * 2 * NI / ROWS; part < (i + 1) * 2 * NI / ROWS; ++part) decode(c1[part >> 1], 1, part);
 #pragma unroll
               for (int f = 0; f < NI; ++f)
                 acc[i][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, wv[s][f]), xr[m % 3],
                                                                    acc[i][f], 0, 0, 0);
               __builtin_amdgcn_sched_barrier(0);
             }
-            if (h == 1 && st + 1 < stages) store_s(st + 1);
+            if (h == 0 && first_half) store_s(wb ^ 1);
             wait_cnt<0>();
             wg_barrier();
           }
@@ -567,35 +637,35 @@ void mx_tiled(MxArgs a) {
       }
     };
     // rows 16 (WM i + wm) .. + 16 are tile i of wavefront row wm: the tile's rows in steps of a quarter
-    if (vrows > TM / 4 * 3) loop(std::integral_constant<int, MI>{});
-    else if (vrows > TM / 2) loop(std::integral_constant<int, MI / 4 * 3>{});
-    else if (vrows > TM / 4) loop(std::integral_constant<int, MI / 2>{});
+    if (cur.vrows > TM / 4 * 3) loop(std::integral_constant<int, MI>{});
+    else if (cur.vrows > TM / 2) loop(std::integral_constant<int, MI / 4 * 3>{});
+    else if (cur.vrows > TM / 4) loop(std::integral_constant<int, MI / 2>{});
     else loop(std::integral_constant<int, MI / 4>{});
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
       const int t = 16 * (WM * i + wm) + r;
-      const bool live = t < vrows;
+      const bool live = t < cur.vrows;
       if constexpr (MODE == 0) {
         float v[8];
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
           for (int j = 0; j < 4; ++j) v[4 * c + j] = silu_mul(acc[i][c][j], acc[i][2 + c][j]);
-        const int64_t col = nt * COLS + wn * 32;
+        const int64_t col = cur.nt * COLS + wn * 32;
         if constexpr (Q) {
           const int byte = block_scale(v);
           const uint32_t c = block_codes(v, byte);
           if (live) {
-            *(uint32_t*)(a.act + (row0 + t) * (a.I / 2) + col / 2 + q * 4) = c;
-            if (q == 0) a.act_scales[(row0 + t) * (a.I / 32) + col / 32] = (uint8_t)byte;
+            *(uint32_t*)(a.act + (cur.row0 + t) * (a.I / 2) + col / 2 + q * 4) = c;
+            if (q == 0) a.act_scales[(cur.row0 + t) * (a.I / 32) + col / 32] = (uint8_t)byte;
           }
         } else if (live) {
-          *(u32x4*)(a.act + ((row0 + t) * a.I + col + q * 8) * 2) =
+          *(u32x4*)(a.act + ((cur.row0 + t) * a.I + col + q * 8) * 2) =
               u32x4{pk_bf16(v[0], v[1]), pk_bf16(v[2], v[3]), pk_bf16(v[4], v[5]), pk_bf16(v[6], v[7])};
         }
       } else if (live) {
-        const float wt = wt_s[t];
-        bf16_t* const o = a.out + (int64_t)orow_s[t] * a.H + nt * COLS + wn * 64 + q * 8;
+        const float wt = __uint_as_float((uint32_t)wt_s[set][t] << 16);
+        bf16_t* const o = a.out + (int64_t)orow_s[set][t] * a.H + cur.nt * COLS + wn * 64 + q * 8;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           u32x4 y;
@@ -608,7 +678,7 @@ void mx_tiled(MxArgs a) {
         }
       }
     }
-    __syncthreads();   // the next tile rewrites the row tables and the buffers
+    cur = next;
   }
 }
 

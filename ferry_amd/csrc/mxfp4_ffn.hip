@@ -36,9 +36,9 @@ struct MxArgs {
   const int64_t* rows;      // [R*k]
   const int64_t* cols;      // [R*k]
   uint8_t* act;             // bf16 [R*k, I], or codes [R*k, I / 2]
-  uint8_t* act_scales;      // [R*k, I / 32] (Q)
+  uint8_t* act_scales;      // [I / 128, R*k, 4] (Q): 128 columns' bytes of the rows together
   bf16_t* out;              // [R*k, H]
-  int64_t H, I, k;
+  int64_t H, I, k, pairs;
   int32_t out_mode;
   int32_t known;            // the listed experts' row counts were given
   ExpertList list;
@@ -169,7 +169,8 @@ __global__ __launch_bounds__(256) void mx_small(MxArgs a) {
   const uint8_t* xp = MODE == 0 ? a.x : a.act;
   const uint8_t* xs = MODE == 0 ? a.x_scales : a.act_scales;
   xp += Q ? src * (K / 2) + q * 16 : src * K * 2 + q * 64;
-  if (Q) xs += src * (K / 32) + q;
+  const int64_t xstep = MODE == 0 ? 4 : a.pairs * 4;
+  if (Q) xs += (MODE == 0 ? src * (K / 32) : src * 4) + q;
   floatx4 acc[NF];
 #pragma unroll
   for (int f = 0; f < NF; ++f) acc[f] = floatx4{0, 0, 0, 0};
@@ -190,7 +191,7 @@ __global__ __launch_bounds__(256) void mx_small(MxArgs a) {
           if (u + b < u1 && c < chunks) {
 #pragma unroll
             for (int s = 0; s < XL; ++s) xv[b][j][s] = *(const u32x4*)(xp + (int64_t)c * (Q ? 64 : 256) + s * 16);
-            if (Q) xb[b][j] = xs[c * 4];
+            if (Q) xb[b][j] = xs[c * xstep];
           }
         }
 #pragma unroll
@@ -252,7 +253,7 @@ __global__ __launch_bounds__(256) void mx_small(MxArgs a) {
         uint8_t* o = a.act + p * (a.I / 2) + bx * 16 + q * 2;
         *(uint16_t*)o = (uint16_t)c;
         *(uint16_t*)(o + 8) = (uint16_t)(c >> 16);
-        if (q == 0) a.act_scales[p * (a.I / 32) + bx] = (uint8_t)byte;
+        if (q == 0) a.act_scales[((bx / 4) * a.pairs + p) * 4 + bx % 4] = (uint8_t)byte;
       }
     } else {
       if (wave >= NF / 2) return;
@@ -290,396 +291,516 @@ int small_launch(const MxArgs& a, hipStream_t s) {
 // Larger experts: tiles of TM rows x TN weight rows
 // =============================================================================================
 
-// WM x WN wavefronts, each MI x 4 tiles of 16 rows x 16 weight rows.  Activations and weights are staged in
-// LDS by direct loads, in rows of 128 bytes (whole cache lines, eight lanes a row): 256 along K of 4-bit
-// values (a stage), 64 of bf16 (four steps to a stage).  Loading the weights to registers in operand order
-// instead takes no LDS, but its lanes touch 64 places of 16 bytes: address processing then bounds the kernel
-// (5 us for 128 along K, whatever the products).  Two buffers each, the loads one stage or step ahead of
-// the products, across tiles too: the last ones of a tile load the first of the next, whose rows are looked
-// up meanwhile.  A row's 16-byte pieces are stored at slot piece ^ swizzle(row), so that the 16 rows that a
-// quarter of a wavefront reads lie on 16 different 16-byte bank groups.
-// Rows of a tile that hold no row of the expert are neither loaded nor multiplied, in steps of a quarter.
-// (bf16) The weights of a step are read before the barrier that its rows wait for.
+// A wavefront multiplies 8 x 4 tiles of 16 rows x 16 weight rows.  Activations and weights are staged in LDS by
+// direct loads.  Loading the weights to registers in operand order instead takes no LDS, but its lanes touch 64
+// places of 16 bytes: address processing then bounds the kernels (5 us for 128 along K, whatever the products).
+// A row's 16-byte pieces are stored at slot piece ^ swizzle(row), so that the 16 rows that a quarter of a
+// wavefront reads lie on 16 different 16-byte bank groups (any LDS read of up to 16 bytes a lane takes the
+// same 7 clocks).
+//
+// The barrier of a step along K stands before its last products, whose operands are in registers by then:
+// behind it the next step's first operands are read, and the loads of the freed buffers issued, between those
+// products.  The same goes on from tile to tile; the next tile's rows are looked up meanwhile.
+// Rows of a tile that hold no row of the expert are not loaded, in steps of a quarter, nor multiplied, from
+// half a tile on.
+//
 // MODE 0: of a wavefront's four weight tiles, two are gate rows and two the up rows of the same 32 columns.
 // The weight rows of the two tiles c of 32 columns interleave in groups of four, 8 g + 4 c + [0, 4):
 // a lane then holds 8 consecutive output columns of one row.
-__device__ __forceinline__ int swz_x(int row) { return (row >> 1) & 7; }
-__device__ __forceinline__ int swz_w(int row) { return ((row >> 1) & 1) | (((row >> 3) & 3) << 1); }
+constexpr int kTileCols = 256;   // weight rows of a tile: 128 or 256 output columns
+template <int MODE>
+constexpr int kOutCols = MODE == 0 ? kTileCols / 2 : kTileCols;
+// first weight row (of the tile's) of a wavefront's weight tile f
+template <int MODE>
+__device__ __forceinline__ constexpr int wtile(int f) {
+  return (f >> 1) * (MODE == 0 ? kTileCols / 2 : 32) + (f & 1) * 4;
+}
 
-template <int MODE, bool Q, int WM, int WN, int MI>
-__global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM * WN / 4, WM * WN / 4)))
-void mx_tiled(MxArgs a) {
-  constexpr int NI = 4, W = WM * WN, TM = 16 * WM * MI, TN = 16 * NI * WN;
-  constexpr int COLS = MODE == 0 ? TN / 2 : TN;          // output columns of a tile
-  constexpr int kX = TM * 128, kW = TN * 128;            // bytes of a buffer
-  constexpr int LX = kX / (1024 * W), LW = kW / (1024 * W);   // direct loads of a wavefront for one
-  constexpr int kXS = Q ? TM * 8 : 0, kWS = TN * 8;      // scale bytes of a stage
-  constexpr int kScaleRows = TN + (Q ? TM : 0);
-  static_assert(LX == 4 && TM == 32 * W && LW >= 1 && kScaleRows <= 64 * W && TM <= 64 * W && MI % 4 == 0);
+struct MxTile {
+  int64_t row0;        // grouped row of the tile's first row
+  int vrows, nt, slot; // rows from there on (> 0), number of its columns' tile, cache slot
+};
+template <int TM>
+__device__ __forceinline__ MxTile mx_locate(const MxArgs& a, const TileTable& tt, int tile, int ntn) {
+  MxTile t;
+  const int mt = tile / ntn;
+  t.nt = tile - mt * ntn;
+  const int li = __builtin_amdgcn_readfirstlane(find_entry(tt, mt));
+  const int m0 = (mt - __builtin_amdgcn_readfirstlane(tt.cum[li])) * TM;
+  t.row0 = uniform64(tt.start[li]) + m0;
+  t.vrows = __builtin_amdgcn_readfirstlane(tt.rows[li]) - m0;
+  t.slot = a.list.slot[li];
+  return t;
+}
+
+// Per tile row, two sets taken in turn: the token, and for MODE 1 the slot index, the output row and the
+// routing weight (bf16 bits).
+template <int MODE, int TM>
+struct __attribute__((aligned(256))) RowTables {
+  int32_t row[2][TM], col[MODE == 1 ? 2 : 1][MODE == 1 ? TM : 64], orow[MODE == 1 ? 2 : 1][MODE == 1 ? TM : 64],
+      wt[MODE == 1 ? 2 : 1][MODE == 1 ? TM : 64];
+  // the tile rows' indices (low words; rows past the last: the first row's) into set p
+  __device__ __forceinline__ void load(const MxArgs& a, const MxTile& t, int p, int wave, int lane) {
+    if (wave < TM / 64) {
+      const int v = 64 * wave + lane;
+      const uint32_t off = (uint32_t)((v < t.vrows ? v : 0) * 8);
+      dma4(reinterpret_cast<const char*>(uniform_ptr(a.rows + t.row0)), off, lds_addr(row[p]) + 256 * wave);
+      if constexpr (MODE == 1)
+        dma4(reinterpret_cast<const char*>(uniform_ptr(a.cols + t.row0)), off, lds_addr(col[p]) + 256 * wave);
+    }
+  }
+  // output row and routing weight of the rows of set p, before the epilogue reads them
+  __device__ __forceinline__ void outputs(const MxArgs& a, const MxTile& t, int p, int wave, int lane) {
+    if (MODE == 1 && wave < TM / 64) {
+      const int v = 64 * wave + lane;
+      const int64_t tj = (int64_t)row[p][v] * a.k + col[p][v];
+      dma2(reinterpret_cast<const char*>(a.w), (uint32_t)(tj * 2), lds_addr(wt[p]) + 256 * wave);
+      orow[p][v] = a.out_mode == 0 ? (int32_t)tj : (int32_t)(t.row0 + (v < t.vrows ? v : 0));
+    }
+  }
+};
+
+// a lane's number where what follows from it is to be computed on the spot, not kept through the loops
+__device__ __forceinline__ int fresh(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+// The sums of a wavefront's tiles into the activations or the outputs: tile i of group wm of WM holds the tile's
+// rows 16 (WM i + wm) ..
+template <int MODE, bool Q, int WM, int TM>
+__device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxTile& t, const RowTables<MODE, TM>& tab, int set,
+                                            const floatx4 (&acc)[8][4], int wm, int wn, int lane_) {
+  const int lane = fresh(lane_), r = lane & 15, q = lane >> 4;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int row = 16 * (WM * i + wm) + r;
+    const bool live = row < t.vrows;
+    if constexpr (MODE == 0) {
+      float v[8];
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[4 * c + j] = silu_mul(acc[i][c][j], acc[i][2 + c][j]);
+      const int64_t col = t.nt * kOutCols<0> + wn * 32;
+      if constexpr (Q) {
+        const int byte = block_scale(v);
+        const uint32_t c = block_codes(v, byte);
+        if (live) {
+          *(uint32_t*)(a.act + (t.row0 + row) * (a.I / 2) + col / 2 + q * 4) = c;
+          if (q == 0) a.act_scales[((col / 128) * a.pairs + t.row0 + row) * 4 + (col / 32) % 4] = (uint8_t)byte;
+        }
+      } else if (live) {
+        *(u32x4*)(a.act + ((t.row0 + row) * a.I + col + q * 8) * 2) =
+            u32x4{pk_bf16(v[0], v[1]), pk_bf16(v[2], v[3]), pk_bf16(v[4], v[5]), pk_bf16(v[6], v[7])};
+      }
+    } else if (live) {
+      const float wt = __uint_as_float((uint32_t)tab.wt[set][row] << 16);
+      bf16_t* const o = a.out + (int64_t)tab.orow[set][row] * a.H + t.nt * kOutCols<1> + wn * 64 + q * 8;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        u32x4 y;
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int j = 0; j < 4; j += 2)
+            y[2 * c + j / 2] = pk_bf16(acc[i][2 * h + c][j] * wt, acc[i][2 * h + c][j + 1] * wt);
+        *(u32x4*)(o + 32 * h) = y;
+      }
+    }
+  }
+}
+
+// XCD-aware order: workgroup b runs on XCD b % 8, whose workgroups take a contiguous run of tiles; tiles of one
+// expert follow each other, columns fastest, and share their rows and weights in that XCD's L2.
+__device__ __forceinline__ int first_tile() {
+  const int per_xcd = gridDim.x % 8 == 0 ? (int)gridDim.x / 8 : 0;
+  return per_xcd ? (int)(blockIdx.x % 8) * per_xcd + (int)(blockIdx.x / 8) : (int)blockIdx.x;
+}
+
+// bf16 activations.  Four wavefronts share 128 rows; two such workgroups run on a CU, each in its own time, so
+// that one's barriers, epilogues and loads fall into the other's products.  A step is 64 along K: rows of 128
+// bytes, two buffers, the loads one step ahead; weights in pieces of 128 along K.
+template <int MODE>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void mx_tiled16(MxArgs a) {
+  constexpr int NI = 4, W = 4, TM = 128, MI = 8, TN = kTileCols, COLS = kOutCols<MODE>;
+  constexpr int RW = 64;                                 // a weight row's bytes in a buffer
+  constexpr int kX = TM * 128, kW = TN * RW, kS = TN * 4;   // bytes of a buffer: rows, weights, scales
+  constexpr int LX = 4, LW = 4;                          // direct loads of a wavefront for one
   __shared__ TileTable tt;
-  __shared__ __attribute__((aligned(1024))) char smem[2 * (kX + kW + kXS + kWS)];
-  // per tile row, two sets taken in turn: the token, and for MODE 1 the slot index, the output row and the
-  // routing weight (bf16 bits)
-  __shared__ __attribute__((aligned(256))) int32_t row_s[2][TM], col_s[MODE == 1 ? 2 : 1][MODE == 1 ? TM : 1];
-  __shared__ __attribute__((aligned(256))) int32_t orow_s[MODE == 1 ? 2 : 1][MODE == 1 ? TM : 1],
-      wt_s[MODE == 1 ? 2 : 1][MODE == 1 ? TM : 1];
+  __shared__ __attribute__((aligned(1024))) char smem[2 * (kX + kW + kS)];
+  __shared__ RowTables<MODE, TM> tab;
   build_tile_table<TM, kSmallRows>(a, tt);
   const int64_t K = MODE == 0 ? a.H : a.I;
   const int ntn = (int)((MODE == 0 ? a.I : a.H) / COLS);
   const int total = __builtin_amdgcn_readfirstlane(tt.total) * ntn;
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave / WN, wn = wave % WN;
+  const int lane = threadIdx.x & 63, wn = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, q = lane >> 4;
-  const int chunks = (int)(K / 128), stages = (chunks + 1) / 2;
-  const uint32_t smem0 = lds_addr(smem);
-  const uint32_t wbuf = smem0 + 2 * kX, xsbuf = wbuf + 2 * kW, wsbuf = xsbuf + 2 * kXS;
+  const int chunks = (int)(K / 128);
+  const uint32_t smem0 = lds_addr(smem), wbuf = smem0 + 2 * kX, sbuf = wbuf + 2 * kW;
   const char* const xbase = reinterpret_cast<const char*>(MODE == 0 ? a.x : a.act);
-  const uint8_t* const xsbase = MODE == 0 ? a.x_scales : a.act_scales;
-
+  auto swz_x = [](int row) { return (row >> 1) & 7; };
+  auto swz_w = [](int row) { return (row >> 3) & 3; };
   // fragment reads: addresses of tile 0, the others at constant offsets
-  const int xrow = 16 * wm + r;
   const int wrow = (MODE == 0 ? wn * 32 : wn * 64) + 8 * (r >> 2) + (r & 3);
-  const uint32_t xa = smem0 + (uint32_t)(xrow * 128 + (((Q ? q : 2 * q) ^ swz_x(xrow)) << 4));
-  const uint32_t wa = wbuf + (uint32_t)(wrow * 128 + (((Q ? q : q >> 1) ^ swz_w(wrow)) << 4) + (Q ? 0 : (q & 1) * 8));
-  constexpr int kXTile = 16 * WM * 128;
-  auto wtile = [](int f) { return (f >> 1) * (MODE == 0 ? TN / 2 : 32) + (f & 1) * 4; };   // in rows
+  const uint32_t xa = smem0 + (uint32_t)(r * 128 + (((2 * q) ^ swz_x(r)) << 4));
+  const uint32_t wa = wbuf + (uint32_t)(wrow * RW + (((q >> 1) ^ swz_w(wrow)) << 4) + (q & 1) * 8);
+  const uint32_t wsa = sbuf + (uint32_t)(wn * 256 + r * 16);
+  constexpr int kXTile = 16 * 128;
 
-  struct Tile {
-    int64_t row0;        // grouped row of the tile's first row
-    int vrows, nt, slot;
-  };
-  auto locate = [&](int tile) {
-    Tile t;
-    const int mt = tile / ntn;
-    t.nt = tile - mt * ntn;
-    const int li = __builtin_amdgcn_readfirstlane(find_entry(tt, mt));
-    const int m0 = (mt - __builtin_amdgcn_readfirstlane(tt.cum[li])) * TM;
-    t.row0 = uniform64(tt.start[li]) + m0;
-    t.vrows = __builtin_amdgcn_readfirstlane(tt.rows[li]) - m0;   // > 0
-    t.slot = a.list.slot[li];
-    return t;
-  };
-  // the tile rows' indices (low words; rows past the last: the first row's) into set p, direct loads
-  auto load_rows = [&](const Tile& t, int p) {
-    if (wave < TM / 64) {
-      const int v = 64 * wave + lane;
-      const uint32_t off = (uint32_t)((v < t.vrows ? v : 0) * 8);
-      dma4(reinterpret_cast<const char*>(uniform_ptr(a.rows + t.row0)), off, lds_addr(row_s[p]) + 256 * wave);
-      if constexpr (MODE == 1)
-        dma4(reinterpret_cast<const char*>(uniform_ptr(a.cols + t.row0)), off, lds_addr(col_s[p]) + 256 * wave);
-    }
-  };
-
-  // The tiles whose activations and weights are being loaded.  Direct load j of a wavefront moves 8 rows, lane / 8 of them,
-  // its lane % 8 the piece (lane % 8) ^ swizzle: rows 64 j .. of the activations over all wavefronts (W = 8),
-  // so that a tile of few rows takes the first loads only.
-  const int r8 = lane >> 3, slot8 = lane & 7;
-  auto xload_row = [&](int j) { return 8 * (W * j + wave) + r8; };
-  uint32_t xoff[LX], woff[LW], sdst;
-  const char* wbase[LW];
-  const uint8_t* sp = nullptr;   // this thread's row of scales: a weight row, or (Q) an activation row
+  // The tile whose steps are being loaded.  Load j of a wavefront moves 1 KiB of rows in a row's order of
+  // slots: 8 rows of 128 bytes or 16 of 64.  Load j of the activations moves rows 32 j .. over all wavefronts.
+  uint32_t xoff[LX], woff, soff;
+  const char *wbase[2], *sbase;   // MODE 0: gate rows (the first half of the loads), up rows
   int xloads = LX;
-  if (tid < TN) sdst = wsbuf + (uint32_t)(tid * 8);
-  else sdst = xsbuf + (uint32_t)((tid - TN) * 8);
-  auto aim_x = [&](const Tile& t, int p) {
-    auto src_row = [&](int v) {
-      return MODE == 0 ? (uint32_t)row_s[p][v] : (uint32_t)(t.row0 + (v < t.vrows ? v : 0));
-    };
-    xloads = t.vrows > TM / 4 * 3 ? 4 : (t.vrows > TM / 2 ? 3 : (t.vrows > TM / 4 ? 2 : 1));
+  auto aim = [&](const MxTile& t, int p) {
+    const int l = fresh(lane);
+    xloads = min((t.vrows + 31) / 32, LX);
 #pragma unroll
     for (int j = 0; j < LX; ++j) {
-      const int v = xload_row(j);
-      xoff[j] = src_row(v) * (uint32_t)(Q ? K / 2 : K * 2) + (uint32_t)((slot8 ^ swz_x(v)) * 16);
+      const int v = 8 * (W * j + wn) + l / 8;
+      const uint32_t src = MODE == 0 ? (uint32_t)tab.row[p][v] : (uint32_t)(t.row0 + (v < t.vrows ? v : 0));
+      xoff[j] = (src * (uint32_t)K + (uint32_t)(((l & 7) ^ swz_x(v)) * 8)) * 2u;
     }
-    if (Q && tid >= TN && tid < kScaleRows) sp = xsbase + (int64_t)src_row(tid - TN) * (K / 32);
-  };
-  auto aim_w = [&](const Tile& t) {
     const Weights m0 = weights_at<MODE>(a, t.slot, 0, t.nt * COLS);
-    const Weights m1 = MODE == 0 ? weights_at<MODE>(a, t.slot, 1, t.nt * COLS) : m0;
-#pragma unroll
-    for (int j = 0; j < LW; ++j) {
-      const int t0 = 8 * (wave * LW + j), part = MODE == 0 ? t0 / (TN / 2) : 0;
-      wbase[j] = reinterpret_cast<const char*>(uniform_ptr(part ? m1.codes : m0.codes));
-      woff[j] = (uint32_t)(t0 - part * (TN / 2) + r8) * (uint32_t)(K / 2) + (uint32_t)((slot8 ^ swz_w(t0 + r8)) * 16);
-    }
-    if (tid < TN) {
-      const int part = MODE == 0 ? tid / (TN / 2) : 0;
-      sp = (part ? m1.scales : m0.scales) + (int64_t)(tid - part * (TN / 2)) * (K / 32);
-    }
+    const Weights m1 = weights_at<MODE>(a, t.slot, MODE == 0 ? 1 : 0, MODE == 0 ? t.nt * COLS : t.nt * COLS + TN / 2);
+    wbase[0] = reinterpret_cast<const char*>(uniform_ptr(m0.codes));
+    wbase[1] = reinterpret_cast<const char*>(uniform_ptr(m1.codes));
+    const int v = 16 * wn + l / 4;   // load j: 64 j rows on, in the same order of slots
+    woff = (uint32_t)v * (uint32_t)(K / 2) + (uint32_t)(((l & 3) ^ swz_w(v)) * 16);
+    // scales: those of a lane's four weight tiles adjacent
+    const int row = 8 * (l >> 4) + ((l >> 2) & 3), f = l & 3;
+    sbase = reinterpret_cast<const char*>(uniform_ptr(m0.scales));
+    soff = (uint32_t)(wn * (MODE == 0 ? 32 : 64) + row + (MODE == 0 ? (f & 1) * 4 : wtile<1>(f))) * (uint32_t)(K / 32) +
+           (MODE == 0 && f >= 2 ? (uint32_t)(a.H * a.I / 32) : 0u);
   };
-  u32x2 sv = {0, 0};
-  auto load_s = [&](int st) {
-    if (tid < kScaleRows) {
-      if (2 * st + 1 < chunks) __builtin_memcpy(&sv, sp + st * 8, 8);
-      else __builtin_memcpy(&sv, sp + st * 8, 4);
-    }
+  auto load_x = [&](int j, int n, int b) {   // load j of step n of the loaded tile into buffer b
+    if (j < xloads) dma16(xbase + (int64_t)n * 128, xoff[j], smem0 + (uint32_t)(b * kX + (W * j + wn) * 1024));
   };
-  auto store_s = [&](int b) {
-    if (tid < kScaleRows)
-      *reinterpret_cast<__attribute__((address_space(3))) u32x2*>((uintptr_t)(sdst + (uint32_t)(b * (tid < TN ? kWS : kXS)))) = sv;
+  auto load_w = [&](int j, int c, int b) {   // of 128 along K number c
+    dma16(wbase[j >> 1] + (j & 1) * 32 * K + (int64_t)c * RW, woff, wbuf + (uint32_t)(b * kW + (W * j + wn) * 1024));
   };
-  // Where the number of chunks is odd, the last stage's rows of 4-bit values end in its middle: the lanes of
-  // the second half read the first half again (it is not multiplied).
-  auto back = [&](int piece) { return (uint32_t)((piece & 4) << 4); };
-  auto load_x = [&](int n, int b) {   // Q: stage n; bf16: step n
-    const uint32_t dst = smem0 + (uint32_t)(b * kX + wave * 1024);
-#pragma unroll
-    for (int j = 0; j < LX; ++j)
-      if (j < xloads) {
-        const uint32_t tail = Q && 2 * n + 1 >= chunks ? back(slot8 ^ swz_x(xload_row(j))) : 0u;
-        dma16(xbase + (int64_t)n * 128, xoff[j] - tail, dst + (uint32_t)(W * j * 1024));
-      }
-  };
-  auto load_w = [&](int st, int b) {
-#pragma unroll
-    for (int j = 0; j < LW; ++j) {
-      const uint32_t tail = 2 * st + 1 >= chunks ? back(slot8 ^ swz_w(8 * (wave * LW + j) + r8)) : 0u;
-      dma16(wbase[j] + (int64_t)st * 128, woff[j] - tail, wbuf + (uint32_t)(b * kW + (wave * LW + j) * 1024));
-    }
-  };
+  auto load_s = [&](int c, int b) { dma4(sbase + (int64_t)c * 4, soff, sbuf + (uint32_t)(b * kS + wn * 256)); };
 
-  // XCD-aware order: workgroup b runs on XCD b % 8, whose workgroups take a contiguous run of tiles; tiles of
-  // one expert follow each other, columns fastest, and share their rows and weights in that XCD's L2.
-  const int per_xcd = gridDim.x % 8 == 0 ? (int)gridDim.x / 8 : 0;
-  const int first = per_xcd ? (int)(blockIdx.x % 8) * per_xcd + (int)(blockIdx.x / 8) : (int)blockIdx.x;
+  const int first = first_tile();
   if (first >= total) return;
-  Tile cur = locate(first);
-  load_rows(cur, 0);
+  MxTile cur = mx_locate<TM>(a, tt, first, ntn);
+  tab.load(a, cur, 0, wn, lane);
   wait_cnt<0>();
   wg_barrier();
-  aim_x(cur, 0);
-  aim_w(cur);
-  load_s(0);
-  load_w(0, 0);
-  load_x(0, 0);
-  store_s(0);
+  aim(cur, 0);
+#pragma unroll
+  for (int j = 0; j < LX; ++j) load_x(j, 0, 0), load_x(j, 1, 1);
+#pragma unroll
+  for (int j = 0; j < LW; ++j) load_w(j, 0, 0);
+  load_s(0, 0);
   wait_cnt<0>();
   wg_barrier();
-  int set = 0, wb = 0;   // set of row tables; buffer of the present stage (Q: of its activations too)
 
-  // bf16: the weights' codes of the next step, their scales of its chunk
+  // read ahead: the next step's weights and scales, its first fragments
   u32x2 wr[NI];
-  uint32_t ws[NI];
-  auto read_w = [&](uint32_t at) {
-#pragma unroll
-    for (int f = 0; f < NI; ++f) wr[f] = lds_get<lds_u32x2>(at + (uint32_t)(wtile(f) * 128));
+  u32x4 wsc, xf[4];
+  auto read_x = [&](int to, int s, int i, int b) {   // half s, tile i of the step in buffer b
+    xf[to] = lds_get<lds_u32x4>(((xa + (uint32_t)(b * kX)) ^ (uint32_t)(s << 4)) + (uint32_t)(kXTile * i));
   };
-  auto read_s = [&](uint32_t at) {
+  auto read_w = [&](int h, int w) {                  // half h of the 128 along K in buffer w
+    const uint32_t at = (wa + (uint32_t)(w * kW)) ^ (uint32_t)(h << 5);
 #pragma unroll
-    for (int f = 0; f < NI; ++f) ws[f] = lds_get<lds_u32>(at + (uint32_t)((wrow + wtile(f)) * 8));
+    for (int f = 0; f < NI; ++f) wr[f] = lds_get<lds_u32x2>(at + (uint32_t)(wtile<MODE>(f) * RW));
+    wsc = lds_get<lds_u32x4>(wsa + (uint32_t)(w * kS));
   };
-  if constexpr (!Q) {
-    read_w(wa);
-    read_s(wsbuf);
-  }
+  read_w(0, 0);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) read_x(i, 0, i, 0);
+  int set = 0, wb = 0;   // set of row tables; buffer of the present weights
   for (int tile = first; tile < total; tile += gridDim.x, set ^= 1) {
-    // the tile after this one; after the last tile its own first stage is loaded again
+    // the tile after this one; after the last tile its own first steps are loaded again
     const bool more = tile + (int)gridDim.x < total;
-    const Tile next = more ? locate(tile + gridDim.x) : cur;
-    load_rows(next, set ^ 1);
-    if constexpr (MODE == 1) {
-      // output row and routing weight of tile row tid, in LDS before the epilogue reads them
-      if (wave < TM / 64) {
-        const int64_t tj = (int64_t)row_s[set][tid] * a.k + col_s[set][tid];
-        dma2(reinterpret_cast<const char*>(a.w), (uint32_t)(tj * 2), lds_addr(wt_s[set]) + 256 * wave);
-        orow_s[set][tid] = a.out_mode == 0 ? (int32_t)tj : (int32_t)(cur.row0 + (tid < cur.vrows ? tid : 0));
-      }
-    }
+    const MxTile next = more ? mx_locate<TM>(a, tt, tile + gridDim.x, ntn) : cur;
+    tab.load(a, next, set ^ 1, wn, lane);
+    tab.outputs(a, cur, set, wn, lane);
     floatx4 acc[MI][NI];
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
       for (int f = 0; f < NI; ++f) acc[i][f] = floatx4{0, 0, 0, 0};
-    // In the last stage (bf16 activations: step) the loads turn to the next tile, whose row indices may still
-    // be on their way where it is the only one.
-    auto turn_x = [&]() {
-      if (stages == 1) {
-        wait_cnt<0>();
-        wg_barrier();
+    // ROWS: tiles of 16 rows that are multiplied; the others hold no row of the expert
+    auto loop = [&](auto rows) {
+      constexpr int ROWS = decltype(rows)::value;
+      for (int c = 0; c < chunks; ++c) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          // the first 32 along K are decoded here, the second 32 between the products of the first
+          u32x4 wv[2][NI];
+          auto decode = [&](int s, int part) {   // half of a weight tile's 8 elements a lane
+            const int f = part >> 1, half = part & 1;
+            const float sc = scale_of(__builtin_amdgcn_ubfe(wsc[f], 16 * h + 8 * (q >> 1), 8));
+            const uint32_t v = wr[f][s];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const bf16x2 d = half ? (j ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, sc, 3)
+                                         : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, sc, 2))
+                                    : (j ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, sc, 1)
+                                         : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, sc, 0));
+              wv[s][f][2 * half + j] = __builtin_bit_cast(uint32_t, d);
+            }
+          };
+#pragma unroll
+          for (int part = 0; part < 2 * NI; ++part) decode(0, part);
+          __builtin_amdgcn_sched_barrier(0);
+          const bool last = c == chunks - 1;
+#pragma unroll
+          for (int n = 0; n < 2 * ROWS; ++n) {
+            const int s = n / ROWS, i = n % ROWS, k = n - (2 * ROWS - 4);
+            if (k == 0) {
+              wait_cnt<0>();   // the next step's loads have landed, this one's fragments are read
+              wg_barrier();
+              if (h == 0 && last) aim(next, set ^ 1);
+              if (h == 1) wb ^= 1;
+              read_w(h ^ 1, wb);
+            }
+            if (s == 0)
+#pragma unroll
+              for (int part = i * 2 * NI / ROWS; part < (i + 1) * 2 * NI / ROWS; ++part) decode(1, part);
+#pragma unroll
+            for (int f = 0; f < NI; ++f)
+              acc[i][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, wv[s][f]),
+                                                                 __builtin_bit_cast(bf16x8, xf[n & 3]), acc[i][f], 0, 0, 0);
+            // the fragment four products on, of this step or the next
+            if (k < 0) read_x(n & 3, (n + 4) / ROWS, (n + 4) % ROWS, h);
+            else read_x(n & 3, 0, k, h ^ 1);
+            if (k >= 0) {   // the loads of the buffers that are free now
+              load_x(k, last ? h : 2 * c + 2 + h, h);
+              if (h == 0) load_w(k, last ? 0 : c + 1, wb ^ 1);
+              if (h == 0 && k == 3) load_s(last ? 0 : c + 1, wb ^ 1);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
       }
-      aim_x(next, set ^ 1);
     };
+    if (cur.vrows > TM / 4 * 3) loop(std::integral_constant<int, MI>{});
+    else if (cur.vrows > TM / 2) loop(std::integral_constant<int, MI / 4 * 3>{});
+    else loop(std::integral_constant<int, MI / 2>{});
+    mx_epilogue<MODE, false, 1, TM>(a, cur, tab, set, acc, 0, wn, lane);
+    cur = next;
+  }
+  wait_cnt<0>();   // no load may write this workgroup's LDS after its end
+}
+
+// 4-bit activations.  Eight wavefronts in two rows share 256 rows.  A step is 256 along K: rows of 128 bytes of
+// activations and of weights, two buffers, the loads one step ahead.  A CU receives about 64 bytes a clock, in
+// lines of 128; the scales therefore come 16 bytes of a row, 512 along K, at a time, and a lane keeps those of
+// its rows' blocks in a register a tile, the present one in the low byte.
+template <int MODE>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void mx_tiled4(MxArgs a) {
+  constexpr int WM = 2, WN = 4, MI = 8, NI = 4, W = WM * WN, TM = 256, TN = kTileCols, COLS = kOutCols<MODE>;
+  constexpr int kX = TM * 128, kW = TN * 128;            // bytes of a buffer
+  constexpr int LX = 4, LW = 4, LS = 4;                  // direct loads of a wavefront for one
+  constexpr int kS = (TN + TM) * 16;                     // scale bytes of two steps: weight rows, activation rows
+  __shared__ TileTable tt;
+  __shared__ __attribute__((aligned(1024))) char smem[2 * (kX + kW + kS)];
+  __shared__ RowTables<MODE, TM> tab;
+  build_tile_table<TM, kSmallRows>(a, tt);
+  const int64_t K = MODE == 0 ? a.H : a.I;
+  const int ntn = (int)((MODE == 0 ? a.I : a.H) / COLS);
+  const int total = __builtin_amdgcn_readfirstlane(tt.total) * ntn;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  const int r = lane & 15, q = lane >> 4;
+  // steps; a tile takes at least two, so that the loads ahead stay within the next tile (what lies past the
+  // last 128 along K is not multiplied, and loads those again)
+  const int chunks = (int)(K / 128), steps = (chunks + 1) / 2, span = max(steps, 2);
+  const uint32_t smem0 = lds_addr(smem), wbuf = smem0 + 2 * kX, sbuf = wbuf + 2 * kW;
+  const char* const xbase = reinterpret_cast<const char*>(MODE == 0 ? a.x : a.act);
+  auto swz_x = [](int row) { return (row >> 1) & 7; };
+  auto swz_w = [](int row) { return ((row >> 1) & 1) | (((row >> 3) & 3) << 1); };
+  // fragment reads: addresses of tile 0, the others at constant offsets
+  const int xrow = 16 * wm + r, wrow = (MODE == 0 ? wn * 32 : wn * 64) + 8 * (r >> 2) + (r & 3);
+  const uint32_t xa = smem0 + (uint32_t)(xrow * 128 + ((q ^ swz_x(xrow)) << 4));
+  const uint32_t wa = wbuf + (uint32_t)(wrow * 128 + ((q ^ swz_w(wrow)) << 4));
+  const uint32_t xsa = sbuf + (uint32_t)((TN + xrow) * 16), wsa = sbuf + (uint32_t)(wrow * 16);
+  constexpr int kXTile = 16 * WM * 128;
+  const uint32_t pick = (uint32_t)(q | (4 + q) << 8);   // byte q of two words
+
+  // The tile whose steps are being loaded.  Load j of a wavefront moves 8 rows of 128 bytes in a row's order of
+  // slots; rows 64 j .. over all wavefronts.  A load of scales moves 16 bytes of 16 rows, four lanes a row.
+  uint32_t xoff[LX], woff, soff[LS];
+  const char *wbase[2], *sbase;   // MODE 0: gate rows (the first half of the loads), up rows
+  int xloads = LX;
+  auto aim = [&](const MxTile& t, int p) {
+    const int l = fresh(lane);
+    auto src_row = [&](int v) {
+      return MODE == 0 ? (uint32_t)tab.row[p][v] : (uint32_t)(t.row0 + (v < t.vrows ? v : 0));
+    };
+    xloads = min((t.vrows + 63) / 64, LX);
+#pragma unroll
+    for (int j = 0; j < LX; ++j) {
+      const int v = 8 * (W * j + wave) + l / 8;
+      xoff[j] = src_row(v) * (uint32_t)(K / 2) + (uint32_t)(((l & 7) ^ swz_x(v)) * 16);
+    }
+    const Weights m0 = weights_at<MODE>(a, t.slot, 0, t.nt * COLS);
+    const Weights m1 = weights_at<MODE>(a, t.slot, MODE == 0 ? 1 : 0, MODE == 0 ? t.nt * COLS : t.nt * COLS + TN / 2);
+    wbase[0] = reinterpret_cast<const char*>(uniform_ptr(m0.codes));
+    wbase[1] = reinterpret_cast<const char*>(uniform_ptr(m1.codes));
+    const int v = 8 * wave + l / 8;   // load j: 64 j rows on, in the same order of slots
+    woff = (uint32_t)v * (uint32_t)(K / 2) + (uint32_t)(((l & 7) ^ swz_w(v)) * 16);
+    if (wave < WN) {
+      sbase = reinterpret_cast<const char*>(uniform_ptr(wave < 2 ? m0.scales : m1.scales));
+#pragma unroll
+      for (int j = 0; j < LS; ++j) soff[j] = (uint32_t)(64 * (wave & 1) + 16 * j + l / 4) * (uint32_t)(K / 32);
+    } else {
+      sbase = reinterpret_cast<const char*>(MODE == 0 ? a.x_scales : a.act_scales);
+#pragma unroll
+      for (int j = 0; j < LS; ++j) {
+        const uint32_t row = src_row(64 * (wave - WN) + 16 * j + l / 4);
+        soff[j] = row * (MODE == 0 ? (uint32_t)(K / 32) : 4u);
+      }
+    }
+  };
+  // Where the number of chunks is odd, the last step's rows end in its middle: the lanes of the second half
+  // read the first half again.
+  auto tail = [&](int piece) { return (uint32_t)((piece & 4) << 4); };
+  auto load_x = [&](int j, int n, int b) {   // load j of step n of the loaded tile into buffer b
+    if (j >= xloads) return;
+    const int at = min(n, steps - 1);
+    uint32_t off = xoff[j];
+    if (2 * at + 1 >= chunks) {
+      const int l = fresh(lane);
+      off -= tail((l & 7) ^ swz_x(8 * (W * j + wave) + l / 8));
+    }
+    dma16(xbase + (int64_t)at * 128, off, smem0 + (uint32_t)(b * kX + (W * j + wave) * 1024));
+  };
+  auto load_w = [&](int j, int n, int b) {
+    const int at = min(n, steps - 1);
+    uint32_t off = woff;
+    if (2 * at + 1 >= chunks) {
+      const int l = fresh(lane);
+      off -= tail((l & 7) ^ swz_w(8 * wave + l / 8));
+    }
+    dma16(wbase[j >> 1] + (j & 1) * 32 * K + (int64_t)at * 128, off, wbuf + (uint32_t)(b * kW + (W * j + wave) * 1024));
+  };
+  auto load_s = [&](int j, int n, int b) {   // of steps n and n + 1
+    const int c = min(2 * n + (fresh(lane) & 3), chunks - 1);
+    const uint32_t per = MODE == 1 && wave >= WN ? (uint32_t)(a.pairs * 4) : 4u;
+    dma4(sbase, soff[j] + (uint32_t)c * per, sbuf + (uint32_t)(b * kS + (4 * wave + j) * 256));
+  };
+
+  const int first = first_tile();
+  if (first >= total) return;
+  MxTile cur = mx_locate<TM>(a, tt, first, ntn);
+  tab.load(a, cur, 0, wave, lane);
+  wait_cnt<0>();
+  wg_barrier();
+  aim(cur, 0);
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+#pragma unroll
+    for (int j = 0; j < LX; ++j) load_x(j, n, n);
+#pragma unroll
+    for (int j = 0; j < LW; ++j) load_w(j, n, n);
+  }
+#pragma unroll
+  for (int j = 0; j < LS; ++j) load_s(j, 0, 0);
+  wait_cnt<0>();
+  wg_barrier();
+
+  // read ahead: the next chunk's weights and first four fragments; the scale bytes of the weight tiles and the
+  // activation tiles
+  u32x4 wf[2][NI], xf[2][4];
+  uint32_t ws[NI], xs[MI];
+  int xb = 0, sb = 0;   // buffers of the present step, of its scales
+  auto read = [&](int to, int j, int b) {   // chunk j of the step in buffer b
+    const uint32_t at = (wa + (uint32_t)(b * kW)) ^ (uint32_t)(j << 6), xat = (xa + (uint32_t)(b * kX)) ^ (uint32_t)(j << 6);
+#pragma unroll
+    for (int f = 0; f < NI; ++f) wf[to][f] = lds_get<lds_u32x4>(at + (uint32_t)(wtile<MODE>(f) * 128));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) xf[to][i] = lds_get<lds_u32x4>(xat + (uint32_t)(kXTile * i));
+  };
+  auto read_s = [&](int b) {   // four chunks' words of each row -> its bytes q
+    auto bytes = [&](uint32_t at) {
+      const u32x4 v = lds_get<lds_u32x4>(at + (uint32_t)(b * kS));
+      const uint32_t lo = __builtin_amdgcn_perm(v[1], v[0], pick), hi = __builtin_amdgcn_perm(v[3], v[2], pick);
+      return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+    };
+#pragma unroll
+    for (int f = 0; f < NI; ++f) ws[f] = bytes(wsa + (uint32_t)(wtile<MODE>(f) * 16));
+#pragma unroll
+    for (int i = 0; i < MI; ++i) xs[i] = bytes(xsa + (uint32_t)(16 * WM * 16 * i));
+  };
+  read(0, 0, 0);
+  int set = 0;   // set of row tables
+  for (int tile = first; tile < total; tile += gridDim.x, set ^= 1) {
+    // the tile after this one; after the last tile its own first steps are loaded again
+    const bool more = tile + (int)gridDim.x < total;
+    const MxTile next = more ? mx_locate<TM>(a, tt, tile + gridDim.x, ntn) : cur;
+    tab.load(a, next, set ^ 1, wave, lane);
+    tab.outputs(a, cur, set, wave, lane);
+    floatx4 acc[MI][NI];
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int f = 0; f < NI; ++f) acc[i][f] = floatx4{0, 0, 0, 0};
     // ROWS: tiles of 16 rows of a wavefront that are multiplied; the others hold no row of the expert
     auto loop = [&](auto rows) {
       constexpr int ROWS = decltype(rows)::value;
-      if constexpr (Q) {
-        for (int st = 0; st < stages; ++st, wb ^= 1) {
-          const uint32_t xb = xa + (uint32_t)(wb * kX), wbb = wa + (uint32_t)(wb * kW);
-          const uint32_t xsb = xsbuf + (uint32_t)(wb * kXS + xrow * 8), wsb = wsbuf + (uint32_t)(wb * kWS + wrow * 8);
-          u32x4 xn[2], wf[NI];
-          uint32_t xsn[2], wsf[NI];
-          auto read_x = [&](int j, int i) {
+      for (int st = 0; st < span; ++st) {
+        if ((st & 1) == 0) read_s(sb);
+        // the step whose loads take the buffers that this one frees
+        const int ls = st + 2 < span ? st + 2 : st + 2 - span;
 #pragma unroll
-            for (int v = 0; v < 2; ++v) {
-              xn[v] = lds_get<lds_u32x4>((xb ^ (uint32_t)(j << 6)) + (uint32_t)(kXTile * (i + v)));
-              xsn[v] = lds_get<lds_u32>(xsb + (uint32_t)(16 * WM * 8 * (i + v) + 4 * j));
-            }
-          };
-          auto read_wq = [&](int j) {
+        for (int j = 0; j < 2; ++j) {
+          const bool there = 2 * st + j < chunks;
+          u32x4 xg[ROWS > 4 ? ROWS - 4 : 1];   // the fragments from the fifth on
+          const uint32_t xat = (xa + (uint32_t)(xb * kX)) ^ (uint32_t)(j << 6);
 #pragma unroll
-            for (int f = 0; f < NI; ++f) {
-              wf[f] = lds_get<lds_u32x4>((wbb ^ (uint32_t)(j << 6)) + (uint32_t)(wtile(f) * 128));
-              wsf[f] = lds_get<lds_u32>(wsb + (uint32_t)(wtile(f) * 8 + 4 * j));
-            }
-          };
-          read_wq(0);
-          read_x(0, 0);
-          const bool last = st + 1 == stages;
-          if (last) {
-            turn_x();
-            aim_w(next);
-          }
-          const int ls = last ? 0 : st + 1;
-          load_s(ls);
-          load_w(ls, wb ^ 1);
-          load_x(ls, wb ^ 1);
-          const bool two = 2 * st + 1 < chunks;
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            if (j == 1 && !two) break;
-            u32x4 cw[NI];
-            int cs[NI];
-#pragma unroll
-            for (int f = 0; f < NI; ++f) cw[f] = wf[f], cs[f] = (int)(wsf[f] >> (8 * q));
-#pragma unroll
-            for (int i = 0; i < ROWS; i += 2) {
-              const u32x4 x0 = xn[0], x1 = xn[1];
-              const int s0 = (int)(xsn[0] >> (8 * q)), s1 = (int)(xsn[1] >> (8 * q));
-              if (i + 2 < ROWS) {
-                read_x(j, i + 2);
-              } else if (j == 0) {
-                read_x(1, 0);
-                read_wq(1);
-              }
-#pragma unroll
-              for (int f = 0; f < NI; ++f) acc[i][f] = mma_fp4(cw[f], cs[f], x0, s0, acc[i][f]);
-#pragma unroll
-              for (int f = 0; f < NI; ++f) acc[i + 1][f] = mma_fp4(cw[f], cs[f], x1, s1, acc[i + 1][f]);
-              __builtin_amdgcn_sched_barrier(0);
-            }
-          }
-          store_s(wb ^ 1);
-          wait_cnt<0>();   // the next stage's loads have landed, this one's fragments are read
-          wg_barrier();
-        }
-      } else {
-        for (int c = 0; c < chunks; ++c) {
-          const bool first_half = (c & 1) == 0, last = c + 1 == chunks;
-          const bool stage_end = !first_half || last;   // the next chunk lies in the other buffer
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t xb = xa, wat = wa;   // computed here, not kept in registers through the loop
-            asm volatile("" : "+v"(xb), "+v"(wat));
-            xb += (uint32_t)(h * kX);
-            bf16x8 xr[3];
-            auto read = [&](int m) {
-              xr[m % 3] = lds_read16((xb ^ (uint32_t)((m / ROWS) << 4)) + (uint32_t)(kXTile * (m % ROWS)));
-            };
-            read(0);
-            read(1);
-            // the first 32 along K are decoded while the first fragments are on their way, the second 32
-            // between the products of the first
-            u32x4 wv[2][NI];
-            uint32_t c1[NI];
-            float sc[NI];
-            auto decode = [&](uint32_t v, int s, int part) {   // half of a weight tile's 8 elements a lane
-              const int f = part >> 1, half = part & 1;
-#pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                const bf16x2 d = half ? (j ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, sc[f], 3)
-                                           : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, sc[f], 2))
-                                      : (j ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, sc[f], 1)
-                                           : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, sc[f], 0));
-                wv[s][f][2 * half + j] = __builtin_bit_cast(uint32_t, d);
-              }
-            };
+          for (int i = 4; i < ROWS; ++i) xg[i - 4] = lds_get<lds_u32x4>(xat + (uint32_t)(kXTile * i));
+          auto multiply = [&](int i) {
 #pragma unroll
             for (int f = 0; f < NI; ++f)
-              c1[f] = wr[f][1], sc[f] = scale_of(__builtin_amdgcn_ubfe(ws[f], 16 * h + 8 * (q >> 1), 8));
-#pragma unroll
-            for (int part = 0; part < 2 * NI; ++part) decode(wr[part >> 1][0], 0, part);
+              acc[i][f] = mma_fp4(wf[j][f], (int)ws[f], i < 4 ? xf[j][i] : xg[i < 4 ? 0 : i - 4], (int)xs[i], acc[i][f]);
             __builtin_amdgcn_sched_barrier(0);
-            if (h == 0) {
-              if (first_half) {   // the next stage's weights: there one step later
-                const bool final_stage = c + 2 >= chunks;
-                if (final_stage) aim_w(next);
-                load_s(final_stage ? 0 : c / 2 + 1);
-                load_w(final_stage ? 0 : c / 2 + 1, wb ^ 1);
-              }
-              load_x(2 * c + 1, 1);
-              read_w((wat + (uint32_t)(wb * kW)) ^ (uint32_t)((c & 1) << 6) ^ 32u);
-            } else {
-              if (last) turn_x();
-              load_x(last ? 0 : 2 * c + 2, 0);
-              if (stage_end) wb ^= 1;
-              read_w((wat + (uint32_t)(wb * kW)) ^ (uint32_t)(stage_end ? 0 : 64));
-              read_s(wsbuf + (uint32_t)(wb * kWS + (stage_end ? 0 : 4)));
-            }
+          };
+          if (there)
 #pragma unroll
-            for (int m = 0; m < 2 * ROWS; ++m) {
-              const int s = m / ROWS, i = m % ROWS;
-              if (m + 2 < 2 * ROWS) read(m + 2);
-              if (s == 0)
-#pragma unroll
-                for (int part = i * 2 * NI / ROWS; part < (i + 1) * 2 * NI / ROWS; ++part) decode(c1[part >> 1], 1, part);
-#pragma unroll
-              for (int f = 0; f < NI; ++f)
-                acc[i][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, wv[s][f]), xr[m % 3],
-                                                                   acc[i][f], 0, 0, 0);
-              __builtin_amdgcn_sched_barrier(0);
-            }
-            if (h == 0 && first_half) store_s(wb ^ 1);
-            wait_cnt<0>();
+            for (int i = 0; i < 4; ++i) multiply(i);
+          if (j == 0) {
+            read(1, 1, xb);
+          } else {
+            wait_cnt<0>();   // the next step's loads have landed, this one's fragments are read
             wg_barrier();
+            if (st == span - 2) aim(next, set ^ 1);
+            read(0, 0, xb ^ 1);
           }
+          // the loads of the buffers that are free now, between the last products
+          auto loads = [&](int k) {
+            if (j == 0) return;
+            load_x(k, ls, xb);
+            load_w(k, ls, xb);
+            if ((ls & 1) == 0) load_s(k, ls, (st & 1) ? sb : sb ^ 1);   // not the next step's scales
+          };
+#pragma unroll
+          for (int i = 4; i < 8; ++i) {
+            if (i < ROWS && there) multiply(i);
+            loads(i - 4);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+#pragma unroll
+          for (int f = 0; f < NI; ++f) ws[f] >>= 8;
+#pragma unroll
+          for (int i = 0; i < ROWS; ++i) xs[i] >>= 8;
         }
+        xb ^= 1;
+        if ((st & 1) == 1 || st == span - 1) sb ^= 1;
       }
     };
-    // rows 16 (WM i + wm) .. + 16 are tile i of wavefront row wm: the tile's rows in steps of a quarter
     if (cur.vrows > TM / 4 * 3) loop(std::integral_constant<int, MI>{});
     else if (cur.vrows > TM / 2) loop(std::integral_constant<int, MI / 4 * 3>{});
-    else if (cur.vrows > TM / 4) loop(std::integral_constant<int, MI / 2>{});
-    else loop(std::integral_constant<int, MI / 4>{});
-#pragma unroll
-    for (int i = 0; i < MI; ++i) {
-      const int t = 16 * (WM * i + wm) + r;
-      const bool live = t < cur.vrows;
-      if constexpr (MODE == 0) {
-        float v[8];
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) v[4 * c + j] = silu_mul(acc[i][c][j], acc[i][2 + c][j]);
-        const int64_t col = cur.nt * COLS + wn * 32;
-        if constexpr (Q) {
-          const int byte = block_scale(v);
-          const uint32_t c = block_codes(v, byte);
-          if (live) {
-            *(uint32_t*)(a.act + (cur.row0 + t) * (a.I / 2) + col / 2 + q * 4) = c;
-            if (q == 0) a.act_scales[(cur.row0 + t) * (a.I / 32) + col / 32] = (uint8_t)byte;
-          }
-        } else if (live) {
-          *(u32x4*)(a.act + ((cur.row0 + t) * a.I + col + q * 8) * 2) =
-              u32x4{pk_bf16(v[0], v[1]), pk_bf16(v[2], v[3]), pk_bf16(v[4], v[5]), pk_bf16(v[6], v[7])};
-        }
-      } else if (live) {
-        const float wt = __uint_as_float((uint32_t)wt_s[set][t] << 16);
-        bf16_t* const o = a.out + (int64_t)orow_s[set][t] * a.H + cur.nt * COLS + wn * 64 + q * 8;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          u32x4 y;
-#pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int j = 0; j < 4; j += 2)
-              y[2 * c + j / 2] = pk_bf16(acc[i][2 * h + c][j] * wt, acc[i][2 * h + c][j + 1] * wt);
-          *(u32x4*)(o + 32 * h) = y;
-        }
-      }
-    }
+    else loop(std::integral_constant<int, MI / 2>{});
+    mx_epilogue<MODE, true, WM, TM>(a, cur, tab, set, acc, wm, wn, lane);
     cur = next;
   }
+  wait_cnt<0>();   // no load may write this workgroup's LDS after its end
 }
 
 int device_cus(int* cus) {
@@ -690,8 +811,11 @@ int device_cus(int* cus) {
   return 0;
 }
 
-// The launches of one list in one kind of activations; tiles: row tiles of 256 rows of the experts with more
-// than kSmallRows rows (an upper bound).
+template <bool Q>
+constexpr int kTileRows = Q ? 256 : 128;
+
+// The launches of one list in one kind of activations; tiles: row tiles of kTileRows rows of the experts with
+// more than kSmallRows rows (an upper bound).
 template <bool Q>
 int launch_list(const MxArgs& a, bool small, int64_t tiles, int32_t phases, int64_t cus, hipStream_t s) {
   for (int mode = 0; mode < 2; ++mode) {
@@ -699,9 +823,12 @@ int launch_list(const MxArgs& a, bool small, int64_t tiles, int32_t phases, int6
     if (small)
       if (const int rc = mode == 0 ? small_launch<0, Q, Q ? 4 : 2>(a, s) : small_launch<1, Q, 4>(a, s)) return rc;
     if (tiles) {
-      const int64_t t = tiles * (mode == 0 ? a.I / 128 : a.H / 256);
-      launch(mode == 0 ? "mx_tiled_up" : "mx_tiled_down", mode == 0 ? mx_tiled<0, Q, 2, 4, 8> : mx_tiled<1, Q, 2, 4, 8>,
-             dim3((unsigned)(t < cus ? t : cus)), dim3(512), 0, s, a);
+      const int64_t t = tiles * (mode == 0 ? a.I / kOutCols<0> : a.H / kOutCols<1>), most = Q ? cus : 2 * cus;
+      const dim3 grid((unsigned)(t < most ? t : most));
+      if constexpr (Q)
+        launch(mode == 0 ? "mx_tiled_up" : "mx_tiled_down", mode == 0 ? mx_tiled4<0> : mx_tiled4<1>, grid, dim3(512), 0, s, a);
+      else
+        launch(mode == 0 ? "mx_tiled_up" : "mx_tiled_down", mode == 0 ? mx_tiled16<0> : mx_tiled16<1>, grid, dim3(256), 0, s, a);
       FERRY_LAUNCHED("mx_tiled");
     }
   }
@@ -740,6 +867,8 @@ extern "C" int ferry_mxfp4_expert_ffn(const void* cache, int64_t cache_rows, int
   // the kernels address activations with 32-bit byte offsets
   FERRY_CHECK_ARG(rows_in < ((int64_t)1 << 31) / hidden && rows_in * topk < ((int64_t)1 << 31) / inter,
                   "x / act must hold fewer than 2^31 elements");
+  // and scales with 32-bit ones from a matrix of the expert's cache row
+  FERRY_CHECK_ARG(hidden * inter < ((int64_t)1 << 32), "hidden * intermediate must be under 2^32");
   if (n_list == 0 || rows_in == 0) return 0;
   FERRY_CHECK_ARG(cache && x && w_sorted && starts && rows && cols && expert_list && slot_of && act && out,
                   "null pointer argument");
@@ -760,7 +889,7 @@ extern "C" int ferry_mxfp4_expert_ffn(const void* cache, int64_t cache_rows, int
   if (const int rc = device_cus(&cus)) return rc;
   if (cus > 2 * spare_cus) cus -= spare_cus;
   const bool quantised = x_scales != nullptr;
-  const int64_t pairs = rows_in * topk;
+  const int64_t pairs = rows_in * topk, tile_rows = quantised ? kTileRows<true> : kTileRows<false>;
   MxArgs a;
   a.cache = (const uint8_t*)cache;
   a.x = (const uint8_t*)x;
@@ -775,6 +904,7 @@ extern "C" int ferry_mxfp4_expert_ffn(const void* cache, int64_t cache_rows, int
   a.H = hidden;
   a.I = inter;
   a.k = topk;
+  a.pairs = pairs;
   a.out_mode = out_mode;
   a.known = list_rows != nullptr;
   a.list.n_mid = 0;
@@ -786,8 +916,9 @@ extern "C" int ferry_mxfp4_expert_ffn(const void* cache, int64_t cache_rows, int
     a.list.n = 0;
     auto flush = [&]() {
       if (a.list.n == 0) return 0;
-      // row counts unknown: sum ceil(n / 256) <= pairs / 256 + the experts with more than kSmallRows rows
-      if (big && !list_rows) tiles = pairs / 256 + (a.list.n < pairs / (kSmallRows + 1) + 1 ? a.list.n : pairs / (kSmallRows + 1) + 1);
+      // row counts unknown: sum ceil(n / rows) <= pairs / rows + the experts with more than kSmallRows rows
+      if (big && !list_rows)
+        tiles = pairs / tile_rows + (a.list.n < pairs / (kSmallRows + 1) + 1 ? a.list.n : pairs / (kSmallRows + 1) + 1);
       const int rc = quantised ? launch_list<true>(a, !big, tiles, phases, cus, (hipStream_t)stream)
                                : launch_list<false>(a, !big, tiles, phases, cus, (hipStream_t)stream);
       a.list.n = 0;
@@ -797,7 +928,7 @@ extern "C" int ferry_mxfp4_expert_ffn(const void* cache, int64_t cache_rows, int
     for (int32_t i = 0; i < n_list; ++i) {
       if (list_rows) {
         if (list_rows[i] < 1 || (list_rows[i] > kSmallRows) != (big != 0)) continue;
-        if (big) tiles += ceil_div(list_rows[i], 256);
+        if (big) tiles += ceil_div(list_rows[i], tile_rows);
       }
       a.list.expert[a.list.n] = (int16_t)expert_list[i];
       a.list.slot[a.list.n++] = slot_of[expert_list[i]];

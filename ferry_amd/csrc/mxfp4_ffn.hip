@@ -36,9 +36,9 @@ struct MxArgs {
   const int64_t* rows;      // [R*k]
   const int64_t* cols;      // [R*k]
   uint8_t* act;             // bf16 [R*k, I], or codes [R*k, I / 2]
-  uint8_t* act_scales;      // [I / 128, R*k, 4] (Q): 128 columns' bytes of the rows together
+  uint8_t* act_scales;      // [R*k, I / 32] (Q)
   bf16_t* out;              // [R*k, H]
-  int64_t H, I, k, pairs;
+  int64_t H, I, k;
   int32_t out_mode;
   int32_t known;            // the listed experts' row counts were given
   ExpertList list;
@@ -169,8 +169,7 @@ __global__ __launch_bounds__(256) void mx_small(MxArgs a) {
   const uint8_t* xp = MODE == 0 ? a.x : a.act;
   const uint8_t* xs = MODE == 0 ? a.x_scales : a.act_scales;
   xp += Q ? src * (K / 2) + q * 16 : src * K * 2 + q * 64;
-  const int64_t xstep = MODE == 0 ? 4 : a.pairs * 4;
-  if (Q) xs += (MODE == 0 ? src * (K / 32) : src * 4) + q;
+  if (Q) xs += src * (K / 32) + q;
   floatx4 acc[NF];
 #pragma unroll
   for (int f = 0; f < NF; ++f) acc[f] = floatx4{0, 0, 0, 0};
@@ -191,7 +190,7 @@ __global__ __launch_bounds__(256) void mx_small(MxArgs a) {
           if (u + b < u1 && c < chunks) {
 #pragma unroll
             for (int s = 0; s < XL; ++s) xv[b][j][s] = *(const u32x4*)(xp + (int64_t)c * (Q ? 64 : 256) + s * 16);
-            if (Q) xb[b][j] = xs[c * xstep];
+            if (Q) xb[b][j] = xs[c * 4];
           }
         }
 #pragma unroll
@@ -253,7 +252,7 @@ __global__ __launch_bounds__(256) void mx_small(MxArgs a) {
         uint8_t* o = a.act + p * (a.I / 2) + bx * 16 + q * 2;
         *(uint16_t*)o = (uint16_t)c;
         *(uint16_t*)(o + 8) = (uint16_t)(c >> 16);
-        if (q == 0) a.act_scales[((bx / 4) * a.pairs + p) * 4 + bx % 4] = (uint8_t)byte;
+        if (q == 0) a.act_scales[p * (a.I / 32) + bx] = (uint8_t)byte;
       }
     } else {
       if (wave >= NF / 2) return;
@@ -298,9 +297,7 @@ int small_launch(const MxArgs& a, hipStream_t s) {
 // wavefront reads lie on 16 different 16-byte bank groups (any LDS read of up to 16 bytes a lane takes the
 // same 7 clocks).
 //
-// The barrier of a step along K stands before its last products, whose operands are in registers by then:
-// behind it the next step's first operands are read, and the loads of the freed buffers issued, between those
-// products.  The same goes on from tile to tile; the next tile's rows are looked up meanwhile.
+// The loads run on from tile to tile; the next tile's rows are looked up meanwhile.
 // Rows of a tile that hold no row of the expert are not loaded, in steps of a quarter, nor multiplied, from
 // half a tile on.
 //
@@ -388,7 +385,7 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxTile& t, co
         const uint32_t c = block_codes(v, byte);
         if (live) {
           *(uint32_t*)(a.act + (t.row0 + row) * (a.I / 2) + col / 2 + q * 4) = c;
-          if (q == 0) a.act_scales[((col / 128) * a.pairs + t.row0 + row) * 4 + (col / 32) % 4] = (uint8_t)byte;
+          if (q == 0) a.act_scales[(t.row0 + row) * (a.I / 32) + col / 32] = (uint8_t)byte;
         }
       } else if (live) {
         *(u32x4*)(a.act + ((t.row0 + row) * a.I + col + q * 8) * 2) =
@@ -420,7 +417,9 @@ __device__ __forceinline__ int first_tile() {
 
 // bf16 activations.  Four wavefronts share 128 rows; two such workgroups run on a CU, each in its own time, so
 // that one's barriers, epilogues and loads fall into the other's products.  A step is 64 along K: rows of 128
-// bytes, two buffers, the loads one step ahead; weights in pieces of 128 along K.
+// bytes, two buffers, the loads one step ahead; weights in pieces of 128 along K.  The barrier of a step stands before
+// its last products, whose operands are in registers by then: behind it the next step's first operands are read, and
+// the loads of the freed buffers issued, between those products.
 template <int MODE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void mx_tiled16(MxArgs a) {
   constexpr int NI = 4, W = 4, TM = 128, MI = 8, TN = kTileCols, COLS = kOutCols<MODE>;
@@ -589,15 +588,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 }
 
 // 4-bit activations.  Eight wavefronts in two rows share 256 rows.  A step is 256 along K: rows of 128 bytes of
-// activations and of weights, two buffers, the loads one step ahead.  A CU receives about 64 bytes a clock, in
-// lines of 128; the scales therefore come 16 bytes of a row, 512 along K, at a time, and a lane keeps those of
-// its rows' blocks in a register a tile, the present one in the low byte.
+// activations and of weights, whole cache lines (with lines of 64 bytes loaded up to three steps ahead, 90 us instead
+// of 70 at 32,768 rows x 2048 x 768 up: a CU receives about 64 bytes a clock, in lines of 128), two buffers,
+// the loads one step ahead.  Here the barrier stands at a step's end: before its last products, as above, it took
+// 69 to 78 us, with scales for two steps at a time 74.
 template <int MODE>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void mx_tiled4(MxArgs a) {
   constexpr int WM = 2, WN = 4, MI = 8, NI = 4, W = WM * WN, TM = 256, TN = kTileCols, COLS = kOutCols<MODE>;
   constexpr int kX = TM * 128, kW = TN * 128;            // bytes of a buffer
-  constexpr int LX = 4, LW = 4, LS = 4;                  // direct loads of a wavefront for one
-  constexpr int kS = (TN + TM) * 16;                     // scale bytes of two steps: weight rows, activation rows
+  constexpr int LX = 4, LW = 4;                          // direct loads of a wavefront for one
+  constexpr int kS = (TN + TM) * 8;                      // scale bytes of a step: weight rows, activation rows
   __shared__ TileTable tt;
   __shared__ __attribute__((aligned(1024))) char smem[2 * (kX + kW + kS)];
   __shared__ RowTables<MODE, TM> tab;
@@ -605,12 +605,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int64_t K = MODE == 0 ? a.H : a.I;
   const int ntn = (int)((MODE == 0 ? a.I : a.H) / COLS);
   const int total = __builtin_amdgcn_readfirstlane(tt.total) * ntn;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
   const int r = lane & 15, q = lane >> 4;
-  // steps; a tile takes at least two, so that the loads ahead stay within the next tile (what lies past the
-  // last 128 along K is not multiplied, and loads those again)
-  const int chunks = (int)(K / 128), steps = (chunks + 1) / 2, span = max(steps, 2);
+  const int chunks = (int)(K / 128), steps = (chunks + 1) / 2;
   const uint32_t smem0 = lds_addr(smem), wbuf = smem0 + 2 * kX, sbuf = wbuf + 2 * kW;
   const char* const xbase = reinterpret_cast<const char*>(MODE == 0 ? a.x : a.act);
   auto swz_x = [](int row) { return (row >> 1) & 7; };
@@ -619,14 +617,14 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int xrow = 16 * wm + r, wrow = (MODE == 0 ? wn * 32 : wn * 64) + 8 * (r >> 2) + (r & 3);
   const uint32_t xa = smem0 + (uint32_t)(xrow * 128 + ((q ^ swz_x(xrow)) << 4));
   const uint32_t wa = wbuf + (uint32_t)(wrow * 128 + ((q ^ swz_w(wrow)) << 4));
-  const uint32_t xsa = sbuf + (uint32_t)((TN + xrow) * 16), wsa = sbuf + (uint32_t)(wrow * 16);
+  const uint32_t xsa = sbuf + (uint32_t)((TN + xrow) * 8), wsa = sbuf + (uint32_t)(wrow * 8);
   constexpr int kXTile = 16 * WM * 128;
-  const uint32_t pick = (uint32_t)(q | (4 + q) << 8);   // byte q of two words
 
   // The tile whose steps are being loaded.  Load j of a wavefront moves 8 rows of 128 bytes in a row's order of
-  // slots; rows 64 j .. over all wavefronts.  A load of scales moves 16 bytes of 16 rows, four lanes a row.
-  uint32_t xoff[LX], woff, soff[LS];
-  const char *wbase[2], *sbase;   // MODE 0: gate rows (the first half of the loads), up rows
+  // slots; rows 64 j .. over all wavefronts.  A thread moves the scales of one row, a weight or activation row.
+  uint32_t xoff[LX], woff;
+  const char* wbase[2];   // MODE 0: gate rows (the first half of the loads), up rows
+  const uint8_t* sp = nullptr;
   int xloads = LX;
   auto aim = [&](const MxTile& t, int p) {
     const int l = fresh(lane);
@@ -645,45 +643,39 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     wbase[1] = reinterpret_cast<const char*>(uniform_ptr(m1.codes));
     const int v = 8 * wave + l / 8;   // load j: 64 j rows on, in the same order of slots
     woff = (uint32_t)v * (uint32_t)(K / 2) + (uint32_t)(((l & 7) ^ swz_w(v)) * 16);
-    if (wave < WN) {
-      sbase = reinterpret_cast<const char*>(uniform_ptr(wave < 2 ? m0.scales : m1.scales));
-#pragma unroll
-      for (int j = 0; j < LS; ++j) soff[j] = (uint32_t)(64 * (wave & 1) + 16 * j + l / 4) * (uint32_t)(K / 32);
+    if (wave < W / 2) {
+      sp = (wave < W / 4 ? m0.scales : m1.scales) + (int64_t)(64 * (wave & 1) + l) * (K / 32);
     } else {
-      sbase = reinterpret_cast<const char*>(MODE == 0 ? a.x_scales : a.act_scales);
-#pragma unroll
-      for (int j = 0; j < LS; ++j) {
-        const uint32_t row = src_row(64 * (wave - WN) + 16 * j + l / 4);
-        soff[j] = row * (MODE == 0 ? (uint32_t)(K / 32) : 4u);
-      }
+      sp = (MODE == 0 ? a.x_scales : a.act_scales) + (int64_t)src_row(64 * (wave - W / 2) + l) * (K / 32);
     }
   };
   // Where the number of chunks is odd, the last step's rows end in its middle: the lanes of the second half
-  // read the first half again.
+  // read the first half again (it is not multiplied).
   auto tail = [&](int piece) { return (uint32_t)((piece & 4) << 4); };
   auto load_x = [&](int j, int n, int b) {   // load j of step n of the loaded tile into buffer b
     if (j >= xloads) return;
-    const int at = min(n, steps - 1);
     uint32_t off = xoff[j];
-    if (2 * at + 1 >= chunks) {
+    if (2 * n + 1 >= chunks) {
       const int l = fresh(lane);
       off -= tail((l & 7) ^ swz_x(8 * (W * j + wave) + l / 8));
     }
-    dma16(xbase + (int64_t)at * 128, off, smem0 + (uint32_t)(b * kX + (W * j + wave) * 1024));
+    dma16(xbase + (int64_t)n * 128, off, smem0 + (uint32_t)(b * kX + (W * j + wave) * 1024));
   };
   auto load_w = [&](int j, int n, int b) {
-    const int at = min(n, steps - 1);
     uint32_t off = woff;
-    if (2 * at + 1 >= chunks) {
+    if (2 * n + 1 >= chunks) {
       const int l = fresh(lane);
       off -= tail((l & 7) ^ swz_w(8 * wave + l / 8));
     }
-    dma16(wbase[j >> 1] + (j & 1) * 32 * K + (int64_t)at * 128, off, wbuf + (uint32_t)(b * kW + (W * j + wave) * 1024));
+    dma16(wbase[j >> 1] + (j & 1) * 32 * K + (int64_t)n * 128, off, wbuf + (uint32_t)(b * kW + (W * j + wave) * 1024));
   };
-  auto load_s = [&](int j, int n, int b) {   // of steps n and n + 1
-    const int c = min(2 * n + (fresh(lane) & 3), chunks - 1);
-    const uint32_t per = MODE == 1 && wave >= WN ? (uint32_t)(a.pairs * 4) : 4u;
-    dma4(sbase, soff[j] + (uint32_t)c * per, sbuf + (uint32_t)(b * kS + (4 * wave + j) * 256));
+  u32x2 sv = {0, 0};
+  auto load_s = [&](int n) {
+    if (2 * n + 1 < chunks) __builtin_memcpy(&sv, sp + n * 8, 8);
+    else __builtin_memcpy(&sv, sp + n * 8, 4);
+  };
+  auto store_s = [&](int b) {
+    *reinterpret_cast<__attribute__((address_space(3))) u32x2*>((uintptr_t)(sbuf + (uint32_t)(b * kS + tid * 8))) = sv;
   };
 
   const int first = first_tile();
@@ -693,45 +685,17 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   wait_cnt<0>();
   wg_barrier();
   aim(cur, 0);
+  load_s(0);
 #pragma unroll
-  for (int n = 0; n < 2; ++n) {
+  for (int j = 0; j < LW; ++j) load_w(j, 0, 0);
 #pragma unroll
-    for (int j = 0; j < LX; ++j) load_x(j, n, n);
-#pragma unroll
-    for (int j = 0; j < LW; ++j) load_w(j, n, n);
-  }
-#pragma unroll
-  for (int j = 0; j < LS; ++j) load_s(j, 0, 0);
+  for (int j = 0; j < LX; ++j) load_x(j, 0, 0);
+  store_s(0);
   wait_cnt<0>();
   wg_barrier();
-
-  // read ahead: the next chunk's weights and first four fragments; the scale bytes of the weight tiles and the
-  // activation tiles
-  u32x4 wf[2][NI], xf[2][4];
-  uint32_t ws[NI], xs[MI];
-  int xb = 0, sb = 0;   // buffers of the present step, of its scales
-  auto read = [&](int to, int j, int b) {   // chunk j of the step in buffer b
-    const uint32_t at = (wa + (uint32_t)(b * kW)) ^ (uint32_t)(j << 6), xat = (xa + (uint32_t)(b * kX)) ^ (uint32_t)(j << 6);
-#pragma unroll
-    for (int f = 0; f < NI; ++f) wf[to][f] = lds_get<lds_u32x4>(at + (uint32_t)(wtile<MODE>(f) * 128));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) xf[to][i] = lds_get<lds_u32x4>(xat + (uint32_t)(kXTile * i));
-  };
-  auto read_s = [&](int b) {   // four chunks' words of each row -> its bytes q
-    auto bytes = [&](uint32_t at) {
-      const u32x4 v = lds_get<lds_u32x4>(at + (uint32_t)(b * kS));
-      const uint32_t lo = __builtin_amdgcn_perm(v[1], v[0], pick), hi = __builtin_amdgcn_perm(v[3], v[2], pick);
-      return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
-    };
-#pragma unroll
-    for (int f = 0; f < NI; ++f) ws[f] = bytes(wsa + (uint32_t)(wtile<MODE>(f) * 16));
-#pragma unroll
-    for (int i = 0; i < MI; ++i) xs[i] = bytes(xsa + (uint32_t)(16 * WM * 16 * i));
-  };
-  read(0, 0, 0);
-  int set = 0;   // set of row tables
+  int set = 0, b = 0;   // set of row tables; buffer of the present step
   for (int tile = first; tile < total; tile += gridDim.x, set ^= 1) {
-    // the tile after this one; after the last tile its own first steps are loaded again
+    // the tile after this one; after the last tile its own first step is loaded again
     const bool more = tile + (int)gridDim.x < total;
     const MxTile next = more ? mx_locate<TM>(a, tt, tile + gridDim.x, ntn) : cur;
     tab.load(a, next, set ^ 1, wave, lane);
@@ -744,59 +708,75 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     // ROWS: tiles of 16 rows of a wavefront that are multiplied; the others hold no row of the expert
     auto loop = [&](auto rows) {
       constexpr int ROWS = decltype(rows)::value;
-      for (int st = 0; st < span; ++st) {
-        if ((st & 1) == 0) read_s(sb);
-        // the step whose loads take the buffers that this one frees
-        const int ls = st + 2 < span ? st + 2 : st + 2 - span;
+      for (int st = 0; st < steps; ++st, b ^= 1) {
+        const uint32_t xb = xa + (uint32_t)(b * kX), wb = wa + (uint32_t)(b * kW);
+        const uint32_t xsb = xsa + (uint32_t)(b * kS), wsb = wsa + (uint32_t)(b * kS);
+        // fragments are read two ahead of their products
+        u32x4 xn[2], wf[NI];
+        uint32_t xsn[2], wsf[NI];
+        auto read_x = [&](int j, int i) {
+#pragma unroll
+          for (int v = 0; v < 2; ++v) {
+            xn[v] = lds_get<lds_u32x4>((xb ^ (uint32_t)(j << 6)) + (uint32_t)(kXTile * (i + v)));
+            xsn[v] = lds_get<lds_u32>(xsb + (uint32_t)(16 * WM * 8 * (i + v) + 4 * j));
+          }
+        };
+        auto read_w = [&](int j) {
+#pragma unroll
+          for (int f = 0; f < NI; ++f) {
+            wf[f] = lds_get<lds_u32x4>((wb ^ (uint32_t)(j << 6)) + (uint32_t)(wtile<MODE>(f) * 128));
+            wsf[f] = lds_get<lds_u32>(wsb + (uint32_t)(wtile<MODE>(f) * 8 + 4 * j));
+          }
+        };
+        read_w(0);
+        read_x(0, 0);
+        const bool last = st + 1 == steps;
+        if (last) {   // the loads turn to the next tile
+          if (steps == 1) {   // its row indices may still be on their way
+            wait_cnt<0>();
+            wg_barrier();
+          }
+          aim(next, set ^ 1);
+        }
+        const int ls = last ? 0 : st + 1;
+        load_s(ls);
+#pragma unroll
+        for (int j = 0; j < LW; ++j) load_w(j, ls, b ^ 1);
+#pragma unroll
+        for (int j = 0; j < LX; ++j) load_x(j, ls, b ^ 1);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const bool there = 2 * st + j < chunks;
-          u32x4 xg[ROWS > 4 ? ROWS - 4 : 1];   // the fragments from the fifth on
-          const uint32_t xat = (xa + (uint32_t)(xb * kX)) ^ (uint32_t)(j << 6);
+          if (j == 1 && 2 * st + 1 >= chunks) break;
+          u32x4 cw[NI];
+          int cs[NI];
 #pragma unroll
-          for (int i = 4; i < ROWS; ++i) xg[i - 4] = lds_get<lds_u32x4>(xat + (uint32_t)(kXTile * i));
-          auto multiply = [&](int i) {
+          for (int f = 0; f < NI; ++f) cw[f] = wf[f], cs[f] = (int)(wsf[f] >> (8 * q));
 #pragma unroll
-            for (int f = 0; f < NI; ++f)
-              acc[i][f] = mma_fp4(wf[j][f], (int)ws[f], i < 4 ? xf[j][i] : xg[i < 4 ? 0 : i - 4], (int)xs[i], acc[i][f]);
-            __builtin_amdgcn_sched_barrier(0);
-          };
-          if (there)
+          for (int i = 0; i < ROWS; i += 2) {
+            const u32x4 x0 = xn[0], x1 = xn[1];
+            const int s0 = (int)(xsn[0] >> (8 * q)), s1 = (int)(xsn[1] >> (8 * q));
+            if (i + 2 < ROWS) {
+              read_x(j, i + 2);
+            } else if (j == 0) {
+              read_x(1, 0);
+              read_w(1);
+            }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) multiply(i);
-          if (j == 0) {
-            read(1, 1, xb);
-          } else {
-            wait_cnt<0>();   // the next step's loads have landed, this one's fragments are read
-            wg_barrier();
-            if (st == span - 2) aim(next, set ^ 1);
-            read(0, 0, xb ^ 1);
-          }
-          // the loads of the buffers that are free now, between the last products
-          auto loads = [&](int k) {
-            if (j == 0) return;
-            load_x(k, ls, xb);
-            load_w(k, ls, xb);
-            if ((ls & 1) == 0) load_s(k, ls, (st & 1) ? sb : sb ^ 1);   // not the next step's scales
-          };
+            for (int f = 0; f < NI; ++f) acc[i][f] = mma_fp4(cw[f], cs[f], x0, s0, acc[i][f]);
 #pragma unroll
-          for (int i = 4; i < 8; ++i) {
-            if (i < ROWS && there) multiply(i);
-            loads(i - 4);
+            for (int f = 0; f < NI; ++f) acc[i + 1][f] = mma_fp4(cw[f], cs[f], x1, s1, acc[i + 1][f]);
             __builtin_amdgcn_sched_barrier(0);
           }
-#pragma unroll
-          for (int f = 0; f < NI; ++f) ws[f] >>= 8;
-#pragma unroll
-          for (int i = 0; i < ROWS; ++i) xs[i] >>= 8;
         }
-        xb ^= 1;
-        if ((st & 1) == 1 || st == span - 1) sb ^= 1;
+        store_s(b ^ 1);
+        wait_cnt<0>();   // the next step's loads have landed, this one's fragments are read
+        wg_barrier();
       }
     };
     if (cur.vrows > TM / 4 * 3) loop(std::integral_constant<int, MI>{});
     else if (cur.vrows > TM / 2) loop(std::integral_constant<int, MI / 4 * 3>{});
-    else loop(std::integral_constant<int, MI / 2>{});
+    else if (cur.vrows > TM / 4) loop(std::integral_constant<int, MI / 2>{});
+    else loop(std::integral_constant<int, MI / 4>{});
     mx_epilogue<MODE, true, WM, TM>(a, cur, tab, set, acc, wm, wn, lane);
     cur = next;
   }
@@ -904,7 +884,6 @@ extern "C" int ferry_mxfp4_expert_ffn(const void* cache, int64_t cache_rows, int
   a.H = hidden;
   a.I = inter;
   a.k = topk;
-  a.pairs = pairs;
   a.out_mode = out_mode;
   a.known = list_rows != nullptr;
   a.list.n_mid = 0;

@@ -52,10 +52,11 @@ def check(logits, k, scoring='softmax', bias=None, groups=1, topk_groups=None, g
     np.testing.assert_array_equal(ids.cpu().numpy(), want)
     got = w.double().cpu().numpy()
     # one rounding to bf16 (half a step: 2^-9 of the next power of two, 2^-8 relative at most) of a value
-    # that is 64-bit but for a rounding to fp32 before it (2^-24)
+    # that is 64-bit but for a rounding to fp32 before it (2^-24); below the least normal 2^-126 the steps are
+    # 2^-133 and 2^-149, whatever the value
     np.testing.assert_array_equal(np.isnan(got), np.isnan(ws))
     fine = ~np.isnan(ws)
-    assert (np.abs(got - ws)[fine] <= (2 ** -8 + 2 ** -23) * np.abs(ws[fine])).all()
+    assert (np.abs(got - ws)[fine] <= (2 ** -8 + 2 ** -23) * np.abs(ws[fine]) + 2.0 ** -134 + 2.0 ** -150).all()
     return w, ids
 
 
@@ -132,6 +133,54 @@ def test_masked_and_special_logits(device, scoring, groups):
         assert all(len(set(r)) == k for r in ids.tolist()) and (ids >= 0).all() and (ids < E).all()
     w, _ = check(x[:1], k, scoring, None, groups, tg)
     assert (w == 0).all()
+
+
+# more tokens than the library gives a wavefront each: four to a wavefront, fp32 scores where they decide
+BATCH_GATES = [(1, 1, 1, 1), (6, 3, 3, 2), (64, 6, 1, 1), (65, 8, 5, 2), (128, 8, 1, 1), (160, 6, 8, 3),
+               (256, 8, 8, 4), (252, 7, 4, 4), (256, 16, 128, 9), (129, 4, 3, 1), (256, 17, 1, 1)]
+
+
+@pytest.mark.parametrize('E,k,G,TG', BATCH_GATES)
+@pytest.mark.parametrize('scoring', ['softmax', 'sigmoid'])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_gates_on_batches(device, E, k, G, TG, scoring, dtype):
+    logits = randn((2051, E), 5, dtype)
+    logits[100:200] = logits[100:200].round()   # ties
+    logits[200:210] = 0.5                       # nothing but ties
+    bias = randn((E,), 6, scale=0.2)
+    score = 'top2' if E // G >= 2 else 'max'
+    check(logits, k, scoring, bias, G, TG, score, True, 2.5)
+    check(logits, k, scoring, None, G, TG, 'max', False, 16.0)
+
+
+@pytest.mark.parametrize('scoring', ['softmax', 'sigmoid'])
+@pytest.mark.parametrize('E,k,G,TG', [(64, 6, 1, 1), (256, 8, 8, 4)])
+def test_special_batches(device, E, k, G, TG, scoring):
+    logits = randn((2400, E), 7)
+    inf, nan = float('inf'), float('nan')
+    logits[0:50, 3:] = -inf            # three experts left, then none
+    logits[50:60] = -inf
+    logits[60:100, ::5] = -inf
+    logits[100:120, 7] = nan
+    logits[120:140, 9] = inf
+    logits[140:160, 2] = nan
+    logits[140:160, 40:] = -inf
+    logits[160:400] *= 40              # scores from next to 1 down to 2^-250
+    logits[400:600] -= 80
+    logits[600:800] *= 2.0 ** -18      # scores that fp32 cannot tell apart, in part
+    logits[800:1000] = 10 + logits[800:1000] * 2.0 ** -16
+    check(logits, k, scoring, None, G, TG, 'max')
+    check(logits, k, scoring, None, G, TG, 'top2', False)
+    bias = randn((E,), 8, scale=0.01)
+    check(logits, k, scoring, bias, G, TG, 'top2')
+    # choice scores far below the scores' own size, or far above it
+    check(logits, k, scoring, -torch.ones(E, device='cuda'), G, TG, 'top2')
+    bias[::2] += 1000
+    bias[1::4] -= 1000
+    check(logits, k, scoring, bias, G, TG, 'top2')
+    bias[5], bias[6], bias[7] = inf, -inf, nan
+    check(logits, k, scoring, bias, G, TG, 'top2')
+    check(logits, k, scoring, bias, G, TG, 'max')
 
 
 def test_empty_and_large_batches(device):

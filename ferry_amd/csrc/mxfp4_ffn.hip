@@ -833,7 +833,16 @@ extern "C" int ferry_mxfp4_expert_ffn(const void* cache, int64_t cache_rows, int
   FERRY_CHECK_ARG(hidden > 0 && hidden % 128 == 0, "hidden must be a positive multiple of 128");
   FERRY_CHECK_ARG(inter > 0 && inter % 128 == 0, "intermediate must be a positive multiple of 128");
   FERRY_CHECK_ARG(hidden <= 1 << 20 && inter <= 1 << 20, "hidden and intermediate must be at most 2^20");
-  FERRY_CHECK_ARG(topk >= 1 && rows_in >= 0 && n_list >= 0 && max_rows_per_expert >= 0, "bad sizes");
+  FERRY_CHECK_ARG(topk >= 1 && rows_in >= 0 && n_list >= 0, "bad sizes");
+  if (list_rows && max_rows_per_expert == -1) {
+    max_rows_per_expert = 0;
+    min_rows_per_expert = n_list ? list_rows[0] : 0;
+    for (int32_t i = 0; i < n_list; ++i) {
+      if (list_rows[i] > max_rows_per_expert) max_rows_per_expert = list_rows[i];
+      if (list_rows[i] < min_rows_per_expert) min_rows_per_expert = list_rows[i];
+    }
+  }
+  FERRY_CHECK_ARG(max_rows_per_expert >= 0, "bad sizes");
   FERRY_CHECK_ARG(min_rows_per_expert >= 0 && min_rows_per_expert <= max_rows_per_expert,
                   "min_rows_per_expert must be in [0, max_rows_per_expert]");
   FERRY_CHECK_ARG(experts >= 1 && experts <= FERRY_MAX_EXPERTS, "experts must be in [1, %d]",

@@ -173,7 +173,7 @@ def _native(t, what, fn, *args):
 
 
 def _on_device(t, name, like):
-    if not isinstance(t, torch.Tensor) or t.device != like.device:
+    if not isinstance(t, torch.Tensor) or t.get_device() != like.get_device():
         raise RuntimeError(f'{name} must be on {like.device}')
 
 
@@ -189,9 +189,8 @@ def _row_stride(t, name):
     return t.shape[-1]
 
 
-def _mxfp4_quantize(x, codes, ldc, scales, lds):
+def _mxfp4_quantize(x, stride, codes, ldc, scales, lds):
     cols = x.shape[-1]
-    stride = _row_stride(x, 'x')
     _native(x, 'mxfp4_quantize', lib().ferry_mxfp4_quantize, x.data_ptr(), _DTYPES[x.dtype],
             x.numel() // cols if cols else 0, cols, stride, codes, ldc, scales, lds)
 
@@ -208,11 +207,12 @@ def mxfp4_quantize(x):
         raise RuntimeError('x must be a tensor of rows')
     if x.dtype not in _DTYPES:
         raise RuntimeError('x must be bf16, fp32 or fp16')
-    blocks = -(-x.shape[-1] // 32)
-    _row_stride(x, 'x')
-    codes = torch.empty((*x.shape[:-1], blocks * 16), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((*x.shape[:-1], blocks), dtype=torch.uint8, device=x.device)
-    _mxfp4_quantize(x, codes.data_ptr(), blocks * 16, scales.data_ptr(), blocks)
+    *lead, cols = x.shape
+    blocks = -(-cols // 32)
+    stride, device = _row_stride(x, 'x'), x.device
+    codes = torch.empty((*lead, blocks * 16), dtype=torch.uint8, device=device)
+    scales = torch.empty((*lead, blocks), dtype=torch.uint8, device=device)
+    _mxfp4_quantize(x, stride, codes.data_ptr(), blocks * 16, scales.data_ptr(), blocks)
     return codes, scales
 
 
@@ -248,7 +248,7 @@ def mxfp4_expert_rows(rows, out=None):
     n, elements = rows.shape
     if elements % 128:
         raise RuntimeError('a row must hold a multiple of 128 elements')
-    _row_stride(rows, 'rows')
+    stride = _row_stride(rows, 'rows')
     width = elements // 32 * 17
     if out is None:
         out = torch.empty((n, width), dtype=torch.uint8, device=rows.device)
@@ -256,7 +256,7 @@ def mxfp4_expert_rows(rows, out=None):
         raise RuntimeError(f'out must be uint8 [{n}, {width}]')
     at = _dev(out, 'out', torch.uint8)
     _on_device(out, 'out', rows)
-    _mxfp4_quantize(rows, at, width, at + elements // 2, width)
+    _mxfp4_quantize(rows, stride, at, width, at + elements // 2, width)
     return out
 
 
@@ -448,8 +448,6 @@ def mxfp4_expert_ffn(cache, x, w_sorted, starts, rows, cols, expert_list, slot_o
     E = int(experts if experts is not None else len(so))
     if E > len(so) or (counts is not None and E > len(counts)):
         raise RuntimeError('slot_of and counts must have an entry for every expert')
-    if len(el) and not 0 <= int(el.min()) <= int(el.max()) < E:
-        raise RuntimeError(f'expert_list must name experts in [0, {E})')
     idx = [v if isinstance(v, int) else _dev(v, name, torch.int64) for v, name in ((rows, 'rows'), (cols, 'cols'))]
     weights, first = _dev(w_sorted, 'w_sorted', torch.bfloat16), _dev(starts, 'starts', torch.int64)
     if starts.numel() < E + 1:
@@ -462,16 +460,16 @@ def mxfp4_expert_ffn(cache, x, w_sorted, starts, rows, cols, expert_list, slot_o
                     (cols, 'cols'), (act, 'act'), (out, 'out')):
         if isinstance(t, torch.Tensor):
             _on_device(t, name, cache)
-    list_rows, most, least = None, int(max_rows if max_rows is not None else R), 0
+    list_rows, most = None, int(max_rows if max_rows is not None else R)
     if isinstance(rows, torch.Tensor) and not rows.numel():
         return out   # no pairs
-    if counts is not None:
-        c = np.ascontiguousarray(np.asarray(counts, dtype=np.int64)[el], dtype=np.int32)
-        if not len(c):
-            return out
-        list_rows, most, least = c.tobytes(), int(c.max()), int(c.min())
+    if counts is not None and len(el):
+        try:
+            list_rows, most = np.asarray(counts)[el].astype(np.int32).tobytes(), -1
+        except IndexError:
+            raise RuntimeError(f'expert_list must name experts in [0, {E})') from None
     _native(cache, 'mxfp4_expert_ffn', lib().ferry_mxfp4_expert_ffn, at[0], cache.shape[0], H, I, at[1], at[2],
-            R, k, weights, first, idx[0], idx[1], el.tobytes(), len(el), so.tobytes(), E, most, least,
+            R, k, weights, first, idx[0], idx[1], el.tobytes(), len(el), so.tobytes(), E, most, 0,
             list_rows, act_at, out_at, int(out_mode), int(phases), int(spare_cus))
     return out
 

@@ -214,7 +214,8 @@ int ferry_expert_ffn_spare(const void* cache, int64_t cache_rows, int64_t hidden
  * x_scales the scales [R, H / 32] of MXFP4 rows, and act is R * k * I / 32 * 17 bytes: the codes
  * [R * k, I / 2] and then the scales [R * k, I / 32] of silu(g) * u, quantised from fp32.  The sums and
  * the SwiGLU are fp32 and an output is rounded once, after its routing weight.  All other arguments as
- * ferry_expert_ffn_spare's; experts with at most 16 rows run the bandwidth-bound kernels.  Output rows of
+ * ferry_expert_ffn_spare's, but that with list_rows max_rows_per_expert = -1 takes the most and the least rows
+ * from there; experts with at most 16 rows run the bandwidth-bound kernels.  Output rows of
  * experts that are not listed stay as they were.  hidden and intermediate are multiples of 128,
  * hidden one of 256 when an expert has more than 16 rows; cache, x, act and out 16-byte aligned.
  */

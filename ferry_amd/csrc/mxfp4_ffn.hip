@@ -17,6 +17,7 @@
 // weights go from the plain row-major rows straight to registers, with no LDS, shuffle or repacking.
 #include "ffn_common.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace ferry {
@@ -408,11 +409,17 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxTile& t, co
   }
 }
 
-// XCD-aware order: workgroup b runs on XCD b % 8, whose workgroups take a contiguous run of tiles; tiles of one
-// expert follow each other, columns fastest, and share their rows and weights in that XCD's L2.
-__device__ __forceinline__ int first_tile() {
-  const int per_xcd = gridDim.x % 8 == 0 ? (int)gridDim.x / 8 : 0;
-  return per_xcd ? (int)(blockIdx.x % 8) * per_xcd + (int)(blockIdx.x / 8) : (int)blockIdx.x;
+// A workgroup's tile of a round, `total` if it has none.  Workgroup b runs on XCD b % 8, whose workgroups take a run of
+// tiles: tiles of one expert follow each other, columns fastest, and share their rows and weights in that XCD's
+// L2.  What is left for a last round is spread over the XCDs, so that no CU has two tiles of it where another
+// has none (777 tokens, top 6 of 64 experts of 2048 x 1408, up: 72 us; with the rest on the first XCDs 89).
+__device__ __forceinline__ int tile_of(int round, int total) {
+  const int g = (int)gridDim.x, x = (int)(blockIdx.x % 8), j = (int)(blockIdx.x / 8);   // g: a multiple of 8
+  const int left = total - round * g;
+  if (left >= g) return round * g + x * (g / 8) + j;
+  if (left <= 0) return total;
+  const int from = left * x / 8, to = left * (x + 1) / 8;
+  return j < to - from ? round * g + from + j : total;
 }
 
 // bf16 activations.  Four wavefronts share 128 rows; two such workgroups run on a CU, each in its own time, so
@@ -481,9 +488,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   };
   auto load_s = [&](int c, int b) { dma4(sbase + (int64_t)c * 4, soff, sbuf + (uint32_t)(b * kS + wn * 256)); };
 
-  const int first = first_tile();
-  if (first >= total) return;
-  MxTile cur = mx_locate<TM>(a, tt, first, ntn);
+  int tile = tile_of(0, total);
+  if (tile >= total) return;
+  MxTile cur = mx_locate<TM>(a, tt, tile, ntn);
   tab.load(a, cur, 0, wn, lane);
   wait_cnt<0>();
   wg_barrier();
@@ -512,10 +519,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
   for (int i = 0; i < 4; ++i) read_x(i, 0, i, 0);
   int set = 0, wb = 0;   // set of row tables; buffer of the present weights
-  for (int tile = first; tile < total; tile += gridDim.x, set ^= 1) {
+  for (int round = 1, later; tile < total; tile = later, ++round, set ^= 1) {
     // the tile after this one; after the last tile its own first steps are loaded again
-    const bool more = tile + (int)gridDim.x < total;
-    const MxTile next = more ? mx_locate<TM>(a, tt, tile + gridDim.x, ntn) : cur;
+    later = tile_of(round, total);
+    const MxTile next = later < total ? mx_locate<TM>(a, tt, later, ntn) : cur;
     tab.load(a, next, set ^ 1, wn, lane);
     tab.outputs(a, cur, set, wn, lane);
     floatx4 acc[MI][NI];
@@ -678,9 +685,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     *reinterpret_cast<__attribute__((address_space(3))) u32x2*>((uintptr_t)(sbuf + (uint32_t)(b * kS + tid * 8))) = sv;
   };
 
-  const int first = first_tile();
-  if (first >= total) return;
-  MxTile cur = mx_locate<TM>(a, tt, first, ntn);
+  int tile = tile_of(0, total);
+  if (tile >= total) return;
+  MxTile cur = mx_locate<TM>(a, tt, tile, ntn);
   tab.load(a, cur, 0, wave, lane);
   wait_cnt<0>();
   wg_barrier();
@@ -694,10 +701,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   wait_cnt<0>();
   wg_barrier();
   int set = 0, b = 0;   // set of row tables; buffer of the present step
-  for (int tile = first; tile < total; tile += gridDim.x, set ^= 1) {
+  for (int round = 1, later; tile < total; tile = later, ++round, set ^= 1) {
     // the tile after this one; after the last tile its own first step is loaded again
-    const bool more = tile + (int)gridDim.x < total;
-    const MxTile next = more ? mx_locate<TM>(a, tt, tile + gridDim.x, ntn) : cur;
+    later = tile_of(round, total);
+    const MxTile next = later < total ? mx_locate<TM>(a, tt, later, ntn) : cur;
     tab.load(a, next, set ^ 1, wave, lane);
     tab.outputs(a, cur, set, wave, lane);
     floatx4 acc[MI][NI];
@@ -804,7 +811,7 @@ int launch_list(const MxArgs& a, bool small, int64_t tiles, int32_t phases, int6
       if (const int rc = mode == 0 ? small_launch<0, Q, Q ? 4 : 2>(a, s) : small_launch<1, Q, 4>(a, s)) return rc;
     if (tiles) {
       const int64_t t = tiles * (mode == 0 ? a.I / kOutCols<0> : a.H / kOutCols<1>), most = Q ? cus : 2 * cus;
-      const dim3 grid((unsigned)(t < most ? t : most));
+      const dim3 grid((unsigned)(t < most ? ceil_div(t, 8) * 8 : most / 8 * 8));
       if constexpr (Q)
         launch(mode == 0 ? "mx_tiled_up" : "mx_tiled_down", mode == 0 ? mx_tiled4<0> : mx_tiled4<1>, grid, dim3(512), 0, s, a);
       else
@@ -896,14 +903,29 @@ extern "C" int ferry_mxfp4_expert_ffn(const void* cache, int64_t cache_rows, int
   a.out_mode = out_mode;
   a.known = list_rows != nullptr;
   a.list.n_mid = 0;
-  // one pass over the small experts, one over the others; without row counts every expert is in both, and
-  // the kernels pass over those of the other kind by the device's starts
+  // One pass over the small experts, one over the others; without row counts every expert is in both, and the
+  // kernels pass over those of the other kind by the device's starts.  An expert's own rows decide, so that its
+  // results do not depend on which experts are listed with it (the two kinds sum in different orders): with all
+  // experts in tiles wherever one has more than kSmallRows rows, 512 tokens (128 experts of 2048 x 768, top 8,
+  // Zipf 1.1) take 110 and 87 us (bf16 and 4-bit activations) instead of 122 and 92, 8,192 tokens 644 and 332
+  // instead of 653 and 341.
   for (int big = 0; big < 2; ++big) {
     if (big ? max_rows_per_expert <= kSmallRows : min_rows_per_expert > kSmallRows) continue;
     int64_t tiles = 0;
+    struct Entry {
+      int32_t rows, expert;
+    } entry[kListMax];
     a.list.n = 0;
     auto flush = [&]() {
       if (a.list.n == 0) return 0;
+      // the experts with most rows first: tiles of few rows, which take less time, fill the last round (65 us for the
+      // up phase above)
+      if (big && list_rows)
+        std::sort(entry, entry + a.list.n, [](const Entry& p, const Entry& q) { return p.rows > q.rows; });
+      for (int i = 0; i < a.list.n; ++i) {
+        a.list.expert[i] = (int16_t)entry[i].expert;
+        a.list.slot[i] = slot_of[entry[i].expert];
+      }
       // row counts unknown: sum ceil(n / rows) <= pairs / rows + the experts with more than kSmallRows rows
       if (big && !list_rows)
         tiles = pairs / tile_rows + (a.list.n < pairs / (kSmallRows + 1) + 1 ? a.list.n : pairs / (kSmallRows + 1) + 1);
@@ -918,8 +940,7 @@ extern "C" int ferry_mxfp4_expert_ffn(const void* cache, int64_t cache_rows, int
         if (list_rows[i] < 1 || (list_rows[i] > kSmallRows) != (big != 0)) continue;
         if (big) tiles += ceil_div(list_rows[i], tile_rows);
       }
-      a.list.expert[a.list.n] = (int16_t)expert_list[i];
-      a.list.slot[a.list.n++] = slot_of[expert_list[i]];
+      entry[a.list.n++] = {list_rows ? list_rows[i] : 0, expert_list[i]};
       if (a.list.n == kListMax)
         if (const int rc = flush()) return rc;
     }

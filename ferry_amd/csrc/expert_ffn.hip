@@ -1269,7 +1269,7 @@ __global__ __launch_bounds__(kTiledThreads) __attribute__((amdgpu_waves_per_eu(2
   __shared__ __attribute__((aligned(256))) int32_t row_s[2][BM], col_s[MODE == 1 ? 2 : 1][MODE == 1 ? BM : 1];
   __shared__ __attribute__((aligned(256))) int32_t orow_s[MODE == 1 ? 2 : 1][MODE == 1 ? BM : 1],
       wt_s[MODE == 1 ? 2 : 1][MODE == 1 ? BM : 1];
-  build_tile_table<BM, kSkinnyMax>(a, tt);
+  build_tile_table<kSkinnyMax>(a, tt, BM);
   const int64_t K = MODE == 0 ? a.H : a.I;
   const int ntn = MODE == 0 ? (int)(a.I / 128) : (int)(a.H / BN);
   const int total = __builtin_amdgcn_readfirstlane(tt.total) * ntn;
@@ -1607,7 +1607,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM
   __shared__ __attribute__((aligned(256))) int32_t row_s[MODE == 1 ? TM : 1], col_s[MODE == 1 ? TM : 1];
   __shared__ int32_t orow_s[MODE == 1 ? TM : 1];
   __shared__ float wt_s[MODE == 1 ? TM : 1];
-  build_tile_table<TM, kSkinnyMax>(a, tt);
+  build_tile_table<kSkinnyMax>(a, tt, TM);
   const int64_t K = MODE == 0 ? a.H : a.I;
   const int ntn = MODE == 0 ? (int)(a.I / (TN / 2)) : (int)(a.H / TN);
   const int total = tt.total * ntn;

@@ -118,10 +118,10 @@ struct TileTable {
   int32_t rows[kListMax];
 };
 
-// Wavefront 0 builds the cumulative counts of M tiles of ROWS rows of the listed experts with more than
+// Wavefront 0 builds the cumulative counts of M tiles of `rows` rows of the listed experts with more than
 // LEAST rows.
-template <int ROWS, int LEAST, typename Args>
-__device__ void build_tile_table(const Args& a, TileTable& tt) {
+template <int LEAST, typename Args>
+__device__ __forceinline__ void build_tile_table(const Args& a, TileTable& tt, uint32_t rows) {
   if (threadIdx.x < 64) {
     const int lane = threadIdx.x;
     int cnt[4];
@@ -134,7 +134,7 @@ __device__ void build_tile_table(const Args& a, TileTable& tt) {
         const int e = a.list.expert[li];
         const int64_t s0 = a.starts[e];
         const int64_t n = a.starts[e + 1] - s0;
-        c = n > LEAST ? (int)((n + ROWS - 1) / ROWS) : 0;
+        c = n > LEAST ? (int)(((uint32_t)n + rows - 1) / rows) : 0;
         tt.start[li] = s0;
         tt.rows[li] = (int32_t)n;
       }

@@ -41,6 +41,7 @@ struct MxArgs {
   bf16_t* out;              // [R*k, H]
   int64_t H, I, k;
   int32_t out_mode;
+  int32_t tile_rows;        // of the tiled kernels: at most theirs
   int32_t known;            // the listed experts' row counts were given
   ExpertList list;
 };
@@ -316,17 +317,16 @@ __device__ __forceinline__ constexpr int wtile(int f) {
 
 struct MxTile {
   int64_t row0;        // grouped row of the tile's first row
-  int vrows, nt, slot; // rows from there on (> 0), number of its columns' tile, cache slot
+  int vrows, nt, slot; // its rows (> 0), number of its columns' tile, cache slot
 };
-template <int TM>
 __device__ __forceinline__ MxTile mx_locate(const MxArgs& a, const TileTable& tt, int tile, int ntn) {
   MxTile t;
   const int mt = tile / ntn;
   t.nt = tile - mt * ntn;
   const int li = __builtin_amdgcn_readfirstlane(find_entry(tt, mt));
-  const int m0 = (mt - __builtin_amdgcn_readfirstlane(tt.cum[li])) * TM;
+  const int m0 = (mt - __builtin_amdgcn_readfirstlane(tt.cum[li])) * a.tile_rows;
   t.row0 = uniform64(tt.start[li]) + m0;
-  t.vrows = __builtin_amdgcn_readfirstlane(tt.rows[li]) - m0;
+  t.vrows = min(__builtin_amdgcn_readfirstlane(tt.rows[li]) - m0, a.tile_rows);
   t.slot = a.list.slot[li];
   return t;
 }
@@ -436,7 +436,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   __shared__ TileTable tt;
   __shared__ __attribute__((aligned(1024))) char smem[2 * (kX + kW + kS)];
   __shared__ RowTables<MODE, TM> tab;
-  build_tile_table<TM, kSmallRows>(a, tt);
+  build_tile_table<kSmallRows>(a, tt, (uint32_t)a.tile_rows);
   const int64_t K = MODE == 0 ? a.H : a.I;
   const int ntn = (int)((MODE == 0 ? a.I : a.H) / COLS);
   const int total = __builtin_amdgcn_readfirstlane(tt.total) * ntn;
@@ -490,18 +490,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 
   int tile = tile_of(0, total);
   if (tile >= total) return;
-  MxTile cur = mx_locate<TM>(a, tt, tile, ntn);
+  MxTile cur = mx_locate(a, tt, tile, ntn);
   tab.load(a, cur, 0, wn, lane);
-  wait_cnt<0>();
-  wg_barrier();
-  aim(cur, 0);
-#pragma unroll
-  for (int j = 0; j < LX; ++j) load_x(j, 0, 0), load_x(j, 1, 1);
-#pragma unroll
-  for (int j = 0; j < LW; ++j) load_w(j, 0, 0);
-  load_s(0, 0);
-  wait_cnt<0>();
-  wg_barrier();
 
   // read ahead: the next step's weights and scales, its first fragments
   u32x2 wr[NI];
@@ -515,21 +505,116 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     for (int f = 0; f < NI; ++f) wr[f] = lds_get<lds_u32x2>(at + (uint32_t)(wtile<MODE>(f) * RW));
     wsc = lds_get<lds_u32x4>(wsa + (uint32_t)(w * kS));
   };
-  read_w(0, 0);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) read_x(i, 0, i, 0);
   int set = 0, wb = 0;   // set of row tables; buffer of the present weights
+  bool primed = false;   // the tile's first steps are loaded, its first operands read
   for (int round = 1, later; tile < total; tile = later, ++round, set ^= 1) {
     // the tile after this one; after the last tile its own first steps are loaded again
     later = tile_of(round, total);
-    const MxTile next = later < total ? mx_locate<TM>(a, tt, later, ntn) : cur;
+    const MxTile next = later < total ? mx_locate(a, tt, later, ntn) : cur;
+    const bool few = cur.vrows <= TM / 2;
+    if (few || !primed) {
+      wait_cnt<0>();   // the tile's row table has landed; the buffers are free behind the barrier
+      wg_barrier();
+      aim(cur, set);
+      wb = 0;
+    }
     tab.load(a, next, set ^ 1, wn, lane);
     tab.outputs(a, cur, set, wn, lane);
+    if (!few && !primed) {
+#pragma unroll
+      for (int j = 0; j < LX; ++j) load_x(j, 0, 0), load_x(j, 1, 1);
+#pragma unroll
+      for (int j = 0; j < LW; ++j) load_w(j, 0, 0);
+      load_s(0, 0);
+      wait_cnt<0>();
+      wg_barrier();
+      read_w(0, 0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) read_x(i, 0, i, 0);
+    }
     floatx4 acc[MI][NI];
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
       for (int f = 0; f < NI; ++f) acc[i][f] = floatx4{0, 0, 0, 0};
+    // one of 32 along K of step h: half a weight tile's 8 elements a lane
+    u32x4 wv[2][NI];
+    auto decode = [&](int h, int s, int part) {
+      const int f = part >> 1, half = part & 1;
+      const float sc = scale_of(__builtin_amdgcn_ubfe(wsc[f], 16 * h + 8 * (q >> 1), 8));
+      const uint32_t v = wr[f][s];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const bf16x2 d = half ? (j ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, sc, 3)
+                                   : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, sc, 2))
+                              : (j ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, sc, 1)
+                                   : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, sc, 0));
+        wv[s][f][2 * half + j] = __builtin_bit_cast(uint32_t, d);
+      }
+    };
+    // Up to 64 rows: a tile of these waits for its loads, not for products.  The rows' buffers hold 128 along K of
+    // ROWS tiles, two halves, so that a barrier comes every 128 along K with the loads as far ahead: one
+    // tile of up to 32 rows takes 15 us for 2048 along K, with the loop below 22.
+    auto loop_few = [&](auto rows) {
+      constexpr int ROWS = decltype(rows)::value, XH = ROWS / 2;   // loads of a half
+      auto load = [&](int p, int c, int b) {                       // part p of 4 of 128 along K number c
+        if (p < 2 * XH)
+          dma16(xbase + (int64_t)(2 * c + p / XH) * 128, xoff[p % XH],
+                smem0 + (uint32_t)(b * kX + (p / XH) * (kX / 2) + (W * (p % XH) + wn) * 1024));
+        load_w(p, c, b);
+        if (p == 3) load_s(c, b);
+      };
+      auto read = [&](int to, int m, int h, int b) {   // fragment m of half h
+        xf[to] = lds_get<lds_u32x4>(((xa + (uint32_t)(b * kX + h * (kX / 2))) ^ (uint32_t)((m / ROWS) << 4)) +
+                                    (uint32_t)(kXTile * (m % ROWS)));
+      };
+#pragma unroll
+      for (int p = 0; p < 4; ++p) load(p, 0, 0);
+      if (chunks > 1)
+#pragma unroll
+        for (int p = 0; p < 4; ++p) load(p, 1, 1);
+      wait_cnt<0>();
+      wg_barrier();
+      read_w(0, 0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) read(i, i, 0, 0);
+      for (int c = 0; c < chunks; ++c) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int part = 0; part < 2 * NI; ++part) decode(h, 0, part);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int n = 0; n < 2 * ROWS; ++n) {
+            const int s = n / ROWS, i = n % ROWS, k = n - (2 * ROWS - 4);
+            if (s == 0)
+#pragma unroll
+              for (int part = i * 2 * NI / ROWS; part < (i + 1) * 2 * NI / ROWS; ++part) decode(h, 1, part);
+            if (n == ROWS) {   // the weights are decoded
+              if (h == 1) {
+                wait_cnt<0>();   // the next loads have landed, this buffer's fragments are read
+                wg_barrier();
+                wb ^= 1;
+              }
+              read_w(h ^ 1, wb);
+            }
+#pragma unroll
+            for (int f = 0; f < NI; ++f)
+              acc[i][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, wv[s][f]),
+                                                                 __builtin_bit_cast(bf16x8, xf[n & 3]), acc[i][f], 0, 0, 0);
+            if (k < 0) read(n & 3, n + 4, h, wb);
+            else if (h == 0 || n >= ROWS) read(n & 3, k, h ^ 1, wb);
+            if (h == 1 && n >= ROWS) {   // behind the barrier; with two tiles the reads of the first two, too
+              if (ROWS == 2) read(n - 2, k - 2, 0, wb);
+              if (c + 2 < chunks)
+#pragma unroll
+                for (int p = (n - ROWS) * 4 / ROWS; p < (n - ROWS + 1) * 4 / ROWS; ++p) load(p, c + 2, wb ^ 1);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+      }
+    };
     // ROWS: tiles of 16 rows that are multiplied; the others hold no row of the expert
     auto loop = [&](auto rows) {
       constexpr int ROWS = decltype(rows)::value;
@@ -537,22 +622,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           // the first 32 along K are decoded here, the second 32 between the products of the first
-          u32x4 wv[2][NI];
-          auto decode = [&](int s, int part) {   // half of a weight tile's 8 elements a lane
-            const int f = part >> 1, half = part & 1;
-            const float sc = scale_of(__builtin_amdgcn_ubfe(wsc[f], 16 * h + 8 * (q >> 1), 8));
-            const uint32_t v = wr[f][s];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const bf16x2 d = half ? (j ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, sc, 3)
-                                         : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, sc, 2))
-                                    : (j ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, sc, 1)
-                                         : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, sc, 0));
-              wv[s][f][2 * half + j] = __builtin_bit_cast(uint32_t, d);
-            }
-          };
-#pragma unroll
-          for (int part = 0; part < 2 * NI; ++part) decode(0, part);
+          for (int part = 0; part < 2 * NI; ++part) decode(h, 0, part);
           __builtin_amdgcn_sched_barrier(0);
           const bool last = c == chunks - 1;
 #pragma unroll
@@ -567,7 +638,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             }
             if (s == 0)
 #pragma unroll
-              for (int part = i * 2 * NI / ROWS; part < (i + 1) * 2 * NI / ROWS; ++part) decode(1, part);
+              for (int part = i * 2 * NI / ROWS; part < (i + 1) * 2 * NI / ROWS; ++part) decode(h, 1, part);
 #pragma unroll
             for (int f = 0; f < NI; ++f)
               acc[i][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, wv[s][f]),
@@ -587,7 +658,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     };
     if (cur.vrows > TM / 4 * 3) loop(std::integral_constant<int, MI>{});
     else if (cur.vrows > TM / 2) loop(std::integral_constant<int, MI / 4 * 3>{});
-    else loop(std::integral_constant<int, MI / 2>{});
+    else if (cur.vrows > TM / 4) loop_few(std::integral_constant<int, MI / 2>{});
+    else loop_few(std::integral_constant<int, MI / 4>{});
+    primed = !few;
     mx_epilogue<MODE, false, 1, TM>(a, cur, tab, set, acc, 0, wn, lane);
     cur = next;
   }
@@ -608,7 +681,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   __shared__ TileTable tt;
   __shared__ __attribute__((aligned(1024))) char smem[2 * (kX + kW + kS)];
   __shared__ RowTables<MODE, TM> tab;
-  build_tile_table<TM, kSmallRows>(a, tt);
+  build_tile_table<kSmallRows>(a, tt, (uint32_t)a.tile_rows);
   const int64_t K = MODE == 0 ? a.H : a.I;
   const int ntn = (int)((MODE == 0 ? a.I : a.H) / COLS);
   const int total = __builtin_amdgcn_readfirstlane(tt.total) * ntn;
@@ -687,7 +760,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 
   int tile = tile_of(0, total);
   if (tile >= total) return;
-  MxTile cur = mx_locate<TM>(a, tt, tile, ntn);
+  MxTile cur = mx_locate(a, tt, tile, ntn);
   tab.load(a, cur, 0, wave, lane);
   wait_cnt<0>();
   wg_barrier();
@@ -704,7 +777,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   for (int round = 1, later; tile < total; tile = later, ++round, set ^= 1) {
     // the tile after this one; after the last tile its own first step is loaded again
     later = tile_of(round, total);
-    const MxTile next = later < total ? mx_locate<TM>(a, tt, later, ntn) : cur;
+    const MxTile next = later < total ? mx_locate(a, tt, later, ntn) : cur;
     tab.load(a, next, set ^ 1, wave, lane);
     tab.outputs(a, cur, set, wave, lane);
     floatx4 acc[MI][NI];
@@ -801,17 +874,24 @@ int device_cus(int* cus) {
 template <bool Q>
 constexpr int kTileRows = Q ? 256 : 128;
 
-// The launches of one list in one kind of activations; tiles: row tiles of kTileRows rows of the experts with
-// more than kSmallRows rows (an upper bound).
+// The launches of one list in one kind of activations.  tiles: the row tiles of kTileRows, a half and a quarter of
+// that many rows of the experts with more than kSmallRows rows (upper bounds).  Halves where they all run at once and
+// quarters where each has a CU of its own: they read the weights more often, and the longest takes less time.  Up,
+// down and up with 4-bit activations, whole tiles against those (128 experts of 2048 x 768, top 8, Zipf 1.1): 100
+// tokens 30, 16 and 17 us against 17, 11 and 15, 200 tokens 31, 18 and 23 against 22, 14 and 17; quarters
+// two to a CU were slower than halves there (24 and 15 us).
 template <bool Q>
-int launch_list(const MxArgs& a, bool small, int64_t tiles, int32_t phases, int64_t cus, hipStream_t s) {
+int launch_list(MxArgs& a, bool small, const int64_t (&tiles)[3], int32_t phases, int64_t cus, hipStream_t s) {
   for (int mode = 0; mode < 2; ++mode) {
     if (!(phases & (1 << mode))) continue;
     if (small)
       if (const int rc = mode == 0 ? small_launch<0, Q, Q ? 4 : 2>(a, s) : small_launch<1, Q, 4>(a, s)) return rc;
-    if (tiles) {
-      const int64_t t = tiles * (mode == 0 ? a.I / kOutCols<0> : a.H / kOutCols<1>), most = Q ? cus : 2 * cus;
-      const dim3 grid((unsigned)(t < most ? ceil_div(t, 8) * 8 : most / 8 * 8));
+    if (tiles[0]) {
+      const int64_t most = (Q ? cus : 2 * cus) / 8 * 8, cols = mode == 0 ? a.I / kOutCols<0> : a.H / kOutCols<1>;
+      const int by = tiles[2] * cols <= cus ? 2 : tiles[1] * cols <= most ? 1 : 0;
+      a.tile_rows = kTileRows<Q> >> by;
+      const int64_t t = tiles[by] * cols;
+      const dim3 grid((unsigned)(t < most ? ceil_div(t, 8) * 8 : most));
       if constexpr (Q)
         launch(mode == 0 ? "mx_tiled_up" : "mx_tiled_down", mode == 0 ? mx_tiled4<0> : mx_tiled4<1>, grid, dim3(512), 0, s, a);
       else
@@ -911,7 +991,7 @@ extern "C" int ferry_mxfp4_expert_ffn(const void* cache, int64_t cache_rows, int
   // instead of 653 and 341.
   for (int big = 0; big < 2; ++big) {
     if (big ? max_rows_per_expert <= kSmallRows : min_rows_per_expert > kSmallRows) continue;
-    int64_t tiles = 0;
+    int64_t tiles[3] = {0, 0, 0};
     struct Entry {
       int32_t rows, expert;
     } entry[kListMax];
@@ -927,18 +1007,21 @@ extern "C" int ferry_mxfp4_expert_ffn(const void* cache, int64_t cache_rows, int
         a.list.slot[i] = slot_of[entry[i].expert];
       }
       // row counts unknown: sum ceil(n / rows) <= pairs / rows + the experts with more than kSmallRows rows
-      if (big && !list_rows)
-        tiles = pairs / tile_rows + (a.list.n < pairs / (kSmallRows + 1) + 1 ? a.list.n : pairs / (kSmallRows + 1) + 1);
+      if (big && !list_rows) {
+        const int64_t most = pairs / (kSmallRows + 1);
+        for (int by = 0; by < 3; ++by) tiles[by] = pairs / (tile_rows >> by) + (a.list.n < most ? a.list.n : most);
+      }
       const int rc = quantised ? launch_list<true>(a, !big, tiles, phases, cus, (hipStream_t)stream)
                                : launch_list<false>(a, !big, tiles, phases, cus, (hipStream_t)stream);
       a.list.n = 0;
-      tiles = 0;
+      tiles[0] = tiles[1] = tiles[2] = 0;
       return rc;
     };
     for (int32_t i = 0; i < n_list; ++i) {
       if (list_rows) {
         if (list_rows[i] < 1 || (list_rows[i] > kSmallRows) != (big != 0)) continue;
-        if (big) tiles += ceil_div(list_rows[i], tile_rows);
+        if (big)
+          for (int by = 0; by < 3; ++by) tiles[by] += ceil_div(list_rows[i], tile_rows >> by);
       }
       entry[a.list.n++] = {list_rows ? list_rows[i] : 0, expert_list[i]};
       if (a.list.n == kListMax)

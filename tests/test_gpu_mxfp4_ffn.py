@@ -169,6 +169,20 @@ def test_many_rows(device, H, I, counts, quantised):
 
 
 @pytest.mark.parametrize('quantised', QUANTISED)
+def test_more_tiles_than_workgroups(device, quantised):
+    """Whole tiles, several to a workgroup, with every count of rows that tiles are cut to; an expert by itself runs
+    in smaller ones and gives the same bits."""
+    c = Case([1380, 17, 720, 1224, 90, 1046, 562, 0, 276, 129, 3], 2048, 1024, seed=5)
+    whole = c.check(quantised)
+    out = torch.full_like(whole, 7.0)
+    for e in range(c.E):
+        c.run(quantised, [e], out=out)
+    assert torch.equal(out, whole)
+    assert torch.equal(c.run(quantised, spare_cus=100), whole)
+    assert torch.equal(c.run(quantised, counts=False), whole)
+
+
+@pytest.mark.parametrize('quantised', QUANTISED)
 def test_forms_of_a_call_give_the_same_bits(device, quantised):
     """Without row counts, phase by phase, on parts of the list, with spare CUs."""
     c = Case([3, 0, 70, 16, 17, 300, 1], 512, 256, seed=4)

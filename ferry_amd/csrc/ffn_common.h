@@ -22,7 +22,7 @@ struct ExpertList {
 };
 
 __device__ __forceinline__ float silu_mul(float g, float u) {
-  // silu(g) * u in fp32 on the bf16-rounded GEMM outputs: g * u / (1 + e^-g) with the
+  // silu(g) * u in fp32 on the up projections' results: g * u / (1 + e^-g) with the
   // hardware exp2 and reciprocal (relative error ~1e-6, far below the bf16 rounding that
   // follows); a large negative g gives e^-g = inf and a zero result, the exact formula's limit
   return g * u * __builtin_amdgcn_rcpf(1.0f + __expf(-g));

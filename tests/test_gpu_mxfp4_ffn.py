@@ -323,6 +323,46 @@ def test_gate_to_combine(device):
     assert err.max().item() < 3 * 2.0 ** -8
 
 
+@pytest.mark.parametrize('quantised', QUANTISED)
+def test_fetched_experts(device, quantised):
+    """MXFP4 rows in a pinned pool, fetched into fewer cache slots than experts while the resident ones run."""
+    from ferry_amd import expert_ops as ops
+    c = Case([5, 40, 0, 16, 200, 3, 30, 9], 256, 384, seed=8)
+    want = c.run(quantised, out_mode=0)
+    pool = torch.empty((c.E, c.cache.shape[1]), dtype=torch.uint8, pin_memory=True)
+    pool.copy_(c.cache[torch.from_numpy(c.slot_of.astype(np.int64)).cuda()])
+    cache = torch.zeros((5, c.cache.shape[1]), dtype=torch.uint8, device='cuda')
+    torch.cuda.synchronize()   # the engine's streams do not wait for this one's work on the cache
+    x = ops.mxfp4_quantize(c.x) if quantised else c.x
+    P = c.R * c.k
+    act = (torch.empty(P * (c.I // 32 * 17), dtype=torch.uint8, device='cuda') if quantised else
+           torch.empty((P, c.I), dtype=torch.bfloat16, device='cuda'))
+    out = torch.full((P, c.H), 7.0, dtype=torch.bfloat16, device='cuda')
+    eng = ops.H2DEngine(cache, pool)
+    slot_of = np.full(c.E, -1, np.int32)
+
+    def fetch(slots, experts):
+        eng.fetch(slots, experts)
+        slot_of[np.isin(slot_of, slots)] = -1
+        slot_of[experts] = slots
+
+    def run(experts):
+        eng.wait_stream(slot_of[experts])
+        ops.mxfp4_expert_ffn(cache, x, c.w, c.starts, c.rows, c.cols, experts, slot_of, c.H, c.I, act, out,
+                             counts=c.counts)
+        eng.mark_used(slot_of[experts])
+    fetch([0, 1, 2], [0, 1, 3])
+    fetch([3, 4], [4, 5])
+    run([0, 1, 3])
+    fetch([1, 2], [6, 7])
+    run([4, 5])
+    run([6, 7])
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    with pytest.raises(RuntimeError, match='not cached'):
+        ops.mxfp4_expert_ffn(cache, x, c.w, c.starts, c.rows, c.cols, [1], slot_of, c.H, c.I, act, out, counts=c.counts)
+
+
 def test_refusals(device):
     from ferry_amd import expert_ops as ops
     c = Case([3, 20], 256, 128, k=2)

@@ -184,6 +184,7 @@ __global__ __launch_bounds__(256) void mx_small(MxArgs a) {
 #pragma unroll
   for (int f = 0; f < NF; ++f) acc[f] = floatx4{0, 0, 0, 0};
   for (int u = u0; u < u1; u += kUnits) {
+    if (u > u0) wait_cnt<0>();   // the last units' operands are read
     if (u > u0 || !a.known)
 #pragma unroll
       for (int b = 0; b < kUnits; ++b)

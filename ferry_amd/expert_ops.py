@@ -181,6 +181,8 @@ def _row_stride(t, name):
     """Elements from one row of [rows, cols] to the next; the elements of a row follow each other."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise RuntimeError(f'{name} must be a CUDA tensor')
+    if not t.dim():
+        raise RuntimeError(f'{name} must hold rows')
     if t.dim() == 2 and (t.shape[1] <= 1 or t.stride(1) == 1) and (
             t.shape[0] <= 1 or t.stride(0) >= t.shape[1]):
         return t.stride(0) if t.shape[0] > 1 else t.shape[1]
@@ -203,13 +205,11 @@ def mxfp4_quantize(x):
     A block's scale is 2^(floor(log2(its largest magnitude)) - 2), elements round to the nearest of 0,
     0.5, 1, 1.5, 2, 3, 4, 6 (ties to the even code) and saturate at 6; a block with an infinity or a NaN
     reads back as NaN.  No counterpart in the reference, whose expert rows are bf16."""
-    if not isinstance(x, torch.Tensor) or x.dim() < 1:
-        raise RuntimeError('x must be a tensor of rows')
+    stride = _row_stride(x, 'x')
     if x.dtype not in _DTYPES:
         raise RuntimeError('x must be bf16, fp32 or fp16')
     *lead, cols = x.shape
-    blocks = -(-cols // 32)
-    stride, device = _row_stride(x, 'x'), x.device
+    blocks, device = -(-cols // 32), x.device
     codes = torch.empty((*lead, blocks * 16), dtype=torch.uint8, device=device)
     scales = torch.empty((*lead, blocks), dtype=torch.uint8, device=device)
     _mxfp4_quantize(x, stride, codes.data_ptr(), blocks * 16, scales.data_ptr(), blocks)

@@ -162,6 +162,23 @@ def test_long_row_and_many_rows(device):
         np.testing.assert_array_equal(s[r:r + 1].cpu().numpy(), want[1])
 
 
+@pytest.mark.parametrize('rows,cols', [(70001, 65536), (140001, 65536), (70001, 65530)])
+def test_more_than_2_32_elements(device, rows, cols):
+    """One row in every 10,000 and the last ones are not zero; 2^33 elements are past a flattened row."""
+    from ferry_amd import expert_ops as ops
+    x = torch.zeros((rows, cols), dtype=torch.bfloat16, device='cuda')
+    at = torch.cat([torch.arange(0, rows - 3, 10000), torch.arange(rows - 3, rows)]).cuda()
+    some = torch.randn((len(at), cols), generator=torch.Generator(device='cuda').manual_seed(1), device='cuda').bfloat16()
+    x[at] = some
+    codes, scales = ops.mxfp4_quantize(x)
+    want = ops.mxfp4_quantize(some)
+    assert torch.equal(codes[at], want[0]) and torch.equal(scales[at], want[1])
+    assert int((scales != 0).any(1).sum()) == len(at)
+    back = ops.mxfp4_dequantize(codes, scales, columns=cols)
+    assert torch.equal(back[at], ops.mxfp4_dequantize(*want, columns=cols))
+    assert int((back != 0).any(1).sum()) == len(at)
+
+
 def test_refusals(device):
     from ferry_amd import expert_ops as ops
     x = torch.zeros((4, 64), device='cuda')

@@ -324,6 +324,24 @@ def test_gate_to_combine(device):
 
 
 @pytest.mark.parametrize('quantised', QUANTISED)
+def test_an_expert_listed_twice(device, quantised):
+    c = Case([5, 40, 0, 17], 256, 384, seed=9)
+    assert torch.equal(c.run(quantised, [1, 0, 3, 1, 0]), c.run(quantised))
+
+
+@pytest.mark.parametrize('quantised', QUANTISED)
+def test_slots_past_4_gib(device, quantised):
+    c = Case([4, 60, 130], 2048, 768, seed=10)
+    want = c.run(quantised)
+    cache = torch.zeros((2000, c.cache.shape[1]), dtype=torch.uint8, device='cuda')   # 5 GB
+    slots = np.array([1997, 1999, 1800], np.int32)
+    for e in range(c.E):
+        cache[int(slots[e])] = c.cache[int(c.slot_of[e])]
+    c.cache, c.slot_of = cache, slots
+    assert torch.equal(c.run(quantised), want)
+
+
+@pytest.mark.parametrize('quantised', QUANTISED)
 def test_fetched_experts(device, quantised):
     """MXFP4 rows in a pinned pool, fetched into fewer cache slots than experts while the resident ones run."""
     from ferry_amd import expert_ops as ops

@@ -197,6 +197,17 @@ def test_empty_and_large_batches(device):
     assert torch.equal(ids[pick.cuda()], ids2) and torch.equal(w[pick.cuda()], w2)
 
 
+def test_more_tokens_than_a_launch_takes(device):
+    from ferry_amd import expert_ops as ops
+    T = 2 ** 24 + 2500
+    logits = randn((T, 4), 12, torch.bfloat16)
+    w, ids = ops.route_experts(logits, 2, scoring='sigmoid')
+    pick = torch.cat([torch.arange(50), torch.arange(2 ** 24 - 50, 2 ** 24 + 50), torch.arange(T - 50, T)]).cuda()
+    w2, ids2 = check(logits[pick], 2, 'sigmoid')
+    assert torch.equal(ids[pick], ids2) and torch.equal(w[pick], w2)
+    assert bool((ids[:, 0] != ids[:, 1]).all()) and int(ids.min()) == 0 and int(ids.max()) == 3
+
+
 def test_graph_replays_and_streams(device):
     from ferry_amd import expert_ops as ops
     logits = randn((50, 256), 11)

@@ -49,7 +49,13 @@ struct MxArgs {
   int32_t out_mode;
   int32_t tile_rows;        // of the tiled kernels: at most theirs
   int32_t known;            // the listed experts' row counts were given
+};
+struct SmallArgs : MxArgs {
   ExpertList list;
+};
+struct TiledArgs : MxArgs {
+  int32_t tile_wgs;         // workgroups that take tiles; the others take the small experts
+  ExpertList list, small;
 };
 
 // 8 elements of a code word as bf16, scaled (exact)
@@ -127,13 +133,15 @@ __device__ __forceinline__ uint32_t block_codes(const float (&v)[8], int byte) {
 constexpr int kUnits = 2;
 __device__ __forceinline__ int swz_w16(int row) { return (row >> 1) & 7; }   // 16 consecutive rows
 
+template <int NF>
+constexpr int kUnitBytes = 16 * NF * 136;   // LDS of a unit: codes, scales
+template <int NF>
+constexpr int kSmallBytes = 4 * kUnits * kUnitBytes<NF>;   // LDS of a workgroup, at most
+// bx: number of its weight rows; tid: 0 to 255
 template <int MODE, bool Q, int NF>
-__global__ __launch_bounds__(256) void mx_small(MxArgs a) {
-  extern __shared__ __attribute__((aligned(1024))) char smem[];
-  constexpr int kRowsW = 16 * NF, kW = kRowsW * 128, kUnit = kW + kRowsW * 8;   // LDS of a unit: codes, scales
-  const int li = blockIdx.y, bx = blockIdx.x;
-  const int e = a.list.expert[li], slot = a.list.slot[li];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+__device__ __forceinline__ void small_rows(const MxArgs& a, int e, int slot, int bx, char* smem, int tid) {
+  constexpr int kRowsW = 16 * NF, kW = kRowsW * 128, kUnit = kUnitBytes<NF>;
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, q = lane >> 4;
   const int64_t K = MODE == 0 ? a.H : a.I;
   const int chunks = (int)(K / 128), units = (chunks + 1) / 2;
@@ -286,12 +294,28 @@ __global__ __launch_bounds__(256) void mx_small(MxArgs a) {
   }
 }
 
-template <int MODE, bool Q, int NF>
-int small_launch(const MxArgs& a, hipStream_t s) {
+// weight rows of a workgroup, in tiles of 16
+template <int MODE, bool Q>
+constexpr int kSmallNF = MODE == 0 && !Q ? 2 : 4;
+template <int MODE, bool Q>
+__device__ __host__ __forceinline__ int small_cols(const MxArgs& a) {   // workgroups of an expert
+  return (int)(MODE == 0 ? a.I / (8 * kSmallNF<0, Q>) : a.H / (16 * kSmallNF<1, Q>));
+}
+
+template <int MODE, bool Q>
+__global__ __launch_bounds__(256) void mx_small(SmallArgs a) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  small_rows<MODE, Q, kSmallNF<MODE, Q>>(a, a.list.expert[blockIdx.y], a.list.slot[blockIdx.y], blockIdx.x, smem,
+                                         threadIdx.x);
+}
+
+template <int MODE, bool Q>
+int small_launch(const SmallArgs& a, hipStream_t s) {
+  constexpr int NF = kSmallNF<MODE, Q>;
   const int64_t K = MODE == 0 ? a.H : a.I, units = ceil_div(K, 256);
-  const dim3 g((unsigned)(MODE == 0 ? a.I / (8 * NF) : a.H / (16 * NF)), (unsigned)a.list.n);
-  const int64_t bytes = 4 * (units > 4 ? kUnits : 1) * (16 * NF * 136), sums = 4 * NF * 1024;
-  launch(MODE == 0 ? "mx_small_up" : "mx_small_down", mx_small<MODE, Q, NF>, g, dim3(256),
+  const dim3 g((unsigned)small_cols<MODE, Q>(a), (unsigned)a.list.n);
+  const int64_t bytes = units > 4 ? kSmallBytes<NF> : kSmallBytes<NF> / kUnits, sums = 4 * NF * 1024;
+  launch(MODE == 0 ? "mx_small_up" : "mx_small_down", mx_small<MODE, Q>, g, dim3(256),
          (uint32_t)(bytes > sums ? bytes : sums), s, a);
   FERRY_LAUNCHED("mx_small");
   return 0;
@@ -328,7 +352,7 @@ struct MxTile {
   int64_t row0;        // grouped row of the tile's first row
   int vrows, nt, slot; // its rows (> 0), number of its columns' tile, cache slot
 };
-__device__ __forceinline__ MxTile mx_locate(const MxArgs& a, const TileTable& tt, int tile, int ntn) {
+__device__ __forceinline__ MxTile mx_locate(const TiledArgs& a, const TileTable& tt, int tile, int ntn) {
   MxTile t;
   const int mt = tile / ntn;
   t.nt = tile - mt * ntn;
@@ -422,8 +446,8 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxTile& t, co
 // tiles: tiles of one expert follow each other, columns fastest, and share their rows and weights in that XCD's
 // L2.  What is left for a last round is spread over the XCDs, so that no CU has two tiles of it where another
 // has none (777 tokens, top 6 of 64 experts of 2048 x 1408, up: 72 us; with the rest on the first XCDs 89).
-__device__ __forceinline__ int tile_of(int round, int total) {
-  const int g = (int)gridDim.x, x = (int)(blockIdx.x % 8), j = (int)(blockIdx.x / 8);   // g: a multiple of 8
+__device__ __forceinline__ int tile_of(int round, int total, int wgs) {
+  const int g = wgs, x = (int)(blockIdx.x % 8), j = (int)(blockIdx.x / 8);   // g: a multiple of 8
   const int left = total - round * g;
   if (left >= g) return round * g + x * (g / 8) + j;
   if (left <= 0) return total;
@@ -437,14 +461,20 @@ __device__ __forceinline__ int tile_of(int round, int total) {
 // its last products, whose operands are in registers by then: behind it the next step's first operands are read, and
 // the loads of the freed buffers issued, between those products.
 template <int MODE>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void mx_tiled16(MxArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void mx_tiled16(TiledArgs a) {
   constexpr int NI = 4, W = 4, TM = 128, MI = 8, TN = kTileCols, COLS = kOutCols<MODE>;
   constexpr int RW = 64;                                 // a weight row's bytes in a buffer
   constexpr int kX = TM * 128, kW = TN * RW, kS = TN * 4;   // bytes of a buffer: rows, weights, scales
   constexpr int LX = 4, LW = 4;                          // direct loads of a wavefront for one
+  constexpr int kTileBytes = 2 * (kX + kW + kS), kSmall = kSmallBytes<kSmallNF<MODE, false>>;
   __shared__ TileTable tt;
-  __shared__ __attribute__((aligned(1024))) char smem[2 * (kX + kW + kS)];
+  __shared__ __attribute__((aligned(1024))) char smem[kTileBytes > kSmall ? kTileBytes : kSmall];
   __shared__ RowTables<MODE, TM> tab;
+  if ((int)blockIdx.x >= a.tile_wgs) {
+    const int per = small_cols<MODE, false>(a), b = (int)blockIdx.x - a.tile_wgs, li = b / per;
+    small_rows<MODE, false, kSmallNF<MODE, false>>(a, a.small.expert[li], a.small.slot[li], b - li * per, smem, threadIdx.x);
+    return;
+  }
   build_tile_table<kSmallRows>(a, tt, (uint32_t)a.tile_rows);
   const int64_t K = MODE == 0 ? a.H : a.I;
   const int ntn = (int)((MODE == 0 ? a.I : a.H) / COLS);
@@ -497,7 +527,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   };
   auto load_s = [&](int c, int b) { dma4(sbase + (int64_t)c * 4, soff, sbuf + (uint32_t)(b * kS + wn * 256)); };
 
-  int tile = tile_of(0, total);
+  int tile = tile_of(0, total, a.tile_wgs);
   if (tile >= total) return;
   MxTile cur = mx_locate(a, tt, tile, ntn);
   tab.load(a, cur, 0, wn, lane);
@@ -518,7 +548,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   bool primed = false;   // the tile's first steps are loaded, its first operands read
   for (int round = 1, later; tile < total; tile = later, ++round, set ^= 1) {
     // the tile after this one; after the last tile its own first steps are loaded again
-    later = tile_of(round, total);
+    later = tile_of(round, total, a.tile_wgs);
     const MxTile next = later < total ? mx_locate(a, tt, later, ntn) : cur;
     const bool few = cur.vrows <= TM / 2;
     if (few || !primed) {
@@ -682,14 +712,22 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 // the loads one step ahead.  Here the barrier stands at a step's end: before its last products, as above, it took
 // 69 to 78 us, with scales for two steps at a time 74.
 template <int MODE>
-__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void mx_tiled4(MxArgs a) {
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void mx_tiled4(TiledArgs a) {
   constexpr int WM = 2, WN = 4, MI = 8, NI = 4, W = WM * WN, TM = 256, TN = kTileCols, COLS = kOutCols<MODE>;
   constexpr int kX = TM * 128, kW = TN * 128;            // bytes of a buffer
   constexpr int LX = 4, LW = 4;                          // direct loads of a wavefront for one
   constexpr int kS = (TN + TM) * 8;                      // scale bytes of a step: weight rows, activation rows
+  constexpr int kTileBytes = 2 * (kX + kW + kS), kSmall = 2 * kSmallBytes<kSmallNF<MODE, true>>;
   __shared__ TileTable tt;
-  __shared__ __attribute__((aligned(1024))) char smem[2 * (kX + kW + kS)];
+  __shared__ __attribute__((aligned(1024))) char smem[kTileBytes > kSmall ? kTileBytes : kSmall];
   __shared__ RowTables<MODE, TM> tab;
+  if ((int)blockIdx.x >= a.tile_wgs) {
+    const int per = small_cols<MODE, true>(a) / 2, b = (int)blockIdx.x - a.tile_wgs, li = b / per;
+    const int half = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);   // two workgroups' work of one expert
+    small_rows<MODE, true, kSmallNF<MODE, true>>(a, a.small.expert[li], a.small.slot[li], 2 * (b - li * per) + half,
+                                                 smem + half * (kSmall / 2), threadIdx.x & 255);
+    return;
+  }
   build_tile_table<kSmallRows>(a, tt, (uint32_t)a.tile_rows);
   const int64_t K = MODE == 0 ? a.H : a.I;
   const int ntn = (int)((MODE == 0 ? a.I : a.H) / COLS);
@@ -767,7 +805,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     *reinterpret_cast<__attribute__((address_space(3))) u32x2*>((uintptr_t)(sbuf + (uint32_t)(b * kS + tid * 8))) = sv;
   };
 
-  int tile = tile_of(0, total);
+  int tile = tile_of(0, total, a.tile_wgs);
   if (tile >= total) return;
   MxTile cur = mx_locate(a, tt, tile, ntn);
   tab.load(a, cur, 0, wave, lane);
@@ -785,7 +823,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   int set = 0, b = 0;   // set of row tables; buffer of the present step
   for (int round = 1, later; tile < total; tile = later, ++round, set ^= 1) {
     // the tile after this one; after the last tile its own first step is loaded again
-    later = tile_of(round, total);
+    later = tile_of(round, total, a.tile_wgs);
     const MxTile next = later < total ? mx_locate(a, tt, later, ntn) : cur;
     tab.load(a, next, set ^ 1, wave, lane);
     tab.outputs(a, cur, set, wave, lane);
@@ -890,23 +928,29 @@ constexpr int kTileRows = Q ? 256 : 128;
 // tokens 30, 16 and 17 us against 17, 11 and 15, 200 tokens 31, 18 and 23 against 22, 14 and 17; quarters
 // two to a CU were slower than halves there (24 and 15 us).
 template <bool Q>
-int launch_list(MxArgs& a, bool small, const int64_t (&tiles)[3], int32_t phases, int64_t cus, hipStream_t s) {
+int launch_lists(TiledArgs& a, const int64_t (&tiles)[3], int32_t phases, int64_t cus, hipStream_t s) {
   for (int mode = 0; mode < 2; ++mode) {
     if (!(phases & (1 << mode))) continue;
-    if (small)
-      if (const int rc = mode == 0 ? small_launch<0, Q, Q ? 4 : 2>(a, s) : small_launch<1, Q, 4>(a, s)) return rc;
-    if (tiles[0]) {
-      const int64_t most = (Q ? cus : 2 * cus) / 8 * 8, cols = mode == 0 ? a.I / kOutCols<0> : a.H / kOutCols<1>;
-      const int by = tiles[2] * cols <= cus ? 2 : tiles[1] * cols <= most ? 1 : 0;
-      a.tile_rows = kTileRows<Q> >> by;
-      const int64_t t = tiles[by] * cols;
-      const dim3 grid((unsigned)(t < most ? ceil_div(t, 8) * 8 : most));
-      if constexpr (Q)
-        launch(mode == 0 ? "mx_tiled_up" : "mx_tiled_down", mode == 0 ? mx_tiled4<0> : mx_tiled4<1>, grid, dim3(512), 0, s, a);
-      else
-        launch(mode == 0 ? "mx_tiled_up" : "mx_tiled_down", mode == 0 ? mx_tiled16<0> : mx_tiled16<1>, grid, dim3(256), 0, s, a);
-      FERRY_LAUNCHED("mx_tiled");
+    if (tiles[0] == 0) {
+      if (a.small.n == 0) continue;
+      SmallArgs b;
+      (MxArgs&)b = a;
+      b.list = a.small;
+      if (const int rc = mode == 0 ? small_launch<0, Q>(b, s) : small_launch<1, Q>(b, s)) return rc;
+      continue;
     }
+    const int64_t most = (Q ? cus : 2 * cus) / 8 * 8, cols = mode == 0 ? a.I / kOutCols<0> : a.H / kOutCols<1>;
+    const int by = tiles[2] * cols <= cus ? 2 : tiles[1] * cols <= most ? 1 : 0;
+    a.tile_rows = kTileRows<Q> >> by;
+    const int64_t t = tiles[by] * cols;
+    a.tile_wgs = (int32_t)(t < most ? ceil_div(t, 8) * 8 : most);
+    const int small = a.small.n * (mode == 0 ? small_cols<0, Q>(a) : small_cols<1, Q>(a)) / (Q ? 2 : 1);
+    const dim3 grid((unsigned)(a.tile_wgs + small));
+    if constexpr (Q)
+      launch(mode == 0 ? "mx_tiled_up" : "mx_tiled_down", mode == 0 ? mx_tiled4<0> : mx_tiled4<1>, grid, dim3(512), 0, s, a);
+    else
+      launch(mode == 0 ? "mx_tiled_up" : "mx_tiled_down", mode == 0 ? mx_tiled16<0> : mx_tiled16<1>, grid, dim3(256), 0, s, a);
+    FERRY_LAUNCHED("mx_tiled");
   }
   return 0;
 }
@@ -975,7 +1019,7 @@ extern "C" int ferry_mxfp4_expert_ffn(const void* cache, int64_t cache_rows, int
   if (cus > 2 * spare_cus) cus -= spare_cus;
   const bool quantised = x_scales != nullptr;
   const int64_t pairs = rows_in * topk, tile_rows = quantised ? kTileRows<true> : kTileRows<false>;
-  MxArgs a;
+  TiledArgs a;
   a.cache = (const uint8_t*)cache;
   a.x = (const uint8_t*)x;
   a.x_scales = (const uint8_t*)x_scales;
@@ -991,52 +1035,45 @@ extern "C" int ferry_mxfp4_expert_ffn(const void* cache, int64_t cache_rows, int
   a.k = topk;
   a.out_mode = out_mode;
   a.known = list_rows != nullptr;
-  a.list.n_mid = 0;
-  // One pass over the small experts, one over the others; without row counts every expert is in both, and the
+  // Small experts and the others, each up to kListMax of a launch; without row counts every expert is in both, and the
   // kernels pass over those of the other kind by the device's starts.  An expert's own rows decide, so that its
   // results do not depend on which experts are listed with it (the two kinds sum in different orders): with all
   // experts in tiles wherever one has more than kSmallRows rows, 512 tokens (128 experts of 2048 x 768, top 8,
   // Zipf 1.1) take 110 and 87 us (bf16 and 4-bit activations) instead of 122 and 92, 8,192 tokens 644 and 332
   // instead of 653 and 341.
-  for (int big = 0; big < 2; ++big) {
-    if (big ? max_rows_per_expert <= kSmallRows : min_rows_per_expert > kSmallRows) continue;
+  struct Entry {
+    int32_t rows, expert;
+  } entry[kListMax];
+  const bool any[2] = {min_rows_per_expert <= kSmallRows, max_rows_per_expert > kSmallRows};   // small, others
+  int32_t at[2] = {any[0] ? 0 : n_list, any[1] ? 0 : n_list};
+  for (;;) {
     int64_t tiles[3] = {0, 0, 0};
-    struct Entry {
-      int32_t rows, expert;
-    } entry[kListMax];
-    a.list.n = 0;
-    auto flush = [&]() {
-      if (a.list.n == 0) return 0;
+    for (int big = 0; big < 2; ++big) {
+      ExpertList& list = big ? a.list : a.small;
+      list.n = list.n_mid = 0;
+      for (int32_t& i = at[big]; i < n_list && list.n < kListMax; ++i) {
+        if (list_rows && (list_rows[i] < 1 || (list_rows[i] > kSmallRows) != (big != 0))) continue;
+        if (list_rows && big)
+          for (int by = 0; by < 3; ++by) tiles[by] += ceil_div(list_rows[i], tile_rows >> by);
+        entry[list.n++] = {list_rows ? list_rows[i] : 0, expert_list[i]};
+      }
       // the experts with most rows first: tiles of few rows, which take less time, fill the last round (65 us for the
       // up phase above)
       if (big && list_rows)
-        std::sort(entry, entry + a.list.n, [](const Entry& p, const Entry& q) { return p.rows > q.rows; });
-      for (int i = 0; i < a.list.n; ++i) {
-        a.list.expert[i] = (int16_t)entry[i].expert;
-        a.list.slot[i] = slot_of[entry[i].expert];
+        std::sort(entry, entry + list.n, [](const Entry& p, const Entry& q) { return p.rows > q.rows; });
+      for (int i = 0; i < list.n; ++i) {
+        list.expert[i] = (int16_t)entry[i].expert;
+        list.slot[i] = slot_of[entry[i].expert];
       }
-      // row counts unknown: sum ceil(n / rows) <= pairs / rows + the experts with more than kSmallRows rows
-      if (big && !list_rows) {
-        const int64_t most = pairs / (kSmallRows + 1);
-        for (int by = 0; by < 3; ++by) tiles[by] = pairs / (tile_rows >> by) + (a.list.n < most ? a.list.n : most);
-      }
-      const int rc = quantised ? launch_list<true>(a, !big, tiles, phases, cus, (hipStream_t)stream)
-                               : launch_list<false>(a, !big, tiles, phases, cus, (hipStream_t)stream);
-      a.list.n = 0;
-      tiles[0] = tiles[1] = tiles[2] = 0;
-      return rc;
-    };
-    for (int32_t i = 0; i < n_list; ++i) {
-      if (list_rows) {
-        if (list_rows[i] < 1 || (list_rows[i] > kSmallRows) != (big != 0)) continue;
-        if (big)
-          for (int by = 0; by < 3; ++by) tiles[by] += ceil_div(list_rows[i], tile_rows >> by);
-      }
-      entry[a.list.n++] = {list_rows ? list_rows[i] : 0, expert_list[i]};
-      if (a.list.n == kListMax)
-        if (const int rc = flush()) return rc;
     }
-    if (const int rc = flush()) return rc;
+    if (a.list.n + a.small.n == 0) return 0;
+    // row counts unknown: sum ceil(n / rows) <= pairs / rows + the experts with more than kSmallRows rows
+    if (!list_rows && a.list.n) {
+      const int64_t most = pairs / (kSmallRows + 1);
+      for (int by = 0; by < 3; ++by) tiles[by] = pairs / (tile_rows >> by) + (a.list.n < most ? a.list.n : most);
+    }
+    const int rc = quantised ? launch_lists<true>(a, tiles, phases, cus, (hipStream_t)stream)
+                             : launch_lists<false>(a, tiles, phases, cus, (hipStream_t)stream);
+    if (rc) return rc;
   }
-  return 0;
 }

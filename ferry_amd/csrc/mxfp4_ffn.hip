@@ -17,10 +17,9 @@
 // without any repacking.
 //
 // Measured, all experts (2048 x 768, 128 of them, top 8, Zipf 1.1): one token 5.4 + 3.9 us (up + down; launch
-// latency), 16 tokens 15 + 9 us (3.4 and 2.8 TB/s of weights), with 4-bit activations 13 + 7; 8,192 tokens 28 + 15 us
-// for the 47 experts of at most 16 rows and 330 + 228 for the others (1,240 and 900 TFLOP/s; a library product of
-// bf16 matrices of 32768 x 2048 x 1536 runs at 1,372), with 4-bit activations 25 + 14 and 163 + 127 (2,500
-// and 1,620 TFLOP/s).
+// latency), 16 tokens 15 + 9 us (3.4 and 2.8 TB/s of weights), with 4-bit activations 13 + 7; 8,192 tokens 348 + 238 us
+// (1,180 and 860 TFLOP/s, without the 47 experts of at most 16 rows 1,240 and 900; a library product of bf16
+// matrices of 32768 x 2048 x 1536 runs at 1,372), with 4-bit activations 177 + 136 (2,320 and 1,510 TFLOP/s).
 #include "ffn_common.h"
 
 #include <algorithm>
@@ -921,14 +920,19 @@ int device_cus(int* cus) {
 template <bool Q>
 constexpr int kTileRows = Q ? 256 : 128;
 
-// The launches of one list in one kind of activations.  tiles: the row tiles of kTileRows, a half and a quarter of
-// that many rows of the experts with more than kSmallRows rows (upper bounds).  Halves where they all run at once and
-// quarters where each has a CU of its own: they read the weights more often, and the longest takes less time.  Up,
-// down and up with 4-bit activations, whole tiles against those (128 experts of 2048 x 768, top 8, Zipf 1.1): 100
-// tokens 30, 16 and 17 us against 17, 11 and 15, 200 tokens 31, 18 and 23 against 22, 14 and 17; quarters
-// two to a CU were slower than halves there (24 and 15 us).
+// The launches of a.list and a.small in one kind of activations.  tiles: the row tiles of kTileRows and of half as many
+// rows of the experts with more than kSmallRows rows (upper bounds).
+//
+// Halves where each has a CU of its own: they read the weights twice, and the longest takes less time.  Up and
+// down, whole tiles against halves (128 experts of 2048 x 768, top 8, Zipf 1.1): 100 tokens 34 + 19 us against
+// 28 + 18; halves two to a CU, and quarters, were level with these or slower (29 + 19).
+//
+// The small experts' workgroups come behind those of the tiles and run where a CU has no tile (left): up + down, with
+// bf16 and with 4-bit activations, 20 tokens take 37 and 37 us, with launches of their own 57 and 49, 777 tokens (64
+// experts of 2048 x 1408, top 6) 137 and 109 against 157 and 121, 8,192 tokens 615 and 319 against 627 and 339;
+// before the tiles' they delay them (153 and 116 us at 777 tokens).
 template <bool Q>
-int launch_lists(TiledArgs& a, const int64_t (&tiles)[3], int32_t phases, int64_t cus, hipStream_t s) {
+int launch_lists(TiledArgs& a, const int64_t (&tiles)[2], int32_t phases, int64_t cus, hipStream_t s) {
   for (int mode = 0; mode < 2; ++mode) {
     if (!(phases & (1 << mode))) continue;
     if (tiles[0] == 0) {
@@ -940,7 +944,7 @@ int launch_lists(TiledArgs& a, const int64_t (&tiles)[3], int32_t phases, int64_
       continue;
     }
     const int64_t most = (Q ? cus : 2 * cus) / 8 * 8, cols = mode == 0 ? a.I / kOutCols<0> : a.H / kOutCols<1>;
-    const int by = tiles[2] * cols <= cus ? 2 : tiles[1] * cols <= most ? 1 : 0;
+    const int by = tiles[1] * cols <= cus;
     a.tile_rows = kTileRows<Q> >> by;
     const int64_t t = tiles[by] * cols;
     a.tile_wgs = (int32_t)(t < most ? ceil_div(t, 8) * 8 : most);
@@ -1047,14 +1051,14 @@ extern "C" int ferry_mxfp4_expert_ffn(const void* cache, int64_t cache_rows, int
   const bool any[2] = {min_rows_per_expert <= kSmallRows, max_rows_per_expert > kSmallRows};   // small, others
   int32_t at[2] = {any[0] ? 0 : n_list, any[1] ? 0 : n_list};
   for (;;) {
-    int64_t tiles[3] = {0, 0, 0};
+    int64_t tiles[2] = {0, 0};
     for (int big = 0; big < 2; ++big) {
       ExpertList& list = big ? a.list : a.small;
       list.n = list.n_mid = 0;
       for (int32_t& i = at[big]; i < n_list && list.n < kListMax; ++i) {
         if (list_rows && (list_rows[i] < 1 || (list_rows[i] > kSmallRows) != (big != 0))) continue;
         if (list_rows && big)
-          for (int by = 0; by < 3; ++by) tiles[by] += ceil_div(list_rows[i], tile_rows >> by);
+          for (int by = 0; by < 2; ++by) tiles[by] += ceil_div(list_rows[i], tile_rows >> by);
         entry[list.n++] = {list_rows ? list_rows[i] : 0, expert_list[i]};
       }
       // the experts with most rows first: tiles of few rows, which take less time, fill the last round (65 us for the
@@ -1070,7 +1074,7 @@ extern "C" int ferry_mxfp4_expert_ffn(const void* cache, int64_t cache_rows, int
     // row counts unknown: sum ceil(n / rows) <= pairs / rows + the experts with more than kSmallRows rows
     if (!list_rows && a.list.n) {
       const int64_t most = pairs / (kSmallRows + 1);
-      for (int by = 0; by < 3; ++by) tiles[by] = pairs / (tile_rows >> by) + (a.list.n < most ? a.list.n : most);
+      for (int by = 0; by < 2; ++by) tiles[by] = pairs / (tile_rows >> by) + (a.list.n < most ? a.list.n : most);
     }
     const int rc = quantised ? launch_lists<true>(a, tiles, phases, cus, (hipStream_t)stream)
                              : launch_lists<false>(a, tiles, phases, cus, (hipStream_t)stream);

@@ -338,13 +338,13 @@ int small_launch(const SmallArgs& a, hipStream_t s) {
 // MODE 0: of a wavefront's four weight tiles, two are gate rows and two the up rows of the same 32 columns.
 // The weight rows of the two tiles c of 32 columns interleave in groups of four, 8 g + 4 c + [0, 4):
 // a lane then holds 8 consecutive output columns of one row.
-constexpr int kTileCols = 256;   // weight rows of a tile: 128 or 256 output columns
-template <int MODE>
-constexpr int kOutCols = MODE == 0 ? kTileCols / 2 : kTileCols;
+constexpr int kTileCols = 256;   // weight rows of a large tile: 128 or 256 output columns
+template <int MODE, int TN = kTileCols>
+constexpr int kOutCols = MODE == 0 ? TN / 2 : TN;
 // first weight row (of the tile's) of a wavefront's weight tile f
-template <int MODE>
+template <int MODE, int TN = kTileCols>
 __device__ __forceinline__ constexpr int wtile(int f) {
-  return (f >> 1) * (MODE == 0 ? kTileCols / 2 : 32) + (f & 1) * 4;
+  return (f >> 1) * (MODE == 0 ? TN / 2 : 32) + (f & 1) * 4;
 }
 
 struct MxTile {
@@ -398,12 +398,12 @@ __device__ __forceinline__ int fresh(int v) {
 
 // The sums of a wavefront's tiles into the activations or the outputs: tile i of group wm of WM holds the tile's
 // rows 16 (WM i + wm) ..
-template <int MODE, bool Q, int WM, int TM>
+template <int MODE, bool Q, int WM, int TM, int TN, int MI>
 __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxTile& t, const RowTables<MODE, TM>& tab, int set,
-                                            const floatx4 (&acc)[8][4], int wm, int wn, int lane_) {
+                                            const floatx4 (&acc)[MI][4], int wm, int wn, int lane_) {
   const int lane = fresh(lane_), r = lane & 15, q = lane >> 4;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < MI; ++i) {
     const int row = 16 * (WM * i + wm) + r;
     const bool live = row < t.vrows;
     if constexpr (MODE == 0) {
@@ -412,7 +412,7 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxTile& t, co
       for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[4 * c + j] = silu_mul(acc[i][c][j], acc[i][2 + c][j]);
-      const int64_t col = t.nt * kOutCols<0> + wn * 32;
+      const int64_t col = t.nt * kOutCols<0, TN> + wn * 32;
       if constexpr (Q) {
         const int byte = block_scale(v);
         const uint32_t c = block_codes(v, byte);
@@ -426,7 +426,7 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxTile& t, co
       }
     } else if (live) {
       const float wt = __uint_as_float((uint32_t)tab.wt[set][row] << 16);
-      bf16_t* const o = a.out + (int64_t)tab.orow[set][row] * a.H + t.nt * kOutCols<1> + wn * 64 + q * 8;
+      bf16_t* const o = a.out + (int64_t)tab.orow[set][row] * a.H + t.nt * kOutCols<1, TN> + wn * 64 + q * 8;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         u32x4 y;
@@ -699,32 +699,35 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     else if (cur.vrows > TM / 4) loop_few(std::integral_constant<int, MI / 2>{});
     else loop_few(std::integral_constant<int, MI / 4>{});
     primed = !few;
-    mx_epilogue<MODE, false, 1, TM>(a, cur, tab, set, acc, 0, wn, lane);
+    mx_epilogue<MODE, false, 1, TM, TN, MI>(a, cur, tab, set, acc, 0, wn, lane);
     cur = next;
   }
   wait_cnt<0>();   // no load may write this workgroup's LDS after its end
 }
 
-// 4-bit activations.  Eight wavefronts in two rows share 256 rows.  A step is 256 along K: rows of 128 bytes of
-// activations and of weights, whole cache lines (with lines of 64 bytes loaded up to three steps ahead, 90 us instead
-// of 70 at 32,768 rows x 2048 x 768 up: a CU receives about 64 bytes a clock, in lines of 128), two buffers,
-// the loads one step ahead.  Here the barrier stands at a step's end: before its last products, as above, it took
-// 69 to 78 us, with scales for two steps at a time 74.
-template <int MODE>
-__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void mx_tiled4(TiledArgs a) {
-  constexpr int WM = 2, WN = 4, MI = 8, NI = 4, W = WM * WN, TM = 256, TN = kTileCols, COLS = kOutCols<MODE>;
+// 4-bit activations.  LARGE: eight wavefronts in two rows share 256 x 256, one workgroup on a CU; else four share 128 x
+// 128, two workgroups on a CU, each in its own time.  A step is 256 along K: rows of 128 bytes of activations
+// and of weights, whole cache lines (with lines of 64 bytes loaded up to three steps ahead, 90 us instead of 70 at
+// 32,768 rows x 2048 x 768 up: a CU receives about 64 bytes a clock, in lines of 128), two buffers, the loads
+// one step ahead.  Here the barrier stands at a step's end: before its last products, as above, it took 69 to 78 us,
+// with scales for two steps at a time 74.  The large tiles load and read half and two thirds as much for
+// each product (32,768 rows: 70 us against 86); the small ones' epilogues and waits fall into the other workgroup's products.
+template <int MODE, bool LARGE>
+__global__ __launch_bounds__(LARGE ? 512 : 256) __attribute__((amdgpu_waves_per_eu(2, 2))) void mx_tiled4(TiledArgs a) {
+  constexpr int WM = 2, WN = LARGE ? 4 : 2, MI = LARGE ? 8 : 4, NI = 4, W = WM * WN;
+  constexpr int TM = 16 * WM * MI, TN = 64 * WN, COLS = kOutCols<MODE, TN>;
   constexpr int kX = TM * 128, kW = TN * 128;            // bytes of a buffer
   constexpr int LX = 4, LW = 4;                          // direct loads of a wavefront for one
   constexpr int kS = (TN + TM) * 8;                      // scale bytes of a step: weight rows, activation rows
-  constexpr int kTileBytes = 2 * (kX + kW + kS), kSmall = 2 * kSmallBytes<kSmallNF<MODE, true>>;
+  constexpr int kTileBytes = 2 * (kX + kW + kS), kSmall = W / 4 * kSmallBytes<kSmallNF<MODE, true>>;
   __shared__ TileTable tt;
   __shared__ __attribute__((aligned(1024))) char smem[kTileBytes > kSmall ? kTileBytes : kSmall];
   __shared__ RowTables<MODE, TM> tab;
   if ((int)blockIdx.x >= a.tile_wgs) {
-    const int per = small_cols<MODE, true>(a) / 2, b = (int)blockIdx.x - a.tile_wgs, li = b / per;
-    const int half = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);   // two workgroups' work of one expert
-    small_rows<MODE, true, kSmallNF<MODE, true>>(a, a.small.expert[li], a.small.slot[li], 2 * (b - li * per) + half,
-                                                 smem + half * (kSmall / 2), threadIdx.x & 255);
+    const int per = small_cols<MODE, true>(a) / (W / 4), b = (int)blockIdx.x - a.tile_wgs, li = b / per;
+    const int part = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);   // LARGE: two workgroups' work of one expert
+    small_rows<MODE, true, kSmallNF<MODE, true>>(a, a.small.expert[li], a.small.slot[li], W / 4 * (b - li * per) + part,
+                                                 smem + part * (kSmall / (W / 4)), threadIdx.x & 255);
     return;
   }
   build_tile_table<kSmallRows>(a, tt, (uint32_t)a.tile_rows);
@@ -757,7 +760,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     auto src_row = [&](int v) {
       return MODE == 0 ? (uint32_t)tab.row[p][v] : (uint32_t)(t.row0 + (v < t.vrows ? v : 0));
     };
-    xloads = min((t.vrows + 63) / 64, LX);
+    xloads = min((t.vrows + 8 * W - 1) / (8 * W), LX);
 #pragma unroll
     for (int j = 0; j < LX; ++j) {
       const int v = 8 * (W * j + wave) + l / 8;
@@ -770,7 +773,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const int v = 8 * wave + l / 8;   // load j: 64 j rows on, in the same order of slots
     woff = (uint32_t)v * (uint32_t)(K / 2) + (uint32_t)(((l & 7) ^ swz_w(v)) * 16);
     if (wave < W / 2) {
-      sp = (wave < W / 4 ? m0.scales : m1.scales) + (int64_t)(64 * (wave & 1) + l) * (K / 32);
+      sp = (wave < W / 4 ? m0.scales : m1.scales) + (int64_t)(64 * (wave & (W / 4 - 1)) + l) * (K / 32);
     } else {
       sp = (MODE == 0 ? a.x_scales : a.act_scales) + (int64_t)src_row(64 * (wave - W / 2) + l) * (K / 32);
     }
@@ -793,7 +796,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       const int l = fresh(lane);
       off -= tail((l & 7) ^ swz_w(8 * wave + l / 8));
     }
-    dma16(wbase[j >> 1] + (j & 1) * 32 * K + (int64_t)n * 128, off, wbuf + (uint32_t)(b * kW + (W * j + wave) * 1024));
+    dma16(wbase[j >> 1] + (j & 1) * (4 * W) * K + (int64_t)n * 128, off, wbuf + (uint32_t)(b * kW + (W * j + wave) * 1024));
   };
   u32x2 sv = {0, 0};
   auto load_s = [&](int n) {
@@ -850,8 +853,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         auto read_w = [&](int j) {
 #pragma unroll
           for (int f = 0; f < NI; ++f) {
-            wf[f] = lds_get<lds_u32x4>((wb ^ (uint32_t)(j << 6)) + (uint32_t)(wtile<MODE>(f) * 128));
-            wsf[f] = lds_get<lds_u32>(wsb + (uint32_t)(wtile<MODE>(f) * 8 + 4 * j));
+            wf[f] = lds_get<lds_u32x4>((wb ^ (uint32_t)(j << 6)) + (uint32_t)(wtile<MODE, TN>(f) * 128));
+            wsf[f] = lds_get<lds_u32>(wsb + (uint32_t)(wtile<MODE, TN>(f) * 8 + 4 * j));
           }
         };
         read_w(0);
@@ -899,11 +902,11 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         wg_barrier();
       }
     };
-    if (cur.vrows > TM / 4 * 3) loop(std::integral_constant<int, MI>{});
-    else if (cur.vrows > TM / 2) loop(std::integral_constant<int, MI / 4 * 3>{});
-    else if (cur.vrows > TM / 4) loop(std::integral_constant<int, MI / 2>{});
-    else loop(std::integral_constant<int, MI / 4>{});
-    mx_epilogue<MODE, true, WM, TM>(a, cur, tab, set, acc, wm, wn, lane);
+    if (LARGE && cur.vrows <= TM / 4) loop(std::integral_constant<int, LARGE ? MI / 4 : MI>{});
+    else if (cur.vrows <= TM / 2) loop(std::integral_constant<int, MI / 2>{});
+    else if (LARGE && cur.vrows <= TM / 4 * 3) loop(std::integral_constant<int, LARGE ? MI / 4 * 3 : MI>{});
+    else loop(std::integral_constant<int, MI>{});
+    mx_epilogue<MODE, true, WM, TM, TN, MI>(a, cur, tab, set, acc, wm, wn, lane);
     cur = next;
   }
   wait_cnt<0>();   // no load may write this workgroup's LDS after its end
@@ -917,22 +920,23 @@ int device_cus(int* cus) {
   return 0;
 }
 
-template <bool Q>
-constexpr int kTileRows = Q ? 256 : 128;
-
-// The launches of a.list and a.small in one kind of activations.  tiles: the row tiles of kTileRows and of half as many
-// rows of the experts with more than kSmallRows rows (upper bounds).
+// The launches of a.list and a.small in one kind of activations.  tiles: the row tiles of 256, 128 and 64 rows of the
+// experts with more than kSmallRows rows (upper bounds).
 //
-// Halves where each has a CU of its own: they read the weights twice, and the longest takes less time.  Up and
-// down, whole tiles against halves (128 experts of 2048 x 768, top 8, Zipf 1.1): 100 tokens 34 + 19 us against
-// 28 + 18; halves two to a CU, and quarters, were level with these or slower (29 + 19).
+// 4-bit activations: the large tiles where the rows make at least six quarters of them for each CU.  Up and down, large
+// tiles against small ones: 512 tokens (128 experts of 2048 x 768, top 8, Zipf 1.1; 1.2 and 1.6 quarters) 43 + 32 us
+// against 39 + 29, 2,048 tokens (7 and 9.4) 78 + 54 against 79 + 54, 4,096 (13 and 17) 113 + 79 against 120
+// + 84; evenly spread, 1,024 tokens (3 and 4) 62 + 37 against 56 + 36, 2,048 (6 and 8) 72 + 46 against 79 + 52.
+// Tiles of 128 rows become tiles of 64 where each has a CU of its own: they read the weights twice, and the longest
+// takes less time.  Up and down, bf16 activations (128 experts of 2048 x 768, top 8, Zipf 1.1): 100 tokens 34 + 19
+// us against 28 + 18; 64 rows two to a CU, and 32, were level with these or slower (29 + 19).
 //
 // The small experts' workgroups come behind those of the tiles and run where a CU has no tile (left): up + down, with
 // bf16 and with 4-bit activations, 20 tokens take 37 and 37 us, with launches of their own 57 and 49, 777 tokens (64
 // experts of 2048 x 1408, top 6) 137 and 109 against 157 and 121, 8,192 tokens 615 and 319 against 627 and 339;
 // before the tiles' they delay them (153 and 116 us at 777 tokens).
 template <bool Q>
-int launch_lists(TiledArgs& a, const int64_t (&tiles)[2], int32_t phases, int64_t cus, hipStream_t s) {
+int launch_lists(TiledArgs& a, const int64_t (&tiles)[3], int32_t phases, int64_t cus, hipStream_t s) {
   for (int mode = 0; mode < 2; ++mode) {
     if (!(phases & (1 << mode))) continue;
     if (tiles[0] == 0) {
@@ -943,17 +947,19 @@ int launch_lists(TiledArgs& a, const int64_t (&tiles)[2], int32_t phases, int64_
       if (const int rc = mode == 0 ? small_launch<0, Q>(b, s) : small_launch<1, Q>(b, s)) return rc;
       continue;
     }
-    const int64_t most = (Q ? cus : 2 * cus) / 8 * 8, cols = mode == 0 ? a.I / kOutCols<0> : a.H / kOutCols<1>;
-    const int by = tiles[1] * cols <= cus;
-    a.tile_rows = kTileRows<Q> >> by;
+    const int64_t large = mode == 0 ? a.I / kOutCols<0> : a.H / kOutCols<1>;   // column tiles
+    const bool use_large = Q && tiles[2] * large >= 6 * cus;
+    const int64_t cols = Q && !use_large ? 2 * large : large, most = (use_large ? cus : 2 * cus) / 8 * 8;
+    const int by = use_large ? 0 : tiles[2] * cols <= cus ? 2 : 1;
+    a.tile_rows = 256 >> by;
     const int64_t t = tiles[by] * cols;
     a.tile_wgs = (int32_t)(t < most ? ceil_div(t, 8) * 8 : most);
-    const int small = a.small.n * (mode == 0 ? small_cols<0, Q>(a) : small_cols<1, Q>(a)) / (Q ? 2 : 1);
-    const dim3 grid((unsigned)(a.tile_wgs + small));
-    if constexpr (Q)
-      launch(mode == 0 ? "mx_tiled_up" : "mx_tiled_down", mode == 0 ? mx_tiled4<0> : mx_tiled4<1>, grid, dim3(512), 0, s, a);
-    else
-      launch(mode == 0 ? "mx_tiled_up" : "mx_tiled_down", mode == 0 ? mx_tiled16<0> : mx_tiled16<1>, grid, dim3(256), 0, s, a);
+    const int small = a.small.n * (mode == 0 ? small_cols<0, Q>(a) : small_cols<1, Q>(a)) / (use_large ? 2 : 1);
+    const dim3 grid((unsigned)(a.tile_wgs + small)), block(use_large ? 512 : 256);
+    const char* const name = mode == 0 ? "mx_tiled_up" : "mx_tiled_down";
+    if constexpr (!Q) launch(name, mode == 0 ? mx_tiled16<0> : mx_tiled16<1>, grid, block, 0, s, a);
+    else if (use_large) launch(name, mode == 0 ? mx_tiled4<0, true> : mx_tiled4<1, true>, grid, block, 0, s, a);
+    else launch(name, mode == 0 ? mx_tiled4<0, false> : mx_tiled4<1, false>, grid, block, 0, s, a);
     FERRY_LAUNCHED("mx_tiled");
   }
   return 0;
@@ -1022,7 +1028,7 @@ extern "C" int ferry_mxfp4_expert_ffn(const void* cache, int64_t cache_rows, int
   if (const int rc = device_cus(&cus)) return rc;
   if (cus > 2 * spare_cus) cus -= spare_cus;
   const bool quantised = x_scales != nullptr;
-  const int64_t pairs = rows_in * topk, tile_rows = quantised ? kTileRows<true> : kTileRows<false>;
+  const int64_t pairs = rows_in * topk;
   TiledArgs a;
   a.cache = (const uint8_t*)cache;
   a.x = (const uint8_t*)x;
@@ -1051,14 +1057,14 @@ extern "C" int ferry_mxfp4_expert_ffn(const void* cache, int64_t cache_rows, int
   const bool any[2] = {min_rows_per_expert <= kSmallRows, max_rows_per_expert > kSmallRows};   // small, others
   int32_t at[2] = {any[0] ? 0 : n_list, any[1] ? 0 : n_list};
   for (;;) {
-    int64_t tiles[2] = {0, 0};
+    int64_t tiles[3] = {0, 0, 0};
     for (int big = 0; big < 2; ++big) {
       ExpertList& list = big ? a.list : a.small;
       list.n = list.n_mid = 0;
       for (int32_t& i = at[big]; i < n_list && list.n < kListMax; ++i) {
         if (list_rows && (list_rows[i] < 1 || (list_rows[i] > kSmallRows) != (big != 0))) continue;
         if (list_rows && big)
-          for (int by = 0; by < 2; ++by) tiles[by] += ceil_div(list_rows[i], tile_rows >> by);
+          for (int by = 0; by < 3; ++by) tiles[by] += ceil_div(list_rows[i], 256 >> by);
         entry[list.n++] = {list_rows ? list_rows[i] : 0, expert_list[i]};
       }
       // the experts with most rows first: tiles of few rows, which take less time, fill the last round (65 us for the
@@ -1074,7 +1080,7 @@ extern "C" int ferry_mxfp4_expert_ffn(const void* cache, int64_t cache_rows, int
     // row counts unknown: sum ceil(n / rows) <= pairs / rows + the experts with more than kSmallRows rows
     if (!list_rows && a.list.n) {
       const int64_t most = pairs / (kSmallRows + 1);
-      for (int by = 0; by < 2; ++by) tiles[by] = pairs / (tile_rows >> by) + (a.list.n < most ? a.list.n : most);
+      for (int by = 0; by < 3; ++by) tiles[by] = pairs / (256 >> by) + (a.list.n < most ? a.list.n : most);
     }
     const int rc = quantised ? launch_lists<true>(a, tiles, phases, cus, (hipStream_t)stream)
                              : launch_lists<false>(a, tiles, phases, cus, (hipStream_t)stream);

@@ -169,10 +169,12 @@ def test_many_rows(device, H, I, counts, quantised):
 
 
 @pytest.mark.parametrize('quantised', QUANTISED)
-def test_more_tiles_than_workgroups(device, quantised):
-    """Whole tiles, several to a workgroup, with every count of rows that tiles are cut to; an expert by itself runs
-    in smaller ones and gives the same bits."""
-    c = Case([1380, 17, 720, 1224, 90, 1046, 562, 0, 276, 129, 3], 2048, 1024, seed=5)
+@pytest.mark.parametrize('counts', [[1380, 17, 720, 1224, 90, 1046, 562, 0, 276, 129, 3],
+                                    [3380, 17, 1720, 2224, 90, 3046, 562, 0, 1276, 129, 3, 200]])
+def test_more_tiles_than_workgroups(device, counts, quantised):
+    """Tiles of every size, several to a workgroup, with every count of rows that they are cut to; an expert by itself
+    runs in smaller ones and gives the same bits."""
+    c = Case(counts, 2048, 1024, seed=5)
     whole = c.check(quantised)
     out = torch.full_like(whole, 7.0)
     for e in range(c.E):

@@ -17,7 +17,7 @@
 // without any repacking.
 //
 // Measured, all experts (2048 x 768, 128 of them, top 8, Zipf 1.1): one token 5.4 + 3.9 us (up + down; launch
-// latency), 16 tokens 15 + 9 us (3.4 and 2.8 TB/s of weights), with 4-bit activations 13 + 7; 8,192 tokens 348 + 238 us
+// latency), 16 tokens 14 + 9 us (3.6 and 2.8 TB/s of weights), with 4-bit activations 12 + 7; 8,192 tokens 348 + 238 us
 // (1,180 and 860 TFLOP/s, without the 47 experts of at most 16 rows 1,240 and 900; a library product of bf16
 // matrices of 32768 x 2048 x 1536 runs at 1,372), with 4-bit activations 177 + 136 (2,320 and 1,510 TFLOP/s).
 #include "ffn_common.h"
@@ -50,10 +50,12 @@ struct MxArgs {
   int32_t known;            // the listed experts' row counts were given
 };
 struct SmallArgs : MxArgs {
+  int32_t items, bufs;      // small_rows
   ExpertList list;
 };
 struct TiledArgs : MxArgs {
   int32_t tile_wgs;         // workgroups that take tiles; the others take the small experts
+  int32_t items;            // small_rows
   ExpertList list, small;
 };
 
@@ -121,14 +123,15 @@ __device__ __forceinline__ uint32_t block_codes(const float (&v)[8], int byte) {
 // Experts with at most 16 rows (decode, and the smallest experts of a prefill)
 // =============================================================================================
 
-// One workgroup: 16 NF weight rows (MODE 0: 8 NF columns of gate and of up; MODE 1: 16 NF hidden rows) x the
-// expert's rows.  Its four wavefronts split K in units of 256, whose sums meet in LDS in wavefront order.
-// Bound by the weight bytes: a wavefront brings up to kUnits units of its weights at once, by direct loads
-// of whole cache lines (8 rows x 128 bytes) into LDS, from where it reads the operands (swizzled as in the
-// tiles below); straight to registers in operand order, the lanes' 64 places of 16 bytes a load bound the
-// kernel at 3 TB/s.  The rows' activations go to registers: only the lanes of rows that are there load.
-// 41 experts of 2048 x 1408: up 30 us, down 20 us (4.1 and 3.1 TB/s), with 4-bit activations 26 and 17 (4.8 and 3.7,
-// a large copy's rate is 5.2); the decoding of the weights to bf16 is what the 4-bit form saves.
+// One workgroup: `items` times 16 NF weight rows (MODE 0: 8 NF columns of gate and of up; MODE 1: 16 NF hidden rows) x
+// the expert's rows.  Its four wavefronts split K in units of 256, whose sums meet in LDS in wavefront order.
+// Bound by the weight bytes: a wavefront brings its weights by direct loads of whole cache lines (8 rows x
+// 128 bytes) into LDS, from where it reads the operands (swizzled as in the tiles below), two units in two
+// buffers, from item to item; straight to registers in operand order, the lanes' 64 places of 16 bytes a load
+// bound the kernel at 3 TB/s.  The rows' activations go to registers, once for all items where two units hold them:
+// only the lanes of rows that are there load.
+// 31 experts of 2048 x 768 (16 tokens, Zipf 1.1): up 14 us, down 9 us (3.6 and 2.8 TB/s), with 4-bit activations 12
+// and 7 (4.4 and 3.4; a large copy's rate is 5.2).  The decoding of the weights to bf16 is what the 4-bit form saves.
 constexpr int kUnits = 2;
 __device__ __forceinline__ int swz_w16(int row) { return (row >> 1) & 7; }   // 16 consecutive rows
 
@@ -136,44 +139,52 @@ template <int NF>
 constexpr int kUnitBytes = 16 * NF * 136;   // LDS of a unit: codes, scales
 template <int NF>
 constexpr int kSmallBytes = 4 * kUnits * kUnitBytes<NF>;   // LDS of a workgroup, at most
-// bx: number of its weight rows; tid: 0 to 255
+// bx: number of its first item; bufs: buffers of a wavefront, 1 only for one item of up to one unit a wavefront; tid:
+// 0 to 255
 template <int MODE, bool Q, int NF>
-__device__ __forceinline__ void small_rows(const MxArgs& a, int e, int slot, int bx, char* smem, int tid) {
+__device__ __forceinline__ void small_rows(const MxArgs& a, int e, int slot, int bx, int items, int bufs, char* smem,
+                                           int tid) {
   constexpr int kRowsW = 16 * NF, kW = kRowsW * 128, kUnit = kUnitBytes<NF>;
+  constexpr int kRowsItem = MODE == 0 ? 8 * NF : 16 * NF, kLoads = 2 * NF + NF / 2;   // direct loads of a unit
   const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, q = lane >> 4;
   const int64_t K = MODE == 0 ? a.H : a.I;
   const int chunks = (int)(K / 128), units = (chunks + 1) / 2;
-  const int u0 = wave * units / 4, u1 = (wave + 1) * units / 4;
-  const uint32_t lds0 = lds_addr(smem) + (uint32_t)(wave * min(kUnits, (units + 3) / 4) * kUnit);
+  auto first_unit = [&](int w) { return w * units / 4; };
+  const int u0 = first_unit(wave), mine = first_unit(wave + 1) - u0, steps = mine * items;
+  const uint32_t lds0 = lds_addr(smem) + (uint32_t)(wave * bufs * kUnit);
 
-  const Weights wp0 = weights_at<MODE>(a, slot, 0, MODE == 0 ? bx * (8 * NF) : bx * (16 * NF));
-  const Weights wp1 = MODE == 0 ? weights_at<MODE>(a, slot, 1, bx * (8 * NF)) : wp0;
-  u32x2 sv[kUnits];
-  auto load_w = [&](int u, int b) {
-    const uint32_t dst = lds0 + (uint32_t)(b * kUnit);
+  // the loads run over the items' units: the next one's item and unit
+  const Weights w0 = weights_at<MODE>(a, slot, 0, (int64_t)bx * kRowsItem);
+  int issued = 0, item = 0, unit = 0;
+  auto load_next = [&]() {
+    if (issued == steps) return;
+    const uint32_t dst = lds0 + (uint32_t)((issued & 1) * kUnit);
+    const int u = u0 + unit;
     const bool tail = 2 * u + 1 >= chunks;   // half a unit: its other half is read again, not multiplied
+    const int64_t row = (int64_t)item * kRowsItem;
+    const uint8_t* const codes = w0.codes + row * (K / 2) + u * 128;
 #pragma unroll
     for (int j = 0; j < 2 * NF; ++j) {
       const int t = 8 * j + (lane >> 3), part = MODE == 0 ? j / NF : 0;
       const int piece = (lane & 7) ^ swz_w16(t);
       const uint32_t off = (uint32_t)(t - part * 8 * NF) * (uint32_t)(K / 2) + (uint32_t)((tail ? piece & 3 : piece) * 16);
-      dma16(reinterpret_cast<const char*>(uniform_ptr((part ? wp1.codes : wp0.codes) + u * 128)), off,
-            dst + (uint32_t)(j * 1024));
+      dma16(reinterpret_cast<const char*>(uniform_ptr(codes + (part ? a.H * a.I / 2 : 0))), off, dst + (uint32_t)(j * 1024));
     }
-    const int part = MODE == 0 && lane >= 8 * NF;
-    const uint8_t* sp = (part ? wp1.scales : wp0.scales) + (int64_t)(lane - part * 8 * NF) * (K / 32) + u * 8;
-    if (lane < kRowsW) {
-      if (tail) __builtin_memcpy(&sv[b], sp, 4);
-      else __builtin_memcpy(&sv[b], sp, 8);
+    const uint8_t* const scales = w0.scales + row * (K / 32) + u * 8;   // 8 bytes a row, two lanes
+#pragma unroll
+    for (int j = 0; j < NF / 2; ++j) {
+      const int t = 32 * j + (lane >> 1), part = MODE == 0 && t >= 8 * NF;
+      const uint32_t off = (uint32_t)(t - part * 8 * NF) * (uint32_t)(K / 32) + (tail ? 0u : (uint32_t)((lane & 1) * 4)) +
+                           (part ? (uint32_t)(a.H * a.I / 32) : 0u);
+      dma4(reinterpret_cast<const char*>(uniform_ptr(scales)), off, dst + (uint32_t)(kW + j * 256));
     }
+    ++issued;
+    if (++unit == mine) unit = 0, ++item;
   };
   // the first units' weights do not depend on the expert's rows: where those are known to be 1 to 16, their
   // loads go first
-  if (a.known)
-#pragma unroll
-    for (int b = 0; b < kUnits; ++b)
-      if (u0 + b < u1) load_w(u0 + b, b);
+  if (a.known) load_next(), load_next();
   const int64_t start = a.starts[e];
   const int64_t n = a.starts[e + 1] - start;
   if (n < 1 || n > kSmallRows) {
@@ -187,108 +198,149 @@ __device__ __forceinline__ void small_rows(const MxArgs& a, int e, int slot, int
   const uint8_t* xs = MODE == 0 ? a.x_scales : a.act_scales;
   xp += Q ? src * (K / 2) + q * 16 : src * K * 2 + q * 64;
   if (Q) xs += src * (K / 32) + q;
-  floatx4 acc[NF];
-#pragma unroll
-  for (int f = 0; f < NF; ++f) acc[f] = floatx4{0, 0, 0, 0};
-  for (int u = u0; u < u1; u += kUnits) {
-    if (u > u0) wait_cnt<0>();   // the last units' operands are read
-    if (u > u0 || !a.known)
-#pragma unroll
-      for (int b = 0; b < kUnits; ++b)
-        if (u + b < u1) load_w(u + b, b);
-    constexpr int XL = Q ? 1 : 4;   // 16-byte loads of a lane and chunk
-    u32x4 xv[kUnits][2][XL] = {};
-    uint32_t xb[kUnits][2] = {};
+  constexpr int XL = Q ? 1 : 4;   // 16-byte loads of a lane and chunk
+  u32x4 xv[kUnits][2][XL] = {};
+  uint32_t xb[kUnits][2] = {};
+  auto load_x = [&](int lu) {     // of the units lu, lu + 1 of the wavefront's
     if (live)
 #pragma unroll
       for (int b = 0; b < kUnits; ++b)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const int c = 2 * (u + b) + j;
-          if (u + b < u1 && c < chunks) {
+          const int c = 2 * (u0 + lu + b) + j;
+          if (lu + b < mine && c < chunks) {
 #pragma unroll
             for (int s = 0; s < XL; ++s) xv[b][j][s] = *(const u32x4*)(xp + (int64_t)c * (Q ? 64 : 256) + s * 16);
             if (Q) xb[b][j] = xs[c * 4];
           }
         }
+  };
+  int64_t o = 0;
+  float wt = 0;
+  if constexpr (MODE == 1) {
+    const int64_t t = a.rows[p] * a.k + a.cols[p];
+    wt = bf16_to_f32(a.w[t]);
+    o = a.out_mode == 0 ? t : p;
+  }
+  load_x(0);
+  if (!a.known) load_next(), load_next();
+  // what was loaded to registers is awaited here: later waits leave the direct loads that they do not need
 #pragma unroll
-    for (int b = 0; b < kUnits; ++b)
-      if (u + b < u1 && lane < kRowsW)
-        *reinterpret_cast<__attribute__((address_space(3))) u32x2*>(
-            (uintptr_t)(lds0 + (uint32_t)(b * kUnit + kW + lane * 8))) = sv[b];
-    wait_cnt<0>();   // the wavefront's own LDS: no barrier
+  for (int b = 0; b < kUnits; ++b)
 #pragma unroll
-    for (int b = 0; b < kUnits; ++b) {
-      if (u + b >= u1) break;
-      const uint32_t at = lds0 + (uint32_t)(b * kUnit);
+    for (int j = 0; j < 2; ++j) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        if (2 * (u + b) + j >= chunks) break;
+      for (int s = 0; s < XL; ++s) asm volatile("" : "+v"(xv[b][j][s]));
+      if (Q) asm volatile("" : "+v"(xb[b][j]));
+    }
+  if constexpr (MODE == 1) asm volatile("" : "+v"(wt), "+v"(o));
+
+  int step = 0;
+  for (int m = 0; m < items; ++m) {
+    floatx4 acc[NF];
 #pragma unroll
-        for (int f = 0; f < NF; ++f) {
-          const u32x4 c = lds_get<lds_u32x4>(at + (uint32_t)(f * 2048 + r * 128 + (((4 * j + q) ^ swz_w16(r)) << 4)));
-          const uint32_t sw = lds_get<lds_u32>(at + (uint32_t)(kW + (f * 16 + r) * 8 + j * 4));
-          if constexpr (Q) {
-            acc[f] = mma_fp4(c, (int)(sw >> (8 * q)), xv[b][j][0], (int)xb[b][j], acc[f]);
-          } else {
-            const float sc = scale_of(__builtin_amdgcn_ubfe(sw, 8 * q, 8));
+    for (int f = 0; f < NF; ++f) acc[f] = floatx4{0, 0, 0, 0};
+    for (int lu = 0; lu < mine; lu += kUnits) {
+      if (mine > kUnits && lu + m > 0) load_x(lu);
 #pragma unroll
-            for (int s = 0; s < 4; ++s)
-              acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(decode8(c[s], sc), __builtin_bit_cast(bf16x8, xv[b][j][s]),
-                                                               acc[f], 0, 0, 0);
+      for (int b = 0; b < kUnits; ++b) {
+        if (lu + b >= mine) break;
+        if (issued > step + 1) wait_cnt<kLoads>();   // the wavefront's own LDS: no barrier
+        else wait_cnt<0>();
+        const uint32_t at = lds0 + (uint32_t)((step & 1) * kUnit);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          if (2 * (u0 + lu + b) + j >= chunks) break;
+#pragma unroll
+          for (int f = 0; f < NF; ++f) {
+            const u32x4 c = lds_get<lds_u32x4>(at + (uint32_t)(f * 2048 + r * 128 + (((4 * j + q) ^ swz_w16(r)) << 4)));
+            const uint32_t sw = lds_get<lds_u32>(at + (uint32_t)(kW + (f * 16 + r) * 8 + j * 4));
+            if constexpr (Q) {
+              acc[f] = mma_fp4(c, (int)(sw >> (8 * q)), xv[b][j][0], (int)xb[b][j], acc[f]);
+            } else {
+              const float sc = scale_of(__builtin_amdgcn_ubfe(sw, 8 * q, 8));
+#pragma unroll
+              for (int s = 0; s < 4; ++s)
+                acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(decode8(c[s], sc), __builtin_bit_cast(bf16x8, xv[b][j][s]),
+                                                                 acc[f], 0, 0, 0);
+            }
           }
+        }
+        ++step;
+        // the buffer that is free now; the item's last one takes its sums first
+        if (lu + b + 1 < mine) {
+          wait_cnt<63>();   // its reads have ended
+          load_next();
         }
       }
     }
-  }
-  __syncthreads();   // the weights' LDS becomes that of the sums
-  floatx4(*part)[NF][64] = reinterpret_cast<floatx4(*)[NF][64]>(smem);
+    // a wavefront's sums go where its last unit of the item was
+    auto sums_of = [&](int w) {
+      const int of = first_unit(w + 1) - first_unit(w), last = of ? (of * (m + 1) - 1) & 1 : 0;
+      return lds_addr(smem) + (uint32_t)((w * bufs + last) * kUnit);
+    };
+    wait_cnt<63>();
 #pragma unroll
-  for (int f = 0; f < NF; ++f) part[wave][f][lane] = acc[f];
-  __syncthreads();
-  // lane l of a tile holds the columns (l / 16) * 4 + i of row l % 16
-  auto sum = [&](int f) {
-    floatx4 v = part[0][f][lane];
+    for (int f = 0; f < NF; ++f)
+      *reinterpret_cast<__attribute__((address_space(3))) floatx4*>((uintptr_t)(sums_of(wave) + (uint32_t)((f * 64 + lane) * 16))) =
+          acc[f];
+    wait_cnt<63>();
+    wg_barrier();
+    // lane l of a tile holds the columns (l / 16) * 4 + i of row l % 16
+    auto sum = [&](int f) {
+      floatx4 v = {};
 #pragma unroll
-    for (int w = 1; w < 4; ++w) v += part[w][f][lane];
-    return v;
-  };
-  if constexpr (MODE == 0) {
-    if constexpr (Q) {
-      static_assert(NF == 4);   // a block of 32 columns
-      if (wave != 0) return;
-      float v[8];   // columns 16 (i / 4) + 4 q + i % 4
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const floatx4 g = sum(b), u = sum(2 + b);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[4 * b + i] = silu_mul(g[i], u[i]);
+      for (int w = 0; w < 4; ++w) {
+        const floatx4 part = lds_get<__attribute__((address_space(3))) floatx4>(sums_of(w) + (uint32_t)((f * 64 + lane) * 16));
+        v = w ? v + part : part;
       }
-      const int byte = block_scale(v);
-      const uint32_t c = block_codes(v, byte);
-      if (live) {
-        uint8_t* o = a.act + p * (a.I / 2) + bx * 16 + q * 2;
-        *(uint16_t*)o = (uint16_t)c;
-        *(uint16_t*)(o + 8) = (uint16_t)(c >> 16);
-        if (q == 0) a.act_scales[p * (a.I / 32) + bx] = (uint8_t)byte;
+      return v;
+    };
+    const int at = bx + m;
+    auto next = [&]() {   // the sums are read: the next loads into their place
+      if (m + 1 < items) {
+        wait_cnt<63>();
+        wg_barrier();
+        if (mine) load_next();
+      }
+    };
+    if constexpr (MODE == 0 && Q) {
+      static_assert(NF == 4);   // a block of 32 columns
+      floatx4 g[2], u[2];       // columns 16 b + 4 q + i
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+        if (wave == 0) g[b] = sum(b), u[b] = sum(2 + b);
+      next();
+      if (wave == 0) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = silu_mul(g[i / 4][i & 3], u[i / 4][i & 3]);
+        const int byte = block_scale(v);
+        const uint32_t c = block_codes(v, byte);
+        if (live) {
+          uint8_t* o = a.act + p * (a.I / 2) + at * 16 + q * 2;
+          *(uint16_t*)o = (uint16_t)c;
+          *(uint16_t*)(o + 8) = (uint16_t)(c >> 16);
+          if (q == 0) a.act_scales[p * (a.I / 32) + at] = (uint8_t)byte;
+        }
+      }
+    } else if constexpr (MODE == 0) {
+      floatx4 g = {}, u = {};
+      if (wave < NF / 2) g = sum(wave), u = sum(NF / 2 + wave);
+      next();
+      if (wave < NF / 2) {
+        u32x2 y;
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) y[i / 2] = pk_bf16(silu_mul(g[i], u[i]), silu_mul(g[i + 1], u[i + 1]));
+        if (live) *(u32x2*)(a.act + (p * a.I + at * (8 * NF) + wave * 16 + q * 4) * 2) = y;
       }
     } else {
-      if (wave >= NF / 2) return;
-      const floatx4 g = sum(wave), u = sum(NF / 2 + wave);
-      u32x2 y;
-#pragma unroll
-      for (int i = 0; i < 4; i += 2) y[i / 2] = pk_bf16(silu_mul(g[i], u[i]), silu_mul(g[i + 1], u[i + 1]));
-      if (live) *(u32x2*)(a.act + (p * a.I + bx * (8 * NF) + wave * 16 + q * 4) * 2) = y;
-    }
-  } else {
-    if (wave >= NF) return;
-    const floatx4 y = sum(wave);
-    if (live) {
-      const int64_t t = a.rows[p] * a.k + a.cols[p];
-      const float wt = bf16_to_f32(a.w[t]);
-      const int64_t o = a.out_mode == 0 ? t : p;
-      *(u32x2*)(a.out + o * a.H + bx * (16 * NF) + wave * 16 + q * 4) =
-          u32x2{pk_bf16(y[0] * wt, y[1] * wt), pk_bf16(y[2] * wt, y[3] * wt)};
+      static_assert(NF == 4);   // a tile for each wavefront
+      const floatx4 y = sum(wave);
+      next();
+      if (live)
+        *(u32x2*)(a.out + o * a.H + at * (16 * NF) + wave * 16 + q * 4) =
+            u32x2{pk_bf16(y[0] * wt, y[1] * wt), pk_bf16(y[2] * wt, y[3] * wt)};
     }
   }
 }
@@ -297,25 +349,36 @@ __device__ __forceinline__ void small_rows(const MxArgs& a, int e, int slot, int
 template <int MODE, bool Q>
 constexpr int kSmallNF = MODE == 0 && !Q ? 2 : 4;
 template <int MODE, bool Q>
-__device__ __host__ __forceinline__ int small_cols(const MxArgs& a) {   // workgroups of an expert
+__device__ __host__ __forceinline__ int small_cols(const MxArgs& a) {   // items of an expert
   return (int)(MODE == 0 ? a.I / (8 * kSmallNF<0, Q>) : a.H / (16 * kSmallNF<1, Q>));
+}
+// Items of a workgroup, a power of two that divides an expert's, so many that at most `per_cu` workgroups come to a CU:
+// those that run at once by their LDS (up at 16 tokens 13.5 us, with one item a workgroup 17.5, with 4-bit
+// activations 12 and 15.5), behind tiles twice as many, which level the end (256 tokens of 64 experts of 2048 x 1408
+// 53 + 35 us, with half as many 58 + 40, with one item each 64 + 35).
+inline int small_items(int experts, int cols, int64_t per_cu, int64_t cus) {
+  int items = 1;
+  while (cols % (2 * items) == 0 && (int64_t)experts * (cols / items) > per_cu * cus) items *= 2;
+  return items;
 }
 
 template <int MODE, bool Q>
 __global__ __launch_bounds__(256) void mx_small(SmallArgs a) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
-  small_rows<MODE, Q, kSmallNF<MODE, Q>>(a, a.list.expert[blockIdx.y], a.list.slot[blockIdx.y], blockIdx.x, smem,
-                                         threadIdx.x);
+  small_rows<MODE, Q, kSmallNF<MODE, Q>>(a, a.list.expert[blockIdx.y], a.list.slot[blockIdx.y], blockIdx.x * a.items,
+                                         a.items, a.bufs, smem, threadIdx.x);
 }
 
 template <int MODE, bool Q>
-int small_launch(const SmallArgs& a, hipStream_t s) {
+int small_launch(SmallArgs& a, int64_t cus, hipStream_t s) {
   constexpr int NF = kSmallNF<MODE, Q>;
-  const int64_t K = MODE == 0 ? a.H : a.I, units = ceil_div(K, 256);
-  const dim3 g((unsigned)small_cols<MODE, Q>(a), (unsigned)a.list.n);
-  const int64_t bytes = units > 4 ? kSmallBytes<NF> : kSmallBytes<NF> / kUnits, sums = 4 * NF * 1024;
+  const int64_t K = MODE == 0 ? a.H : a.I;
+  const int cols = small_cols<MODE, Q>(a);
+  a.items = small_items(a.list.n, cols, NF == 2 ? 4 : 2, cus);
+  a.bufs = K > 1024 || a.items > 1 ? kUnits : 1;
+  const dim3 g((unsigned)(cols / a.items), (unsigned)a.list.n);
   launch(MODE == 0 ? "mx_small_up" : "mx_small_down", mx_small<MODE, Q>, g, dim3(256),
-         (uint32_t)(bytes > sums ? bytes : sums), s, a);
+         (uint32_t)(kSmallBytes<NF> / kUnits * a.bufs), s, a);
   FERRY_LAUNCHED("mx_small");
   return 0;
 }
@@ -470,8 +533,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   __shared__ __attribute__((aligned(1024))) char smem[kTileBytes > kSmall ? kTileBytes : kSmall];
   __shared__ RowTables<MODE, TM> tab;
   if ((int)blockIdx.x >= a.tile_wgs) {
-    const int per = small_cols<MODE, false>(a), b = (int)blockIdx.x - a.tile_wgs, li = b / per;
-    small_rows<MODE, false, kSmallNF<MODE, false>>(a, a.small.expert[li], a.small.slot[li], b - li * per, smem, threadIdx.x);
+    const int per = small_cols<MODE, false>(a) / a.items, b = (int)blockIdx.x - a.tile_wgs, li = b / per;
+    small_rows<MODE, false, kSmallNF<MODE, false>>(a, a.small.expert[li], a.small.slot[li], (b - li * per) * a.items, a.items,
+                                                   kUnits, smem, threadIdx.x);
     return;
   }
   build_tile_table<kSmallRows>(a, tt, (uint32_t)a.tile_rows);
@@ -724,9 +788,10 @@ __global__ __launch_bounds__(LARGE ? 512 : 256) __attribute__((amdgpu_waves_per_
   __shared__ __attribute__((aligned(1024))) char smem[kTileBytes > kSmall ? kTileBytes : kSmall];
   __shared__ RowTables<MODE, TM> tab;
   if ((int)blockIdx.x >= a.tile_wgs) {
-    const int per = small_cols<MODE, true>(a) / (W / 4), b = (int)blockIdx.x - a.tile_wgs, li = b / per;
+    const int per = small_cols<MODE, true>(a) / (W / 4 * a.items), b = (int)blockIdx.x - a.tile_wgs, li = b / per;
     const int part = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);   // LARGE: two workgroups' work of one expert
-    small_rows<MODE, true, kSmallNF<MODE, true>>(a, a.small.expert[li], a.small.slot[li], W / 4 * (b - li * per) + part,
+    small_rows<MODE, true, kSmallNF<MODE, true>>(a, a.small.expert[li], a.small.slot[li],
+                                                 (W / 4 * (b - li * per) + part) * a.items, a.items, kUnits,
                                                  smem + part * (kSmall / (W / 4)), threadIdx.x & 255);
     return;
   }
@@ -944,7 +1009,7 @@ int launch_lists(TiledArgs& a, const int64_t (&tiles)[3], int32_t phases, int64_
       SmallArgs b;
       (MxArgs&)b = a;
       b.list = a.small;
-      if (const int rc = mode == 0 ? small_launch<0, Q>(b, s) : small_launch<1, Q>(b, s)) return rc;
+      if (const int rc = mode == 0 ? small_launch<0, Q>(b, cus, s) : small_launch<1, Q>(b, cus, s)) return rc;
       continue;
     }
     const int64_t large = mode == 0 ? a.I / kOutCols<0> : a.H / kOutCols<1>;   // column tiles
@@ -954,7 +1019,9 @@ int launch_lists(TiledArgs& a, const int64_t (&tiles)[3], int32_t phases, int64_
     a.tile_rows = 256 >> by;
     const int64_t t = tiles[by] * cols;
     a.tile_wgs = (int32_t)(t < most ? ceil_div(t, 8) * 8 : most);
-    const int small = a.small.n * (mode == 0 ? small_cols<0, Q>(a) : small_cols<1, Q>(a)) / (use_large ? 2 : 1);
+    const int part = use_large ? 2 : 1, items = (mode == 0 ? small_cols<0, Q>(a) : small_cols<1, Q>(a)) / part;
+    a.items = small_items(a.small.n, items, use_large ? 2 : 4, cus);
+    const int small = a.small.n * (items / a.items);
     const dim3 grid((unsigned)(a.tile_wgs + small)), block(use_large ? 512 : 256);
     const char* const name = mode == 0 ? "mx_tiled_up" : "mx_tiled_down";
     if constexpr (!Q) launch(name, mode == 0 ? mx_tiled16<0> : mx_tiled16<1>, grid, block, 0, s, a);

@@ -184,7 +184,9 @@ __device__ __forceinline__ void small_rows(const MxArgs& a, int e, int slot, int
   };
   // the first units' weights do not depend on the expert's rows: where those are known to be 1 to 16, their
   // loads go first
-  if (a.known) load_next(), load_next();
+  if (a.known)
+#pragma unroll 1
+    for (int i = 0; i < kUnits; ++i) load_next();
   const int64_t start = a.starts[e];
   const int64_t n = a.starts[e + 1] - start;
   if (n < 1 || n > kSmallRows) {
@@ -223,7 +225,9 @@ __device__ __forceinline__ void small_rows(const MxArgs& a, int e, int slot, int
     o = a.out_mode == 0 ? t : p;
   }
   load_x(0);
-  if (!a.known) load_next(), load_next();
+  if (!a.known)
+#pragma unroll 1
+    for (int i = 0; i < kUnits; ++i) load_next();
   // what was loaded to registers is awaited here: later waits leave the direct loads that they do not need
 #pragma unroll
   for (int b = 0; b < kUnits; ++b)
@@ -245,6 +249,10 @@ __device__ __forceinline__ void small_rows(const MxArgs& a, int e, int slot, int
 #pragma unroll
       for (int b = 0; b < kUnits; ++b) {
         if (lu + b >= mine) break;
+        if (step > 0) {   // into the last unit's buffer, whose operands or sums have been read
+          wait_cnt<63>();
+          load_next();
+        }
         if (issued > step + 1) wait_cnt<kLoads>();   // the wavefront's own LDS: no barrier
         else wait_cnt<0>();
         const uint32_t at = lds0 + (uint32_t)((step & 1) * kUnit);
@@ -267,11 +275,6 @@ __device__ __forceinline__ void small_rows(const MxArgs& a, int e, int slot, int
           }
         }
         ++step;
-        // the buffer that is free now; the item's last one takes its sums first
-        if (lu + b + 1 < mine) {
-          wait_cnt<63>();   // its reads have ended
-          load_next();
-        }
       }
     }
     // a wavefront's sums go where its last unit of the item was
@@ -297,11 +300,10 @@ __device__ __forceinline__ void small_rows(const MxArgs& a, int e, int slot, int
       return v;
     };
     const int at = bx + m;
-    auto next = [&]() {   // the sums are read: the next loads into their place
+    auto next = [&]() {   // the sums are read: their place is free
       if (m + 1 < items) {
         wait_cnt<63>();
         wg_barrier();
-        if (mine) load_next();
       }
     };
     if constexpr (MODE == 0 && Q) {
@@ -374,8 +376,10 @@ int small_launch(SmallArgs& a, int64_t cus, hipStream_t s) {
   constexpr int NF = kSmallNF<MODE, Q>;
   const int64_t K = MODE == 0 ? a.H : a.I;
   const int cols = small_cols<MODE, Q>(a);
-  a.items = small_items(a.list.n, cols, NF == 2 ? 4 : 2, cus);
-  a.bufs = K > 1024 || a.items > 1 ? kUnits : 1;
+  // up to one unit a wavefront: one buffer, twice as many workgroups at once (down at 16 tokens, 4-bit activations,
+  // 7.0 us, with two items and two buffers 8.2)
+  a.items = K > 1024 ? small_items(a.list.n, cols, NF == 2 ? 4 : 2, cus) : 1;
+  a.bufs = K > 1024 ? kUnits : 1;
   const dim3 g((unsigned)(cols / a.items), (unsigned)a.list.n);
   launch(MODE == 0 ? "mx_small_up" : "mx_small_down", mx_small<MODE, Q>, g, dim3(256),
          (uint32_t)(kSmallBytes<NF> / kUnits * a.bufs), s, a);

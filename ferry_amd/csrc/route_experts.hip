@@ -20,9 +20,9 @@
 // index (unique: a drawing needs no second search for its owner), until the key is below the k-th's by more than
 // the margin.  The candidates, one to a lane, are ranked by their 64-bit scores.  A row with more than 16 of
 // them, or whose group scores are too near each other for fp32, goes to exact_row.  One token of 256 experts in 8
-// groups, top 8: 6.1 us; 32,768 of them, fp32: 32 us, against 105 with a wavefront a token and 6.5 for the bytes at
-// the rate of a large copy; what is left is instructions (1,360 vector and 570 scalar ones for four tokens, 18 us of
-// issue).
+// groups, top 8: 6.1 us; 32,768 of them, fp32: 30 us, against 105 with a wavefront a token and 6.5 for the bytes at
+// the rate of a large copy; what is left is instructions (1,220 vector and 320 scalar ones for four tokens, 16 us of
+// issue) and, at the end, the last rows of exact_row (about 6 us).  An eighth wavefront on a SIMD changes nothing.
 //
 // The margin.  e^y as 2^(y log2 e) in fp32 is off by at most (2.5 |y| + 2) 2^-24 of itself: y's and the product's
 // rounding, the constant's and the instruction's.  Without a bias an expert's choice score is 1 / (1 + e^-x) or
@@ -473,22 +473,31 @@ __global__ __launch_bounds__(64 * kWaves) void route_many(RouteArgs a) {
   }
   // Each lane sorts its keys; a drawing takes the largest of the lanes' first ones.  The r-th goes to lane r.
   sort_keys(key);
-  uint32_t mine = 0, floor = 0;
-  bool more = !exact;
-  for (int r = 0; r < 17 && __any(more); ++r) {
-    const uint32_t m = largest16(key[0]);
-    more = more && m != 0 && (r < a.topk || (m & ~kLow) >= floor);
-    if (more) {
-      if (r == a.topk - 1) {
-        const float v = unordered(m & ~kLow);
-        floor = fabsf(v) < 0x1p100f ? ordered(v - margin_of(a, v)) & ~kLow : 0u;
-      }
-      if (l == r) mine = m;
-      exact = r == 16;
-      const uint32_t owner = key[0] == m ? ~0u : 0u;   // its keys move up
+  uint32_t mine = 0, m = 0;
+  auto draw = [&](int r) {
+    if (l == r) mine = m;
+    const bool owner = key[0] == m;   // its keys move up
 #pragma unroll
-      for (int j = 0; j + 1 < N; ++j) key[j] = (key[j + 1] & owner) | (key[j] & ~owner);
-      key[N - 1] &= ~owner;
+    for (int j = 0; j < N; ++j) {
+      const uint32_t up = j + 1 < N ? key[j + 1] : 0u;
+      const uint32_t stay = key[j];   // values, not places: a chosen place would become a search through all keys
+      key[j] = owner ? up : stay;
+    }
+  };
+  for (int r = 0; r < a.topk; ++r) {
+    m = largest16(key[0]);
+    draw(r);
+  }
+  const float kth = unordered(m & ~kLow);
+  const uint32_t floor = fabsf(kth) < 0x1p100f ? ordered(kth - margin_of(a, kth)) & ~kLow : 0u;
+  bool more = !exact;
+  for (int r = a.topk; r < 17; ++r) {
+    m = largest16(key[0]);
+    more = more && m != 0 && (m & ~kLow) >= floor;
+    if (!__any(more)) break;
+    if (more) {
+      draw(r);
+      exact = r == 16;
     }
   }
   const bool cand = mine != 0;
@@ -496,13 +505,18 @@ __global__ __launch_bounds__(64 * kWaves) void route_many(RouteArgs a) {
   const double logit = load_logit<T>(a.logits, t * a.experts + e);
   const double s = score_of<SIGMOID>(logit, (double)most, inv);
   const double v = cand ? choice_of(a, logit, s, e) : __builtin_nan("");
-  double ov = v;
-  int oe = e, rank = 0;
+  // the r-th lane's is the r-th best, unless two near ones are the other way round
+  double ov = dpp64<kRor1>(v);
+  int oe = (int)dpp<kRor1>((uint32_t)e), ol = (int)dpp<kRor1>((uint32_t)l), rank = l;
+  const bool ahead = ov > v || (ov == v && oe < e);
+  if (__any(cand && ((ol == l - 1 && !ahead) || (ol == l + 1 && ahead)))) {
+    rank = ahead;
 #pragma unroll
-  for (int i = 0; i < 15; ++i) {
-    ov = dpp64<kRor1>(ov);
-    oe = (int)dpp<kRor1>((uint32_t)oe);
-    rank += ov > v || (ov == v && oe < e);
+    for (int i = 1; i < 15; ++i) {
+      ov = dpp64<kRor1>(ov);
+      oe = (int)dpp<kRor1>((uint32_t)oe);
+      rank += ov > v || (ov == v && oe < e);
+    }
   }
   const bool chosen = cand && rank < a.topk;
   const double total = reduce16(chosen ? s : 0.0, Sum());

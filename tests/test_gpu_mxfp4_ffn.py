@@ -169,6 +169,19 @@ def test_many_rows(device, H, I, counts, quantised):
 
 
 @pytest.mark.parametrize('quantised', QUANTISED)
+@pytest.mark.parametrize('H,I,more', [(4224, 2944, []), (4352, 2816, [40, 130])])
+def test_many_small_experts_with_long_rows(device, H, I, more, quantised):
+    """Several groups of weight rows a workgroup, rows of more units than it holds; alone and behind tiles."""
+    c = Case([int(v) for v in np.random.default_rng(1).integers(0, 17, 40)] + more, H, I, k=8, seed=11, scale=0.02)
+    whole = c.check(quantised)
+    out = torch.full_like(whole, 7.0)
+    for e in range(0, c.E, 3):
+        c.run(quantised, [e], out=out)
+        at = slice(int(c.starts[e]), int(c.starts[e + 1]))
+        assert torch.equal(out[at], whole[at])
+
+
+@pytest.mark.parametrize('quantised', QUANTISED)
 @pytest.mark.parametrize('counts', [[1380, 17, 720, 1224, 90, 1046, 562, 0, 276, 129, 3],
                                     [3380, 17, 1720, 2224, 90, 3046, 562, 0, 1276, 129, 3, 200]])
 def test_more_tiles_than_workgroups(device, counts, quantised):

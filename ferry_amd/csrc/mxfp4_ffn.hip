@@ -17,7 +17,7 @@
 // without any repacking.
 //
 // Measured, all experts (2048 x 768, 128 of them, top 8, Zipf 1.1): one token 5.4 + 3.9 us (up + down; launch
-// latency), 16 tokens 14 + 9 us (3.6 and 2.8 TB/s of weights), with 4-bit activations 12 + 7; 8,192 tokens 348 + 238 us
+// latency), 16 tokens 14 + 8.6 us (3.6 and 3.0 TB/s of weights), with 4-bit activations 12 + 7; 8,192 tokens 348 + 238 us
 // (1,180 and 860 TFLOP/s, without the 47 experts of at most 16 rows 1,240 and 900; a library product of bf16
 // matrices of 32768 x 2048 x 1536 runs at 1,372), with 4-bit activations 177 + 136 (2,320 and 1,510 TFLOP/s).
 #include "ffn_common.h"
@@ -130,7 +130,7 @@ __device__ __forceinline__ uint32_t block_codes(const float (&v)[8], int byte) {
 // buffers, from item to item; straight to registers in operand order, the lanes' 64 places of 16 bytes a load
 // bound the kernel at 3 TB/s.  The rows' activations go to registers, once for all items where two units hold them:
 // only the lanes of rows that are there load.
-// 31 experts of 2048 x 768 (16 tokens, Zipf 1.1): up 14 us, down 9 us (3.6 and 2.8 TB/s), with 4-bit activations 12
+// 31 experts of 2048 x 768 (16 tokens, Zipf 1.1): up 14 us, down 8.6 us (3.6 and 3.0 TB/s), with 4-bit activations 12
 // and 7 (4.4 and 3.4; a large copy's rate is 5.2).  The decoding of the weights to bf16 is what the 4-bit form saves.
 constexpr int kUnits = 2;
 __device__ __forceinline__ int swz_w16(int row) { return (row >> 1) & 7; }   // 16 consecutive rows
@@ -364,8 +364,9 @@ inline int small_items(int experts, int cols, int64_t per_cu, int64_t cus) {
   return items;
 }
 
+// Down with bf16 activations: within the registers of four workgroups a CU (16 tokens 8.6 us, with three 9.7).
 template <int MODE, bool Q>
-__global__ __launch_bounds__(256) void mx_small(SmallArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(MODE == 1 && !Q ? 4 : 1))) void mx_small(SmallArgs a) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   small_rows<MODE, Q, kSmallNF<MODE, Q>>(a, a.list.expert[blockIdx.y], a.list.slot[blockIdx.y], blockIdx.x * a.items,
                                          a.items, a.bufs, smem, threadIdx.x);

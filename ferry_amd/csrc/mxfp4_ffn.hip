@@ -5,8 +5,8 @@
 //   out = bf16(y * w[rows[p], cols[p]])
 // with cache[slot] = [codes of Wg (I x H) | Wu (I x H) | Wd (H x I), then their scales], the MXFP4 form
 // of the bf16 cache row (mxfp4.hip).  Sums are fp32.  Two kinds of activations:
-//  * bf16 (Q = false): x is bf16 and a is rounded to bf16, an operand of the bf16 matrix instruction.
-//    The 4-bit weights become bf16 in registers, which is exact.
+//  * bf16 (Q = false): x is bf16 and a is rounded to bf16, an operand of the bf16 matrix instruction (but for
+//    calls of very few rows: small_rows).  The 4-bit weights become bf16 in registers, which is exact.
 //  * MXFP4 (Q = true): x is codes and scales, and a is quantised from fp32 in the up epilogue, per 32
 //    columns, as mxfp4_quantize does; both products run on the scaled 4-bit matrix instruction.
 //
@@ -48,6 +48,7 @@ struct MxArgs {
   int32_t out_mode;
   int32_t tile_rows;        // of the tiled kernels: at most theirs
   int32_t known;            // the listed experts' row counts were given
+  int32_t fine;             // small_rows
 };
 struct SmallArgs : MxArgs {
   int32_t items, bufs;      // small_rows
@@ -132,7 +133,49 @@ __device__ __forceinline__ uint32_t block_codes(const float (&v)[8], int byte) {
 // only the lanes of rows that are there load.
 // 31 experts of 2048 x 768 (16 tokens, Zipf 1.1): up 14 us, down 8.6 us (3.6 and 3.0 TB/s), with 4-bit activations 12
 // and 7 (4.4 and 3.4; a large copy's rate is 5.2).  The decoding of the weights to bf16 is what the 4-bit form saves.
+//
+// In calls of at most kFinePairs (token, expert) pairs the activations of experts with at most kFineRows rows are not
+// rounded to bf16 between up and down: in the space of four bf16 columns stand four 14-bit integers and their
+// power of two.  Down multiplies the integers' upper bits in the rows 0 to 7 of the instruction and their lower bits, both exact in
+// bf16, in the rows 8 to 15 that such experts leave empty, and adds the two.  The rounding to bf16 costs an output as
+// much as its own does, 1.4 times the error in the mean over many rows, up to 1.55 times over eight.  Down of
+// one token takes 5.5 us so, otherwise 4.6; larger calls would pay more (16 tokens 14.5 us instead of 8.4) for less.
+constexpr int kFineRows = 8, kFinePairs = 64;
 constexpr int kUnits = 2;
+
+// v as integers of 14 bits times 2^(e - 139), e the biased exponent of the largest (at least 13); 255: NaNs
+__device__ __forceinline__ u32x2 fine_pack(const float (&v)[4]) {
+  uint32_t amax = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) amax = max(amax, __float_as_uint(v[i]) & 0x7fffffffu);
+  const uint32_t e = max(amax >> 23, 13u);
+  const float up = __uint_as_float((266u - e) << 23);   // 2^(139 - e)
+  uint32_t n[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) n[i] = (uint32_t)(int)fminf(fmaxf(__builtin_rintf(v[i] * up), -8191.0f), 8191.0f) & 0x3fffu;
+  return u32x2{n[0] | n[1] << 14 | n[2] << 28, n[2] >> 4 | n[3] << 10 | e << 24};
+}
+// eight of them: the upper bits, or with `low` the others, as bf16
+__device__ __forceinline__ u32x4 fine_unpack(u32x4 c, bool low) {
+  const uint32_t mask = low ? 0xffff0000u : 0u;
+  u32x4 y;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t a = c[2 * h], b = c[2 * h + 1], e = b >> 24;
+    const float s = __uint_as_float(e == 255 ? 0x7fc00000u : (e - 12) << 23);
+    const uint32_t n[4] = {a & 0x3fffu, (a >> 14) & 0x3fffu, __builtin_amdgcn_alignbit(b, a, 28) & 0x3fffu, (b >> 10) & 0x3fffu};
+    uint32_t x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      // 2^23 + 2^13 + the signed integer, as a float's bits
+      const float f = (__uint_as_float((n[i] ^ 0x2000u) | 0x4b000000u) - 8396800.0f) * s;
+      x[i] = __float_as_uint(f - __uint_as_float(__float_as_uint(f) & mask));
+    }
+    y[2 * h] = __builtin_amdgcn_perm(x[1], x[0], 0x07060302u);
+    y[2 * h + 1] = __builtin_amdgcn_perm(x[3], x[2], 0x07060302u);
+  }
+  return y;
+}
 __device__ __forceinline__ int swz_w16(int row) { return (row >> 1) & 7; }   // 16 consecutive rows
 
 template <int NF>
@@ -193,8 +236,10 @@ __device__ __forceinline__ void small_rows(const MxArgs& a, int e, int slot, int
     wait_cnt<0>();
     return;
   }
-  const bool live = r < n;
-  const int64_t p = start + (live ? r : 0);
+  const bool fine = !Q && a.fine && n <= kFineRows;
+  const int row = MODE == 1 && fine ? r & 7 : r;
+  const bool live = row < n;
+  const int64_t p = start + (live ? row : 0);
   const int64_t src = MODE == 0 ? a.rows[p] : p;
   const uint8_t* xp = MODE == 0 ? a.x : a.act;
   const uint8_t* xs = MODE == 0 ? a.x_scales : a.act_scales;
@@ -238,6 +283,18 @@ __device__ __forceinline__ void small_rows(const MxArgs& a, int e, int slot, int
       if (Q) asm volatile("" : "+v"(xb[b][j]));
     }
   if constexpr (MODE == 1) asm volatile("" : "+v"(wt), "+v"(o));
+  auto unpack_x = [&]() {
+    if constexpr (MODE == 1 && !Q)
+      if (fine)
+#pragma unroll
+        for (int b = 0; b < kUnits; ++b)
+          if (b < mine)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int s = 0; s < XL; ++s) xv[b][j][s] = fine_unpack(xv[b][j][s], r >= 8);
+  };
+  unpack_x();
 
   int step = 0;
   for (int m = 0; m < items; ++m) {
@@ -245,7 +302,7 @@ __device__ __forceinline__ void small_rows(const MxArgs& a, int e, int slot, int
 #pragma unroll
     for (int f = 0; f < NF; ++f) acc[f] = floatx4{0, 0, 0, 0};
     for (int lu = 0; lu < mine; lu += kUnits) {
-      if (mine > kUnits && lu + m > 0) load_x(lu);
+      if (mine > kUnits && lu + m > 0) load_x(lu), unpack_x();
 #pragma unroll
       for (int b = 0; b < kUnits; ++b) {
         if (lu + b >= mine) break;
@@ -331,16 +388,20 @@ __device__ __forceinline__ void small_rows(const MxArgs& a, int e, int slot, int
       if (wave < NF / 2) g = sum(wave), u = sum(NF / 2 + wave);
       next();
       if (wave < NF / 2) {
-        u32x2 y;
+        float v[4];
 #pragma unroll
-        for (int i = 0; i < 4; i += 2) y[i / 2] = pk_bf16(silu_mul(g[i], u[i]), silu_mul(g[i + 1], u[i + 1]));
+        for (int i = 0; i < 4; ++i) v[i] = silu_mul(g[i], u[i]);
+        const u32x2 y = fine ? fine_pack(v) : u32x2{pk_bf16(v[0], v[1]), pk_bf16(v[2], v[3])};
         if (live) *(u32x2*)(a.act + (p * a.I + at * (8 * NF) + wave * 16 + q * 4) * 2) = y;
       }
     } else {
       static_assert(NF == 4);   // a tile for each wavefront
-      const floatx4 y = sum(wave);
+      floatx4 y = sum(wave);
       next();
-      if (live)
+      if (fine)   // the lower bits' rows
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] += __shfl_xor(y[i], 8, 64);
+      if (live && (!fine || r < 8))
         *(u32x2*)(a.out + o * a.H + at * (16 * NF) + wave * 16 + q * 4) =
             u32x2{pk_bf16(y[0] * wt, y[1] * wt), pk_bf16(y[2] * wt, y[3] * wt)};
     }
@@ -1117,6 +1178,7 @@ extern "C" int ferry_mxfp4_expert_ffn(const void* cache, int64_t cache_rows, int
   a.k = topk;
   a.out_mode = out_mode;
   a.known = list_rows != nullptr;
+  a.fine = pairs <= kFinePairs;
   // Small experts and the others, each up to kListMax of a launch; without row counts every expert is in both, and the
   // kernels pass over those of the other kind by the device's starts.  An expert's own rows decide, so that its
   // results do not depend on which experts are listed with it (the two kinds sum in different orders): with all

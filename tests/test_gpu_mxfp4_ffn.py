@@ -65,8 +65,9 @@ class Case:
         n = self.H * self.I
         return m[:n].view(self.I, self.H), m[n:2 * n].view(self.I, self.H), m[2 * n:].view(self.H, self.I)
 
-    def reference(self, quantised, experts, x=None):
-        """(values, error bound) float64 [P, H] of the grouped rows; NaN rows for experts not in the list."""
+    def reference(self, quantised, experts, x=None, fine=False):
+        """(values, error bound) float64 [P, H] of the grouped rows; NaN rows for experts not in the list.  fine: the
+        activations keep 13 bits of the largest of four columns."""
         P = self.rows.numel()
         out = torch.full((P, self.H), float('nan'), dtype=torch.float64, device='cuda')
         tol = torch.zeros_like(out)
@@ -103,6 +104,9 @@ class Case:
                     near |= (y - m).abs() <= d / step
                 da = torch.where(near | flips, 2 * top, torch.zeros_like(b)).reshape(a.shape)
                 a = av
+            elif fine:   # steps of 2^-12 of the largest's power of two, at most 2^-12 of it; the largest can be 8191 of 8192
+                most = (a.abs() + da).reshape(-1, 4).amax(1, keepdim=True).expand(-1, 4).reshape(a.shape)
+                da = da + 2.0 ** -13 * most
             else:
                 da = da + 2.0 ** -8 * (a.abs() + da)   # the operand's rounding to bf16
             y = a @ wd.t()
@@ -129,10 +133,10 @@ class Case:
                                  counts=self.counts if counts else None, **kw)
         return out
 
-    def check(self, quantised, experts=None, out_mode=1, **kw):
+    def check(self, quantised, experts=None, out_mode=1, fine=False, **kw):
         out = self.run(quantised, experts, out_mode, **kw)
         experts = range(self.E) if experts is None else experts
-        want, tol = self.reference(quantised, experts, kw.get('x'))
+        want, tol = self.reference(quantised, experts, kw.get('x'), fine)
         n = self.rows.numel()
         at = self.rows * self.k + self.cols if out_mode == 0 else torch.arange(n, device='cuda')
         live = ~torch.isnan(want[:, 0])
@@ -166,6 +170,17 @@ def test_many_rows(device, H, I, counts, quantised):
     c = Case(counts, H, I, seed=H + I)
     c.check(quantised)
     c.check(quantised, out_mode=0)
+
+
+@pytest.mark.parametrize('H,I,counts,k', [(2048, 768, [1] * 8, 8), (512, 2816, [8, 5, 1, 0, 8], 4), (128, 128, [1], 1),
+                                          (384, 640, [2, 3, 7, 8, 1], 8), (2048, 4352, [3, 1], 2)])
+@pytest.mark.parametrize('scale', [1.0, 2.0 ** -40, 2.0 ** 25])
+def test_few_pairs_keep_more_than_bf16(device, H, I, counts, k, scale):
+    c = Case(counts, H, I, k=k, seed=H + I)
+    assert c.R * c.k <= 64
+    x = (c.x.float() * scale).to(torch.bfloat16)
+    c.check(False, x=x, fine=True)
+    c.check(False, x=x, fine=True, out_mode=0, counts=False, max_rows=16)
 
 
 @pytest.mark.parametrize('quantised', QUANTISED)

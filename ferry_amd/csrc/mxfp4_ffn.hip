@@ -143,7 +143,8 @@ __device__ __forceinline__ uint32_t block_codes(const float (&v)[8], int byte) {
 constexpr int kFineRows = 8, kFinePairs = 64;
 constexpr int kUnits = 2;
 
-// v as integers of 14 bits times 2^(e - 139), e the biased exponent of the largest (at least 13); 255: NaNs
+// v as integers from -8191 to 8191 (plus 8192) times 2^(e - 139), e the biased exponent of the largest (at least 13);
+// 255: NaNs
 __device__ __forceinline__ u32x2 fine_pack(const float (&v)[4]) {
   uint32_t amax = 0;
 #pragma unroll
@@ -152,25 +153,23 @@ __device__ __forceinline__ u32x2 fine_pack(const float (&v)[4]) {
   const float up = __uint_as_float((266u - e) << 23);   // 2^(139 - e)
   uint32_t n[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) n[i] = (uint32_t)(int)fminf(fmaxf(__builtin_rintf(v[i] * up), -8191.0f), 8191.0f) & 0x3fffu;
+  for (int i = 0; i < 4; ++i) n[i] = (uint32_t)((int)fminf(fmaxf(__builtin_rintf(v[i] * up), -8191.0f), 8191.0f) + 8192);
   return u32x2{n[0] | n[1] << 14 | n[2] << 28, n[2] >> 4 | n[3] << 10 | e << 24};
 }
-// eight of them: the upper bits, or with `low` the others, as bf16
+// eight of them as bf16: what their upper 8 bits stand for, or with `low` the lower 6
 __device__ __forceinline__ u32x4 fine_unpack(u32x4 c, bool low) {
-  const uint32_t mask = low ? 0xffff0000u : 0u;
+  const uint32_t bits = low ? 0x3fu : 0x3fc0u;
+  const float zero = low ? 8388608.0f : 8396800.0f;   // 2^23, and 8192 more
   u32x4 y;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const uint32_t a = c[2 * h], b = c[2 * h + 1], e = b >> 24;
     const float s = __uint_as_float(e == 255 ? 0x7fc00000u : (e - 12) << 23);
-    const uint32_t n[4] = {a & 0x3fffu, (a >> 14) & 0x3fffu, __builtin_amdgcn_alignbit(b, a, 28) & 0x3fffu, (b >> 10) & 0x3fffu};
-    uint32_t x[4];
+    const uint32_t n[4] = {a, a >> 14, __builtin_amdgcn_alignbit(b, a, 28), b >> 10};
+    uint32_t x[4];   // 0x4b000000: 2^23, whose last bit is 1
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      // 2^23 + 2^13 + the signed integer, as a float's bits
-      const float f = (__uint_as_float((n[i] ^ 0x2000u) | 0x4b000000u) - 8396800.0f) * s;
-      x[i] = __float_as_uint(f - __uint_as_float(__float_as_uint(f) & mask));
-    }
+    for (int i = 0; i < 4; ++i)
+      x[i] = __float_as_uint((__uint_as_float((n[i] & bits) | 0x4b000000u) - zero) * s);
     y[2 * h] = __builtin_amdgcn_perm(x[1], x[0], 0x07060302u);
     y[2 * h + 1] = __builtin_amdgcn_perm(x[3], x[2], 0x07060302u);
   }

@@ -262,6 +262,20 @@ def test_special_rows(device, quantised):
     assert bool((got[:n][tok == 2] == 0).all())
 
 
+def test_special_rows_of_few_pairs(device):
+    c = Case([4, 2], 256, 128, k=2, seed=6)
+    x = c.x.clone()
+    want = c.run(False)
+    x[0, 3] = float('inf')
+    x[1, 5] = float('nan')
+    x[2] = 0
+    got = c.run(False, x=x)
+    n, tok = c.rows.numel(), c.rows
+    assert torch.equal(got[:n][tok == 3], want[:n][tok == 3]) and bool((got[n:] == 7).all())
+    assert bool(torch.isnan(got[:n][tok == 1]).all()) and not bool(torch.isfinite(got[:n][tok == 0]).any())
+    assert bool((got[:n][tok == 2] == 0).all())
+
+
 @pytest.mark.parametrize('quantised', QUANTISED)
 def test_scale_bytes_at_the_ends(device, quantised):
     """Weight blocks with the smallest scale, and an expert row with a NaN scale."""

@@ -31,7 +31,7 @@ namespace {
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
-constexpr int kSmallRows = 16;   // experts with at most this many rows run mx_small
+constexpr int kSmallRows = 16;   // experts with at most this many rows run small_rows
 
 struct MxArgs {
   const uint8_t* cache;

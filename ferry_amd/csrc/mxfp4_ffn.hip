@@ -5,8 +5,8 @@
 //   out = bf16(y * w[rows[p], cols[p]])
 // with cache[slot] = [codes of Wg (I x H) | Wu (I x H) | Wd (H x I), then their scales], the MXFP4 form
 // of the bf16 cache row (mxfp4.hip).  Sums are fp32.  Two kinds of activations:
-//  * bf16 (Q = false): x is bf16 and a is rounded to bf16, an operand of the bf16 matrix instruction (but for
-//    calls of very few rows: small_rows).  The 4-bit weights become bf16 in registers, which is exact.
+//  * bf16 (Q = false): x is bf16 and a is rounded to bf16, an operand of the bf16 matrix instruction (in
+//    calls of few pairs to 11 bits: small_rows).  The 4-bit weights become bf16 in registers, which is exact.
 //  * MXFP4 (Q = true): x is codes and scales, and a is quantised from fp32 in the up epilogue, per 32
 //    columns, as mxfp4_quantize does; both products run on the scaled 4-bit matrix instruction.
 //
@@ -135,43 +135,54 @@ __device__ __forceinline__ uint32_t block_codes(const float (&v)[8], int byte) {
 // and 7 (4.4 and 3.4; a large copy's rate is 5.2).  The decoding of the weights to bf16 is what the 4-bit form saves.
 //
 // In calls of at most kFinePairs (token, expert) pairs the activations of experts with at most kFineRows rows are not
-// rounded to bf16 between up and down: in the space of four bf16 columns stand four 14-bit integers and their
-// power of two.  Down multiplies the integers' upper bits in the rows 0 to 7 of the instruction and their lower bits, both exact in
-// bf16, in the rows 8 to 15 that such experts leave empty, and adds the two.  The rounding to bf16 costs an output as
-// much as its own does, 1.4 times the error in the mean over many rows, up to 1.55 times over eight.  Down of
-// one token takes 5.5 us so, otherwise 4.6; larger calls would pay more (16 tokens 14.5 us instead of 8.4) for less.
+// rounded to bf16 between up and down: in their 16 bits stand fp16 numbers below 2, and eight columns share the largest
+// one's 8-bit exponent, a bit of it in each one's highest exponent bit, which is 0.  A column of down to 2^-14 of the
+// largest so has 11 bits and one of down to 2^-17 at least bf16's 8, whatever its neighbours hold; smaller ones are off by at
+// most 2^-25 of the largest.  An infinity stays one, a NaN makes eight of them.  Down multiplies the upper 8 bits in the
+// rows 0 to 7 of the instruction and the lower three, both exact in bf16, in the rows 8 to 15 that such experts leave
+// empty, and adds the two.  An output's mean error is 0.0017 of its size so, its own rounding to bf16, otherwise 0.0023.
+// Down of one token takes 5.7 us so, otherwise 4.9; of 8 tokens 8.9 and 7.0; larger calls would pay more for less (16 tokens
+// 10.2 us instead of 8.2, error 0.0020: experts of more rows keep bf16).
 constexpr int kFineRows = 8, kFinePairs = 64;
 constexpr int kUnits = 2;
 
-// v as integers from -8191 to 8191 (plus 8192) times 2^(e - 139), e the biased exponent of the largest (at least 13);
-// 255: NaNs
-__device__ __forceinline__ u32x2 fine_pack(const float (&v)[4]) {
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+// The shared exponent e is that of the largest column rounded to 11 bits (255: infinite); e - 1 is stored, with a NaN 255 and
+// nothing but ones: its bit 3 - i in column 2 i, its bit 7 - i in column 2 i + 1.
+// This lane's four of eight columns, the others in the lane ^ 16: `upper` the last four.
+__device__ __forceinline__ u32x2 fine_pack(const float (&v)[4], bool upper) {
   uint32_t amax = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) amax = max(amax, __float_as_uint(v[i]) & 0x7fffffffu);
-  const uint32_t e = max(amax >> 23, 13u);
-  const float up = __uint_as_float((266u - e) << 23);   // 2^(139 - e)
-  uint32_t n[4];
+  amax = max(amax, (uint32_t)__shfl_xor((int)amax, 16, 64));
+  const uint32_t e = max((amax + 0x1000u) >> 23, 1u);
+  u32x2 y;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) n[i] = (uint32_t)((int)fminf(fmaxf(__builtin_rintf(v[i] * up), -8191.0f), 8191.0f) + 8192);
-  return u32x2{n[0] | n[1] << 14 | n[2] << 28, n[2] >> 4 | n[3] << 10 | e << 24};
+  for (int j = 0; j < 2; ++j) {
+    const f16x2 n = {(_Float16)__builtin_amdgcn_ldexpf(v[2 * j], 127 - (int)e),
+                     (_Float16)__builtin_amdgcn_ldexpf(v[2 * j + 1], 127 - (int)e)};
+    const uint32_t k = (e - 1) >> (3 - (j + (upper ? 2 : 0)));
+    // an infinity's exponent bits 31 become 15: 2^128
+    y[j] = amax > 0x7f800000u ? ~0u : (__builtin_bit_cast(uint32_t, n) & 0xbfffbfffu) | (k & 1u) << 14 | (k >> 4 & 1u) << 30;
+  }
+  return y;
 }
-// eight of them as bf16: what their upper 8 bits stand for, or with `low` the lower 6
+// the eight as bf16: their upper 8 bits, or with `low` the lower three
 __device__ __forceinline__ u32x4 fine_unpack(u32x4 c, bool low) {
-  const uint32_t bits = low ? 0x3fu : 0x3fc0u;
-  const float zero = low ? 8388608.0f : 8396800.0f;   // 2^23, and 8192 more
+  uint32_t t = c[0] & 0x40004000u;
+#pragma unroll
+  for (int i = 1; i < 4; ++i) t |= c[i] >> i & (0x40004000u >> i);
+  const uint32_t e = (t >> 11 & 15u) | (t >> 23 & 0xf0u);   // less 1
+  const uint32_t bits = (e == 255 ? 0xffffffffu : 0xbfffbfffu) & (low ? ~0u : 0xfff8fff8u);
+  const uint32_t upper = low ? bits & 0xfff8fff8u : 0u;
   u32x4 y;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const uint32_t a = c[2 * h], b = c[2 * h + 1], e = b >> 24;
-    const float s = __uint_as_float(e == 255 ? 0x7fc00000u : (e - 12) << 23);
-    const uint32_t n[4] = {a, a >> 14, __builtin_amdgcn_alignbit(b, a, 28), b >> 10};
-    uint32_t x[4];   // 0x4b000000: 2^23, whose last bit is 1
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      x[i] = __float_as_uint((__uint_as_float((n[i] & bits) | 0x4b000000u) - zero) * s);
-    y[2 * h] = __builtin_amdgcn_perm(x[1], x[0], 0x07060302u);
-    y[2 * h + 1] = __builtin_amdgcn_perm(x[3], x[2], 0x07060302u);
+  for (int i = 0; i < 4; ++i) {
+    const f16x2 part = __builtin_bit_cast(f16x2, c[i] & bits) - __builtin_bit_cast(f16x2, c[i] & upper);
+    const uint32_t x0 = __float_as_uint(__builtin_amdgcn_ldexpf((float)part[0], (int)e - 126));
+    const uint32_t x1 = __float_as_uint(__builtin_amdgcn_ldexpf((float)part[1], (int)e - 126));
+    y[i] = __builtin_amdgcn_perm(x1, x0, 0x07060302u);
   }
   return y;
 }
@@ -390,7 +401,7 @@ __device__ __forceinline__ void small_rows(const MxArgs& a, int e, int slot, int
         float v[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = silu_mul(g[i], u[i]);
-        const u32x2 y = fine ? fine_pack(v) : u32x2{pk_bf16(v[0], v[1]), pk_bf16(v[2], v[3])};
+        const u32x2 y = fine ? fine_pack(v, q & 1) : u32x2{pk_bf16(v[0], v[1]), pk_bf16(v[2], v[3])};
         if (live) *(u32x2*)(a.act + (p * a.I + at * (8 * NF) + wave * 16 + q * 4) * 2) = y;
       }
     } else {
@@ -1179,8 +1190,9 @@ extern "C" int ferry_mxfp4_expert_ffn(const void* cache, int64_t cache_rows, int
   a.known = list_rows != nullptr;
   a.fine = pairs <= kFinePairs;
   // Small experts and the others, each up to kListMax of a launch; without row counts every expert is in both, and the
-  // kernels pass over those of the other kind by the device's starts.  An expert's own rows decide, so that its
-  // results do not depend on which experts are listed with it (the two kinds sum in different orders): with all
+  // kernels pass over those of the other kind by the device's starts.  An expert's own rows (and with a.fine the call's
+  // pairs) decide, so that its results do not depend on which experts are listed with it (the two kinds sum in different
+  // orders): with all
   // experts in tiles wherever one has more than kSmallRows rows, 512 tokens (128 experts of 2048 x 768, top 8,
   // Zipf 1.1) take 110 and 87 us (bf16 and 4-bit activations) instead of 122 and 92, 8,192 tokens 644 and 332
   // instead of 653 and 341.

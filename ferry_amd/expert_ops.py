@@ -435,7 +435,8 @@ def mxfp4_expert_ffn(cache, x, w_sorted, starts, rows, cols, expert_list, slot_o
     """``expert_ffn`` over cache slots of MXFP4 rows (``mxfp4_expert_rows``: uint8 [slots, 3 * hidden *
     intermediate / 32 * 17]), read as they are: 4.25 bits a weight.
 
-    ``x`` is bf16 [R, hidden], with ``act`` bf16 scratch of R * topk * intermediate elements; or
+    ``x`` is bf16 [R, hidden], with ``act`` bf16 scratch of R * topk * intermediate elements (silu(g) * u rounded to
+    bf16; with R * topk <= 64 experts of at most 8 rows keep 11 bits of it, in a format of their own); or
     ``mxfp4_quantize``'s (codes, scales) of the rows, with ``act`` uint8 scratch of R * topk *
     intermediate / 32 * 17 bytes: both products then take 4-bit operands on either side, which is the
     faster form for prompts, and silu(g) * u is quantised on the way.  Sums and SwiGLU are fp32; an

@@ -210,8 +210,8 @@ int ferry_expert_ffn_spare(const void* cache, int64_t cache_rows, int64_t hidden
  * ferry_expert_ffn on MXFP4 cache rows (no counterpart in the reference): cache[slot] holds the codes
  * of [gate I*H | up I*H | down H*I] and then their scales, 3 * H * I / 32 * 17 bytes (ferry_mxfp4_quantize
  * of the bf16 row, or of its three matrices' rows).  With x_scales null, x is bf16 [R, H] and act bf16
- * scratch of R * k * I elements, rounded once from fp32 (with R * k <= 64 and at most 8 rows an expert kept to 13
- * bits of the largest of four columns instead); otherwise x holds the codes [R, H / 2] and
+ * scratch of R * k * I elements, rounded once from fp32 (with R * k <= 64 and at most 8 rows an expert to 11
+ * bits instead of 8, in another format: so an expert's outputs depend on R * k); otherwise x holds the codes [R, H / 2] and
  * x_scales the scales [R, H / 32] of MXFP4 rows, and act is R * k * I / 32 * 17 bytes: the codes
  * [R * k, I / 2] and then the scales [R * k, I / 32] of silu(g) * u, quantised from fp32.  The sums and
  * the SwiGLU are fp32 and an output is rounded once, after its routing weight.  All other arguments as

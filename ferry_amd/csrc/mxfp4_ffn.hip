@@ -23,6 +23,7 @@
 #include "ffn_common.h"
 
 #include <algorithm>
+#include <bitset>
 #include <type_traits>
 
 namespace ferry {
@@ -1157,6 +1158,8 @@ extern "C" int ferry_mxfp4_expert_ffn(const void* cache, int64_t cache_rows, int
   FERRY_CHECK_ARG(((uintptr_t)cache | (uintptr_t)x | (uintptr_t)act | (uintptr_t)out) % 16 == 0,
                   "cache, x, act and out must be 16-byte aligned");
   FERRY_CHECK_ARG((uintptr_t)x_scales % 4 == 0, "x_scales must be 4-byte aligned");
+  std::bitset<FERRY_MAX_EXPERTS> seen;
+  int64_t listed = 0;   // pairs of the listed experts; one may be listed twice
   for (int32_t i = 0; i < n_list; ++i) {
     const int32_t e = expert_list[i];
     FERRY_CHECK_ARG(e >= 0 && e < experts, "expert_list[%d] = %d out of range", i, e);
@@ -1166,7 +1169,10 @@ extern "C" int ferry_mxfp4_expert_ffn(const void* cache, int64_t cache_rows, int
       FERRY_CHECK_ARG(list_rows[i] >= min_rows_per_expert && list_rows[i] <= max_rows_per_expert,
                       "list_rows[%d] = %d outside [min_rows_per_expert, max_rows_per_expert]", i,
                       list_rows[i]);
+    if (list_rows && !seen[e]) listed += list_rows[i];
+    seen[e] = true;
   }
+  FERRY_CHECK_ARG(listed <= rows_in * topk, "list_rows name more than rows * topk pairs");
   int cus = 0;
   if (const int rc = device_cus(&cus)) return rc;
   if (cus > 2 * spare_cus) cus -= spare_cus;

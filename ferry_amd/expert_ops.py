@@ -441,7 +441,8 @@ def mxfp4_expert_ffn(cache, x, w_sorted, starts, rows, cols, expert_list, slot_o
     intermediate / 32 * 17 bytes: both products then take 4-bit operands on either side, which is the
     faster form for prompts, and silu(g) * u is quantised on the way.  Sums and SwiGLU are fp32; an
     output row is rounded to bf16 once, after its routing weight.  The other arguments are
-    ``expert_ffn``'s; rows of ``out`` that belong to experts outside the list are left as they are.
+    ``expert_ffn``'s; ``rows`` and ``cols`` have an entry for every pair of ``starts`` (at least the sum of
+    ``counts``, where those are given); rows of ``out`` that belong to experts outside the list are left as they are.
     No counterpart in the reference.
     """
     R, k = w_sorted.shape
@@ -473,11 +474,22 @@ def mxfp4_expert_ffn(cache, x, w_sorted, starts, rows, cols, expert_list, slot_o
     if act.numel() < R * k * (I // 32 * 17 if quantised else I) or out.numel() < R * k * H:
         raise RuntimeError('act and out must hold the rows of rows * topk (token, expert) pairs')
     list_rows, most = None, int(max_rows if max_rows is not None else R)
-    if isinstance(rows, torch.Tensor) and not rows.numel():
+    # entries of rows and cols; of a list that is an address as many as there are output rows
+    pairs = R * k
+    held = rows.numel() if isinstance(rows, torch.Tensor) else pairs
+    slots = cols.numel() if isinstance(cols, torch.Tensor) else pairs
+    if held != slots and isinstance(rows, torch.Tensor) and isinstance(cols, torch.Tensor):
+        raise RuntimeError('rows and cols must have the same length')
+    if counts is not None:
+        counts = np.asarray(counts)
+        # with lists of the usual length only the listed experts' counts are checked, in the library
+        if (held != pairs or slots != pairs) and np.add.reduce(counts[:E]) > min(held, slots, pairs):
+            raise RuntimeError('counts must name at most rows * topk pairs, with an entry of rows and cols for each')
+    if not held or not slots:
         return out   # no pairs
     if counts is not None and len(el):
         try:
-            list_rows, most = np.asarray(counts)[el].astype(np.int32).tobytes(), -1
+            list_rows, most = counts[el].astype(np.int32).tobytes(), -1
         except IndexError:
             raise RuntimeError(f'expert_list must name experts in [0, {E})') from None
     _native(cache, 'mxfp4_expert_ffn', lib().ferry_mxfp4_expert_ffn, cache.data_ptr(), cache.shape[0], H, I,

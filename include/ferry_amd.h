@@ -216,7 +216,8 @@ int ferry_expert_ffn_spare(const void* cache, int64_t cache_rows, int64_t hidden
  * [R * k, I / 2] and then the scales [R * k, I / 32] of silu(g) * u, quantised from fp32.  The sums and
  * the SwiGLU are fp32 and an output is rounded once, after its routing weight.  All other arguments as
  * ferry_expert_ffn_spare's, but that with list_rows max_rows_per_expert = -1 takes the most and the least rows
- * from there; experts with at most 16 rows run the bandwidth-bound kernels.  Output rows of
+ * from there; the pairs that list_rows names (an expert that is listed twice once) must be at most R * k, and rows
+ * and cols hold starts[experts] entries.  Experts with at most 16 rows run the bandwidth-bound kernels.  Output rows of
  * experts that are not listed stay as they were.  hidden and intermediate are multiples of 128,
  * hidden one of 256 when an expert has more than 16 rows; cache, x, act and out 16-byte aligned.
  */

@@ -447,3 +447,40 @@ def test_refusals(device):
     h = Case([3, 20], 384, 128, k=2)      # tiles cover the hidden dimension in 256 columns
     with pytest.raises(RuntimeError, match='256'):
         h.run(False)
+
+
+@pytest.mark.parametrize('quantised', QUANTISED)
+def test_index_lists_that_are_too_short(device, quantised):
+    """Row and slot lists that end before the pairs of the call do are refused, and counts that name more pairs than there
+    are output rows; longer lists are not."""
+    from ferry_amd import expert_ops as ops
+    c = Case([3, 20, 0], 256, 128, k=2)
+    P = c.R * c.k
+    x = ops.mxfp4_quantize(c.x) if quantised else c.x
+    act = (torch.zeros(P * (c.I // 32 * 17), dtype=torch.uint8, device='cuda') if quantised else
+           torch.zeros((P, c.I), dtype=torch.bfloat16, device='cuda'))
+
+    def call(**other):
+        out = torch.full((P, c.H), 7.0, dtype=torch.bfloat16, device='cuda')
+        args = dict(cache=c.cache, x=x, w_sorted=c.w, starts=c.starts, rows=c.rows, cols=c.cols, expert_list=[0, 1],
+                    slot_of=c.slot_of, hidden=256, intermediate=128, act=act, out=out, counts=c.counts, out_mode=1)
+        return ops.mxfp4_expert_ffn(**{**args, **other})
+    want = call()
+    none = torch.zeros(0, dtype=torch.int64, device='cuda')
+    for bad in (dict(cols=c.cols[:-1]), dict(rows=c.rows[:-1]), dict(rows=c.rows[:-1], cols=c.cols[:-1]),
+                dict(rows=none, cols=none), dict(cols=none), dict(cols=c.cols[:-1], counts=None),
+                dict(rows=none, counts=None), dict(rows=c.rows.data_ptr(), cols=c.cols[:-1]),
+                dict(rows=c.rows[:-1], cols=c.cols.data_ptr()), dict(counts=[3, P - 2, 0]),
+                dict(counts=[3, 20, 18], expert_list=[0])):
+        with pytest.raises(RuntimeError, match='rows'):
+            call(**bad)
+    usual = [torch.cat([t, t[:P - t.numel()]]) for t in (c.rows, c.cols)]   # an entry for every output row
+    with pytest.raises(RuntimeError, match='rows'):
+        call(rows=usual[0], cols=usual[1], counts=[3, P - 2, 0])
+    longer = torch.cat([c.rows, c.rows]), torch.cat([c.cols, c.cols])
+    for good in (dict(counts=list(c.counts)), dict(rows=usual[0], cols=usual[1]), dict(rows=longer[0], cols=longer[1]), dict(counts=None),
+                 dict(rows=c.rows.data_ptr(), cols=c.cols.data_ptr()), dict(counts=[3, 20, 0, 1000], experts=3),
+                 dict(expert_list=[0, 1, 1, 0, 1])):   # 66 pairs if each time counted
+        assert torch.equal(call(**good), want)
+    out = call(rows=none, cols=none, counts=[0, 0, 0], expert_list=[0, 1])
+    assert bool((out == 7).all())

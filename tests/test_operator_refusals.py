@@ -1,5 +1,7 @@
 """CPU tier: the C entry points of the gate and MXFP4 operators refuse bad arguments before any device
 work, and their Python calls refuse host tensors."""
+import ctypes
+
 import pytest
 import torch
 
@@ -43,6 +45,20 @@ def test_mxfp4_arguments(args, word):
 def test_mxfp4_without_elements():
     assert lib().ferry_mxfp4_quantize(None, 0, 0, 64, 64, None, 32, None, 2, None) == 0
     assert lib().ferry_mxfp4_dequantize(None, 32, None, 2, 5, 0, None, 0, 64, None) == 0
+
+
+def test_mxfp4_expert_ffn_of_more_pairs_than_rows():
+    """list_rows of more than rows * topk pairs, an expert that is listed twice counted once."""
+    ints = lambda *v: (ctypes.c_int32 * len(v))(*v)
+    place = ctypes.create_string_buffer(64)           # no address is followed before the refusal
+    at = (ctypes.addressof(place) + 15) // 16 * 16
+
+    def call(experts, counts, rows=4, topk=2):
+        return lib().ferry_mxfp4_expert_ffn(at, 2, 256, 128, at, None, rows, topk, at, at, at, at, ints(*experts),
+                                            len(experts), ints(0, 1, 0, 1), 4, -1, 0, ints(*counts), at, at, 0, 3, 0, None)
+    for experts, counts in (([0], [9]), ([0, 1, 2], [4, 4, 1]), ([0, 1, 0, 2], [4, 4, 4, 1])):
+        assert call(experts, counts) != 0
+        assert 'pairs' in last_error()
 
 
 def test_host_tensors_are_refused():

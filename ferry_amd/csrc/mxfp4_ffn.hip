@@ -21,6 +21,7 @@
 // (1,180 and 860 TFLOP/s, without the 47 experts of at most 16 rows 1,240 and 900; a library product of bf16
 // matrices of 32768 x 2048 x 1536 runs at 1,372), with 4-bit activations 177 + 136 (2,320 and 1,510 TFLOP/s).
 #include "ffn_common.h"
+#include "mxfp4_plan.h"
 
 #include <algorithm>
 #include <bitset>
@@ -425,15 +426,6 @@ constexpr int kSmallNF = MODE == 0 && !Q ? 2 : 4;
 template <int MODE, bool Q>
 __device__ __host__ __forceinline__ int small_cols(const MxArgs& a) {   // items of an expert
   return (int)(MODE == 0 ? a.I / (8 * kSmallNF<0, Q>) : a.H / (16 * kSmallNF<1, Q>));
-}
-// Items of a workgroup, a power of two that divides an expert's, so many that at most `per_cu` workgroups come to a CU:
-// those that run at once by their LDS (up at 16 tokens 13.5 us, with one item a workgroup 17.5, with 4-bit
-// activations 12 and 15.5), behind tiles twice as many, which level the end (256 tokens of 64 experts of 2048 x 1408
-// 53 + 35 us, with half as many 58 + 40, with one item each 64 + 35).
-inline int small_items(int experts, int cols, int64_t per_cu, int64_t cus) {
-  int items = 1;
-  while (cols % (2 * items) == 0 && (int64_t)experts * (cols / items) > per_cu * cus) items *= 2;
-  return items;
 }
 
 // Down with bf16 activations: within the registers of four workgroups a CU (16 tokens 8.6 us, with three 9.7).
@@ -1062,49 +1054,32 @@ int device_cus(int* cus) {
   return 0;
 }
 
-// The launches of a.list and a.small in one kind of activations.  tiles: the row tiles of 256, 128 and 64 rows of the
-// experts with more than kSmallRows rows (upper bounds).
-//
-// 4-bit activations: the large tiles where the rows make at least six quarters of them for each CU.  Up and down, large
-// tiles against small ones: 512 tokens (128 experts of 2048 x 768, top 8, Zipf 1.1; 1.2 and 1.6 quarters) 43 + 32 us
-// against 39 + 29, 2,048 tokens (7 and 9.4) 78 + 54 against 79 + 54, 4,096 (13 and 17) 113 + 79 against 120
-// + 84; evenly spread, 1,024 tokens (3 and 4) 62 + 37 against 56 + 36, 2,048 (6 and 8) 72 + 46 against 79 + 52.
-// Tiles of 128 rows become tiles of 64 where each has a CU of its own: they read the weights twice, and the longest
-// takes less time.  Up and down, bf16 activations (128 experts of 2048 x 768, top 8, Zipf 1.1): 100 tokens 34 + 19
-// us against 28 + 18; 64 rows two to a CU, and 32, were level with these or slower (29 + 19).
-//
-// The small experts' workgroups come behind those of the tiles and run where a CU has no tile (left): up + down, with
-// bf16 and with 4-bit activations, 20 tokens take 37 and 37 us, with launches of their own 57 and 49, 777 tokens (64
-// experts of 2048 x 1408, top 6) 137 and 109 against 157 and 121, 8,192 tokens 615 and 319 against 627 and 339;
-// before the tiles' they delay them (153 and 116 us at 777 tokens).
+// The launches of a.list and a.small in one kind of activations, as plan_tiles cuts them.  tiles: the row tiles of 256,
+// 128 and 64 rows of the experts with more than kSmallRows rows (upper bounds).
 template <bool Q>
-int launch_lists(TiledArgs& a, const int64_t (&tiles)[3], int32_t phases, int64_t cus, hipStream_t s) {
+int launch_lists(TiledArgs& a, const int64_t (&tiles)[3], int32_t phases, int64_t cus, int64_t spare, hipStream_t s) {
   for (int mode = 0; mode < 2; ++mode) {
     if (!(phases & (1 << mode))) continue;
-    if (tiles[0] == 0) {
-      if (a.small.n == 0) continue;
+    if (tiles[0]) {
+      const int64_t cols = mode == 0 ? a.I / kOutCols<0> : a.H / kOutCols<1>;
+      const MxPlan p = plan_tiles(Q, cols, tiles, a.small.n, mode == 0 ? small_cols<0, Q>(a) : small_cols<1, Q>(a), cus, spare);
+      a.tile_rows = p.tile_rows;
+      a.tile_wgs = p.tile_wgs;
+      a.items = p.items;
+      const dim3 grid((unsigned)(p.tile_wgs + p.small_wgs)), block(p.large ? 512 : 256);
+      const char* const name = mode == 0 ? "mx_tiled_up" : "mx_tiled_down";
+      if constexpr (!Q) launch(name, mode == 0 ? mx_tiled16<0> : mx_tiled16<1>, grid, block, 0, s, a);
+      else if (p.large) launch(name, mode == 0 ? mx_tiled4<0, true> : mx_tiled4<1, true>, grid, block, 0, s, a);
+      else launch(name, mode == 0 ? mx_tiled4<0, false> : mx_tiled4<1, false>, grid, block, 0, s, a);
+      FERRY_LAUNCHED("mx_tiled");
+      if (p.small_wgs) continue;
+    }
+    if (a.small.n) {
       SmallArgs b;
       (MxArgs&)b = a;
       b.list = a.small;
       if (const int rc = mode == 0 ? small_launch<0, Q>(b, cus, s) : small_launch<1, Q>(b, cus, s)) return rc;
-      continue;
     }
-    const int64_t large = mode == 0 ? a.I / kOutCols<0> : a.H / kOutCols<1>;   // column tiles
-    const bool use_large = Q && tiles[2] * large >= 6 * cus;
-    const int64_t cols = Q && !use_large ? 2 * large : large, most = (use_large ? cus : 2 * cus) / 8 * 8;
-    const int by = use_large ? 0 : tiles[2] * cols <= cus ? 2 : 1;
-    a.tile_rows = 256 >> by;
-    const int64_t t = tiles[by] * cols;
-    a.tile_wgs = (int32_t)(t < most ? ceil_div(t, 8) * 8 : most);
-    const int part = use_large ? 2 : 1, items = (mode == 0 ? small_cols<0, Q>(a) : small_cols<1, Q>(a)) / part;
-    a.items = small_items(a.small.n, items, use_large ? 2 : 4, cus);
-    const int small = a.small.n * (items / a.items);
-    const dim3 grid((unsigned)(a.tile_wgs + small)), block(use_large ? 512 : 256);
-    const char* const name = mode == 0 ? "mx_tiled_up" : "mx_tiled_down";
-    if constexpr (!Q) launch(name, mode == 0 ? mx_tiled16<0> : mx_tiled16<1>, grid, block, 0, s, a);
-    else if (use_large) launch(name, mode == 0 ? mx_tiled4<0, true> : mx_tiled4<1, true>, grid, block, 0, s, a);
-    else launch(name, mode == 0 ? mx_tiled4<0, false> : mx_tiled4<1, false>, grid, block, 0, s, a);
-    FERRY_LAUNCHED("mx_tiled");
   }
   return 0;
 }
@@ -1175,7 +1150,6 @@ extern "C" int ferry_mxfp4_expert_ffn(const void* cache, int64_t cache_rows, int
   FERRY_CHECK_ARG(listed <= rows_in * topk, "list_rows name more than rows * topk pairs");
   int cus = 0;
   if (const int rc = device_cus(&cus)) return rc;
-  if (cus > 2 * spare_cus) cus -= spare_cus;
   const bool quantised = x_scales != nullptr;
   const int64_t pairs = rows_in * topk;
   TiledArgs a;
@@ -1233,8 +1207,8 @@ extern "C" int ferry_mxfp4_expert_ffn(const void* cache, int64_t cache_rows, int
       const int64_t most = pairs / (kSmallRows + 1);
       for (int by = 0; by < 3; ++by) tiles[by] = pairs / (256 >> by) + (a.list.n < most ? a.list.n : most);
     }
-    const int rc = quantised ? launch_lists<true>(a, tiles, phases, cus, (hipStream_t)stream)
-                             : launch_lists<false>(a, tiles, phases, cus, (hipStream_t)stream);
+    const int rc = quantised ? launch_lists<true>(a, tiles, phases, cus, spare_cus, (hipStream_t)stream)
+                             : launch_lists<false>(a, tiles, phases, cus, spare_cus, (hipStream_t)stream);
     if (rc) return rc;
   }
 }

@@ -442,7 +442,8 @@ def mxfp4_expert_ffn(cache, x, w_sorted, starts, rows, cols, expert_list, slot_o
     faster form for prompts, and silu(g) * u is quantised on the way.  Sums and SwiGLU are fp32; an
     output row is rounded to bf16 once, after its routing weight.  The other arguments are
     ``expert_ffn``'s; ``rows`` and ``cols`` have an entry for every pair of ``starts`` (at least the sum of
-    ``counts``, where those are given); rows of ``out`` that belong to experts outside the list are left as they are.
+    ``counts``, where those are given); ``spare_cus`` leaves the room of that many CUs beside the tiled kernels (half the
+    room of twice as many, where two workgroups share a CU), and gives the small experts launches of their own; rows of ``out`` that belong to experts outside the list are left as they are.
     No counterpart in the reference.
     """
     R, k = w_sorted.shape

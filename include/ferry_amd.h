@@ -211,15 +211,20 @@ int ferry_expert_ffn_spare(const void* cache, int64_t cache_rows, int64_t hidden
  * of [gate I*H | up I*H | down H*I] and then their scales, 3 * H * I / 32 * 17 bytes (ferry_mxfp4_quantize
  * of the bf16 row, or of its three matrices' rows).  With x_scales null, x is bf16 [R, H] and act bf16
  * scratch of R * k * I elements, rounded once from fp32 (with R * k <= 64 and at most 8 rows an expert to 11
- * bits instead of 8, in another format: so an expert's outputs depend on R * k); otherwise x holds the codes [R, H / 2] and
- * x_scales the scales [R, H / 32] of MXFP4 rows, and act is R * k * I / 32 * 17 bytes: the codes
- * [R * k, I / 2] and then the scales [R * k, I / 32] of silu(g) * u, quantised from fp32.  The sums and
- * the SwiGLU are fp32 and an output is rounded once, after its routing weight.  All other arguments as
- * ferry_expert_ffn_spare's, but that with list_rows max_rows_per_expert = -1 takes the most and the least rows
- * from there; the pairs that list_rows names (an expert that is listed twice once) must be at most R * k, and rows
- * and cols hold starts[experts] entries.  Experts with at most 16 rows run the bandwidth-bound kernels.  Output rows of
- * experts that are not listed stay as they were.  hidden and intermediate are multiples of 128,
- * hidden one of 256 when an expert has more than 16 rows; cache, x, act and out 16-byte aligned.
+ * bits instead of 8, in another format: so an expert's outputs depend on R * k); otherwise x holds the
+ * codes [R, H / 2] and x_scales the scales [R, H / 32] of MXFP4 rows, and act is R * k * I / 32 * 17 bytes:
+ * the codes [R * k, I / 2] and then the scales [R * k, I / 32] of silu(g) * u, quantised from fp32.  The sums and
+ * the SwiGLU are fp32 and an output is rounded once, after its routing weight.  All other arguments are
+ * ferry_expert_ffn_spare's, but that
+ *  - with list_rows, max_rows_per_expert = -1 takes the most and the least rows from there; the pairs that it
+ *    names (an expert that is listed twice once) must be at most R * k;
+ *  - spare_cus, where two of the tiled kernels' workgroups share a CU, may leave half the room of twice as
+ *    many CUs; the small experts, whose workgroups otherwise fill what the tiles leave, then have launches of
+ *    their own, on all CUs, as there;
+ *  - experts with at most 16 rows run the bandwidth-bound kernels.
+ * rows and cols hold starts[experts] entries.  Output rows of experts that are not listed stay as they were.
+ * hidden and intermediate are multiples of 128, hidden one of 256 when an expert has more than 16 rows;
+ * cache, x, act and out 16-byte aligned.
  */
 int ferry_mxfp4_expert_ffn(const void* cache, int64_t cache_rows, int64_t hidden, int64_t inter,
                            const void* x, const void* x_scales, int64_t rows_in, int64_t topk,

@@ -484,3 +484,20 @@ def test_index_lists_that_are_too_short(device, quantised):
         assert torch.equal(call(**good), want)
     out = call(rows=none, cols=none, counts=[0, 0, 0], expert_list=[0, 1])
     assert bool((out == 7).all())
+
+
+@pytest.mark.parametrize('H,I', [(2048, 1408), (2048, 128), (2048, 256), (256, 2816)])
+def test_largest_tiles(device, H, I):
+    """4-bit activations with rows enough for tiles of 256 x 256: odd numbers of 128 along K (I = 1408, 128: the last step is
+    half a one), one step in all (I = 128 and 256 down, H = 256 up), and small experts behind them."""
+    counts = [4000, 17, 3300, 3, 12, 2900, 250, 0, 16, 129, 1800, 65, 1, 180]
+    c = Case(counts, H, I, seed=H + I)
+    tiles = sum(-(-n // 64) for n in counts if n > 16)
+    cus = torch.cuda.get_device_properties(0).multi_processor_count
+    assert tiles * max(I // 128 if H == 256 else 0, H // 256) >= 6 * cus   # the rule for these tiles, of the product meant
+    whole = c.check(True)
+    out = torch.full_like(whole, 7.0)
+    for e in range(c.E):      # each by itself: in the smaller tiles
+        c.run(True, [e], out=out)
+    assert torch.equal(out, whole)
+    assert torch.equal(c.run(True, counts=False), whole)

@@ -501,3 +501,19 @@ def test_largest_tiles(device, H, I):
         c.run(True, [e], out=out)
     assert torch.equal(out, whole)
     assert torch.equal(c.run(True, counts=False), whole)
+
+
+@pytest.mark.parametrize('counts', [[40, 9], [300, 2], [40, 30, 70, 17]])
+def test_infinite_rows_of_bf16_activations(device, counts):
+    """An infinity in a token's row makes all of that token's outputs infinities or NaNs, in every kernel, and no others."""
+    c = Case(counts, 256, 128, k=2, seed=6)
+    want = c.run(False)
+    for column in (0, 3, 255):
+        x = c.x.clone()
+        x[0, column] = float('inf')
+        x[5, column] = -float('inf')
+        got = c.run(False, x=x)
+        n = c.rows.numel()
+        hit = (c.rows == 0) | (c.rows == 5)
+        assert bool(hit.any()) and not bool(torch.isfinite(got[:n][hit]).any())
+        assert torch.equal(got[:n][~hit], want[:n][~hit]) and bool((got[n:] == 7).all())

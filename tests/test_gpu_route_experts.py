@@ -250,3 +250,21 @@ def test_refusals(device):
     for bad in (x.double(), x[0], x.t(), torch.zeros((2, 513), device='cuda')):
         with pytest.raises(RuntimeError):
             ops.route_experts(bad, 2)
+
+
+# further batches: logits in fp16, more experts and more of them chosen than 16 lanes hold
+MORE_BATCH_GATES = [(512, 8, 8, 4), (511, 5, 1, 1), (500, 16, 10, 3), (512, 32, 256, 40), (257, 6, 1, 1), (256, 32, 16, 2),
+                    (64, 17, 1, 1)]
+
+
+@pytest.mark.parametrize('E,k,G,TG', BATCH_GATES + MORE_BATCH_GATES)
+@pytest.mark.parametrize('scoring', ['softmax', 'sigmoid'])
+def test_gates_on_fp16_batches(device, E, k, G, TG, scoring):
+    test_gates_on_batches(device, E, k, G, TG, scoring, torch.float16)
+
+
+@pytest.mark.parametrize('E,k,G,TG', MORE_BATCH_GATES)
+@pytest.mark.parametrize('scoring', ['softmax', 'sigmoid'])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_large_gates_on_batches(device, E, k, G, TG, scoring, dtype):
+    test_gates_on_batches(device, E, k, G, TG, scoring, dtype)

@@ -16,10 +16,11 @@
 // inside a product is free as long as both operands share it.  So the plain row-major rows are operands
 // without any repacking.
 //
-// Measured, all experts (2048 x 768, 128 of them, top 8, Zipf 1.1): one token 5.4 + 3.9 us (up + down; launch
-// latency), 16 tokens 14 + 8.6 us (3.6 and 3.0 TB/s of weights), with 4-bit activations 12 + 7; 8,192 tokens 348 + 238 us
-// (1,180 and 860 TFLOP/s, without the 47 experts of at most 16 rows 1,240 and 900; a library product of bf16
-// matrices of 32768 x 2048 x 1536 runs at 1,372), with 4-bit activations 177 + 136 (2,320 and 1,510 TFLOP/s).
+// Measured, all experts (2048 x 768, 128 of them, top 8, Zipf 1.1): one token 7.0 + 5.6 us (up + down; launch
+// latency), 16 tokens 14.6 + 8.2 us, with weights that no cache holds 16.8 + 10.2 (3.2 and 2.7 TB/s of weights), with 4-bit
+// activations 12.5 + 7.3 and 15.2 + 8.8; 8,192 tokens 346 + 237 us (1,190 and 870 TFLOP/s, without the 47 experts of at
+// most 16 rows 1,240 and 900; a library product of bf16 matrices of 32768 x 2048 x 1536 runs at 1,372), with 4-bit
+// activations 178 + 136 (2,300 and 1,510 TFLOP/s).
 #include "ffn_common.h"
 #include "mxfp4_plan.h"
 
@@ -133,8 +134,9 @@ __device__ __forceinline__ uint32_t block_codes(const float (&v)[8], int byte) {
 // buffers, from item to item; straight to registers in operand order, the lanes' 64 places of 16 bytes a load
 // bound the kernel at 3 TB/s.  The rows' activations go to registers, once for all items where two units hold them:
 // only the lanes of rows that are there load.
-// 31 experts of 2048 x 768 (16 tokens, Zipf 1.1): up 14 us, down 8.6 us (3.6 and 3.0 TB/s), with 4-bit activations 12
-// and 7 (4.4 and 3.4; a large copy's rate is 5.2).  The decoding of the weights to bf16 is what the 4-bit form saves.
+// 31 experts of 2048 x 768 (16 tokens, Zipf 1.1): up 14.6 us, down 8.2 us (3.5 and 3.2 TB/s, in part from the last-level
+// cache), with 4-bit activations 12.5 and 7.3 (4.1 and 3.6; a large copy's rate is 5.2).  The decoding of the weights to
+// bf16 is what the 4-bit form saves.
 //
 // In calls of at most kFinePairs (token, expert) pairs the activations of experts with at most kFineRows rows are not
 // rounded to bf16 between up and down: in their 16 bits stand fp16 numbers below 2, and eight columns share the largest
@@ -1172,10 +1174,9 @@ extern "C" int ferry_mxfp4_expert_ffn(const void* cache, int64_t cache_rows, int
   // Small experts and the others, each up to kListMax of a launch; without row counts every expert is in both, and the
   // kernels pass over those of the other kind by the device's starts.  An expert's own rows (and with a.fine the call's
   // pairs) decide, so that its results do not depend on which experts are listed with it (the two kinds sum in different
-  // orders): with all
-  // experts in tiles wherever one has more than kSmallRows rows, 512 tokens (128 experts of 2048 x 768, top 8,
-  // Zipf 1.1) take 110 and 87 us (bf16 and 4-bit activations) instead of 122 and 92, 8,192 tokens 644 and 332
-  // instead of 653 and 341.
+  // orders): with all experts in tiles wherever one has more than kSmallRows rows, 512 tokens (128 experts of 2048 x
+  // 768, top 8, Zipf 1.1) took 10 and 5 % less (bf16 and 4-bit activations), 8,192 tokens 1 and 3 %, when the small ones
+  // had launches of their own.
   struct Entry {
     int32_t rows, expert;
   } entry[kListMax];
@@ -1192,8 +1193,8 @@ extern "C" int ferry_mxfp4_expert_ffn(const void* cache, int64_t cache_rows, int
           for (int by = 0; by < 3; ++by) tiles[by] += ceil_div(list_rows[i], 256 >> by);
         entry[list.n++] = {list_rows ? list_rows[i] : 0, expert_list[i]};
       }
-      // the experts with most rows first: tiles of few rows, which take less time, fill the last round (65 us for the
-      // up phase above)
+      // the experts with most rows first: tiles of few rows, which take less time, fill the last round (777 tokens
+      // of 64 experts as at tile_of: 65 us up instead of 72)
       if (big && list_rows)
         std::sort(entry, entry + list.n, [](const Entry& p, const Entry& q) { return p.rows > q.rows; });
       for (int i = 0; i < list.n; ++i) {

@@ -35,9 +35,9 @@ inline int small_items(int experts, int cols, int64_t per_cu, int64_t cus) {
 // us against 28 + 18; 64 rows two to a CU, and 32, were level with these or slower (29 + 19).
 //
 // The small experts' workgroups come behind those of the tiles and run where a CU has no tile (left): up + down, with
-// bf16 and with 4-bit activations, 20 tokens take 37 and 37 us, with launches of their own 57 and 49, 777 tokens (64
-// experts of 2048 x 1408, top 6) 137 and 109 against 157 and 121, 8,192 tokens 615 and 319 against 627 and 339;
-// before the tiles' they delay them (153 and 116 us at 777 tokens).
+// bf16 and with 4-bit activations, 20 tokens took 37 and 37 us, with launches of their own 57 and 49, 777 tokens (64
+// experts of 2048 x 1408, top 6) 13 and 10 % less than with these, 8,192 tokens 2 and 6 %; before the tiles' they
+// delay them (777 tokens 12 and 6 % more than behind).
 //
 // spare: the tiles' launch leaves the room of that many CUs to other streams' kernels (at least 8 are used).  Nothing
 // comes behind the tiles then, so that what is left is not filled; where two of its workgroups share a CU, the room may be

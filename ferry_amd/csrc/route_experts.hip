@@ -20,9 +20,11 @@
 // index (unique: a drawing needs no second search for its owner), until the key is below the k-th's by more than
 // the margin.  The candidates, one to a lane, are ranked by their 64-bit scores.  A row with more than 16 of
 // them, or whose group scores are too near each other for fp32, goes to exact_row.  One token of 256 experts in 8
-// groups, top 8: 6.1 us; 32,768 of them, fp32: 30 us, against 105 with a wavefront a token and 6.5 for the bytes at
-// the rate of a large copy; what is left is instructions (1,220 vector and 320 scalar ones for four tokens, 16 us of
-// issue) and, at the end, the last rows of exact_row (about 6 us).  An eighth wavefront on a SIMD changes nothing.
+// groups, top 8: 6.2 us; 32,768 of them, fp32: 29 us (27 a call where calls follow each other), against 105 with a
+// wavefront a token and 7 for the bytes at the rate of a large copy; what is left is instructions (1,220 vector and 320
+// scalar ones for four tokens, 16 us of issue) and, at the end, the last rows of exact_row (about 6 us).  An eighth
+// wavefront on a SIMD changes nothing.  Batches of more than 256 experts or more than 16 chosen have a wavefront a token too:
+// 32,768 tokens, 512 experts in 8 groups 104 us (bytes 13), 256 experts and 24 of them 87 (bytes 8).
 //
 // The margin.  e^y as 2^(y log2 e) in fp32 is off by at most (2.5 |y| + 2) 2^-24 of itself: y's and the product's
 // rounding, the constant's and the instruction's.  Without a bias an expert's choice score is 1 / (1 + e^-x) or

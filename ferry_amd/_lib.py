@@ -53,6 +53,17 @@ SIGNATURES = [
     ('ferry_unpack_dispatch', ctypes.c_int, [_c_p, _i64, _i64, _i64, _c_p, _c_p, _c_p]),
     ('ferry_combine_add', ctypes.c_int, [_c_p, _c_p, _i64, _i64, _i64, _c_p, _c_p, _c_p]),
     ('ferry_gate_logits', ctypes.c_int, [_c_p, _i64, _i64, _c_p, _i64, _c_p, _c_p]),
+    ('ferry_linear_workspace_bytes', _i64, [_i32, _i64, _i64, _i64, _i64]),
+    ('ferry_expert_linear', ctypes.c_int,
+     [_c_p, _i32, _i64, _i64, _i64, _c_p, _i64, _c_p, _i64, _c_p, _i64, _i64, _i64, _c_p, _i64, _i32, _c_p,
+      _i64, _c_p, _c_p, _i64, _i32, _c_p, _i64, _c_p]),
+    ('ferry_linear_grad_z', ctypes.c_int,
+     [_c_p, _i32, _i64, _i64, _i64, _c_p, _i32, _c_p, _i64, _c_p, _c_p, _c_p, _i64, _c_p]),
+    ('ferry_expert_linear_grad_x', ctypes.c_int,
+     [_c_p, _i32, _i64, _i64, _i64, _c_p, _i64, _c_p, _i64, _i64, _i64, _c_p, _i32, _c_p, _i64, _c_p]),
+    ('ferry_expert_linear_grad_w', ctypes.c_int,
+     [_c_p, _i32, _i64, _i64, _i64, _c_p, _i64, _i64, _i64, _c_p, _c_p, _i64, _c_p, _c_p, _i64, _c_p]),
+    ('ferry_sum_pairs', ctypes.c_int, [_c_p, _i32, _i64, _i64, _c_p, _i64, _i64, _c_p, _c_p]),
     ('ferry_history_update', ctypes.c_int,
      [_c_p, _i64, _i64, _i64, _i64, _i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _i32, _c_p]),
     ('ferry_history_ready_words', _i64, [_i64, _i64]),

@@ -1,0 +1,286 @@
+// What the kernels of the linear products share: their arguments, the groups' table of tiles, loads of
+// 16-bit operands, the epilogue.
+//
+// Three products over G groups of rows, starts[g] <= p < starts[g + 1] (one group of all rows for a
+// dense layer), with i the index of an output row, j that of an output column, c the contraction:
+//   kFwd  y[p, j]  = sum_c x[row(p), c] w[g][j, c]     i = p, j < N, c < K
+//   kDx   dx[p, j] = sum_c dz[p, c] w[g][c, j]         i = p, j < K, c < N
+//   kDw   dw[g][i, j] = sum_p dz[p, i] x[row(p), j]    i < N, j < K, c = p
+// Operand A belongs to i, B to j.  An operand whose elements follow each other along c (x and w in kFwd,
+// dz in kDx) is staged in LDS by rows of its own index; the others (w in kDx, both of kDw) by rows of c,
+// and their fragments are read with the transposing LDS read, so that no operand is copied in another
+// order first.
+#pragma once
+
+#include "common.h"
+
+namespace ferry {
+namespace lin {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+
+enum { kFwd = 0, kDx = 1, kDw = 2 };
+enum { kNone = 0, kRelu = 1, kSilu = 2, kGelu = 3, kGeluTanh = 4 };   // FERRY_ACT_*
+
+constexpr int kMaxGroups = FERRY_MAX_EXPERTS;
+
+struct Args {
+  const uint16_t* a;    // x (kFwd), dz (kDx, kDw)
+  const uint16_t* b;    // w (kFwd, kDx), x (kDw)
+  int64_t lda, ldb, ldo;           // elements from row to row
+  int64_t b_group, o_group;        // elements from group to group: weights, dw
+  const int64_t* starts;           // null: one group of all pairs
+  const int64_t* rows;             // null: row(p) = p
+  int64_t pairs, x_rows;           // rows of the grouped order, rows of x
+  int64_t I, J, C;                 // sizes of i, j and c; the ragged one is 0
+  int32_t groups, splits;          // parts of the contraction, joined by join_kernel
+  int32_t act, zero_rest;          // zero_rest: rows outside the groups become 0
+  int32_t vec_out;                 // out, residual and pre take 8-byte accesses of four columns
+  int64_t bias_group;
+  const uint16_t* bias;
+  const uint16_t* residual;
+  int64_t ldr;
+  uint16_t* pre;
+  uint16_t* out;
+  float* part;                     // [splits][rows of out][J], with splits > 1
+};
+
+// -- types -------------------------------------------------------------------------------------
+
+struct Bf16 {
+  typedef __bf16 x8 __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ f32x4 mma(s16x8 p, s16x8 q, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(x8, p), __builtin_bit_cast(x8, q), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ float load(uint16_t h) { return bf16_to_f32(h); }
+  static __device__ __forceinline__ uint16_t round(float f) { return f32_to_bf16(f); }
+  static __device__ __forceinline__ uint32_t round2(float lo, float hi) {   // lo | hi << 16
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){lo, hi}, b16x2));
+  }
+};
+struct F16 {
+  typedef _Float16 x8 __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ f32x4 mma(s16x8 p, s16x8 q, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(x8, p), __builtin_bit_cast(x8, q), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ float load(uint16_t h) { return (float)__builtin_bit_cast(_Float16, h); }
+  static __device__ __forceinline__ uint16_t round(float f) { return __builtin_bit_cast(uint16_t, (_Float16)f); }
+  static __device__ __forceinline__ uint32_t round2(float lo, float hi) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef _Float16 h16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){lo, hi}, h16x2));
+  }
+};
+
+// -- activations ---------------------------------------------------------------------------------
+// fp32, with the hardware's exp2 and reciprocal (relative error about 1e-6: the results are rounded to
+// 8 or 11 bits afterwards).  The tanh form is z / (1 + e^-2u), u = sqrt(2 / pi) (z + 0.044715 z^3): no
+// cancellation for negative z.
+
+__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __expf(-z)); }
+
+__device__ __forceinline__ float activate(int act, float z) {
+  switch (act) {
+    case kRelu: return z <= 0.f ? 0.f : z;   // a NaN stays one
+    case kSilu: return z * sigmoid(z);
+    case kGelu: return 0.5f * z * erfcf(z * -0.70710678f);
+    case kGeluTanh: return z * sigmoid(1.5957691f * (z + 0.044715f * z * z * z));
+    default: return z;
+  }
+}
+
+// f'(z).  Beyond |z| = 30 those of gelu are 0 or 1 to all bits; the clamp keeps z^3 finite.
+__device__ __forceinline__ float slope(int act, float z) {
+  if (z != z) return z;
+  switch (act) {
+    case kRelu: return z <= 0.f ? 0.f : 1.f;
+    case kSilu: {
+      const float s = sigmoid(z);
+      return s * (1.0f + z * (1.0f - s));
+    }
+    case kGelu: {
+      z = fminf(fmaxf(z, -30.f), 30.f);
+      return 0.5f * erfcf(z * -0.70710678f) + z * 0.39894228f * __expf(-0.5f * z * z);
+    }
+    case kGeluTanh: {
+      z = fminf(fmaxf(z, -30.f), 30.f);
+      const float s = sigmoid(1.5957691f * (z + 0.044715f * z * z * z));
+      return s + z * s * (1.0f - s) * 1.5957691f * (1.0f + 0.134145f * z * z);
+    }
+    default: return 1.f;
+  }
+}
+
+// -- groups ----------------------------------------------------------------------------------------
+
+struct Table {
+  __attribute__((aligned(16))) int32_t cum[kMaxGroups + 8];   // tiles before the group, 0x7fffffff behind the last
+  int64_t start[kMaxGroups + 1];
+  int32_t total;
+};
+
+// start[g] = starts[g], forced into [0, pairs] and to ascend, so that whatever starts holds every access
+// stays inside the tensors; cum: with RAGGED_I the tiles of `rows` rows of the groups before, else `rows`
+// tiles for each group.  By wavefront 0; all others wait.
+template <bool RAGGED_I>
+__device__ __forceinline__ void build_table(const Args& a, Table& t, int rows) {
+  if (threadIdx.x < 64) {
+    const int lane = threadIdx.x;
+    if (!a.starts) {
+      if (lane == 0) {
+        t.start[0] = 0;
+        t.start[1] = a.pairs;
+        t.cum[0] = 0;
+        t.total = RAGGED_I ? (int32_t)((a.pairs + rows - 1) / rows) : rows;
+      }
+      for (int i = 1 + lane; i < kMaxGroups + 8; i += 64) t.cum[i] = 0x7fffffff;
+    } else {
+      const int G = a.groups;
+      int64_t before = 0;
+      int sum = 0;
+      for (int g0 = 0; g0 <= G; g0 += 64) {
+        const int g = g0 + lane;
+        int64_t s = g <= G ? a.starts[g] : 0;
+        s = s < 0 ? 0 : (s > a.pairs ? a.pairs : s);
+        s = s < before ? before : s;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+          const int64_t v = __shfl_up(s, off, 64);
+          if (lane >= off && v > s) s = v;
+        }
+        if (g <= G) t.start[g] = s;
+        before = __shfl(s, 63, 64);
+      }
+      __threadfence_block();
+      for (int g0 = 0; g0 < kMaxGroups + 8; g0 += 64) {
+        const int g = g0 + lane;
+        int n = 0;
+        if (g < G) n = RAGGED_I ? (int)((t.start[g + 1] - t.start[g] + rows - 1) / rows) : rows;
+        int incl = n;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+          const int v = __shfl_up(incl, off, 64);
+          if (lane >= off) incl += v;
+        }
+        if (g < kMaxGroups + 8) t.cum[g] = g < G ? sum + incl - n : 0x7fffffff;
+        sum += __shfl(incl, 63, 64);
+      }
+      if (lane == 0) t.total = sum;
+    }
+  }
+  __syncthreads();
+}
+
+// the group of tile m: the last g with cum[g] <= m (groups without tiles share their successor's cum)
+__device__ __forceinline__ int find_group(const Table& t, int m) {
+  const int lane = threadIdx.x & 63;
+  int le = 0;
+#pragma unroll
+  for (int q = 0; q < kMaxGroups / 256; ++q) {
+    const u32x4 c = *reinterpret_cast<const u32x4*>(&t.cum[(q * 64 + lane) * 4]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) le += __popcll(__ballot((int)c[k] <= m));
+  }
+  return __builtin_amdgcn_readfirstlane(le - 1);
+}
+
+// -- operands in LDS ---------------------------------------------------------------------------------
+// Rows of 16-byte chunks, chunk c of row r in place c ^ swizzle(r).
+// By index ("direct"): 64 values of c a row (128 bytes); a fragment is 16 rows by one chunk, lane l of the
+// wavefront row l % 16, chunk l / 16 of the step's four: the 16 rows of a quarter wavefront then lie on
+// 16 different chunks of the banks.
+// By c ("across"): W indices a row.  The transposing read takes from each of 16 lanes 8 bytes, lanes
+// 4 r + q four indices 4 q of the row c = r, and gives lane l the index l at four c: two of them make a
+// fragment, lane group g the c = 8 g .. 8 g + 7.  32 lanes read 8 rows (4 of each group) of 32 bytes,
+// which the swizzle puts on 64 different banks.
+__device__ __forceinline__ int swz_direct(int r) { return (r >> 1) & 7; }
+template <int W>
+__device__ __forceinline__ int swz_across(int r) {
+  return W == 64 ? ((((r >> 1) & 1) | (((r >> 3) & 1) << 1)) << 1) : (((r & 3) | (((r >> 3) & 1) << 2)) << 1);
+}
+// fragment of 16 indices from i0 on at K step ks (32 values of c): byte offsets into the staged operand
+__device__ __forceinline__ uint32_t frag_direct(int i0, int ks) {
+  const int lane = threadIdx.x & 63, r = i0 + (lane & 15);
+  return (uint32_t)(r * 128 + (((4 * ks + (lane >> 4)) ^ swz_direct(r)) << 4));
+}
+template <int W>
+__device__ __forceinline__ uint32_t frag_across(int i0, int ks, int h) {
+  const int lane = threadIdx.x & 63, r = (lane & 15) >> 2, q = lane & 3;
+  const int c = 32 * ks + 8 * (lane >> 4) + 4 * h + r;
+  const int i = i0 + 4 * q;
+  return (uint32_t)(c * W * 2 + ((((i >> 3)) ^ swz_across<W>(c)) << 4) + (i & 4) * 2);
+}
+typedef __attribute__((address_space(3))) const s16x8 lds_x8;
+typedef __attribute__((address_space(3))) s16x4 lds_x4;
+__device__ __forceinline__ s16x8 read_direct(uint32_t addr) { return *reinterpret_cast<lds_x8*>((uintptr_t)addr); }
+__device__ __forceinline__ s16x8 read_across(uint32_t lo, uint32_t hi) {
+  const s16x4 p = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_x4*>((uintptr_t)lo));
+  const s16x4 q = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_x4*>((uintptr_t)hi));
+  return s16x8{p[0], p[1], p[2], p[3], q[0], q[1], q[2], q[3]};
+}
+
+// -- epilogue ----------------------------------------------------------------------------------------
+// Four columns j .. j + 3 (of which `n` > 0 are there) of output row `row`: bias, pre, activation,
+// residual, one rounding.  g: the group, for its bias.
+template <typename T>
+__device__ __forceinline__ void finish4(const Args& a, int g, int64_t row, int64_t j, int n, f32x4 v) {
+  uint16_t* const o = a.out + row * a.ldo + j;
+  const bool whole = n >= 4 && a.vec_out;
+  if (a.bias) {
+    const uint16_t* b = a.bias + g * a.bias_group + j;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] += q < n ? T::load(b[q]) : 0.f;
+  }
+  if (a.pre) {
+    uint16_t* const p = a.pre + row * a.J + j;
+    if (whole) {
+      *reinterpret_cast<u32x2*>(p) = u32x2{T::round2(v[0], v[1]), T::round2(v[2], v[3])};
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (q < n) p[q] = T::round(v[q]);
+    }
+  }
+  if (a.act != kNone) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] = activate(a.act, v[q]);
+  }
+  if (a.residual) {
+    const uint16_t* r = a.residual + row * a.ldr + j;
+    if (whole) {
+      const u32x2 w = *reinterpret_cast<const u32x2*>(r);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[q] += T::load((uint16_t)(w[q >> 1] >> (16 * (q & 1))));
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (q < n) v[q] += T::load(r[q]);
+    }
+  }
+  if (whole) {
+    *reinterpret_cast<u32x2*>(o) = u32x2{T::round2(v[0], v[1]), T::round2(v[2], v[3])};
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (q < n) o[q] = T::round(v[q]);
+  }
+}
+
+// rows of the output that belong to no group, by all workgroups of a launch
+__device__ __forceinline__ void zero_rest(const Args& a, const Table& t) {
+  const int64_t first = t.start[0], last = t.start[a.starts ? a.groups : 1];
+  const int64_t n = first + (a.pairs - last);
+  for (int64_t r = blockIdx.x; r < n; r += gridDim.x) {
+    uint16_t* const o = a.out + (r < first ? r : last + (r - first)) * a.ldo;
+    for (int64_t j = threadIdx.x; j < a.J; j += blockDim.x) o[j] = 0;
+  }
+}
+
+}  // namespace lin
+}  // namespace ferry

@@ -1,0 +1,610 @@
+// Dense and expert-grouped linear products with their epilogue and gradients: the kernels that take
+// every size and alignment, and the entry points.  No counterpart in the reference, whose experts are
+// SwiGLU blocks of bf16 matrices without biases or gradients.
+#include "linear.h"
+
+#include <algorithm>
+
+namespace ferry {
+namespace lin {
+namespace {
+
+// =============================================================================================
+// Any size, any alignment
+// =============================================================================================
+
+// eight 16-bit values from p, of which the first n are there (the others 0).  p may lie at any even
+// address: the hardware takes unaligned 16-byte loads.
+__device__ __forceinline__ u32x4 load8(const uint16_t* p, int n) {
+  u32x4 v = {0, 0, 0, 0};
+  if (n >= 8) {
+    __builtin_memcpy(&v, p, 16);
+  } else if (n > 0) {
+    uint16_t h[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) h[q] = q < n ? p[q] : (uint16_t)0;
+    __builtin_memcpy(&v, h, 16);
+  }
+  return v;
+}
+
+// TI x TJ outputs per workgroup of four wavefronts, 64 of the contraction a step through registers into
+// one of two LDS buffers, the loads of a step issued before the products of the one before.  Loads are
+// 16 bytes at any alignment; what lies outside the matrices, the group or the contraction is 0 in LDS, so
+// that nothing a neighbouring row holds, a NaN included, enters a sum.
+template <typename T, int MODE, int TI, int TJ>
+__global__ __launch_bounds__(256) void any_kernel(Args a) {
+  constexpr bool kAcrossA = MODE == kDw, kAcrossB = MODE != kFwd, kRaggedI = MODE != kDw;
+  constexpr int kStage = (TI + TJ) * 128, MI = TI / 32, NJ = TJ / 32;
+  __shared__ Table tt;
+  __shared__ __attribute__((aligned(1024))) char smem[2 * kStage];
+  const int ntj = (int)ceil_div(a.J, TJ);
+  const int nti = kRaggedI ? 0 : (int)ceil_div(a.I, TI);
+  build_table<kRaggedI>(a, tt, kRaggedI ? TI : nti);
+  if (a.zero_rest) zero_rest(a, tt);
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wi = (wave >> 1) * (TI / 2), wj = (wave & 1) * (TJ / 2);
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
+  const int64_t total = (int64_t)tt.total * ntj * a.splits;
+  for (int64_t item = blockIdx.x; item < total; item += gridDim.x) {
+    const int s = (int)(item % a.splits);
+    const int64_t t = item / a.splits;
+    const int jt = (int)(t % ntj), mt = (int)(t / ntj);
+    const int g = a.starts ? find_group(tt, mt) : 0;
+    const int64_t start = tt.start[g], n = tt.start[g + 1] - start;
+    const int64_t i0 = (int64_t)(mt - tt.cum[g]) * TI, j0 = (int64_t)jt * TJ;
+    const int64_t I = kRaggedI ? n : a.I, C = kRaggedI ? a.C : n;
+    const int64_t per = ceil_div(ceil_div(C, a.splits), 64) * 64;
+    const int64_t c0 = s * per, c1 = c0 + per < C ? c0 + per : C;
+    const uint16_t* const bw = a.b + (MODE == kDw ? 0 : g * a.b_group);
+    // operands by index: each thread's rows
+    const uint16_t* pa[MI];
+    const uint16_t* pb[NJ];
+    if constexpr (!kAcrossA) {
+#pragma unroll
+      for (int q = 0; q < MI; ++q) {
+        const int64_t i = i0 + tid / 8 + 32 * q;
+        int64_t r = start + i;
+        bool ok = i < I;
+        if (MODE == kFwd && a.rows && ok) {
+          r = a.rows[r];
+          ok = (uint64_t)r < (uint64_t)a.x_rows;
+        }
+        pa[q] = ok ? a.a + r * a.lda + (tid & 7) * 8 : nullptr;
+      }
+    }
+    if constexpr (!kAcrossB) {
+#pragma unroll
+      for (int q = 0; q < NJ; ++q) {
+        const int64_t j = j0 + tid / 8 + 32 * q;
+        pb[q] = j < a.J ? bw + j * a.ldb + (tid & 7) * 8 : nullptr;
+      }
+    }
+    u32x4 va[MI], vb[NJ];
+    auto load = [&](int64_t c) {
+#pragma unroll
+      for (int q = 0; q < MI; ++q) {
+        if constexpr (!kAcrossA) {
+          va[q] = load8(pa[q] + c, pa[q] ? (int)(c1 - c < 64 ? c1 - c : 64) - (tid & 7) * 8 : 0);
+        } else {
+          constexpr int per_row = TI / 8;
+          const int64_t cc = c + tid / per_row + (256 / per_row) * q, i = i0 + (tid % per_row) * 8;
+          va[q] = load8(a.a + (start + cc) * a.lda + i, cc < c1 ? (int)(I - i < 8 ? I - i : 8) : 0);
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < NJ; ++q) {
+        if constexpr (!kAcrossB) {
+          vb[q] = load8(pb[q] + c, pb[q] ? (int)(c1 - c < 64 ? c1 - c : 64) - (tid & 7) * 8 : 0);
+        } else {
+          constexpr int per_row = TJ / 8;
+          const int64_t cc = c + tid / per_row + (256 / per_row) * q, j = j0 + (tid % per_row) * 8;
+          int64_t r = cc;
+          bool ok = cc < c1;
+          if (MODE == kDw && ok) {
+            r = start + cc;
+            if (a.rows) {
+              r = a.rows[r];
+              ok = (uint64_t)r < (uint64_t)a.x_rows;
+            }
+          }
+          vb[q] = load8(bw + (ok ? r * a.ldb : 0) + j, ok ? (int)(a.J - j < 8 ? a.J - j : 8) : 0);
+        }
+      }
+    };
+    auto store = [&](int buf) {
+      char* const st = smem + buf * kStage;
+#pragma unroll
+      for (int q = 0; q < MI; ++q) {
+        constexpr int per_row = kAcrossA ? TI / 8 : 8;
+        const int r = tid / per_row + (256 / per_row) * q, k = tid % per_row;
+        const int at = kAcrossA ? r * TI * 2 + ((k ^ swz_across<TI>(r)) << 4) : r * 128 + ((k ^ swz_direct(r)) << 4);
+        *reinterpret_cast<u32x4*>(st + at) = va[q];
+      }
+#pragma unroll
+      for (int q = 0; q < NJ; ++q) {
+        constexpr int per_row = kAcrossB ? TJ / 8 : 8;
+        const int r = tid / per_row + (256 / per_row) * q, k = tid % per_row;
+        const int at = kAcrossB ? r * TJ * 2 + ((k ^ swz_across<TJ>(r)) << 4) : r * 128 + ((k ^ swz_direct(r)) << 4);
+        *reinterpret_cast<u32x4*>(st + TI * 128 + at) = vb[q];
+      }
+    };
+    f32x4 acc[MI][NJ];
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+    __syncthreads();   // the tile before has read its last buffer
+    load(c0);
+    store(0);
+    int buf = 0;
+    for (int64_t c = c0; c < c1; c += 64, buf ^= 1) {
+      const bool more = c + 64 < c1;
+      if (more) load(c + 64);
+      __syncthreads();
+      const uint32_t la = lds0 + buf * kStage, lb = la + TI * 128;
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        s16x8 fa[MI], fb[NJ];
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+          fa[i] = kAcrossA ? read_across(la + frag_across<TI>(wi + 16 * i, ks, 0), la + frag_across<TI>(wi + 16 * i, ks, 1))
+                           : read_direct(la + frag_direct(wi + 16 * i, ks));
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+          fb[j] = kAcrossB ? read_across(lb + frag_across<TJ>(wj + 16 * j, ks, 0), lb + frag_across<TJ>(wj + 16 * j, ks, 1))
+                           : read_direct(lb + frag_direct(wj + 16 * j, ks));
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) acc[i][j] = T::mma(fb[j], fa[i], acc[i][j]);
+      }
+      if (more) store(buf ^ 1);
+    }
+    // lane l holds columns 4 (l / 16) + [0, 4) of row l % 16 of each 16 x 16 tile
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const int64_t r = i0 + wi + 16 * i + (lane & 15);
+      if (r >= I) continue;
+      const int64_t row = kRaggedI ? start + r : r;
+#pragma unroll
+      for (int jj = 0; jj < NJ; ++jj) {
+        const int64_t j = j0 + wj + 16 * jj + 4 * (lane >> 4);
+        const int m = (int)(a.J - j < 4 ? a.J - j : 4);
+        if (m <= 0) continue;
+        if (a.splits > 1) {
+          float* const o = a.part + (kRaggedI ? (s * a.pairs + row) : ((int64_t)s * a.groups + g) * a.I + row) * a.J + j;
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (q < m) o[q] = acc[i][jj][q];
+        } else if constexpr (MODE == kDw) {
+          Args d = a;
+          d.out = a.out + g * a.o_group;
+          finish4<T>(d, g, row, j, m, acc[i][jj]);
+        } else {
+          finish4<T>(a, g, row, j, m, acc[i][jj]);
+        }
+      }
+    }
+  }
+}
+
+// The parts of a split contraction added in their order, and the epilogue.  A wavefront takes 256
+// columns of a row.
+template <typename T, int MODE>
+__global__ __launch_bounds__(256) void join_kernel(Args a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t per = ceil_div(a.J, 256), rows = MODE == kDw ? a.groups * a.I : a.pairs, items = rows * per;
+  for (int64_t it = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); it < items; it += (int64_t)gridDim.x * 4) {
+    const int64_t row = it / per, j = (it % per) * 256 + lane * 4;
+    if (j >= a.J) continue;
+    const int m = (int)(a.J - j < 4 ? a.J - j : 4);
+    int g = MODE == kDw ? (int)(row / a.I) : 0;
+    bool in = true;
+    if (MODE != kDw && a.starts) {   // the last group that starts at or before the row
+      int64_t reach = a.starts[0] < 0 ? 0 : a.starts[0];
+      in = row >= reach;
+      g = -1;
+      for (int k = 0; k < a.groups && in; ++k) {
+        const int64_t e = a.starts[k + 1] > reach ? a.starts[k + 1] : reach;
+        if (row < e) {
+          g = k;
+          break;
+        }
+        reach = e;
+      }
+      in = g >= 0;
+    }
+    Args d = a;
+    if (MODE == kDw) d.out = a.out + g * a.o_group;
+    const int64_t orow = MODE == kDw ? row % a.I : row;
+    if (!in) {
+      if (a.zero_rest)
+        for (int q = 0; q < m; ++q) a.out[row * a.ldo + j + q] = 0;
+      continue;
+    }
+    f32x4 v = {0, 0, 0, 0};
+    for (int s = 0; s < a.splits; ++s) {
+      const float* const p = a.part + (s * rows + row) * a.J + j;
+      if (m == 4 && a.J % 4 == 0) {
+        v += *reinterpret_cast<const f32x4*>(p);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] += q < m ? p[q] : 0.f;
+      }
+    }
+    finish4<T>(d, g, orow, j, m, v);
+  }
+}
+
+// =============================================================================================
+// The epilogue's gradient, and sums
+// =============================================================================================
+
+struct SlopeArgs {
+  const uint16_t* dy;
+  const uint16_t* pre;   // act != 0
+  uint16_t* dz;          // null: not wanted (act == 0)
+  uint16_t* db;          // null: not wanted; [groups][N]
+  float* part;           // [splits][groups][N], with splits > 1
+  int64_t ldy, pairs, N;
+  const int64_t* starts;
+  int32_t groups, splits, act, zero_rest, vec;
+};
+
+// rows [lo, hi) of group g, as build_table has them; by every wavefront
+__device__ __forceinline__ void group_rows(const int64_t* __restrict__ starts, int g, int64_t pairs, int64_t& lo,
+                                           int64_t& hi) {
+  int64_t v = 0;
+  for (int k = threadIdx.x & 63; k <= g; k += 64) v = starts[k] > v ? starts[k] : v;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) {
+    const int64_t o = __shfl_xor(v, off, 64);
+    v = o > v ? o : v;
+  }
+  const int64_t e = starts[g + 1];
+  lo = v > pairs ? pairs : v;
+  hi = e > lo ? (e > pairs ? pairs : e) : lo;
+}
+
+// dz = dy f'(pre) rounded, and db = the sum of the unrounded dz over each group's rows.  A workgroup
+// takes 256 columns (8 a thread) of one part of a group's rows, 8 rows at a time.  Bound by memory: dy
+// and pre in, dz out.
+template <typename T>
+__global__ __launch_bounds__(256) void slope_kernel(SlopeArgs a) {
+  __shared__ float sum[8][256 + 8];
+  const int tid = threadIdx.x, rl = tid >> 5, cl = (tid & 31) * 8;
+  const int64_t jb = ceil_div(a.N, 256), items = jb * a.groups * a.splits;
+  for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
+    const int64_t j = (it % jb) * 256 + cl;
+    const int g = (int)(it / jb % a.groups), s = (int)(it / jb / a.groups);
+    int64_t lo = 0, hi = a.pairs;
+    if (a.starts) group_rows(a.starts, g, a.pairs, lo, hi);
+    const int64_t per = ceil_div(hi - lo, a.splits);
+    const int64_t r0 = lo + s * per, r1 = r0 + per < hi ? r0 + per : hi;
+    const int m = (int)(a.N - j < 8 ? a.N - j : 8);
+    float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (m > 0)
+#pragma unroll 2
+      for (int64_t r = r0 + rl; r < r1; r += 8) {
+        const u32x4 y = load8(a.dy + r * a.ldy + j, m);
+        float v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = T::load((uint16_t)(y[q >> 1] >> (16 * (q & 1))));
+        if (a.act != kNone) {
+          const u32x4 z = load8(a.pre + r * a.N + j, m);
+#pragma unroll
+          for (int q = 0; q < 8; ++q) v[q] *= slope(a.act, T::load((uint16_t)(z[q >> 1] >> (16 * (q & 1)))));
+          uint16_t* const o = a.dz + r * a.N + j;
+          u32x4 w;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) w[q] = T::round2(v[2 * q], v[2 * q + 1]);
+          if (m == 8) {
+            __builtin_memcpy(o, &w, 16);
+          } else {
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              if (q < m) o[q] = (uint16_t)(w[q >> 1] >> (16 * (q & 1)));
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < 8; ++q) acc[q] += v[q];
+      }
+    if (!a.db) continue;
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 8; ++q) sum[rl][cl + q] = acc[q];
+    __syncthreads();
+    const int64_t jj = (it % jb) * 256 + tid;
+    if (jj < a.N) {
+      float t = 0;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) t += sum[q][tid];
+      if (a.splits > 1)
+        a.part[((int64_t)s * a.groups + g) * a.N + jj] = t;
+      else
+        a.db[(int64_t)g * a.N + jj] = T::round(t);
+    }
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void slope_join_kernel(const float* __restrict__ part, int64_t n, int splits,
+                                                         uint16_t* __restrict__ db) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    float t = 0;
+    for (int s = 0; s < splits; ++s) t += part[s * n + i];
+    db[i] = T::round(t);
+  }
+}
+
+// out[t] = sum over j ascending of part[pair_pos[t, j]], fp32, rounded once; entries outside the pairs
+// add nothing.  Bound by reading part.
+template <typename T>
+__global__ __launch_bounds__(256) void sum_pairs_kernel(const uint16_t* __restrict__ part, int64_t pairs, int64_t K,
+                                                        int64_t ldp, const int32_t* __restrict__ pos, int64_t tokens,
+                                                        int topk, uint16_t* __restrict__ out) {
+  const int64_t per = ceil_div(K, 8), items = tokens * per;
+  for (int64_t it = (int64_t)blockIdx.x * 256 + threadIdx.x; it < items; it += (int64_t)gridDim.x * 256) {
+    const int64_t t = it / per, k = (it % per) * 8;
+    const int m = (int)(K - k < 8 ? K - k : 8);
+    float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll 4
+    for (int j = 0; j < topk; ++j) {
+      const int32_t p = pos[t * topk + j];
+      if ((uint32_t)p < (uint64_t)pairs) {
+        const u32x4 v = load8(part + p * ldp + k, m);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) acc[q] += T::load((uint16_t)(v[q >> 1] >> (16 * (q & 1))));
+      }
+    }
+    u32x4 w;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) w[q] = T::round2(acc[2 * q], acc[2 * q + 1]);
+    uint16_t* const o = out + t * K + k;
+    if (m == 8) {
+      __builtin_memcpy(o, &w, 16);
+    } else {
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        if (q < m) o[q] = (uint16_t)(w[q >> 1] >> (16 * (q & 1)));
+    }
+  }
+}
+
+// =============================================================================================
+// Host
+// =============================================================================================
+
+int64_t cus() {   // of the current device
+  static int64_t known[64];
+  int dev = 0, n = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+  if (!known[dev]) {
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) return 256;
+    known[dev] = n;
+  }
+  return known[dev];
+}
+
+// Parts of the contraction: as many as give every CU a tile, of at least 256 each.
+int64_t splits_of(int64_t tiles, int64_t c) {
+  const int64_t want = tiles > 0 ? 256 / tiles : 1, most = c / 256;
+  return std::max<int64_t>(1, std::min<int64_t>({want, most, 32}));
+}
+
+struct Plan {
+  int tile;       // rows and columns of a tile
+  int64_t tiles;  // upper bound
+  int64_t splits;
+};
+
+// op: the product; rows: pairs
+Plan plan(int op, int64_t pairs, int64_t n, int64_t k, int64_t groups) {
+  Plan p;
+  const int64_t J = op == kFwd ? n : k;
+  auto tiles = [&](int64_t t) {
+    return (op == kDw ? groups * ceil_div(n, t) : ceil_div(pairs, t) + (groups > 1 ? groups : 0)) * ceil_div(J, t);
+  };
+  p.tile = tiles(128) >= 512 ? 128 : 64;
+  p.tiles = tiles(p.tile);
+  p.splits = splits_of(p.tiles, op == kFwd ? k : (op == kDx ? n : pairs / std::max<int64_t>(groups, 1)));
+  return p;
+}
+
+int64_t part_bytes(int op, const Plan& p, int64_t pairs, int64_t n, int64_t k, int64_t groups) {
+  if (p.splits <= 1) return 0;
+  const int64_t out = op == kDw ? groups * n * k : pairs * (op == kFwd ? n : k);
+  return p.splits * out * 4;
+}
+
+int64_t slope_splits(int64_t pairs, int64_t n, int64_t groups) {
+  const int64_t items = ceil_div(n, 256) * std::max<int64_t>(groups, 1);
+  return std::max<int64_t>(1, std::min<int64_t>({ceil_div(1024, items), ceil_div(pairs / std::max<int64_t>(groups, 1), 64), 64}));
+}
+
+template <typename T, int MODE>
+int run_typed(const Args& a, const Plan& p, hipStream_t s) {
+  static const char* const names[] = {"linear_fwd", "linear_dx", "linear_dw"};
+  const int64_t items = p.tiles * p.splits;
+  const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>(items, cus() * 4)));
+  if (p.tile == 128)
+    launch(names[MODE], any_kernel<T, MODE, 128, 128>, grid, dim3(256), 0, s, a);
+  else
+    launch(names[MODE], any_kernel<T, MODE, 64, 64>, grid, dim3(256), 0, s, a);
+  FERRY_LAUNCHED(names[MODE]);
+  if (a.splits > 1) {
+    const int64_t rows = MODE == kDw ? a.groups * a.I : a.pairs;
+    launch("linear_join", join_kernel<T, MODE>,
+           dim3((unsigned)std::min<int64_t>(ceil_div(rows * ceil_div(a.J, 256), 4), 65536)), dim3(256), 0, s, a);
+    FERRY_LAUNCHED("linear_join");
+  }
+  return 0;
+}
+
+template <int MODE>
+int run(Args& a, int32_t dtype, int64_t pairs, int64_t n, int64_t k, void* workspace, int64_t workspace_bytes,
+        hipStream_t s) {
+  const Plan p = plan(MODE, pairs, n, k, a.groups);
+  const int64_t need = part_bytes(MODE, p, pairs, n, k, a.groups);
+  FERRY_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need), "workspace too small (%lld < %lld bytes)",
+                  (long long)workspace_bytes, (long long)need);
+  FERRY_CHECK_ARG(need == 0 || (uintptr_t)workspace % 16 == 0, "workspace must be 16-byte aligned");
+  a.pairs = pairs;
+  a.splits = (int32_t)p.splits;
+  a.part = (float*)workspace;
+  auto even = [](const void* q, int64_t stride) { return (uintptr_t)q % 8 == 0 && stride % 4 == 0; };
+  a.vec_out = even(a.out, a.ldo) && a.o_group % 4 == 0 && (!a.residual || even(a.residual, a.ldr)) &&
+              (!a.pre || even(a.pre, a.J));
+  return dtype == FERRY_BF16 ? run_typed<Bf16, MODE>(a, p, s) : run_typed<F16, MODE>(a, p, s);
+}
+
+constexpr int64_t kMost = (int64_t)1 << 30;   // rows, columns, pairs: tile numbers are counted in 32 bits
+
+int check_sizes(int32_t dtype, int64_t pairs, int64_t n, int64_t k, int64_t groups, const int64_t* starts) {
+  FERRY_CHECK_ARG(dtype == FERRY_BF16 || dtype == FERRY_F16, "dtype must be bf16 or fp16");
+  FERRY_CHECK_ARG(pairs >= 0 && pairs < kMost && n >= 1 && n < kMost && k >= 1 && k < kMost,
+                  "bad sizes: rows in [0, 2^30), n and k in [1, 2^30)");
+  FERRY_CHECK_ARG(groups >= 1 && groups <= kMaxGroups, "groups must be in [1, %d]", kMaxGroups);
+  FERRY_CHECK_ARG(groups * n <= (int64_t)1 << 36, "bad sizes: groups * n above 2^36");
+  FERRY_CHECK_ARG(starts || groups == 1, "starts must name the rows of several groups");
+  return 0;
+}
+
+}  // namespace
+}  // namespace lin
+}  // namespace ferry
+
+using namespace ferry;
+using namespace ferry::lin;
+
+extern "C" int64_t ferry_linear_workspace_bytes(int32_t op, int64_t pairs, int64_t n, int64_t k, int64_t groups) {
+  if (pairs < 0 || pairs >= kMost || n < 1 || n >= kMost || k < 1 || k >= kMost || groups < 1 || groups > kMaxGroups)
+    return -1;
+  if (op == FERRY_LINEAR_GRAD_Z) {
+    const int64_t s = slope_splits(pairs, n, groups);
+    return s > 1 ? s * groups * n * 4 : 0;
+  }
+  if (op < kFwd || op > kDw) return -1;
+  return part_bytes(op, plan(op, pairs, n, k, groups), pairs, n, k, groups);
+}
+
+extern "C" int ferry_expert_linear(const void* x, int32_t dtype, int64_t x_rows, int64_t k, int64_t x_stride,
+                                   const int64_t* rows, int64_t pairs, const int64_t* starts, int64_t groups,
+                                   const void* w, int64_t n, int64_t w_stride, int64_t w_group_stride,
+                                   const void* bias, int64_t bias_stride, int32_t activation, const void* residual,
+                                   int64_t residual_stride, void* pre, void* out, int64_t out_stride,
+                                   int32_t zero_rest, void* workspace, int64_t workspace_bytes, void* stream) {
+  clear_error();
+  if (int rc = check_sizes(dtype, pairs, n, k, groups, starts)) return rc;
+  FERRY_CHECK_ARG(activation >= kNone && activation <= kGeluTanh, "unknown activation");
+  FERRY_CHECK_ARG(x_rows >= 0 && (rows || x_rows >= pairs), "x must have a row for every output row");
+  FERRY_CHECK_ARG((x_stride >= k || x_rows <= 1) && (w_stride >= k || n == 1) && (out_stride >= n || pairs <= 1) && w_group_stride >= 0 &&
+                      bias_stride >= 0 && (!residual || residual_stride >= 0),
+                  "strides must reach over their rows");
+  if (pairs == 0) return 0;
+  FERRY_CHECK_ARG(x && w && out, "null pointer argument");
+  Args a = {};
+  a.a = (const uint16_t*)x, a.lda = x_stride;
+  a.b = (const uint16_t*)w, a.ldb = w_stride, a.b_group = w_group_stride;
+  a.out = (uint16_t*)out, a.ldo = out_stride;
+  a.starts = starts, a.rows = rows, a.x_rows = x_rows;
+  a.J = n, a.C = k, a.groups = (int32_t)groups;
+  a.act = activation, a.zero_rest = starts && zero_rest;
+  a.bias = (const uint16_t*)bias, a.bias_group = bias_stride;
+  a.residual = (const uint16_t*)residual, a.ldr = residual_stride;
+  a.pre = (uint16_t*)pre;
+  return run<kFwd>(a, dtype, pairs, n, k, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+extern "C" int ferry_linear_grad_z(const void* grad, int32_t dtype, int64_t pairs, int64_t n, int64_t grad_stride,
+                                   const void* pre, int32_t activation, const int64_t* starts, int64_t groups, void* dz,
+                                   void* db, void* workspace, int64_t workspace_bytes, void* stream) {
+  clear_error();
+  if (int rc = check_sizes(dtype, pairs, n, 1, groups, starts)) return rc;
+  FERRY_CHECK_ARG(activation >= kNone && activation <= kGeluTanh, "unknown activation");
+  FERRY_CHECK_ARG(grad_stride >= n || pairs <= 1, "strides must reach over their rows");
+  FERRY_CHECK_ARG(activation == kNone || pairs == 0 || (pre && dz), "pre and dz belong to an activation");
+  FERRY_CHECK_ARG(!starts || activation == kNone, "groups have no activation");
+  if (activation == kNone && !db) return 0;
+  FERRY_CHECK_ARG(pairs == 0 || grad, "null pointer argument");
+  SlopeArgs a = {};
+  a.splits = (int32_t)slope_splits(pairs, n, groups);
+  const int64_t need = db && a.splits > 1 ? a.splits * groups * n * 4 : 0;
+  FERRY_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need), "workspace too small (%lld < %lld bytes)",
+                  (long long)workspace_bytes, (long long)need);
+  FERRY_CHECK_ARG(need == 0 || (uintptr_t)workspace % 16 == 0, "workspace must be 16-byte aligned");
+  a.dy = (const uint16_t*)grad, a.pre = (const uint16_t*)pre, a.dz = (uint16_t*)dz, a.db = (uint16_t*)db;
+  a.part = (float*)workspace, a.ldy = grad_stride, a.pairs = pairs, a.N = n;
+  a.starts = starts, a.groups = (int32_t)groups, a.act = activation;
+  hipStream_t s = (hipStream_t)stream;
+  const dim3 grid((unsigned)std::min<int64_t>(ceil_div(n, 256) * groups * a.splits, kMaxGrid));
+  if (dtype == FERRY_BF16)
+    launch("linear_slope", slope_kernel<Bf16>, grid, dim3(256), 0, s, a);
+  else
+    launch("linear_slope", slope_kernel<F16>, grid, dim3(256), 0, s, a);
+  FERRY_LAUNCHED("linear_slope");
+  if (need) {
+    const dim3 g2((unsigned)std::min<int64_t>(ceil_div(groups * n, 256), 65536));
+    if (dtype == FERRY_BF16)
+      launch("linear_slope_join", slope_join_kernel<Bf16>, g2, dim3(256), 0, s, (const float*)a.part, groups * n, (int)a.splits, a.db);
+    else
+      launch("linear_slope_join", slope_join_kernel<F16>, g2, dim3(256), 0, s, (const float*)a.part, groups * n, (int)a.splits, a.db);
+    FERRY_LAUNCHED("linear_slope_join");
+  }
+  return 0;
+}
+
+extern "C" int ferry_expert_linear_grad_x(const void* dz, int32_t dtype, int64_t pairs, int64_t n, int64_t dz_stride,
+                                          const int64_t* starts, int64_t groups, const void* w, int64_t k,
+                                          int64_t w_stride, int64_t w_group_stride, void* out, int32_t zero_rest,
+                                          void* workspace, int64_t workspace_bytes, void* stream) {
+  clear_error();
+  if (int rc = check_sizes(dtype, pairs, n, k, groups, starts)) return rc;
+  FERRY_CHECK_ARG((dz_stride >= n || pairs <= 1) && (w_stride >= k || n == 1) && w_group_stride >= 0,
+                  "strides must reach over their rows");
+  if (pairs == 0) return 0;
+  FERRY_CHECK_ARG(dz && w && out, "null pointer argument");
+  Args a = {};
+  a.a = (const uint16_t*)dz, a.lda = dz_stride;
+  a.b = (const uint16_t*)w, a.ldb = w_stride, a.b_group = w_group_stride;
+  a.out = (uint16_t*)out, a.ldo = k;
+  a.starts = starts, a.J = k, a.C = n, a.groups = (int32_t)groups, a.zero_rest = starts && zero_rest;
+  return run<kDx>(a, dtype, pairs, n, k, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+extern "C" int ferry_expert_linear_grad_w(const void* dz, int32_t dtype, int64_t pairs, int64_t n, int64_t dz_stride,
+                                          const void* x, int64_t x_rows, int64_t k, int64_t x_stride,
+                                          const int64_t* rows, const int64_t* starts, int64_t groups, void* dw,
+                                          void* workspace, int64_t workspace_bytes, void* stream) {
+  clear_error();
+  if (int rc = check_sizes(dtype, pairs, n, k, groups, starts)) return rc;
+  FERRY_CHECK_ARG(x_rows >= 0 && (rows || x_rows >= pairs), "x must have a row for every row of the gradient");
+  FERRY_CHECK_ARG((dz_stride >= n || pairs <= 1) && (x_stride >= k || x_rows <= 1), "strides must reach over their rows");
+  FERRY_CHECK_ARG(dw && (pairs == 0 || (dz && x)), "null pointer argument");
+  Args a = {};
+  a.a = (const uint16_t*)dz, a.lda = dz_stride;
+  a.b = (const uint16_t*)x, a.ldb = x_stride;
+  a.out = (uint16_t*)dw, a.ldo = k, a.o_group = n * k;
+  a.starts = starts, a.rows = rows, a.x_rows = x_rows;
+  a.I = n, a.J = k, a.groups = (int32_t)groups;
+  return run<kDw>(a, dtype, pairs, n, k, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+extern "C" int ferry_sum_pairs(const void* part, int32_t dtype, int64_t pairs, int64_t k, const int32_t* pair_pos,
+                               int64_t tokens, int64_t topk, void* out, void* stream) {
+  clear_error();
+  FERRY_CHECK_ARG(dtype == FERRY_BF16 || dtype == FERRY_F16, "dtype must be bf16 or fp16");
+  FERRY_CHECK_ARG(pairs >= 0 && pairs < kMost && k >= 1 && k < kMost && tokens >= 0 && tokens < kMost && topk >= 1 && topk < kMost, "bad sizes");
+  if (tokens == 0) return 0;
+  FERRY_CHECK_ARG(out && pair_pos && (part || pairs == 0), "null pointer argument");
+  const dim3 grid((unsigned)std::min<int64_t>(ceil_div(tokens * ceil_div(k, 8), 256), 1 << 20));
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == FERRY_BF16)
+    launch("sum_pairs", sum_pairs_kernel<Bf16>, grid, dim3(256), 0, s, (const uint16_t*)part, pairs, k, k, pair_pos, tokens, (int)topk, (uint16_t*)out);
+  else
+    launch("sum_pairs", sum_pairs_kernel<F16>, grid, dim3(256), 0, s, (const uint16_t*)part, pairs, k, k, pair_pos, tokens, (int)topk, (uint16_t*)out);
+  FERRY_LAUNCHED("sum_pairs");
+  return 0;
+}

@@ -14,6 +14,7 @@ import numpy as np
 import torch
 import torch.nn.functional as F
 from torch.autograd import forward_ad
+from torch.autograd.function import once_differentiable
 
 from ._lib import check, lib
 from ._lib import check as _check_status
@@ -22,7 +23,8 @@ from .h2d import H2DEngine
 __all__ = ['execute_experts', 'pack_dispatch', 'unpack_dispatch', 'reduce_partials',
            'scatter_returned', 'H2DEngine', 'router_topk', 'layout', 'gate_logits', 'expert_ffn',
            'combine', 'SharedExpert', 'route_experts', 'mxfp4_quantize', 'mxfp4_dequantize',
-           'mxfp4_expert_rows', 'mxfp4_expert_ffn', 'history_update', 'history_ready_words', 'current_stream', 'PHASE_UP',
+           'mxfp4_expert_rows', 'mxfp4_expert_ffn', 'linear', 'linear_grad', 'expert_linear', 'expert_linear_grad',
+           'sum_pairs', 'history_update', 'history_ready_words', 'current_stream', 'PHASE_UP',
            'PHASE_DOWN', 'PHASE_BOTH']
 
 MAX_EXPERTS = 512
@@ -496,6 +498,332 @@ def mxfp4_expert_ffn(cache, x, w_sorted, starts, rows, cols, expert_list, slot_o
     _native(cache, 'mxfp4_expert_ffn', lib().ferry_mxfp4_expert_ffn, cache.data_ptr(), cache.shape[0], H, I,
             x_at, scales_at, R, k, weights, first, rows_at, cols_at, el.tobytes(), len(el), so.tobytes(), E, most, 0,
             list_rows, act_at, out_at, int(out_mode), int(phases), int(spare_cus))
+    return out
+
+
+_ACTIVATIONS = {None: 0, 'relu': 1, 'silu': 2, 'gelu': 3, 'gelu_tanh': 4}   # FERRY_ACT_*
+_LINEAR, _GRAD_X, _GRAD_W, _GRAD_Z = 0, 1, 2, 3                                # FERRY_LINEAR*
+_HALF = {torch.bfloat16: 0, torch.float16: 2}                                 # FERRY_BF16, FERRY_F16
+
+
+def _half_rows(t, name, device=None, dtype=None):
+    """(address, row stride) of the rows of a bf16 or fp16 tensor, on ``device`` and of ``dtype`` if given."""
+    stride = _row_stride(t, name)
+    if dtype is None:
+        if t.dtype not in _HALF:
+            raise RuntimeError(f'{name} must be bf16 or fp16')
+    elif t.dtype != dtype:
+        raise RuntimeError(f'{name} must be {dtype}, got {t.dtype}')
+    if device is not None and t.get_device() != device:
+        raise RuntimeError(f'{name} must be on cuda:{device}')
+    return t.data_ptr(), stride
+
+
+def _weight_groups(w, name, device, dtype):
+    """(address, row stride, group stride) of [groups, n, k] weights whose rows are contiguous."""
+    if not isinstance(w, torch.Tensor) or w.get_device() != device:
+        raise RuntimeError(f'{name} must be on cuda:{device}')
+    if w.dtype != dtype:
+        raise RuntimeError(f'{name} must be {dtype}, got {w.dtype}')
+    _, n, k = w.shape
+    group, row, one = w.stride()
+    if (k > 1 and one != 1) or (n > 1 and row < k):
+        raise RuntimeError(f'the rows of {name} must be contiguous')
+    return w.data_ptr(), row if n > 1 else k, group
+
+
+def _workspace(product, pairs, n, k, groups, device):
+    """(tensor or None, address, bytes) of a linear product's scratch memory."""
+    need = lib().ferry_linear_workspace_bytes(product, pairs, n, k, groups)
+    if need <= 0:
+        return None, None, 0
+    ws = torch.empty(need, dtype=torch.uint8, device=device)
+    return ws, ws.data_ptr(), need
+
+
+def _watched(what, *tensors):
+    """Whether autograd takes part in a call on these tensors (None among them)."""
+    if (getattr(forward_ad, '_current_level', 0) >= 0
+            and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)):
+        raise RuntimeError(f'{what} has no forward-mode derivative')
+    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors):
+        return False
+    if torch.cuda.is_current_stream_capturing():
+        # autograd ties a captured backward pass to the streams of every eager one that shares a leaf
+        raise RuntimeError(f'{what}: capture it and {what}_grad under torch.no_grad(); a graph with autograd '
+                           'in it is not supported')
+    return True
+
+
+def _product(x, xs, k, rows, pairs, starts, groups, w, ws, wg, n, bias, bias_stride, act, residual, rs, pre, out,
+             out_stride, zero_rest):
+    scratch, at, size = _workspace(_LINEAR, pairs, n, k, groups, x.device)
+    _native(x, 'linear' if starts is None else 'expert_linear', lib().ferry_expert_linear,
+            x.data_ptr(), _HALF[x.dtype], x.numel() // k, k, xs, rows, pairs, starts, groups, w, n, ws, wg, bias,
+            bias_stride, act, residual, rs, pre, out, out_stride, zero_rest, at, size)
+
+
+def _linear(x, weight, bias, activation, residual, out, keep):
+    """(out, pre or None) of ``linear``."""
+    act = _ACTIVATIONS.get(activation, -1)
+    if act < 0:
+        raise ValueError("activation must be None, 'relu', 'silu', 'gelu' or 'gelu_tanh'")
+    _, xs = _half_rows(x, 'x')
+    dtype, dev = x.dtype, x.get_device()
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or weight.shape[1] != x.shape[-1]:
+        raise RuntimeError('weight must be [n, k] for x [..., k]')
+    w, ws = _half_rows(weight, 'weight', dev, dtype)
+    n, k = weight.shape
+    *lead, _ = x.shape
+    m = math.prod(lead)
+    shape = (*lead, n)
+    if bias is not None and bias.shape != (n,):
+        raise RuntimeError('bias must be [n]')
+    b = _at(bias, 'bias', dtype, dev) if bias is not None else None
+    r, rs = None, 0
+    if residual is not None:
+        r, rs = _half_rows(residual, 'residual', dev, dtype)
+        if residual.shape != shape:
+            raise RuntimeError(f'residual must be {list(shape)}')
+    if out is None:
+        out = _matrix(m, n, dtype, x.device)
+        if len(lead) != 1:
+            out = out.view(shape)
+        at, stride = out.data_ptr(), n
+    else:
+        at, stride = _half_rows(out, 'out', dev, dtype)
+        if out.shape != shape:
+            raise RuntimeError(f'out must be {list(shape)}')
+    pre = _matrix(m, n, dtype, x.device) if keep and act else None
+    if m:
+        _product(x, xs, k, None, m, None, 1, w, ws, 0, n, b, 0, act, r, rs,
+                 pre.data_ptr() if pre is not None else None, at, stride, 0)
+    return out, pre
+
+
+def linear(x, weight, bias=None, activation=None, residual=None, out=None, return_pre=False):
+    """``activation(x @ weight.T + bias) + residual``, rounded once.
+
+    ``x`` [..., k], ``weight`` [n, k] (a matrix may have a row stride), ``bias`` [n] and ``residual``
+    [..., n] are bf16 or fp16, all the same; sums are fp32.  ``activation`` is None, 'relu', 'silu', 'gelu'
+    (the normal distribution's) or 'gelu_tanh'.  ``out`` (optional) receives the result and may be
+    ``residual`` itself.  ``return_pre=True`` returns (result, the activation's rounded argument [rows, n],
+    or None without an activation), what ``linear_grad`` needs.  Rows that start at multiples of 16 bytes
+    are fastest; any other alignment is taken.
+
+    The result carries the gradients of x, weight, bias and residual, except with ``out`` or ``return_pre``
+    and inside a captured graph (there ``linear`` and ``linear_grad`` are called under torch.no_grad()).
+    No counterpart in the reference."""
+    if _watched('linear', x, weight, bias, residual):
+        if out is not None or return_pre:
+            raise RuntimeError('linear: out and return_pre carry no gradients; call it under torch.no_grad()')
+        return _Linear.apply(x, weight, bias, residual, activation)
+    y, pre = _linear(x, weight, bias, activation, residual, out, return_pre)
+    return (y, pre) if return_pre else y
+
+
+def _column_sums(grad, gs, rows, n, starts, groups, pre, act, dz, db):
+    scratch, at, size = _workspace(_GRAD_Z, rows, n, 1, groups, grad.device) if db is not None else (None, None, 0)
+    _native(grad, 'linear_grad', lib().ferry_linear_grad_z, grad.data_ptr(), _HALF[grad.dtype], rows, n, gs,
+            pre.data_ptr() if pre is not None else None, act, starts, groups,
+            dz.data_ptr() if dz is not None else None, db.data_ptr() if db is not None else None, at, size)
+
+
+def _grad_x(dz, zs, pairs, starts, groups, w, ws, wg, n, k, zero_rest):
+    dx = _matrix(pairs, k, dz.dtype, dz.device)
+    if pairs:
+        scratch, at, size = _workspace(_GRAD_X, pairs, n, k, groups, dz.device)
+        _native(dz, 'linear_grad', lib().ferry_expert_linear_grad_x, dz.data_ptr(), _HALF[dz.dtype], pairs, n, zs,
+                starts, groups, w, k, ws, wg, dx.data_ptr(), zero_rest, at, size)
+    return dx
+
+
+def _grad_w(dz, zs, pairs, n, x, xs, k, rows, starts, groups):
+    dw = torch.empty((groups, n, k), dtype=dz.dtype, device=dz.device)
+    scratch, at, size = _workspace(_GRAD_W, pairs, n, k, groups, dz.device)
+    _native(dz, 'linear_grad', lib().ferry_expert_linear_grad_w, dz.data_ptr(), _HALF[dz.dtype], pairs, n, zs,
+            x.data_ptr(), x.numel() // k, k, xs, rows, starts, groups, dw.data_ptr(), at, size)
+    return dw
+
+
+def linear_grad(grad, x, weight, pre=None, activation=None, need_x=True, need_weight=True, need_bias=True):
+    """Gradients (dx, dweight, dbias) of ``linear`` for the gradient ``grad`` [..., n] of its result, None for
+    those that are not needed; ``pre`` is ``linear(..., return_pre=True)``'s.  The residual's is ``grad``.
+
+    dz = grad * f'(pre) is rounded to the inputs' type before the products; the bias's gradient sums it
+    unrounded.  Makes no use of autograd, so it can be captured into a graph."""
+    act = _ACTIVATIONS.get(activation, -1)
+    if act < 0:
+        raise ValueError("activation must be None, 'relu', 'silu', 'gelu' or 'gelu_tanh'")
+    _, xs = _half_rows(x, 'x')
+    dtype, dev = x.dtype, x.get_device()
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or weight.shape[1] != x.shape[-1]:
+        raise RuntimeError('weight must be [n, k] for x [..., k]')
+    w, ws = _half_rows(weight, 'weight', dev, dtype)
+    n, k = weight.shape
+    *lead, _ = x.shape
+    m = math.prod(lead)
+    _, gs = _half_rows(grad, 'grad', dev, dtype)
+    if grad.shape != (*lead, n):
+        raise RuntimeError(f'grad must be {[*lead, n]}')
+    dz, zs = grad, gs
+    db = torch.empty(n, dtype=dtype, device=x.device) if need_bias else None
+    if act:
+        if not isinstance(pre, torch.Tensor) or pre.shape != (m, n):
+            raise RuntimeError('pre must be [rows, n], as linear returns it')
+        _at(pre, 'pre', dtype, dev)
+        dz, zs = _matrix(m, n, dtype, x.device), n
+        _column_sums(grad, gs, m, n, None, 1, pre, act, dz, db)
+    elif need_bias:
+        _column_sums(grad, gs, m, n, None, 1, None, 0, None, db)
+    dx = _grad_x(dz, zs, m, None, 1, w, ws, 0, n, k, 0).view(x.shape) if need_x else None
+    dw = _grad_w(dz, zs, m, n, x, xs, k, None, None, 1).view(n, k) if need_weight else None
+    return dx, dw, db
+
+
+def _rows_of(grad):
+    """``grad`` as autograd hands it over, with contiguous rows."""
+    try:
+        _row_stride(grad, 'grad')
+        return grad
+    except RuntimeError:
+        return grad.contiguous()
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, activation):
+        y, pre = _linear(x, weight, bias, activation, residual, None, any(ctx.needs_input_grad[:3]))
+        ctx.activation = activation
+        ctx.save_for_backward(x, weight, pre)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        x, weight, pre = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx = dw = db = None
+        if any(need[:3]):
+            dx, dw, db = linear_grad(_rows_of(grad), x, weight, pre, ctx.activation, *need[:3])
+        return dx, dw, db, grad if need[3] else None, None
+
+
+def _expert_args(x, weight, starts, rows):
+    """What ``expert_linear`` and its gradients share: x's row stride, the weights' place, the pairs."""
+    _, xs = _half_rows(x, 'x')
+    dtype, dev = x.dtype, x.get_device()
+    if x.dim() != 2 or not isinstance(weight, torch.Tensor) or weight.dim() != 3 or weight.shape[2] != x.shape[1]:
+        raise RuntimeError('x must be [rows, k] and weight [experts, n, k]')
+    w, ws, wg = _weight_groups(weight, 'weight', dev, dtype)
+    first = _at(starts, 'starts', torch.int64, dev)
+    if starts.shape != (weight.shape[0] + 1,):
+        raise RuntimeError('starts must have an entry for every expert, and the end')
+    rows_at, pairs = None, x.shape[0]
+    if rows is not None:
+        rows_at, pairs = _at(rows, 'rows', torch.int64, dev), rows.numel()
+    return xs, w, ws, wg, first, rows_at, pairs
+
+
+def _expert_linear(x, weight, starts, bias, rows, out):
+    xs, w, ws, wg, first, rows_at, pairs = _expert_args(x, weight, starts, rows)
+    E, n, k = weight.shape
+    b, bs = None, 0
+    if bias is not None:
+        b, bs = _half_rows(bias, 'bias', x.get_device(), x.dtype)
+        if bias.shape != (E, n):
+            raise RuntimeError('bias must be [experts, n]')
+    zero = out is None
+    if zero:
+        out = _matrix(pairs, n, x.dtype, x.device)
+        at, stride = out.data_ptr(), n
+    else:
+        at, stride = _half_rows(out, 'out', x.get_device(), x.dtype)
+        if out.shape != (pairs, n):
+            raise RuntimeError(f'out must be [{pairs}, {n}]')
+    if pairs:
+        _product(x, xs, k, rows_at, pairs, first, E, w, ws, wg, n, b, bs, 0, None, 0, None, at, stride, int(zero))
+    return out
+
+
+def expert_linear(x, weight, starts, bias=None, rows=None, pair_pos=None, out=None):
+    """Products grouped by expert: ``out[p] = x[rows[p]] @ weight[e].T + bias[e]`` for ``starts[e] <= p <
+    starts[e + 1]``, [pairs, n], for one matrix of an expert, of any number of rows each.
+
+    ``x`` [rows, k], ``weight`` [experts, n, k] (strides of experts and rows may be larger, as those of a
+    part of cache rows are) and ``bias`` [experts, n] are bf16 or fp16, all the same; sums are fp32, a result
+    is rounded once.  ``starts``, ``rows`` and ``pair_pos`` are ``layout``'s, on the device; without ``rows``
+    ``x`` is in grouped order already.  An entry of ``rows`` that names no row of x reads as zeros.  Rows
+    before ``starts[0]`` and from ``starts[experts]`` on are 0; in an ``out`` that is passed they stay as
+    they were.
+
+    The result carries the gradients of x, weight and bias (x's, with ``rows``, needs ``pair_pos`` [tokens *
+    topk], the places of each row of x), except with ``out`` and inside a captured graph (there
+    ``expert_linear`` and ``expert_linear_grad`` are called under torch.no_grad()).  No counterpart in the
+    reference."""
+    if _watched('expert_linear', x, weight, bias):
+        if out is not None:
+            raise RuntimeError('expert_linear: out carries no gradients; call it under torch.no_grad()')
+        if rows is not None and pair_pos is None and x.requires_grad:
+            raise RuntimeError('expert_linear: the gradient of gathered rows needs pair_pos')
+        return _ExpertLinear.apply(x, weight, starts, bias, rows, pair_pos)
+    return _expert_linear(x, weight, starts, bias, rows, out)
+
+
+def expert_linear_grad(grad, x, weight, starts, rows=None, pair_pos=None, need_x=True, need_weight=True,
+                       need_bias=True):
+    """Gradients (dx, dweight, dbias) of ``expert_linear`` for the gradient ``grad`` [pairs, n] of its result,
+    None for those that are not needed.  With ``rows``, dx[t] is the sum, j ascending, of the (rounded)
+    gradients of the grouped rows ``pair_pos[t, j]``; without ``pair_pos`` it is those, [pairs, k], in
+    grouped order.  Experts without rows have zero gradients; rows of ``grad`` that belong to no expert are
+    not read.  Makes no use of autograd, so it can be captured into a graph."""
+    xs, w, ws, wg, first, rows_at, pairs = _expert_args(x, weight, starts, rows)
+    E, n, k = weight.shape
+    _, gs = _half_rows(grad, 'grad', x.get_device(), x.dtype)
+    if grad.shape != (pairs, n):
+        raise RuntimeError(f'grad must be [{pairs}, {n}]')
+    dx = dw = db = None
+    if need_bias:
+        db = torch.empty((E, n), dtype=x.dtype, device=x.device)
+        _column_sums(grad, gs, pairs, n, first, E, None, 0, None, db)
+    if need_x:
+        dx = _grad_x(grad, gs, pairs, first, E, w, ws, wg, n, k, 1)
+        if rows is not None and pair_pos is not None:
+            dx = sum_pairs(dx, pair_pos, x.shape[0])
+    if need_weight:
+        dw = _grad_w(grad, gs, pairs, n, x, xs, k, rows_at, first, E)
+    return dx, dw, db
+
+
+class _ExpertLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, starts, bias, rows, pair_pos):
+        ctx.save_for_backward(x, weight, starts, rows, pair_pos)
+        return _expert_linear(x, weight, starts, bias, rows, None)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        x, weight, starts, rows, pair_pos = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx, dw, db = expert_linear_grad(_rows_of(grad), x, weight, starts, rows, pair_pos, need[0], need[1], need[3])
+        return dx, dw, None, db, None, None
+
+
+def sum_pairs(part, pair_pos, tokens):
+    """out[t] = the fp32 sum, j ascending, of ``part[pair_pos[t, j]]``, rounded once, [tokens, k]: the gradient of
+    rows that were gathered from tokens.  ``part`` is contiguous bf16 or fp16 [pairs, k], ``pair_pos`` int32
+    with as many entries for every token, ``layout``'s; entries outside [0, pairs) add nothing."""
+    if not isinstance(part, torch.Tensor) or part.dim() != 2 or part.dtype not in _HALF:
+        raise RuntimeError('part must be bf16 or fp16 [pairs, k]')
+    at, (pairs, k) = _dev(part, 'part'), part.shape
+    pos = _at(pair_pos, 'pair_pos', torch.int32, part.get_device())
+    if tokens and (pair_pos.numel() % tokens or not pair_pos.numel()):
+        raise RuntimeError('pair_pos must hold as many entries for every token')
+    out = _matrix(tokens, k, part.dtype, part.device)
+    if tokens:
+        _native(part, 'sum_pairs', lib().ferry_sum_pairs, at, _HALF[part.dtype], pairs, k, pos, tokens,
+                pair_pos.numel() // tokens, out.data_ptr())
     return out
 
 

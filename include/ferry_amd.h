@@ -299,6 +299,59 @@ int ferry_gate_logits(const void* x, int64_t tokens, int64_t hidden, const void*
                       int64_t experts, float* out, void* stream);
 
 /*
+ * Linear products, dense and grouped by expert, with their gradients (no counterpart in the reference,
+ * whose experts are SwiGLU blocks of bf16 matrices without biases).  All matrices are bf16 or fp16
+ * (dtype; every one of a call the same), their rows a stride apart and the elements of a row next to each
+ * other, at any alignment: rows whose address and stride are multiples of 16 bytes are read fastest.
+ * Sums are fp32 (for a contraction in parts, fp32 sums of those in their order); every output is rounded
+ * once.  Results do not depend on the order in which workgroups run.
+ *
+ * Groups: row p of the grouped order belongs to group g with starts[g] <= p < starts[g + 1] (device memory,
+ * int64 [groups + 1], as ferry_layout writes it; null: one group of all `pairs` rows).  Values that do not
+ * ascend within [0, pairs] are read as if they did.  rows (device memory, nullable) names the row of x of
+ * each p; an index outside [0, x_rows) reads as a row of zeros.  Output rows p of no group are set to 0 with
+ * zero_rest and stay as they were without.
+ *
+ * ferry_expert_linear: out[p] = f(x[rows[p]] w[g]^T + bias[g]) + residual[p], with w[g] an [n, k] matrix
+ * at w + g * w_group_stride elements, bias[g] its n values at bias + g * bias_stride (bias and residual
+ * nullable) and f the activation: none, relu, silu, gelu (of the normal distribution) or its tanh form.
+ * pre (nullable, contiguous [pairs, n]) receives the rounded argument of f.  residual may be out itself.
+ * ferry_linear_grad_z: dz = grad * f'(pre) (contiguous [pairs, n]; only with an activation, which a call
+ * with starts has not) and db[g] (nullable, contiguous [groups, n]) = the sum of grad * f'(pre) over the
+ * rows of g.
+ * ferry_expert_linear_grad_x: out[p] = dz[p] w[g], contiguous [pairs, k].
+ * ferry_expert_linear_grad_w: dw[g] = sum over the rows of g of dz[p]^T x[rows[p]], contiguous
+ * [groups, n, k]; 0 for a group without rows.
+ * ferry_sum_pairs: out[t] = sum over j ascending of part[pair_pos[t, j]] (the gradient of rows that were
+ * gathered from tokens; pair_pos as ferry_layout writes it, entries outside [0, pairs) add nothing).
+ * `workspace` (16-byte aligned device memory) must hold ferry_linear_workspace_bytes bytes of the product
+ * (-1 for bad sizes); calls that may run at the same time need one each.
+ * pairs, n and k are below 2^30, groups at most FERRY_MAX_EXPERTS, groups * n at most 2^36.
+ */
+enum { FERRY_ACT_NONE = 0, FERRY_ACT_RELU = 1, FERRY_ACT_SILU = 2, FERRY_ACT_GELU = 3, FERRY_ACT_GELU_TANH = 4 };
+enum { FERRY_LINEAR = 0, FERRY_LINEAR_GRAD_X = 1, FERRY_LINEAR_GRAD_W = 2, FERRY_LINEAR_GRAD_Z = 3 };
+int64_t ferry_linear_workspace_bytes(int32_t product, int64_t pairs, int64_t n, int64_t k, int64_t groups);
+int ferry_expert_linear(const void* x, int32_t dtype, int64_t x_rows, int64_t k, int64_t x_stride,
+                        const int64_t* rows, int64_t pairs, const int64_t* starts, int64_t groups,
+                        const void* w, int64_t n, int64_t w_stride, int64_t w_group_stride,
+                        const void* bias, int64_t bias_stride, int32_t activation, const void* residual,
+                        int64_t residual_stride, void* pre, void* out, int64_t out_stride, int32_t zero_rest,
+                        void* workspace, int64_t workspace_bytes, void* stream);
+int ferry_linear_grad_z(const void* grad, int32_t dtype, int64_t pairs, int64_t n, int64_t grad_stride,
+                        const void* pre, int32_t activation, const int64_t* starts, int64_t groups, void* dz,
+                        void* db, void* workspace, int64_t workspace_bytes, void* stream);
+int ferry_expert_linear_grad_x(const void* dz, int32_t dtype, int64_t pairs, int64_t n, int64_t dz_stride,
+                               const int64_t* starts, int64_t groups, const void* w, int64_t k,
+                               int64_t w_stride, int64_t w_group_stride, void* out, int32_t zero_rest,
+                               void* workspace, int64_t workspace_bytes, void* stream);
+int ferry_expert_linear_grad_w(const void* dz, int32_t dtype, int64_t pairs, int64_t n, int64_t dz_stride,
+                               const void* x, int64_t x_rows, int64_t k, int64_t x_stride,
+                               const int64_t* rows, const int64_t* starts, int64_t groups, void* dw,
+                               void* workspace, int64_t workspace_bytes, void* stream);
+int ferry_sum_pairs(const void* part, int32_t dtype, int64_t pairs, int64_t k, const int32_t* pair_pos,
+                    int64_t tokens, int64_t topk, void* out, void* stream);
+
+/*
  * Selection-frequency history on the device.  Replaces ferry/metadata.py:15-38 (GateHistory
  * update/scores over one-hot rows built by RouteGather.collect, ferry/metadata.py:67-83).
  * State per layer (device memory, caller-owned, zero-initialised):

@@ -2,6 +2,7 @@
 // every size and alignment, and the entry points.  No counterpart in the reference, whose experts are
 // SwiGLU blocks of bf16 matrices without biases or gradients.
 #include "linear.h"
+#include "linear_tile.h"
 
 #include <algorithm>
 
@@ -395,7 +396,7 @@ int64_t splits_of(int64_t tiles, int64_t c) {
 }
 
 struct Plan {
-  int tile;       // rows and columns of a tile
+  int tile;       // rows and columns of a tile; 256: tile256
   int64_t tiles;  // upper bound
   int64_t splits;
 };
@@ -407,10 +408,24 @@ Plan plan(int op, int64_t pairs, int64_t n, int64_t k, int64_t groups) {
   auto tiles = [&](int64_t t) {
     return (op == kDw ? groups * ceil_div(n, t) : ceil_div(pairs, t) + (groups > 1 ? groups : 0)) * ceil_div(J, t);
   };
-  p.tile = tiles(128) >= 512 ? 128 : 64;
+  p.tile = n % 8 == 0 && k % 8 == 0 && tiles(256) >= 48 ? 256 : (tiles(128) >= 512 ? 128 : 64);
   p.tiles = tiles(p.tile);
   p.splits = splits_of(p.tiles, op == kFwd ? k : (op == kDx ? n : pairs / std::max<int64_t>(groups, 1)));
   return p;
+}
+
+// Whether the tiled kernels can read and write the operands: rows at multiples of 16 bytes, offsets that 32
+// bits hold (a tile's, or all of an operand whose rows are gathered or follow the contraction).
+bool tiles_fit(int op, const Args& a, int64_t pairs, int64_t n, int64_t k) {
+  auto even = [](const void* q, int64_t stride) { return (uintptr_t)q % 16 == 0 && stride % 8 == 0; };
+  if (n % 8 || k % 8 || !even(a.a, a.lda) || !even(a.b, a.ldb) || a.b_group % 8 || !even(a.out, a.ldo) || a.o_group % 8 ||
+      (a.bias && !even(a.bias, a.bias_group)) || (a.residual && !even(a.residual, a.ldr)) || (a.pre && !even(a.pre, 0)))
+    return false;
+  const int64_t most = ((int64_t)1 << 31) - (1 << 20);   // elements, with room for a stage behind the end
+  const int64_t ia = op == kDw ? pairs : (a.rows ? a.x_rows : 512), ib = op == kFwd ? 512 : (op == kDx ? n : (a.rows ? a.x_rows : pairs));
+  if (a.lda > most / 512 || a.ldb > most / 512 || ia * a.lda > most || ib * a.ldb > most || a.C > most / 4) return false;
+  // the row numbers of a tile are loaded one tile ahead, which takes a contraction of more than two stages
+  return !(op == kFwd && a.rows) || ceil_div(ceil_div(k, a.splits), 64) * 64 > 128;
 }
 
 int64_t part_bytes(int op, const Plan& p, int64_t pairs, int64_t n, int64_t k, int64_t groups) {
@@ -425,14 +440,18 @@ int64_t slope_splits(int64_t pairs, int64_t n, int64_t groups) {
 }
 
 template <typename T, int MODE>
-int run_typed(const Args& a, const Plan& p, hipStream_t s) {
+int run_typed(const Args& a, const Plan& p, int64_t n, int64_t k, hipStream_t s) {
   static const char* const names[] = {"linear_fwd", "linear_dx", "linear_dw"};
   const int64_t items = p.tiles * p.splits;
-  const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>(items, cus() * 4)));
-  if (p.tile == 128)
-    launch(names[MODE], any_kernel<T, MODE, 128, 128>, grid, dim3(256), 0, s, a);
-  else
-    launch(names[MODE], any_kernel<T, MODE, 64, 64>, grid, dim3(256), 0, s, a);
+  if (p.tile == 256 && tiles_fit(MODE, a, a.pairs, n, k)) {
+    tile_launch(MODE, T::kType, names[MODE], a, items, cus(), s);
+  } else {
+    const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>(items, cus() * 4)));
+    if (p.tile >= 128)
+      launch(names[MODE], any_kernel<T, MODE, 128, 128>, grid, dim3(256), 0, s, a);
+    else
+      launch(names[MODE], any_kernel<T, MODE, 64, 64>, grid, dim3(256), 0, s, a);
+  }
   FERRY_LAUNCHED(names[MODE]);
   if (a.splits > 1) {
     const int64_t rows = MODE == kDw ? a.groups * a.I : a.pairs;
@@ -457,7 +476,7 @@ int run(Args& a, int32_t dtype, int64_t pairs, int64_t n, int64_t k, void* works
   auto even = [](const void* q, int64_t stride) { return (uintptr_t)q % 8 == 0 && stride % 4 == 0; };
   a.vec_out = even(a.out, a.ldo) && a.o_group % 4 == 0 && (!a.residual || even(a.residual, a.ldr)) &&
               (!a.pre || even(a.pre, a.J));
-  return dtype == FERRY_BF16 ? run_typed<Bf16, MODE>(a, p, s) : run_typed<F16, MODE>(a, p, s);
+  return dtype == FERRY_BF16 ? run_typed<Bf16, MODE>(a, p, n, k, s) : run_typed<F16, MODE>(a, p, n, k, s);
 }
 
 constexpr int64_t kMost = (int64_t)1 << 30;   // rows, columns, pairs: tile numbers are counted in 32 bits

@@ -1,0 +1,570 @@
+// The linear products on whole tiles: rows at multiples of 16 bytes, sizes of multiples of 8.
+#include "linear.h"
+#include "linear_tile.h"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace ferry {
+namespace lin {
+namespace {
+
+// -- loads to LDS, waits ---------------------------------------------------------------------------------
+
+// A part of memory as a buffer: reads behind its end give 0, also into LDS.
+__device__ __forceinline__ u32x4 buffer_at(const void* p, int64_t bytes) {
+  const uint64_t v = (uint64_t)(uintptr_t)p;
+  const int64_t n = bytes < 0 ? 0 : (bytes > 0xffffffffll ? 0xffffffffll : bytes);
+  return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v),
+               (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32)) & 0xffffu,
+               (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)n), 0x00020000u};
+}
+constexpr uint32_t kNowhere = 0xfffffff0u;   // an offset behind the end of every buffer
+
+// 16 bytes of each lane from offset soff + voff of the buffer to LDS address lds + 16 * lane; 0 from behind the
+// buffer's end (soff itself must lie in it, or be 0: the hardware compares voff with size - soff).  Inline asm,
+// so that no wait is added: their completion is awaited with wait_cnt.  m0 holds the LDS base; one wait state
+// between its write and the load.
+__device__ __forceinline__ void load_lds(u32x4 r, uint32_t voff, uint32_t soff, uint32_t lds) {
+  asm volatile(
+      "s_mov_b32 m0, %2\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %0, %1, %3 offen lds"
+      :
+      : "v"(voff), "s"(r), "s"(__builtin_amdgcn_readfirstlane((int)lds)), "s"(__builtin_amdgcn_readfirstlane((int)soff))
+      : "memory");
+}
+// 4 bytes of each lane, as above
+__device__ __forceinline__ void load_lds4(u32x4 r, uint32_t voff, uint32_t lds) {
+  asm volatile(
+      "s_mov_b32 m0, %2\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dword %0, %1, 0 offen lds"
+      :
+      : "v"(voff), "s"(r), "s"(lds)
+      : "memory");
+}
+template <int VM>
+__device__ __forceinline__ void wait_cnt() {   // at most VM loads and no LDS reads outstanding
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((VM & 15) | (7 << 4) | ((VM >> 4) << 14));
+  asm volatile("" ::: "memory");
+}
+// barrier of a workgroup without the fence of __syncthreads, which would drain the loads
+__device__ __forceinline__ void wg_barrier() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_barrier" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+__device__ __forceinline__ uint32_t lds_at(const void* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
+}
+
+// -- epilogue ------------------------------------------------------------------------------------------
+
+template <typename T>
+__device__ __forceinline__ void unpack8(const u32x4& v, float (&f)[8]) {
+#pragma unroll
+  for (int q = 0; q < 8; ++q) f[q] = T::load((uint16_t)(v[q >> 1] >> (16 * (q & 1))));
+}
+template <typename T>
+__device__ __forceinline__ u32x4 pack8(const float (&f)[8]) {
+  u32x4 w;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) w[q] = T::round2(f[2 * q], f[2 * q + 1]);
+  return w;
+}
+// columns j .. j + 7 of row `row`: v + bias, pre, activation, residual r, one rounding
+template <typename T, int ACT>
+__device__ __forceinline__ void finish8(const Args& a, uint16_t* out, int64_t row, int64_t j, float (&v)[8],
+                                        const u32x4& bias, const u32x4& r) {
+  float f[8];
+  unpack8<T>(bias, f);
+#pragma unroll
+  for (int q = 0; q < 8; ++q) v[q] += f[q];
+  if constexpr (ACT != kNone) {
+    if (a.pre) *reinterpret_cast<u32x4*>(a.pre + row * a.J + j) = pack8<T>(v);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = activate(ACT, v[q]);
+  }
+  unpack8<T>(r, f);
+#pragma unroll
+  for (int q = 0; q < 8; ++q) v[q] += f[q];
+  *reinterpret_cast<u32x4*>(out + row * a.ldo + j) = pack8<T>(v);
+}
+
+// =============================================================================================
+// 256 x 256 tiles
+// =============================================================================================
+//
+// A workgroup of eight wavefronts, two per SIMD, computes 256 x 256 outputs; bound by the matrix cores.  The
+// schedule is that of the expert FFN's large tiles: a stage holds 64 of the contraction, each operand as two
+// halves of 128 indices (16 KiB); wavefront (wm, wn) = (w / 4, w % 4) computes in each quadrant (A half, B
+// half) the indices 32 i + 16 wm + [0, 16) of A (i < 4) by 32 wn + [0, 32) of B.
+//
+//   phase            1        2        3        4
+//   reads            A0(k)    B1(k)    A1(k)    B0(k+1)
+//   loads            B0(k+2)  A0(k+2)  B1(k+2)  A1(k+2)    (into the half read one phase before)
+//   multiplies       A0 B0    A0 B1    A1 B0    A1 B1
+//
+// Each phase is a memory and a matrix segment with a barrier after each; the wavefronts wm = 1 run one
+// segment behind, so that one of a SIMD's two multiplies while the other reads and loads.  A half is loaded
+// seven phases before it is read, two loads a wavefront and phase, so "at most 12 outstanding" says that the
+// half read next has landed.  The last two stages of a tile load the first two of the next.
+//
+// Loads are buffer loads straight to LDS: whatever lies behind an operand's last row or a group's end reads
+// as 0, so ragged sizes cost no test in the loop.  A contraction that is no multiple of 64 ends inside the
+// rows of an operand staged by index; there the lanes whose chunk lies behind it get an offset behind the
+// buffer before the last stage.
+//
+// The B indices belong to the products' first operand, so a lane holds four consecutive output columns of
+// one row.  Two tiles of 16 columns give 8 and one 16-byte store: of an operand staged by index, whose
+// fragments take any rows, the columns 8 g + 4 c + [0, 4) of tile c; of one staged by c, whose fragments take
+// 16 consecutive ones without bank conflicts, by an exchange between neighbouring rows of lanes at the end.
+constexpr int kHalf = 128 * 128;   // bytes
+__device__ __forceinline__ int swz_pair(int r) { return ((r >> 1) & 1) | (((r >> 3) & 3) << 1); }
+
+template <typename T, int MODE, bool GATHER, int ACT>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void tile256(Args a) {
+  constexpr bool XA = MODE == kDw, XB = MODE != kFwd, RAG = MODE != kDw;
+  constexpr bool GA = GATHER && MODE == kFwd, GB = GATHER && MODE == kDw;
+  __shared__ Table tt;
+  __shared__ __attribute__((aligned(1024))) char smem[8 * kHalf];
+  // GA: the rows of x of a tile's rows, two tiles in turn.  GB: those of 8 stages, each wavefront its own 8
+  // rows of a stage: sets 0 and 1 in turn, 2 and 3 for the first 8 stages of a tile.  Low and high words.
+  __shared__ __attribute__((aligned(256))) uint32_t row_s[GA ? 2 : (GB ? 4 : 1)][2][GA ? 256 : (GB ? 512 : 1)];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int ntj = (int)ceil_div(a.J, 256), nti = RAG ? 0 : (int)ceil_div(a.I, 256);
+  build_table<RAG>(a, tt, RAG ? 256 : nti);
+  if (RAG && a.zero_rest) zero_rest(a, tt);
+  const int mtiles = __builtin_amdgcn_readfirstlane(tt.total);
+  const int total = mtiles * ntj * a.splits;
+  const int wm = wave >> 2, wn = wave & 3;
+  const int j16 = lane & 15, g4 = lane >> 4;
+  const uint32_t smem0 = lds_at(smem);
+
+  // fragment reads.  Staged by index: one address for each K step, tiles at constant distances.  By c: one
+  // for each tile (the swizzle exchanges tiles), K steps and halves of a fragment at constant distances.
+  uint32_t a_addr[XA ? 4 : 2], b_addr[2];
+  if constexpr (XA) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a_addr[i] = smem0 + frag_across<128>(32 * i + 16 * wm, 0, 0);
+  } else {
+    const int r = 16 * wm + j16;
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) a_addr[ks] = smem0 + (uint32_t)(r * 128 + (((4 * ks + g4) ^ swz_direct(r)) << 4));
+  }
+  if constexpr (XB) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) b_addr[c] = smem0 + 4 * kHalf + frag_across<128>(32 * wn + 16 * c, 0, 0);
+  } else {
+    const int r = 32 * wn + 8 * (j16 >> 2) + (j16 & 3);
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+      b_addr[ks] = smem0 + 4 * kHalf + (uint32_t)(r * 128 + (((4 * ks + g4) ^ swz_pair(r)) << 4));
+  }
+
+  struct Tile {
+    u32x4 a, b;
+    int g, s, nc;          // group, part, length of the contraction
+    int64_t row0;          // output row of the tile's first
+    int rows, j0;          // rows from there on (may be more than 256), first column
+    const int64_t* idx;    // GA, GB: the row numbers from the tile's first row or c on
+  };
+  const uint32_t lda2 = (uint32_t)a.lda * 2, ldb2 = (uint32_t)a.ldb * 2;
+  const uint32_t a_step = XA ? 64 * lda2 : 128, b_step = XB ? (GB ? 0 : 64 * ldb2) : 128;
+
+  auto locate = [&](int item) {
+    Tile t;
+    t.s = item % a.splits;
+    const int q = item / a.splits;
+    int mt, jt;
+    // bands of four row tiles, all columns of a band before the next: what runs at one time on an XCD
+    // shares few rows of either operand
+    auto banded = [&](int k, int rows) {
+      const int band = k / (4 * ntj), r = k - band * 4 * ntj, h = rows - 4 * band < 4 ? rows - 4 * band : 4;
+      jt = r / h;
+      mt = 4 * band + r - jt * h;
+    };
+    int i0;
+    if constexpr (RAG) {
+      banded(q, mtiles);
+      t.g = a.starts ? find_group(tt, mt) : 0;
+      i0 = (mt - tt.cum[t.g]) * 256;
+    } else {
+      t.g = q / (nti * ntj);
+      banded(q - t.g * nti * ntj, nti);
+      i0 = mt * 256;
+    }
+    t.g = __builtin_amdgcn_readfirstlane(t.g);
+    const int64_t start = tt.start[t.g], n = tt.start[t.g + 1] - start;
+    t.rows = __builtin_amdgcn_readfirstlane((int)((RAG ? n : a.I) - i0));
+    t.j0 = __builtin_amdgcn_readfirstlane(jt * 256);
+    t.row0 = (RAG ? start : 0) + i0;
+    const int64_t C = RAG ? a.C : n, per = ceil_div(ceil_div(C, a.splits), 64) * 64;
+    const int64_t c0 = t.s * per, c1 = c0 + per < C ? c0 + per : C;
+    t.nc = __builtin_amdgcn_readfirstlane((int)(c1 > c0 ? c1 - c0 : 0));
+    const int64_t nc = t.nc, vi = t.rows < 256 ? t.rows : 256, vj = a.J - t.j0 < 256 ? a.J - t.j0 : 256;
+    auto size = [](int64_t rows, int64_t ld, int64_t last) { return rows > 0 && last > 0 ? ((rows - 1) * ld + last) * 2 : 0; };
+    if constexpr (XA)
+      t.a = buffer_at(a.a + (start + c0) * a.lda + i0, size(nc, a.lda, vi));
+    else if constexpr (GA)
+      t.a = buffer_at(a.a + c0, size(a.x_rows, a.lda, nc));
+    else
+      t.a = buffer_at(a.a + t.row0 * a.lda + c0, size(vi, a.lda, nc));
+    const uint16_t* const w = a.b + (MODE == kDw ? 0 : t.g * a.b_group);
+    if constexpr (!XB)
+      t.b = buffer_at(w + (int64_t)t.j0 * a.ldb + c0, size(vj, a.ldb, nc));
+    else if constexpr (GB)
+      t.b = buffer_at(w + t.j0, size(a.x_rows, a.ldb, vj));
+    else
+      t.b = buffer_at(w + ((MODE == kDw ? start : 0) + c0) * a.ldb + t.j0, size(nc, a.ldb, vj));
+    t.idx = GATHER ? a.rows + (GA ? t.row0 : start + c0) : nullptr;
+    return t;
+  };
+
+  // The load stream: the tile whose stages are being loaded.  Staged by index: a wavefront's rows 16 wave +
+  // 8 q + lane / 8 of a half, place lane % 8.  By c: its rows 8 wave + 4 q + lane / 16, place lane % 16.
+  u32x4 ra, rb;                  // buffers
+  uint32_t sa = 0, sb = 0;       // the stage's offset in them
+  uint32_t a_half, b_half;       // from half 0 to half 1
+  int left = 0;                  // of the contraction, from the stage on
+  const int64_t* idx = nullptr;  // GB: row numbers from the stage on
+  uint32_t avo[GA ? 2 : 1][2], bvo[2];
+  auto chunk_a = [&](int q) {
+    return XA ? (lane & 15) ^ swz_across<128>(8 * wave + 4 * q + (lane >> 4))
+              : (lane & 7) ^ swz_direct(16 * wave + 8 * q + (lane >> 3));
+  };
+  auto chunk_b = [&](int q) {
+    return XB ? (lane & 15) ^ swz_across<128>(8 * wave + 4 * q + (lane >> 4))
+              : (lane & 7) ^ swz_pair(16 * wave + 8 * q + (lane >> 3));
+  };
+  // GA: the row numbers of a tile's `n` rows into set p
+  auto tile_rows = [&](const int64_t* at, int n, int p) {
+    if (wave < 4) {
+      const u32x4 r = buffer_at(at, (int64_t)(n < 256 ? n : 256) * 8);
+      const uint32_t o = (uint32_t)(64 * wave + lane) * 8;
+      load_lds4(r, o, lds_at(row_s[p][0]) + 256 * wave);
+      load_lds4(r, o + 4, lds_at(row_s[p][1]) + 256 * wave);
+    }
+  };
+  // GB: those of 8 stages, `n` c from `at` on, into set p
+  auto stage8_rows = [&](const int64_t* at, int n, int p) {
+    const u32x4 r = buffer_at(at, (int64_t)n * 8);
+    const uint32_t o = (uint32_t)((lane >> 3) * 64 + 8 * wave + (lane & 7)) * 8;
+    load_lds4(r, o, lds_at(row_s[p][0]) + 256 * wave);
+    load_lds4(r, o + 4, lds_at(row_s[p][1]) + 256 * wave);
+  };
+  // the stream goes on with the tile t; GA: p its set of row numbers
+  auto begin_tile = [&](const Tile& t, int p) {
+    ra = t.a, rb = t.b, sa = sb = 0, left = t.nc, idx = t.idx;
+    // a half without rows or columns loads the other's: what it gives is not stored
+    a_half = XA ? 256 : (t.rows > 128 ? 128 * lda2 : 0);
+    b_half = XB ? 256 : (a.J - t.j0 > 128 ? 128 * ldb2 : 0);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const uint32_t ca = (uint32_t)chunk_a(q) * 16, cb = (uint32_t)chunk_b(q) * 16;
+      if constexpr (GA) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = 128 * h + 16 * wave + 8 * q + (lane >> 3);
+          const uint32_t x = row_s[p][0][r];
+          const bool ok = r < t.rows && row_s[p][1][r] == 0 && x < (uint64_t)a.x_rows;
+          avo[h][q] = ok ? x * lda2 + ca : kNowhere;
+        }
+      } else {
+        avo[0][q] = (uint32_t)(XA ? 8 * wave + 4 * q + (lane >> 4) : 16 * wave + 8 * q + (lane >> 3)) * lda2 + ca;
+      }
+      if constexpr (!GB) bvo[q] = (uint32_t)(XB ? 8 * wave + 4 * q + (lane >> 4) : 16 * wave + 8 * q + (lane >> 3)) * ldb2 + cb;
+    }
+  };
+  // before the stage k of the stream's tile is loaded; GB: p the tile's first set is 2 + p
+  auto begin_stage = [&](int k, int p) {
+    if (left <= 0) {   // not there: zeros
+      ra[2] = rb[2] = 0;
+      sa = sb = 0;
+    } else if (!(XA && XB) && left < 64) {   // chunks behind the contraction's end lie nowhere
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        if (!XA && chunk_a(q) * 8 >= left) {
+          avo[0][q] = kNowhere;
+          if constexpr (GA) avo[1][q] = kNowhere;
+        }
+        if (!XB && chunk_b(q) * 8 >= left) bvo[q] = kNowhere;
+      }
+    }
+    if constexpr (GB) {
+      if ((k & 7) == 0) {
+        if (left > 512) stage8_rows(idx + 512, left - 512, ((k >> 3) + 1) & 1);
+        idx += 512;
+      }
+      const int set = k < 8 ? 2 + p : (k >> 3) & 1;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int r = 4 * q + (lane >> 4), at = 64 * wave + 8 * (k & 7) + r;
+        const uint32_t x = row_s[set][0][at];
+        const bool ok = 8 * wave + r < left && row_s[set][1][at] == 0 && x < (uint64_t)a.x_rows;
+        bvo[q] = ok ? x * ldb2 + (uint32_t)chunk_b(q) * 16 : kNowhere;
+      }
+    }
+  };
+  auto end_stage = [&]() {
+    left -= 64;
+    sa += a_step;
+    sb += b_step;
+  };
+  auto load_a = [&](int h, int slot) {
+    const uint32_t dst = smem0 + (uint32_t)((2 * h + slot) * kHalf + 2048 * wave);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) load_lds(ra, avo[GA ? h : 0][q], GA || h == 0 ? sa : sa + (left > 0 ? a_half : 0), dst + 1024 * q);
+  };
+  auto load_b = [&](int h, int slot) {
+    const uint32_t dst = smem0 + (uint32_t)((4 + 2 * h + slot) * kHalf + 2048 * wave);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) load_lds(rb, bvo[q], h == 0 ? sb : sb + (left > 0 ? b_half : 0), dst + 1024 * q);
+  };
+
+  s16x8 ft[4][2], fw[2][2][2];
+  auto read_a = [&](auto hh, auto ss) {
+    constexpr int off = (2 * decltype(hh)::value + decltype(ss)::value) * kHalf;
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (XA)
+          ft[i][ks] = read_across(a_addr[i] + (off + ks * 8192), a_addr[i] + (off + ks * 8192 + 1024));
+        else
+          ft[i][ks] = read_direct(a_addr[ks] + (off + i * 32 * 128));
+      }
+  };
+  auto read_b = [&](auto hh, auto ss) {
+    constexpr int H = decltype(hh)::value, off = (2 * H + decltype(ss)::value) * kHalf;
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        if constexpr (XB)
+          fw[H][c][ks] = read_across(b_addr[c] + (off + ks * 8192), b_addr[c] + (off + ks * 8192 + 1024));
+        else
+          fw[H][c][ks] = read_direct(b_addr[ks] + (off + c * 4 * 128));
+      }
+  };
+
+  // XCD-aware order: workgroup b runs on XCD b % 8; in each round of gridDim tiles those of one XCD take a
+  // contiguous run
+  const int per_xcd = gridDim.x % 8 == 0 ? (int)gridDim.x / 8 : 0;
+  const int first = per_xcd ? (int)(blockIdx.x % 8) * per_xcd + (int)(blockIdx.x / 8) : (int)blockIdx.x;
+  if (first >= total) return;
+  typedef std::integral_constant<int, 0> I0;
+  typedef std::integral_constant<int, 1> I1;
+
+  int set = 0;   // GA: the set of the tile's row numbers; GB: its first set is 2 + set
+  {
+    const Tile t = locate(first);
+    if constexpr (GA) tile_rows(t.idx, t.rows, 0);
+    if constexpr (GB) stage8_rows(t.idx, t.nc, 2);
+    if (GATHER) {
+      wait_cnt<0>();
+      wg_barrier();
+    }
+    begin_tile(t, 0);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      begin_stage(k, 0);
+      load_b(0, k);
+      load_a(0, k);
+      load_b(1, k);
+      load_a(1, k);
+      end_stage();
+    }
+  }
+  wait_cnt<12>();   // B half 0 and A half 0 of stage 0 have landed
+  wg_barrier();
+  read_b(I0{}, I0{});
+  wait_cnt<12>();   // every wavefront has read B half 0 of stage 0 before stage 2's replaces it
+  wg_barrier();
+  if (wm == 1) wg_barrier();   // the second group runs one segment behind the first
+  for (int item = first; item < total; item += gridDim.x, set ^= 1) {
+    // the tile after this one; after the last its own first stages are loaded again
+    const int after = item + (int)gridDim.x < total ? item + (int)gridDim.x : item;
+    if constexpr (GATHER) {
+      const Tile t = locate(after);
+      if constexpr (GA) tile_rows(t.idx, t.rows, set ^ 1);
+      if constexpr (GB) stage8_rows(t.idx, t.nc, 2 + (set ^ 1));
+    }
+    int nf[2], pairs, rows;
+    {
+      const Tile t = locate(item);
+      rows = t.rows;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {   // 16-row tiles of each A half that hold rows
+        const int v = rows - 128 * h - 16 * wm;
+        nf[h] = __builtin_amdgcn_readfirstlane(v >= 128 ? 4 : (v > 0 ? (v + 31) / 32 : 0));
+      }
+      pairs = (t.nc + 127) / 128;   // pairs of stages: what is not there reads as 0
+    }
+    if (GB && pairs <= 1) wait_cnt<0>();   // the next tile's row numbers are needed at once
+
+    auto pipeline = [&](auto part) {
+      constexpr bool PARTIAL = decltype(part)::value;
+      f32x4 acc[2][2][4][2];   // [A half][B half][16-row tile][16-column tile]
+#pragma unroll
+      for (int ha = 0; ha < 2; ++ha)
+#pragma unroll
+        for (int hb = 0; hb < 2; ++hb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) acc[ha][hb][i][c] = f32x4{0, 0, 0, 0};
+      auto mma = [&](auto ha, auto hb) {
+        constexpr int A = decltype(ha)::value, B = decltype(hb)::value;
+        auto tile_row = [&](int i, int ks) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) acc[A][B][i][c] = T::mma(fw[B][c][ks], ft[i][ks], acc[A][B][i][c]);
+        };
+        __builtin_amdgcn_s_setprio(1);
+        if constexpr (!PARTIAL) {
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) tile_row(i, ks);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; i += 2)
+            if (i < nf[A]) {
+#pragma unroll
+              for (int ks = 0; ks < 2; ++ks) {
+                tile_row(i, ks);
+                tile_row(i + 1, ks);
+              }
+            }
+        }
+        __builtin_amdgcn_s_setprio(0);
+        wg_barrier();
+      };
+      auto mem_end = [&]() {   // the next segment's half has landed, this one's fragments are read
+        wait_cnt<12>();
+        wg_barrier();
+      };
+      // a stage in slot S, loading the stage k of the stream into it
+      auto stage = [&](int k, int p, auto ss) {
+        constexpr int S = decltype(ss)::value;
+        typedef std::integral_constant<int, S> IS;
+        typedef std::integral_constant<int, 1 - S> IO;
+        begin_stage(k, p);
+        read_a(I0{}, IS{});
+        load_b(0, S);
+        mem_end();
+        mma(I0{}, I0{});
+        read_b(I1{}, IS{});
+        load_a(0, S);
+        mem_end();
+        mma(I0{}, I1{});
+        read_a(I1{}, IS{});
+        load_b(1, S);
+        mem_end();
+        mma(I1{}, I0{});
+        read_b(I0{}, IO{});
+        load_a(1, S);
+        end_stage();
+        mem_end();
+        mma(I1{}, I1{});
+      };
+      for (int k = 1; k < pairs; ++k) {
+        stage(2 * k, set, I0{});
+        stage(2 * k + 1, set, I1{});
+      }
+      begin_tile(locate(after), set ^ 1);   // the last two stages load the next tile's first two
+      stage(0, set ^ 1, I0{});
+      stage(1, set ^ 1, I1{});
+
+      const Tile cur = locate(item);
+      int erow = 16 * wm + j16;
+      asm volatile("" : "+v"(erow));   // the stores' addresses are computed here, not kept through the loop
+      uint16_t* const out = a.out + (MODE == kDw ? cur.g * a.o_group : 0);
+#pragma unroll
+      for (int hb = 0; hb < 2; ++hb) {
+        const int64_t j = cur.j0 + 128 * hb + 32 * wn + (XB ? 16 * (g4 & 1) + 8 * (g4 >> 1) : 8 * g4);
+        const int rows_in = j < a.J ? cur.rows : 0;   // (all lanes take part in the exchange below)
+        u32x4 bias = {0, 0, 0, 0};
+        if (MODE == kFwd && a.bias && a.splits == 1 && rows_in)
+          bias = *reinterpret_cast<const u32x4*>(a.bias + cur.g * a.bias_group + j);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          u32x4 res[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = 128 * h + 32 * i + erow;
+            res[i] = u32x4{0, 0, 0, 0};
+            if (MODE == kFwd && !GATHER && a.residual && a.splits == 1 && r < rows_in)
+              res[i] = *reinterpret_cast<const u32x4*>(a.residual + (cur.row0 + r) * a.ldr + j);
+          }
+          __builtin_amdgcn_sched_barrier(0);   // one half's residual at a time: registers
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = 128 * h + 32 * i + erow;
+            float v[8];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              float lo = acc[h][hb][i][0][q], hi = acc[h][hb][i][1][q];
+              if constexpr (XB) {
+                const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(lo), __float_as_uint(hi), false, false);
+                lo = __uint_as_float(s[0]);
+                hi = __uint_as_float(s[1]);
+              }
+              v[q] = lo;
+              v[4 + q] = hi;
+            }
+            if (r < rows_in) {
+              const int64_t row = cur.row0 + r;
+              if (a.splits > 1) {
+                float* const o = a.part + (RAG ? cur.s * a.pairs + row : ((int64_t)cur.s * a.groups + cur.g) * a.I + row) * a.J + j;
+                *reinterpret_cast<f32x4*>(o) = f32x4{v[0], v[1], v[2], v[3]};
+                *reinterpret_cast<f32x4*>(o + 4) = f32x4{v[4], v[5], v[6], v[7]};
+              } else {
+                finish8<T, ACT>(a, out, row, j, v, bias, res[i]);
+              }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+      }
+    };
+    if (rows >= 256)
+      pipeline(std::false_type{});
+    else
+      pipeline(std::true_type{});
+  }
+  if (wm == 0) wg_barrier();
+  wait_cnt<0>();   // no load may write this workgroup's LDS after its end
+}
+
+template <typename T, int MODE, bool GATHER, int ACT>
+void go(const char* name, const Args& a, int64_t tiles, int64_t cus, hipStream_t s) {
+  launch(name, tile256<T, MODE, GATHER, ACT>, dim3((unsigned)std::min(tiles, cus)), dim3(512), 0, s, a);
+}
+
+template <typename T>
+void tile_typed(int mode, const char* name, const Args& a, int64_t tiles, int64_t cus, hipStream_t s) {
+  const bool gather = a.rows != nullptr;
+  if (mode == kDx) return go<T, kDx, false, kNone>(name, a, tiles, cus, s);
+  if (mode == kDw) return gather ? go<T, kDw, true, kNone>(name, a, tiles, cus, s) : go<T, kDw, false, kNone>(name, a, tiles, cus, s);
+  if (gather) return go<T, kFwd, true, kNone>(name, a, tiles, cus, s);
+  switch (a.splits > 1 ? kNone : a.act) {
+    case kRelu: return go<T, kFwd, false, kRelu>(name, a, tiles, cus, s);
+    case kSilu: return go<T, kFwd, false, kSilu>(name, a, tiles, cus, s);
+    case kGelu: return go<T, kFwd, false, kGelu>(name, a, tiles, cus, s);
+    case kGeluTanh: return go<T, kFwd, false, kGeluTanh>(name, a, tiles, cus, s);
+    default: return go<T, kFwd, false, kNone>(name, a, tiles, cus, s);
+  }
+}
+
+}  // namespace
+
+void tile_launch(int mode, int32_t dtype, const char* name, const Args& a, int64_t tiles, int64_t cus, hipStream_t s) {
+  dtype == FERRY_BF16 ? tile_typed<Bf16>(mode, name, a, tiles, cus, s) : tile_typed<F16>(mode, name, a, tiles, cus, s);
+}
+
+}  // namespace lin
+}  // namespace ferry

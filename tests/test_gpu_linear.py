@@ -274,6 +274,25 @@ def test_autograd_gives_what_is_asked():
     assert xr.grad.shape == x.shape and bool(xr.grad.isfinite().all())
 
 
+LARGE = [(2056, 2312, 264), (4104, 1032, 72), (1800, 4096, 8), (2304, 2048, 136), (257, 12296, 320), (2500, 2048, 1160)]
+
+
+@pytest.mark.parametrize('dtype', [BF16, F16])
+@pytest.mark.parametrize('m,n,k', LARGE)
+def test_large_tiles(m, n, k, dtype):
+    """Sizes of many tiles, most of them with partial tiles and a contraction that ends inside a stage."""
+    x, w = normal(m, k, dtype=dtype, seed=1), normal(n, k, dtype=dtype, seed=2, scale=k ** -0.5)
+    bias, res, dy = normal(n, dtype=dtype, seed=3), normal(m, n, dtype=dtype, seed=4), normal(m, n, dtype=dtype, seed=5)
+    act = ACTS[(m + n + k) // 8 % 5]
+    y, b, z, zb = layer(x, w, bias, act, res)
+    got, pre = ops().linear(x, w, bias, act, res, return_pre=True)
+    close(got, y, b, act)
+    want = layer_grad(dy, x, w, z, zb, act)
+    for name, v in zip(('dx', 'dw', 'db'), ops().linear_grad(dy, x, w, pre, act)):
+        close(v, *want[name], name)
+    close(ops().linear(x, w), *layer(x, w)[:2], 'plain')
+
+
 # -- experts ------------------------------------------------------------------------------------------
 
 def groups_of(counts, head=0):
@@ -303,7 +322,8 @@ def expert_reference(x, w, starts, bias=None, rows=None, dy=None):
     return out
 
 
-COUNTS = [([1], 8, 8), ([0, 3, 0], 24, 40), ([0, 1, 63, 64, 65, 0, 200, 3], 72, 136), ([5] * 33, 64, 64),
+COUNTS = [([300, 0, 1, 700, 256, 255, 257, 0, 600, 31], 1032, 264), ([0, 900, 513, 0, 64, 2, 1100], 2048, 1032),
+          ([1], 8, 8), ([0, 3, 0], 24, 40), ([0, 1, 63, 64, 65, 0, 200, 3], 72, 136), ([5] * 33, 64, 64),
           ([300, 0, 7], 35, 37), ([0] * 60 + [2] + [0] * 67, 256, 512), ([1, 0, 2] * 100, 40, 72),
           ([129, 127, 255, 257, 1, 16, 17, 33], 264, 200), ([1000, 30, 500, 2], 520, 96), ([0, 0], 16, 16),
           ([64] * 8, 1032, 1032), ([3] * 512, 16, 24)]

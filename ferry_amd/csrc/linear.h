@@ -141,59 +141,61 @@ __device__ __forceinline__ float slope(int act, float z) {
 
 // -- groups ----------------------------------------------------------------------------------------
 
+// The rows of group g are [start, start + n), forced into [0, pairs], so that whatever starts holds every
+// access stays inside the tensors; a group that ends before it starts has none.
+__device__ __forceinline__ int group_start(const Args& a, int g) {
+  const int64_t s = a.starts[g];
+  return (int)(s < 0 ? 0 : (s > a.pairs ? a.pairs : s));
+}
+
 struct Table {
-  __attribute__((aligned(16))) int32_t cum[kMaxGroups + 8];   // tiles before the group, 0x7fffffff behind the last
-  int64_t start[kMaxGroups + 1];
-  int32_t total;
+  __attribute__((aligned(16))) int32_t cum[kMaxGroups];   // tiles before the group, 0x7fffffff behind the last
+  int32_t start[kMaxGroups], rows[kMaxGroups];
+  int32_t total, first, last;   // tiles; rows of the grouped order before the first and behind the last group
 };
 
-// start[g] = starts[g], forced into [0, pairs] and to ascend, so that whatever starts holds every access
-// stays inside the tensors; cum: with RAGGED_I the tiles of `rows` rows of the groups before, else `rows`
-// tiles for each group.  By wavefront 0; all others wait.
+// The groups' starts, rows and tiles: `rows` rows a tile with RAGGED_I, else `rows` tiles for each group.  By
+// wavefront 0, all loads at once; all others wait.
 template <bool RAGGED_I>
 __device__ __forceinline__ void build_table(const Args& a, Table& t, int rows) {
+  constexpr int Q = kMaxGroups / 64;
   if (threadIdx.x < 64) {
-    const int lane = threadIdx.x;
-    if (!a.starts) {
-      if (lane == 0) {
-        t.start[0] = 0;
-        t.start[1] = a.pairs;
-        t.cum[0] = 0;
-        t.total = RAGGED_I ? (int32_t)((a.pairs + rows - 1) / rows) : rows;
-      }
-      for (int i = 1 + lane; i < kMaxGroups + 8; i += 64) t.cum[i] = 0x7fffffff;
-    } else {
-      const int G = a.groups;
-      int64_t before = 0;
-      int sum = 0;
-      for (int g0 = 0; g0 <= G; g0 += 64) {
-        const int g = g0 + lane;
-        int64_t s = g <= G ? a.starts[g] : 0;
-        s = s < 0 ? 0 : (s > a.pairs ? a.pairs : s);
-        s = s < before ? before : s;
+    const int lane = threadIdx.x, G = a.groups;
+    int s[Q], n[Q];
 #pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-          const int64_t v = __shfl_up(s, off, 64);
-          if (lane >= off && v > s) s = v;
-        }
-        if (g <= G) t.start[g] = s;
-        before = __shfl(s, 63, 64);
+    for (int q = 0; q < Q; ++q) {
+      const int g = q * 64 + lane;
+      s[q] = n[q] = 0;
+      if (q * 64 < G && g < G) {
+        s[q] = a.starts ? group_start(a, g) : 0;
+        n[q] = a.starts ? group_start(a, g + 1) : (int)a.pairs;
       }
-      __threadfence_block();
-      for (int g0 = 0; g0 < kMaxGroups + 8; g0 += 64) {
-        const int g = g0 + lane;
-        int n = 0;
-        if (g < G) n = RAGGED_I ? (int)((t.start[g + 1] - t.start[g] + rows - 1) / rows) : rows;
-        int incl = n;
+    }
+    int sum = 0;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      const int g = q * 64 + lane;
+      if (q * 64 < G) {
+        n[q] = n[q] > s[q] ? n[q] - s[q] : 0;
+        const int c = g < G ? (RAGGED_I ? (int)(((uint32_t)n[q] + rows - 1) / (uint32_t)rows) : rows) : 0;
+        int incl = c;
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) {
           const int v = __shfl_up(incl, off, 64);
           if (lane >= off) incl += v;
         }
-        if (g < kMaxGroups + 8) t.cum[g] = g < G ? sum + incl - n : 0x7fffffff;
+        t.cum[g] = g < G ? sum + incl - c : 0x7fffffff;
+        t.start[g] = s[q];
+        t.rows[g] = n[q];
         sum += __shfl(incl, 63, 64);
+      } else {
+        t.cum[g] = 0x7fffffff;
       }
-      if (lane == 0) t.total = sum;
+    }
+    if (lane == 0) {
+      t.total = sum;
+      t.first = a.starts ? group_start(a, 0) : 0;
+      t.last = a.starts ? group_start(a, G) : (int)a.pairs;
     }
   }
   __syncthreads();
@@ -294,9 +296,8 @@ __device__ __forceinline__ void finish4(const Args& a, int g, int64_t row, int64
   }
 }
 
-// rows of the output that belong to no group, by all workgroups of a launch
-__device__ __forceinline__ void zero_rest(const Args& a, const Table& t) {
-  const int64_t first = t.start[0], last = t.start[a.starts ? a.groups : 1];
+// rows of the output before the first and behind the last group, by all workgroups of a launch
+__device__ __forceinline__ void zero_rest(const Args& a, int first, int last) {
   const int64_t n = first + (a.pairs - last);
   for (int64_t r = blockIdx.x; r < n; r += gridDim.x) {
     uint16_t* const o = a.out + (r < first ? r : last + (r - first)) * a.ldo;

@@ -42,7 +42,7 @@ __global__ __launch_bounds__(256) void any_kernel(Args a) {
   const int ntj = (int)ceil_div(a.J, TJ);
   const int nti = kRaggedI ? 0 : (int)ceil_div(a.I, TI);
   build_table<kRaggedI>(a, tt, kRaggedI ? TI : nti);
-  if (a.zero_rest) zero_rest(a, tt);
+  if (a.zero_rest) zero_rest(a, tt.first, tt.last);
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wi = (wave >> 1) * (TI / 2), wj = (wave & 1) * (TJ / 2);
@@ -53,7 +53,7 @@ __global__ __launch_bounds__(256) void any_kernel(Args a) {
     const int64_t t = item / a.splits;
     const int jt = (int)(t % ntj), mt = (int)(t / ntj);
     const int g = a.starts ? find_group(tt, mt) : 0;
-    const int64_t start = tt.start[g], n = tt.start[g + 1] - start;
+    const int64_t start = tt.start[g], n = tt.rows[g];
     const int64_t i0 = (int64_t)(mt - tt.cum[g]) * TI, j0 = (int64_t)jt * TJ;
     const int64_t I = kRaggedI ? n : a.I, C = kRaggedI ? a.C : n;
     const int64_t per = ceil_div(ceil_div(C, a.splits), 64) * 64;
@@ -203,19 +203,10 @@ __global__ __launch_bounds__(256) void join_kernel(Args a) {
     const int m = (int)(a.J - j < 4 ? a.J - j : 4);
     int g = MODE == kDw ? (int)(row / a.I) : 0;
     bool in = true;
-    if (MODE != kDw && a.starts) {   // the last group that starts at or before the row
-      int64_t reach = a.starts[0] < 0 ? 0 : a.starts[0];
-      in = row >= reach;
-      g = -1;
-      for (int k = 0; k < a.groups && in; ++k) {
-        const int64_t e = a.starts[k + 1] > reach ? a.starts[k + 1] : reach;
-        if (row < e) {
-          g = k;
-          break;
-        }
-        reach = e;
-      }
-      in = g >= 0;
+    if (MODE != kDw && a.starts) {
+      in = false;
+      for (int k = 0; k < a.groups && !in; ++k)
+        if (row >= group_start(a, k) && row < group_start(a, k + 1)) g = k, in = true;
     }
     Args d = a;
     if (MODE == kDw) d.out = a.out + g * a.o_group;
@@ -254,21 +245,6 @@ struct SlopeArgs {
   int32_t groups, splits, act, zero_rest, vec;
 };
 
-// rows [lo, hi) of group g, as build_table has them; by every wavefront
-__device__ __forceinline__ void group_rows(const int64_t* __restrict__ starts, int g, int64_t pairs, int64_t& lo,
-                                           int64_t& hi) {
-  int64_t v = 0;
-  for (int k = threadIdx.x & 63; k <= g; k += 64) v = starts[k] > v ? starts[k] : v;
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    const int64_t o = __shfl_xor(v, off, 64);
-    v = o > v ? o : v;
-  }
-  const int64_t e = starts[g + 1];
-  lo = v > pairs ? pairs : v;
-  hi = e > lo ? (e > pairs ? pairs : e) : lo;
-}
-
 // dz = dy f'(pre) rounded, and db = the sum of the unrounded dz over each group's rows.  A workgroup
 // takes 256 columns (8 a thread) of one part of a group's rows, 8 rows at a time.  Bound by memory: dy
 // and pre in, dz out.
@@ -281,7 +257,12 @@ __global__ __launch_bounds__(256) void slope_kernel(SlopeArgs a) {
     const int64_t j = (it % jb) * 256 + cl;
     const int g = (int)(it / jb % a.groups), s = (int)(it / jb / a.groups);
     int64_t lo = 0, hi = a.pairs;
-    if (a.starts) group_rows(a.starts, g, a.pairs, lo, hi);
+    if (a.starts) {
+      lo = a.starts[g];
+      hi = a.starts[g + 1];
+      lo = lo < 0 ? 0 : (lo > a.pairs ? a.pairs : lo);
+      hi = hi < lo ? lo : (hi > a.pairs ? a.pairs : hi);
+    }
     const int64_t per = ceil_div(hi - lo, a.splits);
     const int64_t r0 = lo + s * per, r1 = r0 + per < hi ? r0 + per : hi;
     const int m = (int)(a.N - j < 8 ? a.N - j : 8);
@@ -395,29 +376,55 @@ int64_t splits_of(int64_t tiles, int64_t c) {
   return std::max<int64_t>(1, std::min<int64_t>({want, most, 32}));
 }
 
+enum Kind { kAny = 0, kTiles = 1, kFew = 2 };
 struct Plan {
-  int tile;       // rows and columns of a tile; 256: tile256
-  int64_t tiles;  // upper bound
+  Kind kind;
+  int mt, nb;     // kFew: rows and columns of a tile in 16s
+  int any;        // rows and columns of any_kernel's tile
+  int64_t tiles;  // upper bound (kFew: of row tiles, with one of splits)
   int64_t splits;
 };
 
 // op: the product; rows: pairs
 Plan plan(int op, int64_t pairs, int64_t n, int64_t k, int64_t groups) {
-  Plan p;
-  const int64_t J = op == kFwd ? n : k;
-  auto tiles = [&](int64_t t) {
-    return (op == kDw ? groups * ceil_div(n, t) : ceil_div(pairs, t) + (groups > 1 ? groups : 0)) * ceil_div(J, t);
-  };
-  p.tile = n % 8 == 0 && k % 8 == 0 && tiles(256) >= 48 ? 256 : (tiles(128) >= 512 ? 128 : 64);
-  p.tiles = tiles(p.tile);
+  Plan p = {};
+  const int64_t J = op == kFwd ? n : k, used = std::min(groups, std::max<int64_t>(pairs, 1));
+  auto row_tiles = [&](int64_t t) { return ceil_div(pairs, t) + (groups > 1 ? used : 0); };
+  auto tiles = [&](int64_t t) { return (op == kDw ? groups * ceil_div(n, t) : row_tiles(t)) * ceil_div(J, t); };
+  p.any = tiles(128) >= 512 ? 128 : 64;
+  p.splits = 1;
+  const int64_t rows = pairs / used;   // of a group, on average
+  if (op == kFwd && k % 8 == 0 && rows <= 64) {
+    p.kind = kFew;
+    p.mt = rows <= 16 ? 1 : (rows <= 32 ? 2 : 4);
+    p.tiles = row_tiles(16 * p.mt);
+    const int64_t blocks = used * ceil_div(n, 16);
+    p.nb = p.mt == 1 ? (blocks > 2048 ? 2 : 1) : (p.mt == 2 || blocks < 1024 ? 2 : 4);
+    return p;
+  }
+  if (n % 8 == 0 && k % 8 == 0 && tiles(256) >= 48) {
+    p.kind = kTiles;
+    p.tiles = tiles(256);
+  } else {
+    p.tiles = tiles(p.any);
+  }
   p.splits = splits_of(p.tiles, op == kFwd ? k : (op == kDx ? n : pairs / std::max<int64_t>(groups, 1)));
   return p;
+}
+
+bool even(const void* q, int64_t stride) { return (uintptr_t)q % 16 == 0 && stride % 8 == 0; }
+
+// Whether few_kernel can read the operands: rows at multiples of 16 bytes, offsets that 32 bits hold.
+bool few_fits(const Args& a, int64_t k) {
+  const int64_t most = ((int64_t)1 << 31) - (1 << 20);
+  return k % 8 == 0 && even(a.a, a.lda) && even(a.b, a.ldb) && a.b_group % 8 == 0 && a.ldb <= most / 128 && a.lda <= most / 128 &&
+         k <= most / 4 && (!a.rows || (a.x_rows >= 1 && a.x_rows * a.lda <= most));
 }
 
 // Whether the tiled kernels can read and write the operands: rows at multiples of 16 bytes, offsets that 32
 // bits hold (a tile's, or all of an operand whose rows are gathered or follow the contraction).
 bool tiles_fit(int op, const Args& a, int64_t pairs, int64_t n, int64_t k) {
-  auto even = [](const void* q, int64_t stride) { return (uintptr_t)q % 16 == 0 && stride % 8 == 0; };
+  if (a.rows && a.x_rows < 1) return false;
   if (n % 8 || k % 8 || !even(a.a, a.lda) || !even(a.b, a.ldb) || a.b_group % 8 || !even(a.out, a.ldo) || a.o_group % 8 ||
       (a.bias && !even(a.bias, a.bias_group)) || (a.residual && !even(a.residual, a.ldr)) || (a.pre && !even(a.pre, 0)))
     return false;
@@ -442,12 +449,13 @@ int64_t slope_splits(int64_t pairs, int64_t n, int64_t groups) {
 template <typename T, int MODE>
 int run_typed(const Args& a, const Plan& p, int64_t n, int64_t k, hipStream_t s) {
   static const char* const names[] = {"linear_fwd", "linear_dx", "linear_dw"};
-  const int64_t items = p.tiles * p.splits;
-  if (p.tile == 256 && tiles_fit(MODE, a, a.pairs, n, k)) {
-    tile_launch(MODE, T::kType, names[MODE], a, items, cus(), s);
+  if (p.kind == kFew && few_fits(a, k)) {
+    few_launch(T::kType, p.mt, p.nb, a, p.tiles, cus(), s);
+  } else if (p.kind == kTiles && tiles_fit(MODE, a, a.pairs, n, k)) {
+    tile_launch(MODE, T::kType, names[MODE], a, p.tiles * p.splits, cus(), s);
   } else {
-    const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>(items, cus() * 4)));
-    if (p.tile >= 128)
+    const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>(p.tiles * p.splits * (p.kind == kFew ? 8 : 4), cus() * 4)));
+    if (p.any == 128)
       launch(names[MODE], any_kernel<T, MODE, 128, 128>, grid, dim3(256), 0, s, a);
     else
       launch(names[MODE], any_kernel<T, MODE, 64, 64>, grid, dim3(256), 0, s, a);

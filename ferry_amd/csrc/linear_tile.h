@@ -1,4 +1,4 @@
-// Launches of the linear products' tiled kernels (linear_tile.hip).
+// Launches of the linear products' kernels for aligned operands (linear_tile.hip, linear_few.hip).
 #pragma once
 
 #include "linear.h"
@@ -8,6 +8,9 @@ namespace lin {
 
 // 256 x 256 tiles, `tiles` of them at most, on `cus` CUs
 void tile_launch(int mode, int32_t dtype, const char* name, const Args& a, int64_t tiles, int64_t cus, hipStream_t s);
+
+// kFwd of few rows: tiles of 16 mt rows, at most `tiles` of them, by 16 nb columns
+void few_launch(int32_t dtype, int mt, int nb, const Args& a, int64_t tiles, int64_t cus, hipStream_t s);
 
 }  // namespace lin
 }  // namespace ferry

@@ -1,5 +1,5 @@
 // The linear products on whole tiles: rows at multiples of 16 bytes, sizes of multiples of 8.
-#include "linear.h"
+#include "linear_loads.h"
 #include "linear_tile.h"
 
 #include <algorithm>
@@ -8,57 +8,6 @@
 namespace ferry {
 namespace lin {
 namespace {
-
-// -- loads to LDS, waits ---------------------------------------------------------------------------------
-
-// A part of memory as a buffer: reads behind its end give 0, also into LDS.
-__device__ __forceinline__ u32x4 buffer_at(const void* p, int64_t bytes) {
-  const uint64_t v = (uint64_t)(uintptr_t)p;
-  const int64_t n = bytes < 0 ? 0 : (bytes > 0xffffffffll ? 0xffffffffll : bytes);
-  return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v),
-               (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32)) & 0xffffu,
-               (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)n), 0x00020000u};
-}
-constexpr uint32_t kNowhere = 0xfffffff0u;   // an offset behind the end of every buffer
-
-// 16 bytes of each lane from offset soff + voff of the buffer to LDS address lds + 16 * lane; 0 from behind the
-// buffer's end (soff itself must lie in it, or be 0: the hardware compares voff with size - soff).  Inline asm,
-// so that no wait is added: their completion is awaited with wait_cnt.  m0 holds the LDS base; one wait state
-// between its write and the load.
-__device__ __forceinline__ void load_lds(u32x4 r, uint32_t voff, uint32_t soff, uint32_t lds) {
-  asm volatile(
-      "s_mov_b32 m0, %2\n\t"
-      "s_nop 0\n\t"
-      "buffer_load_dwordx4 %0, %1, %3 offen lds"
-      :
-      : "v"(voff), "s"(r), "s"(__builtin_amdgcn_readfirstlane((int)lds)), "s"(__builtin_amdgcn_readfirstlane((int)soff))
-      : "memory");
-}
-// 4 bytes of each lane, as above
-__device__ __forceinline__ void load_lds4(u32x4 r, uint32_t voff, uint32_t lds) {
-  asm volatile(
-      "s_mov_b32 m0, %2\n\t"
-      "s_nop 0\n\t"
-      "buffer_load_dword %0, %1, 0 offen lds"
-      :
-      : "v"(voff), "s"(r), "s"(lds)
-      : "memory");
-}
-template <int VM>
-__device__ __forceinline__ void wait_cnt() {   // at most VM loads and no LDS reads outstanding
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt((VM & 15) | (7 << 4) | ((VM >> 4) << 14));
-  asm volatile("" ::: "memory");
-}
-// barrier of a workgroup without the fence of __syncthreads, which would drain the loads
-__device__ __forceinline__ void wg_barrier() {
-  __builtin_amdgcn_sched_barrier(0);
-  asm volatile("s_barrier" ::: "memory");
-  __builtin_amdgcn_sched_barrier(0);
-}
-__device__ __forceinline__ uint32_t lds_at(const void* p) {
-  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
-}
 
 // -- epilogue ------------------------------------------------------------------------------------------
 
@@ -137,7 +86,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int ntj = (int)ceil_div(a.J, 256), nti = RAG ? 0 : (int)ceil_div(a.I, 256);
   build_table<RAG>(a, tt, RAG ? 256 : nti);
-  if (RAG && a.zero_rest) zero_rest(a, tt);
+  if (RAG && a.zero_rest) zero_rest(a, tt.first, tt.last);
   const int mtiles = __builtin_amdgcn_readfirstlane(tt.total);
   const int total = mtiles * ntj * a.splits;
   const int wm = wave >> 2, wn = wave & 3;
@@ -198,7 +147,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       i0 = mt * 256;
     }
     t.g = __builtin_amdgcn_readfirstlane(t.g);
-    const int64_t start = tt.start[t.g], n = tt.start[t.g + 1] - start;
+    const int64_t start = tt.start[t.g], n = tt.rows[t.g];
     t.rows = __builtin_amdgcn_readfirstlane((int)((RAG ? n : a.I) - i0));
     t.j0 = __builtin_amdgcn_readfirstlane(jt * 256);
     t.row0 = (RAG ? start : 0) + i0;

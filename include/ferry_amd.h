@@ -307,8 +307,9 @@ int ferry_gate_logits(const void* x, int64_t tokens, int64_t hidden, const void*
  * once.  Results do not depend on the order in which workgroups run.
  *
  * Groups: row p of the grouped order belongs to group g with starts[g] <= p < starts[g + 1] (device memory,
- * int64 [groups + 1], as ferry_layout writes it; null: one group of all `pairs` rows).  Values that do not
- * ascend within [0, pairs] are read as if they did.  rows (device memory, nullable) names the row of x of
+ * int64 [groups + 1], as ferry_layout writes it; null: one group of all `pairs` rows).  Starts must ascend within
+ * [0, pairs]: others are forced into that range, so that nothing outside the matrices is touched, and a group
+ * that ends before it starts has no rows.  rows (device memory, nullable) names the row of x of
  * each p; an index outside [0, x_rows) reads as a row of zeros.  Output rows p of no group are set to 0 with
  * zero_rest and stay as they were without.
  *

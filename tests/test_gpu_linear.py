@@ -274,6 +274,22 @@ def test_autograd_gives_what_is_asked():
     assert xr.grad.shape == x.shape and bool(xr.grad.isfinite().all())
 
 
+FEW = [(m, n, k) for m in (1, 7, 16, 17, 32, 33, 50, 64) for n, k in ((8, 8), (37, 264), (1000, 1032), (2064, 520), (40, 4160))]
+
+
+@pytest.mark.parametrize('m,n,k', FEW)
+def test_few_rows(m, n, k):
+    dtype = F16 if (m + n) % 3 else BF16
+    x, w = normal(m, k, dtype=dtype, seed=1), normal(n, k, dtype=dtype, seed=2, scale=k ** -0.5)
+    bias, res = normal(n, dtype=dtype, seed=3), normal(m, n, dtype=dtype, seed=4)
+    act = ACTS[(m + n + k) % 5]
+    y, b, z, zb = layer(x, w, bias, act, res)
+    got, pre = ops().linear(x, w, bias, act, res, return_pre=True)
+    close(got, y, b, act)
+    if act:
+        close(pre, z, zb + rounding(z, dtype), 'pre')
+
+
 LARGE = [(2056, 2312, 264), (4104, 1032, 72), (1800, 4096, 8), (2304, 2048, 136), (257, 12296, 320), (2500, 2048, 1160)]
 
 
@@ -322,7 +338,9 @@ def expert_reference(x, w, starts, bias=None, rows=None, dy=None):
     return out
 
 
-COUNTS = [([300, 0, 1, 700, 256, 255, 257, 0, 600, 31], 1032, 264), ([0, 900, 513, 0, 64, 2, 1100], 2048, 1032),
+COUNTS = [([1] * 40 + [0] * 30 + [9] * 20 + [200], 520, 1032), ([20, 30, 0, 33, 16, 17] * 5, 2064, 264),
+          ([64, 50, 0, 10] * 9, 1000, 520), ([1], 2000, 2048), ([2, 0, 1], 4104, 72),
+          ([300, 0, 1, 700, 256, 255, 257, 0, 600, 31], 1032, 264), ([0, 900, 513, 0, 64, 2, 1100], 2048, 1032),
           ([1], 8, 8), ([0, 3, 0], 24, 40), ([0, 1, 63, 64, 65, 0, 200, 3], 72, 136), ([5] * 33, 64, 64),
           ([300, 0, 7], 35, 37), ([0] * 60 + [2] + [0] * 67, 256, 512), ([1, 0, 2] * 100, 40, 72),
           ([129, 127, 255, 257, 1, 16, 17, 33], 264, 200), ([1000, 30, 500, 2], 520, 96), ([0, 0], 16, 16),
@@ -403,14 +421,17 @@ def test_weights_in_cache_rows():
 
 
 def test_starts_and_rows_out_of_range():
-    """Starts that do not ascend within the pairs read as if they did, rows of x that are not there as zeros."""
+    """Starts outside the pairs are forced into them, a group that ends before it starts has no rows, and rows of x
+    that are not there read as zeros."""
     x, w = normal(50, 64, seed=1), normal(4, 32, 64, seed=2)
-    wild = torch.tensor([-5, 10, 3, 1 << 40, 20], dtype=torch.int64, device='cuda')
+    wild = torch.tensor([-5, 10, 10, 1 << 40, 1 << 33], dtype=torch.int64, device='cuda')
     tame = torch.tensor([0, 10, 10, 50, 50], dtype=torch.int64, device='cuda')
     assert torch.equal(ops().expert_linear(x, w, wild), ops().expert_linear(x, w, tame))
     dy = normal(50, 32, seed=3)
     for a, b in zip(ops().expert_linear_grad(dy, x, w, wild), ops().expert_linear_grad(dy, x, w, tame)):
         assert torch.equal(a, b)
+    back = torch.tensor([0, 10, 3, 10, 50], dtype=torch.int64, device='cuda')   # group 1 ends before it starts
+    assert bool(ops().expert_linear_grad(dy, x, w, back)[1][1].eq(0).all())
     rows = torch.arange(50, device='cuda')
     rows[[4, 30]] = torch.tensor([-1, 50], device='cuda')
     zeroed = x.clone()

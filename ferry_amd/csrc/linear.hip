@@ -5,6 +5,7 @@
 #include "linear_tile.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace ferry {
 namespace lin {
@@ -370,7 +371,7 @@ int64_t cus() {   // of the current device
   return known[dev];
 }
 
-// Parts of the contraction: as many as give every CU a tile, of at least 256 each.
+// Parts of the contraction for any_kernel: as many as give every CU a tile, of at least 256 each.
 int64_t splits_of(int64_t tiles, int64_t c) {
   const int64_t want = tiles > 0 ? 256 / tiles : 1, most = c / 256;
   return std::max<int64_t>(1, std::min<int64_t>({want, most, 32}));
@@ -379,19 +380,28 @@ int64_t splits_of(int64_t tiles, int64_t c) {
 enum Kind { kAny = 0, kTiles = 1, kFew = 2 };
 struct Plan {
   Kind kind;
+  int shape;      // kTiles: 0 256 x 256, 1 .. 4 of ring_launch
   int mt, nb;     // kFew: rows and columns of a tile in 16s
   int any;        // rows and columns of any_kernel's tile
   int64_t tiles;  // upper bound (kFew: of row tiles, with one of splits)
   int64_t splits;
 };
 
+// The tiles' sizes (indices of A and of B), and their time in us: for a stage of 64 of the contraction, and for
+// what a tile costs besides.
+struct TileCost {
+  int tm, tn;
+  double stage, fixed;
+};
+const TileCost kShapes[] = {{256, 256, 1.31, 5.0}, {256, 128, 0.8, 4.0}, {128, 128, 0.52, 3.0}, {64, 128, 0.38, 2.5}, {64, 64, 0.30, 2.0}};
+
 // op: the product; rows: pairs
 Plan plan(int op, int64_t pairs, int64_t n, int64_t k, int64_t groups) {
   Plan p = {};
   const int64_t J = op == kFwd ? n : k, used = std::min(groups, std::max<int64_t>(pairs, 1));
   auto row_tiles = [&](int64_t t) { return ceil_div(pairs, t) + (groups > 1 ? used : 0); };
-  auto tiles = [&](int64_t t) { return (op == kDw ? groups * ceil_div(n, t) : row_tiles(t)) * ceil_div(J, t); };
-  p.any = tiles(128) >= 512 ? 128 : 64;
+  auto tiles = [&](int64_t tm, int64_t tn) { return (op == kDw ? groups * ceil_div(n, tm) : row_tiles(tm)) * ceil_div(J, tn); };
+  p.any = tiles(128, 128) >= 512 ? 128 : 64;
   p.splits = 1;
   const int64_t rows = pairs / used;   // of a group, on average
   if (op == kFwd && k % 8 == 0 && rows <= 64) {
@@ -402,13 +412,36 @@ Plan plan(int op, int64_t pairs, int64_t n, int64_t k, int64_t groups) {
     p.nb = p.mt == 1 ? (blocks > 2048 ? 2 : 1) : (p.mt == 2 || blocks < 1024 ? 2 : 4);
     return p;
   }
-  if (n % 8 == 0 && k % 8 == 0 && tiles(256) >= 48) {
-    p.kind = kTiles;
-    p.tiles = tiles(256);
-  } else {
-    p.tiles = tiles(p.any);
+  const double c = op == kFwd ? (double)k : (op == kDx ? (double)n : (double)pairs / (double)groups);
+  if (n % 8 || k % 8) {
+    p.tiles = tiles(p.any, p.any);
+    p.splits = splits_of(p.tiles, (int64_t)c);
+    return p;
   }
-  p.splits = splits_of(p.tiles, op == kFwd ? k : (op == kDx ? n : pairs / std::max<int64_t>(groups, 1)));
+  p.kind = kTiles;
+  // The cheapest shape and number of parts: whole rounds of tiles over the CUs, no faster than the operands come
+  // from memory, and the parts' way through memory.
+  const int64_t cu = cus();
+  const double out = (double)(op == kDw ? groups * n * k : pairs * J);
+  const double bytes = 2.0 * (op == kDw ? (double)pairs * (n + k) + out : (double)pairs * (n + k) + (double)used * n * k);
+  double least = 0;
+  for (int i = 0; i < 5; ++i) {
+    const TileCost& t = kShapes[i];
+    const double mt = op == kDw ? (double)(groups * ceil_div(n, t.tm)) : (groups > 1 ? (double)pairs / t.tm + 0.5 * used : (double)ceil_div(pairs, t.tm));
+    for (int64_t parts = 1; parts <= 16; parts *= 2) {
+      if (parts > 1 && c / parts < 256) break;
+      const double items = mt * ceil_div(J, t.tn) * parts, rounds = std::ceil(items / cu);
+      double cost = rounds * (std::ceil(c / 64 / parts) * t.stage + t.fixed);
+      cost = std::max(cost, bytes / 4.5e6 + 1.0);
+      if (parts > 1) cost += 4.0 + out * (8.0 * parts + 2.0) / 4.5e6;
+      if ((i == 0 && parts == 1) || cost < least) {
+        least = cost;
+        p.shape = i;
+        p.splits = parts;
+      }
+    }
+  }
+  p.tiles = tiles(kShapes[p.shape].tm, kShapes[p.shape].tn);
   return p;
 }
 
@@ -431,8 +464,7 @@ bool tiles_fit(int op, const Args& a, int64_t pairs, int64_t n, int64_t k) {
   const int64_t most = ((int64_t)1 << 31) - (1 << 20);   // elements, with room for a stage behind the end
   const int64_t ia = op == kDw ? pairs : (a.rows ? a.x_rows : 512), ib = op == kFwd ? 512 : (op == kDx ? n : (a.rows ? a.x_rows : pairs));
   if (a.lda > most / 512 || a.ldb > most / 512 || ia * a.lda > most || ib * a.ldb > most || a.C > most / 4) return false;
-  // the row numbers of a tile are loaded one tile ahead, which takes a contraction of more than two stages
-  return !(op == kFwd && a.rows) || ceil_div(ceil_div(k, a.splits), 64) * 64 > 128;
+  return true;
 }
 
 int64_t part_bytes(int op, const Plan& p, int64_t pairs, int64_t n, int64_t k, int64_t groups) {
@@ -449,10 +481,15 @@ int64_t slope_splits(int64_t pairs, int64_t n, int64_t groups) {
 template <typename T, int MODE>
 int run_typed(const Args& a, const Plan& p, int64_t n, int64_t k, hipStream_t s) {
   static const char* const names[] = {"linear_fwd", "linear_dx", "linear_dw"};
+  // (tile256 loads the row numbers of a tile one tile ahead, which takes a contraction of more than two stages)
+  const int shape = p.shape == 0 && MODE == kFwd && a.rows && ceil_div(ceil_div(k, a.splits), 64) * 64 <= 128 ? 1 : p.shape;
   if (p.kind == kFew && few_fits(a, k)) {
     few_launch(T::kType, p.mt, p.nb, a, p.tiles, cus(), s);
   } else if (p.kind == kTiles && tiles_fit(MODE, a, a.pairs, n, k)) {
-    tile_launch(MODE, T::kType, names[MODE], a, p.tiles * p.splits, cus(), s);
+    if (shape == 0)
+      tile_launch(MODE, T::kType, names[MODE], a, p.tiles * p.splits, cus(), s);
+    else
+      ring_launch(MODE, T::kType, shape, names[MODE], a, std::max(p.tiles * p.splits, shape == p.shape ? 0 : cus()), cus(), s);
   } else {
     const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>(p.tiles * p.splits * (p.kind == kFew ? 8 : 4), cus() * 4)));
     if (p.any == 128)

@@ -1,5 +1,5 @@
 // The linear products on whole tiles: rows at multiples of 16 bytes, sizes of multiples of 8.
-#include "linear_loads.h"
+#include "linear_stream.h"
 #include "linear_tile.h"
 
 #include <algorithm>
@@ -8,39 +8,6 @@
 namespace ferry {
 namespace lin {
 namespace {
-
-// -- epilogue ------------------------------------------------------------------------------------------
-
-template <typename T>
-__device__ __forceinline__ void unpack8(const u32x4& v, float (&f)[8]) {
-#pragma unroll
-  for (int q = 0; q < 8; ++q) f[q] = T::load((uint16_t)(v[q >> 1] >> (16 * (q & 1))));
-}
-template <typename T>
-__device__ __forceinline__ u32x4 pack8(const float (&f)[8]) {
-  u32x4 w;
-#pragma unroll
-  for (int q = 0; q < 4; ++q) w[q] = T::round2(f[2 * q], f[2 * q + 1]);
-  return w;
-}
-// columns j .. j + 7 of row `row`: v + bias, pre, activation, residual r, one rounding
-template <typename T, int ACT>
-__device__ __forceinline__ void finish8(const Args& a, uint16_t* out, int64_t row, int64_t j, float (&v)[8],
-                                        const u32x4& bias, const u32x4& r) {
-  float f[8];
-  unpack8<T>(bias, f);
-#pragma unroll
-  for (int q = 0; q < 8; ++q) v[q] += f[q];
-  if constexpr (ACT != kNone) {
-    if (a.pre) *reinterpret_cast<u32x4*>(a.pre + row * a.J + j) = pack8<T>(v);
-#pragma unroll
-    for (int q = 0; q < 8; ++q) v[q] = activate(ACT, v[q]);
-  }
-  unpack8<T>(r, f);
-#pragma unroll
-  for (int q = 0; q < 8; ++q) v[q] += f[q];
-  *reinterpret_cast<u32x4*>(out + row * a.ldo + j) = pack8<T>(v);
-}
 
 // =============================================================================================
 // 256 x 256 tiles
@@ -71,7 +38,6 @@ __device__ __forceinline__ void finish8(const Args& a, uint16_t* out, int64_t ro
 // fragments take any rows, the columns 8 g + 4 c + [0, 4) of tile c; of one staged by c, whose fragments take
 // 16 consecutive ones without bank conflicts, by an exchange between neighbouring rows of lanes at the end.
 constexpr int kHalf = 128 * 128;   // bytes
-__device__ __forceinline__ int swz_pair(int r) { return ((r >> 1) & 1) | (((r >> 3) & 3) << 1); }
 
 template <typename T, int MODE, bool GATHER, int ACT>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void tile256(Args a) {
@@ -114,64 +80,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       b_addr[ks] = smem0 + 4 * kHalf + (uint32_t)(r * 128 + (((4 * ks + g4) ^ swz_pair(r)) << 4));
   }
 
-  struct Tile {
-    u32x4 a, b;
-    int g, s, nc;          // group, part, length of the contraction
-    int64_t row0;          // output row of the tile's first
-    int rows, j0;          // rows from there on (may be more than 256), first column
-    const int64_t* idx;    // GA, GB: the row numbers from the tile's first row or c on
-  };
   const uint32_t lda2 = (uint32_t)a.lda * 2, ldb2 = (uint32_t)a.ldb * 2;
   const uint32_t a_step = XA ? 64 * lda2 : 128, b_step = XB ? (GB ? 0 : 64 * ldb2) : 128;
-
-  auto locate = [&](int item) {
-    Tile t;
-    t.s = item % a.splits;
-    const int q = item / a.splits;
-    int mt, jt;
-    // bands of four row tiles, all columns of a band before the next: what runs at one time on an XCD
-    // shares few rows of either operand
-    auto banded = [&](int k, int rows) {
-      const int band = k / (4 * ntj), r = k - band * 4 * ntj, h = rows - 4 * band < 4 ? rows - 4 * band : 4;
-      jt = r / h;
-      mt = 4 * band + r - jt * h;
-    };
-    int i0;
-    if constexpr (RAG) {
-      banded(q, mtiles);
-      t.g = a.starts ? find_group(tt, mt) : 0;
-      i0 = (mt - tt.cum[t.g]) * 256;
-    } else {
-      t.g = q / (nti * ntj);
-      banded(q - t.g * nti * ntj, nti);
-      i0 = mt * 256;
-    }
-    t.g = __builtin_amdgcn_readfirstlane(t.g);
-    const int64_t start = tt.start[t.g], n = tt.rows[t.g];
-    t.rows = __builtin_amdgcn_readfirstlane((int)((RAG ? n : a.I) - i0));
-    t.j0 = __builtin_amdgcn_readfirstlane(jt * 256);
-    t.row0 = (RAG ? start : 0) + i0;
-    const int64_t C = RAG ? a.C : n, per = ceil_div(ceil_div(C, a.splits), 64) * 64;
-    const int64_t c0 = t.s * per, c1 = c0 + per < C ? c0 + per : C;
-    t.nc = __builtin_amdgcn_readfirstlane((int)(c1 > c0 ? c1 - c0 : 0));
-    const int64_t nc = t.nc, vi = t.rows < 256 ? t.rows : 256, vj = a.J - t.j0 < 256 ? a.J - t.j0 : 256;
-    auto size = [](int64_t rows, int64_t ld, int64_t last) { return rows > 0 && last > 0 ? ((rows - 1) * ld + last) * 2 : 0; };
-    if constexpr (XA)
-      t.a = buffer_at(a.a + (start + c0) * a.lda + i0, size(nc, a.lda, vi));
-    else if constexpr (GA)
-      t.a = buffer_at(a.a + c0, size(a.x_rows, a.lda, nc));
-    else
-      t.a = buffer_at(a.a + t.row0 * a.lda + c0, size(vi, a.lda, nc));
-    const uint16_t* const w = a.b + (MODE == kDw ? 0 : t.g * a.b_group);
-    if constexpr (!XB)
-      t.b = buffer_at(w + (int64_t)t.j0 * a.ldb + c0, size(vj, a.ldb, nc));
-    else if constexpr (GB)
-      t.b = buffer_at(w + t.j0, size(a.x_rows, a.ldb, vj));
-    else
-      t.b = buffer_at(w + ((MODE == kDw ? start : 0) + c0) * a.ldb + t.j0, size(nc, a.ldb, vj));
-    t.idx = GATHER ? a.rows + (GA ? t.row0 : start + c0) : nullptr;
-    return t;
-  };
+  auto locate = [&](int item) { return locate_tile<MODE, GATHER, 256, 256>(a, tt, item, mtiles, nti, ntj); };
 
   // The load stream: the tile whose stages are being loaded.  Staged by index: a wavefront's rows 16 wave +
   // 8 q + lane / 8 of a half, place lane % 8.  By c: its rows 8 wave + 4 q + lane / 16, place lane % 16.
@@ -454,27 +365,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
           for (int i = 0; i < 4; ++i) {
             const int r = 128 * h + 32 * i + erow;
             float v[8];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              float lo = acc[h][hb][i][0][q], hi = acc[h][hb][i][1][q];
-              if constexpr (XB) {
-                const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(lo), __float_as_uint(hi), false, false);
-                lo = __uint_as_float(s[0]);
-                hi = __uint_as_float(s[1]);
-              }
-              v[q] = lo;
-              v[4 + q] = hi;
-            }
-            if (r < rows_in) {
-              const int64_t row = cur.row0 + r;
-              if (a.splits > 1) {
-                float* const o = a.part + (RAG ? cur.s * a.pairs + row : ((int64_t)cur.s * a.groups + cur.g) * a.I + row) * a.J + j;
-                *reinterpret_cast<f32x4*>(o) = f32x4{v[0], v[1], v[2], v[3]};
-                *reinterpret_cast<f32x4*>(o + 4) = f32x4{v[4], v[5], v[6], v[7]};
-              } else {
-                finish8<T, ACT>(a, out, row, j, v, bias, res[i]);
-              }
-            }
+            columns8<XB>(acc[h][hb][i][0], acc[h][hb][i][1], v);
+            if (r < rows_in) store8<T, MODE, ACT>(a, cur, out, r, j, v, bias, res[i]);
             __builtin_amdgcn_sched_barrier(0);
           }
         }

@@ -143,10 +143,8 @@ __device__ __forceinline__ float slope(int act, float z) {
 
 // The rows of group g are [start, start + n), forced into [0, pairs], so that whatever starts holds every
 // access stays inside the tensors; a group that ends before it starts has none.
-__device__ __forceinline__ int group_start(const Args& a, int g) {
-  const int64_t s = a.starts[g];
-  return (int)(s < 0 ? 0 : (s > a.pairs ? a.pairs : s));
-}
+__device__ __forceinline__ int in_pairs(const Args& a, int64_t s) { return (int)(s < 0 ? 0 : (s > a.pairs ? a.pairs : s)); }
+__device__ __forceinline__ int group_start(const Args& a, int g) { return in_pairs(a, a.starts[g]); }
 
 struct Table {
   __attribute__((aligned(16))) int32_t cum[kMaxGroups];   // tiles before the group, 0x7fffffff behind the last
@@ -161,16 +159,24 @@ __device__ __forceinline__ void build_table(const Args& a, Table& t, int rows) {
   constexpr int Q = kMaxGroups / 64;
   if (threadIdx.x < 64) {
     const int lane = threadIdx.x, G = a.groups;
+    int64_t lo[Q] = {}, hi[Q] = {};
+    int64_t end = a.pairs, begin = 0;
+    if (a.starts) {
+#pragma unroll
+      for (int q = 0; q < Q; ++q)
+        if (q * 64 < G) {
+          const int g = q * 64 + lane < G ? q * 64 + lane : G - 1;
+          lo[q] = a.starts[g];
+          hi[q] = a.starts[g + 1];
+        }
+      begin = a.starts[0];
+      end = a.starts[G];
+    } else {
+      hi[0] = a.pairs;
+    }
     int s[Q], n[Q];
 #pragma unroll
-    for (int q = 0; q < Q; ++q) {
-      const int g = q * 64 + lane;
-      s[q] = n[q] = 0;
-      if (q * 64 < G && g < G) {
-        s[q] = a.starts ? group_start(a, g) : 0;
-        n[q] = a.starts ? group_start(a, g + 1) : (int)a.pairs;
-      }
-    }
+    for (int q = 0; q < Q; ++q) s[q] = in_pairs(a, lo[q]), n[q] = in_pairs(a, hi[q]);
     int sum = 0;
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
@@ -194,8 +200,8 @@ __device__ __forceinline__ void build_table(const Args& a, Table& t, int rows) {
     }
     if (lane == 0) {
       t.total = sum;
-      t.first = a.starts ? group_start(a, 0) : 0;
-      t.last = a.starts ? group_start(a, G) : (int)a.pairs;
+      t.first = in_pairs(a, begin);
+      t.last = in_pairs(a, end);
     }
   }
   __syncthreads();

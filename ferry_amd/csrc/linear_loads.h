@@ -48,6 +48,9 @@ __device__ __forceinline__ void wait_cnt() {   // at most VM loads and no LDS re
   __builtin_amdgcn_s_waitcnt((VM & 15) | (7 << 4) | ((VM >> 4) << 14));
   asm volatile("" ::: "memory");
 }
+// no loads outstanding, in a form that the compiler counts with: loads to registers behind a condition would
+// otherwise be waited for where the registers are written next, in the loop
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }
 // no LDS reads outstanding
 __device__ __forceinline__ void wait_lds() {
   asm volatile("" ::: "memory");

@@ -30,6 +30,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM
   // row numbers (low and high words), each wavefront its own.  GA: of a tile, two in turn.  GB: of BS stages,
   // sets 0 and 1 in turn, 2 and 3 for the first ones of a tile.
   __shared__ __attribute__((aligned(256))) uint32_t row_s[GA ? 2 : (GB ? 4 : 1)][2][GATHER ? 64 * W : 1];
+  __shared__ __attribute__((aligned(256))) uint32_t bias_s[MODE == kFwd ? 2 : 1][MODE == kFwd ? 64 : 1];   // as in tile256
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int ntj = (int)ceil_div(a.J, TN), nti = RAG ? 0 : (int)ceil_div(a.I, TM);
@@ -127,10 +128,10 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM
     } else if (!(XA && XB) && left < 64) {   // chunks behind the contraction's end lie nowhere
 #pragma unroll
       for (int q = 0; q < LA; ++q)
-        if (!XA && chunk_a(q) * 8 >= left) avo[q] = kNowhere;
+        if constexpr (!XA) avo[q] = chunk_a(q) * 8 >= left ? kNowhere : avo[q];
 #pragma unroll
       for (int q = 0; q < LB; ++q)
-        if (!XB && chunk_b(q) * 8 >= left) bvo[q] = kNowhere;
+        if constexpr (!XB) bvo[q] = chunk_b(q) * 8 >= left ? kNowhere : bvo[q];
     }
     if constexpr (GB) {
       if (sk % BS == 0) {
@@ -213,11 +214,18 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM
   wg_barrier();
   read(0, I0{}, t0, w0);
   int cur = 0;   // slot of the stage
-  for (int item = first; item < total; item += gridDim.x) {
+  constexpr int kStores = MI * NI / 2;   // of a wavefront and whole tile
+  int early = 0;   // stages whose loads are older than the stores of the tile before
+  int bs = 0;
+  for (int item = first; item < total; item += gridDim.x, bs ^= 1) {
     const Tile t = locate(item);
     const int kt = t.nc > 64 ? (t.nc + 63) / 64 : 1;
     const int v = t.rows - 16 * wm;   // 16-row tiles of this wavefront that hold rows
     const int nf = __builtin_amdgcn_readfirstlane(v <= 0 ? 0 : ((v + 16 * WM - 1) / (16 * WM) < MI ? (v + 16 * WM - 1) / (16 * WM) : MI));
+    if (MODE == kFwd && wave == 0) {   // (128 columns)
+      const u32x4 r = buffer_at(a.bias + t.g * a.bias_group + t.j0, a.bias && a.splits == 1 ? (a.J - t.j0) * 2 : 0);
+      load_lds4(r, lane * 4, lds_at(bias_s[bs]));
+    }
     f32x4 acc[MI][NI];
 #pragma unroll
     for (int i = 0; i < MI; ++i)
@@ -236,7 +244,12 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM
 #pragma unroll
       for (int i = 0; i < MI; ++i) mma(i, t0, w0);
       // the stage is read by this wavefront, its loads of the next have landed
-      wait_cnt<(SST - 2) * LPS>();
+      if (early > 0) {   // the stores of the tile before may be outstanding too
+        --early;
+        wait_cnt<(SST - 2) * LPS + kStores>();
+      } else {
+        wait_cnt<(SST - 2) * LPS>();
+      }
       wg_barrier();
       read(nxt, I0{}, t0, w0);
       begin_stage();
@@ -248,25 +261,48 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM
       end_stage();
       cur = nxt;
     }
-    uint16_t* const out = a.out + (MODE == kDw ? t.g * a.o_group : 0);
-#pragma unroll
-    for (int cc = 0; cc < NI / 2; ++cc) {
-      const int64_t j = t.j0 + 16 * NI * wn + 32 * cc + (XB ? 16 * (g4 & 1) + 8 * (g4 >> 1) : 8 * g4);
-      const int rows_in = j < a.J ? t.rows : 0;   // (all lanes take part in the exchange below)
-      u32x4 bias = {0, 0, 0, 0};
-      if (MODE == kFwd && a.bias && a.splits == 1 && rows_in)
-        bias = *reinterpret_cast<const u32x4*>(a.bias + t.g * a.bias_group + j);
-#pragma unroll
-      for (int i = 0; i < MI; ++i) {
-        const int r = 16 * WM * i + 16 * wm + j16;
-        u32x4 res = {0, 0, 0, 0};
-        if (MODE == kFwd && !GATHER && a.residual && a.splits == 1 && r < rows_in)
-          res = *reinterpret_cast<const u32x4*>(a.residual + (t.row0 + r) * a.ldr + j);
-        float v8[8];
-        columns8<XB>(acc[i][2 * cc], acc[i][2 * cc + 1], v8);
-        if (r < rows_in) store8<T, MODE, MODE == kFwd && !GATHER ? -1 : (int)kNone>(a, t, out, r, j, v8, bias, res);
-      }
+    if (MODE == kFwd && kt < SST) {   // the bias was loaded at the tile's start
+      wait_cnt<0>();
+      wg_barrier();
     }
+    uint16_t* const out = a.out + (MODE == kDw ? t.g * a.o_group : 0);
+    early = t.rows >= TM && t.j0 + TN <= a.J ? SST - 1 : 0;
+    const int64_t jc = t.j0 + 16 * NI * wn + (XB ? 16 * (g4 & 1) + 8 * (g4 >> 1) : 8 * g4);
+    // the residual is read before the first store, as in tile256
+    auto finish = [&](auto with_res) {
+      constexpr bool RES = decltype(with_res)::value;
+      u32x4 res[NI / 2][MI] = {};
+      if constexpr (RES) {
+#pragma unroll
+        for (int cc = 0; cc < NI / 2; ++cc)
+#pragma unroll
+          for (int i = 0; i < MI; ++i) {
+            const int r = 16 * WM * i + 16 * wm + j16;
+            if (r < t.rows && jc + 32 * cc < a.J)
+              res[cc][i] = *reinterpret_cast<const u32x4*>(a.residual + (t.row0 + r) * a.ldr + jc + 32 * cc);
+          }
+        wait_loads();
+      }
+#pragma unroll
+      for (int cc = 0; cc < NI / 2; ++cc) {
+        const int64_t j = jc + 32 * cc;
+        const int rows_in = j < a.J ? t.rows : 0;   // (all lanes take part in the exchange below)
+        u32x4 bias = {0, 0, 0, 0};
+        if constexpr (MODE == kFwd)
+          bias = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(bias_s[bs]) + (j - t.j0) * 2);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+          const int r = 16 * WM * i + 16 * wm + j16;
+          float v8[8];
+          columns8<XB>(acc[i][2 * cc], acc[i][2 * cc + 1], v8);
+          if (r < rows_in) store8<T, MODE, MODE == kFwd && !GATHER ? -1 : (int)kNone>(a, t, out, r, j, v8, bias, res[cc][i]);
+        }
+      }
+    };
+    if (MODE == kFwd && !GATHER && a.residual && a.splits == 1)
+      finish(std::true_type{});
+    else
+      finish(std::false_type{});
   }
   wait_cnt<0>();   // no load may write this workgroup's LDS after its end
 }

@@ -48,6 +48,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   // GA: the rows of x of a tile's rows, two tiles in turn.  GB: those of 8 stages, each wavefront its own 8
   // rows of a stage: sets 0 and 1 in turn, 2 and 3 for the first 8 stages of a tile.  Low and high words.
   __shared__ __attribute__((aligned(256))) uint32_t row_s[GA ? 2 : (GB ? 4 : 1)][2][GA ? 256 : (GB ? 512 : 1)];
+  __shared__ __attribute__((aligned(256))) uint32_t bias_s[MODE == kFwd ? 2 : 1][MODE == kFwd ? 128 : 1];   // of the tile's columns, in turn
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int ntj = (int)ceil_div(a.J, 256), nti = RAG ? 0 : (int)ceil_div(a.I, 256);
@@ -245,6 +246,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   wait_cnt<12>();   // every wavefront has read B half 0 of stage 0 before stage 2's replaces it
   wg_barrier();
   if (wm == 1) wg_barrier();   // the second group runs one segment behind the first
+  int stores = 0;   // at least so many stores of the tile before may be outstanding, behind the loads in flight: 0 or 16
   for (int item = first; item < total; item += gridDim.x, set ^= 1) {
     // the tile after this one; after the last its own first stages are loaded again
     const int after = item + (int)gridDim.x < total ? item + (int)gridDim.x : item;
@@ -263,6 +265,11 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         nf[h] = __builtin_amdgcn_readfirstlane(v >= 128 ? 4 : (v > 0 ? (v + 31) / 32 : 0));
       }
       pairs = (t.nc + 127) / 128;   // pairs of stages: what is not there reads as 0
+      if (MODE == kFwd && wave < 2) {   // read behind the loop, 16 loads or more later
+        const int64_t j = t.j0 + 128 * wave;
+        const u32x4 r = buffer_at(a.bias + t.g * a.bias_group + j, a.bias && a.splits == 1 && j < a.J ? (a.J - j) * 2 : 0);
+        load_lds4(r, lane * 4, lds_at(bias_s[set]) + 256 * wave);
+      }
     }
     if (GB && pairs <= 1) wait_cnt<0>();   // the next tile's row numbers are needed at once
 
@@ -303,8 +310,16 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         __builtin_amdgcn_s_setprio(0);
         wg_barrier();
       };
-      auto mem_end = [&]() {   // the next segment's half has landed, this one's fragments are read
-        wait_cnt<12>();
+      // The next segment's half has landed, this one's fragments are read.  The first seven halves of a tile
+      // were loaded before the stores of the tile before: those may be outstanding too.
+      int early = stores ? 7 : 0;
+      auto mem_end = [&]() {
+        if (early > 0) {
+          --early;
+          wait_cnt<28>();
+        } else {
+          wait_cnt<12>();
+        }
         wg_barrier();
       };
       // a stage in slot S, loading the stage k of the stream into it
@@ -343,34 +358,45 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       int erow = 16 * wm + j16;
       asm volatile("" : "+v"(erow));   // the stores' addresses are computed here, not kept through the loop
       uint16_t* const out = a.out + (MODE == kDw ? cur.g * a.o_group : 0);
+      const int64_t jc = cur.j0 + 32 * wn + (XB ? 16 * (g4 & 1) + 8 * (g4 >> 1) : 8 * g4);
+      stores = cur.rows >= 256 && cur.j0 + 256 <= a.J ? 16 : 0;
+      // a B half's residual is read before its first store: a wait for it behind that would wait for the store too
+      auto finish = [&](auto with_res) {
+        constexpr bool RES = decltype(with_res)::value;
 #pragma unroll
-      for (int hb = 0; hb < 2; ++hb) {
-        const int64_t j = cur.j0 + 128 * hb + 32 * wn + (XB ? 16 * (g4 & 1) + 8 * (g4 >> 1) : 8 * g4);
-        const int rows_in = j < a.J ? cur.rows : 0;   // (all lanes take part in the exchange below)
-        u32x4 bias = {0, 0, 0, 0};
-        if (MODE == kFwd && a.bias && a.splits == 1 && rows_in)
-          bias = *reinterpret_cast<const u32x4*>(a.bias + cur.g * a.bias_group + j);
+        for (int hb = 0; hb < 2; ++hb) {
+          const int64_t j = jc + 128 * hb;
+          const int rows_in = j < a.J ? cur.rows : 0;   // (all lanes take part in the exchange below)
+          u32x4 res[2][4] = {};
+          if constexpr (RES) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          u32x4 res[4];
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int r = 128 * h + 32 * i + erow;
-            res[i] = u32x4{0, 0, 0, 0};
-            if (MODE == kFwd && !GATHER && a.residual && a.splits == 1 && r < rows_in)
-              res[i] = *reinterpret_cast<const u32x4*>(a.residual + (cur.row0 + r) * a.ldr + j);
+              for (int i = 0; i < 4; ++i) {
+                const int r = 128 * h + 32 * i + erow;
+                if (r < rows_in) res[h][i] = *reinterpret_cast<const u32x4*>(a.residual + (cur.row0 + r) * a.ldr + j);
+              }
+            wait_loads();
           }
-          __builtin_amdgcn_sched_barrier(0);   // one half's residual at a time: registers
+          u32x4 bias = {0, 0, 0, 0};
+          if constexpr (MODE == kFwd)
+            bias = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(bias_s[set]) + (j - cur.j0) * 2);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int r = 128 * h + 32 * i + erow;
-            float v[8];
-            columns8<XB>(acc[h][hb][i][0], acc[h][hb][i][1], v);
-            if (r < rows_in) store8<T, MODE, ACT>(a, cur, out, r, j, v, bias, res[i]);
-            __builtin_amdgcn_sched_barrier(0);
-          }
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              __builtin_amdgcn_sched_barrier(0);   // one row at a time: registers
+              const int r = 128 * h + 32 * i + erow;
+              float v[8];
+              columns8<XB>(acc[h][hb][i][0], acc[h][hb][i][1], v);
+              if (r < rows_in) store8<T, MODE, ACT>(a, cur, out, r, j, v, bias, res[h][i]);
+            }
         }
-      }
+      };
+      if (MODE == kFwd && !GATHER && a.residual && a.splits == 1)
+        finish(std::true_type{});
+      else
+        finish(std::false_type{});
     };
     if (rows >= 256)
       pipeline(std::false_type{});

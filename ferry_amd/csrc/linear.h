@@ -85,7 +85,13 @@ struct F16 {
 // 8 or 11 bits afterwards).  The tanh form is z / (1 + e^-2u), u = sqrt(2 / pi) (z + 0.044715 z^3): no
 // cancellation for negative z.
 
-__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __expf(-z)); }
+// 1 / (1 + 2^-y): two transcendental instructions, which cost as much as eight others
+__device__ __forceinline__ float sigmoid2(float y) {
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-y));
+}
+__device__ __forceinline__ float sigmoid(float z) { return sigmoid2(1.44269504f * z); }
+// sigmoid(2 u), u = sqrt(2 / pi) (z + 0.044715 z^3), in powers of 2
+__device__ __forceinline__ float gelu_gate(float z) { return sigmoid2(z * fmaf(0.102943240f, z * z, 2.30220819f)); }
 
 // The normal distribution function, erfc(-z / sqrt 2) / 2, with erfc(x) = t e^(P(t) - x^2), t = 1 / (1 + x / 2),
 // for x >= 0: P is a Chebyshev fit of degree 9 over 0 <= x <= 12 to ln(erfc(x) e^(x^2) / t), relative error
@@ -103,7 +109,7 @@ __device__ __forceinline__ float normal_cdf(float z) {
   p = fmaf(p, t, 0.380354122f);
   p = fmaf(p, t, 0.999348078f);
   p = fmaf(p, t, -1.26548227f);
-  const float q = 0.5f * t * __expf(fmaf(-x, x, p));
+  const float q = 0.5f * t * __builtin_amdgcn_exp2f(1.44269504f * fmaf(-x, x, p));
   return z > 0.f ? 1.0f - q : q;
 }
 
@@ -112,7 +118,7 @@ __device__ __forceinline__ float activate(int act, float z) {
     case kRelu: return z <= 0.f ? 0.f : z;   // a NaN stays one
     case kSilu: return z * sigmoid(z);
     case kGelu: return z * normal_cdf(z);
-    case kGeluTanh: return z * sigmoid(1.5957691f * (z + 0.044715f * z * z * z));
+    case kGeluTanh: return z * gelu_gate(z);
     default: return z;
   }
 }
@@ -128,11 +134,11 @@ __device__ __forceinline__ float slope(int act, float z) {
     }
     case kGelu: {
       z = fminf(fmaxf(z, -30.f), 30.f);
-      return normal_cdf(z) + z * 0.39894228f * __expf(-0.5f * z * z);
+      return normal_cdf(z) + z * 0.39894228f * __builtin_amdgcn_exp2f(-0.72134752f * z * z);
     }
     case kGeluTanh: {
       z = fminf(fmaxf(z, -30.f), 30.f);
-      const float s = sigmoid(1.5957691f * (z + 0.044715f * z * z * z));
+      const float s = gelu_gate(z);
       return s + z * s * (1.0f - s) * 1.5957691f * (1.0f + 0.134145f * z * z);
     }
     default: return 1.f;
@@ -150,6 +156,7 @@ struct Table {
   __attribute__((aligned(16))) int32_t cum[kMaxGroups];   // tiles before the group, 0x7fffffff behind the last
   int32_t start[kMaxGroups], rows[kMaxGroups];
   int32_t total, first, last;   // tiles; rows of the grouped order before the first and behind the last group
+  uint16_t order[kMaxGroups];   // not RAGGED_I: the groups by descending rows
 };
 
 // The groups' starts, rows and tiles: `rows` rows a tile with RAGGED_I, else `rows` tiles for each group.  By
@@ -205,6 +212,15 @@ __device__ __forceinline__ void build_table(const Args& a, Table& t, int rows) {
     }
   }
   __syncthreads();
+  if constexpr (!RAGGED_I) {
+    for (int g = threadIdx.x; g < a.groups; g += blockDim.x) {
+      const int n = t.rows[g];
+      int rank = 0;
+      for (int h = 0; h < a.groups; ++h) rank += t.rows[h] > n || (t.rows[h] == n && h < g);
+      t.order[rank] = (uint16_t)g;
+    }
+    __syncthreads();
+  }
 }
 
 // the group of tile m: the last g with cum[g] <= m (groups without tiles share their successor's cum)
@@ -232,6 +248,7 @@ __device__ __forceinline__ int find_group(const Table& t, int m) {
 __device__ __forceinline__ int swz_direct(int r) { return (r >> 1) & 7; }
 template <int W>
 __device__ __forceinline__ int swz_across(int r) {
+  if (W == 32) return ((r >> 3) & 1) << 1;
   return W == 64 ? ((((r >> 1) & 1) | (((r >> 3) & 1) << 1)) << 1) : (((r & 3) | (((r >> 3) & 1) << 2)) << 1);
 }
 // fragment of 16 indices from i0 on at K step ks (32 values of c): byte offsets into the staged operand

@@ -6,6 +6,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace ferry {
 namespace lin {
@@ -246,16 +247,33 @@ struct SlopeArgs {
   int32_t groups, splits, act, zero_rest, vec;
 };
 
-// dz = dy f'(pre) rounded, and db = the sum of the unrounded dz over each group's rows.  A workgroup
-// takes 256 columns (8 a thread) of one part of a group's rows, 8 rows at a time.  Bound by memory: dy
-// and pre in, dz out.
-template <typename T>
+// f[q] = f'(f[q]), the choice of the activation once for eight
+__device__ __forceinline__ void slope8(int act, float (&f)[8]) {
+  auto all = [&](auto a) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) f[q] = slope(decltype(a)::value, f[q]);
+  };
+  switch (act) {
+    case kRelu: return all(std::integral_constant<int, kRelu>{});
+    case kSilu: return all(std::integral_constant<int, kSilu>{});
+    case kGelu: return all(std::integral_constant<int, kGelu>{});
+    default: return all(std::integral_constant<int, kGeluTanh>{});
+  }
+}
+
+// dz = dy f'(pre) rounded, and db = the sum of the unrounded dz over each group's rows.  A workgroup takes
+// 2048 / RL columns (8 a thread) of one part of a group's rows, RL rows side by side and four of those at a
+// time, whose loads are issued together.  Large calls are bound by memory (dy and pre in, dz out) and take RL = 8
+// and parts, which a second launch adds; small ones by the chain of loads of a column's rows, which RL = 32
+// shortens without parts.
+template <typename T, int RL>
 __global__ __launch_bounds__(256) void slope_kernel(SlopeArgs a) {
-  __shared__ float sum[8][256 + 8];
-  const int tid = threadIdx.x, rl = tid >> 5, cl = (tid & 31) * 8;
-  const int64_t jb = ceil_div(a.N, 256), items = jb * a.groups * a.splits;
+  constexpr int CL = 256 / RL, COLS = CL * 8, U = 4;
+  __shared__ float sum[RL][COLS + 8];
+  const int tid = threadIdx.x, rl = tid / CL, cl = (tid % CL) * 8;
+  const int64_t jb = ceil_div(a.N, COLS), items = jb * a.groups * a.splits;
   for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
-    const int64_t j = (it % jb) * 256 + cl;
+    const int64_t j = (it % jb) * COLS + cl;
     const int g = (int)(it / jb % a.groups), s = (int)(it / jb / a.groups);
     int64_t lo = 0, hi = a.pairs;
     if (a.starts) {
@@ -269,41 +287,54 @@ __global__ __launch_bounds__(256) void slope_kernel(SlopeArgs a) {
     const int m = (int)(a.N - j < 8 ? a.N - j : 8);
     float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (m > 0)
-#pragma unroll 2
-      for (int64_t r = r0 + rl; r < r1; r += 8) {
-        const u32x4 y = load8(a.dy + r * a.ldy + j, m);
-        float v[8];
+      for (int64_t rr = r0 + rl; rr < r1; rr += U * RL) {
+        u32x4 y[U], z[U];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) v[q] = T::load((uint16_t)(y[q >> 1] >> (16 * (q & 1))));
-        if (a.act != kNone) {
-          const u32x4 z = load8(a.pre + r * a.N + j, m);
-#pragma unroll
-          for (int q = 0; q < 8; ++q) v[q] *= slope(a.act, T::load((uint16_t)(z[q >> 1] >> (16 * (q & 1)))));
-          uint16_t* const o = a.dz + r * a.N + j;
-          u32x4 w;
-#pragma unroll
-          for (int q = 0; q < 4; ++q) w[q] = T::round2(v[2 * q], v[2 * q + 1]);
-          if (m == 8) {
-            __builtin_memcpy(o, &w, 16);
-          } else {
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-              if (q < m) o[q] = (uint16_t)(w[q >> 1] >> (16 * (q & 1)));
-          }
+        for (int u = 0; u < U; ++u) {
+          const int64_t r = rr + u * RL;
+          y[u] = load8(a.dy + r * a.ldy + j, r < r1 ? m : 0);
+          z[u] = load8(a.pre + r * a.N + j, a.act != kNone && r < r1 ? m : 0);
         }
 #pragma unroll
-        for (int q = 0; q < 8; ++q) acc[q] += v[q];
+        for (int u = 0; u < U; ++u) {
+          const int64_t r = rr + u * RL;
+          if (r >= r1) continue;
+          float v[8];
+#pragma unroll
+          for (int q = 0; q < 8; ++q) v[q] = T::load((uint16_t)(y[u][q >> 1] >> (16 * (q & 1))));
+          if (a.act != kNone) {
+            float f[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) f[q] = T::load((uint16_t)(z[u][q >> 1] >> (16 * (q & 1))));
+            slope8(a.act, f);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v[q] *= f[q];
+            uint16_t* const o = a.dz + r * a.N + j;
+            u32x4 w;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) w[q] = T::round2(v[2 * q], v[2 * q + 1]);
+            if (m == 8) {
+              __builtin_memcpy(o, &w, 16);
+            } else {
+#pragma unroll
+              for (int q = 0; q < 8; ++q)
+                if (q < m) o[q] = (uint16_t)(w[q >> 1] >> (16 * (q & 1)));
+            }
+          }
+#pragma unroll
+          for (int q = 0; q < 8; ++q) acc[q] += v[q];
+        }
       }
     if (!a.db) continue;
     __syncthreads();
 #pragma unroll
     for (int q = 0; q < 8; ++q) sum[rl][cl + q] = acc[q];
     __syncthreads();
-    const int64_t jj = (it % jb) * 256 + tid;
-    if (jj < a.N) {
+    const int64_t jj = (it % jb) * COLS + tid;
+    if (tid < COLS && jj < a.N) {
       float t = 0;
 #pragma unroll
-      for (int q = 0; q < 8; ++q) t += sum[q][tid];
+      for (int q = 0; q < RL; ++q) t += sum[q][tid];
       if (a.splits > 1)
         a.part[((int64_t)s * a.groups + g) * a.N + jj] = t;
       else
@@ -388,12 +419,20 @@ struct Plan {
 };
 
 // The tiles' sizes (indices of A and of B), and their time in us: for a stage of 64 of the contraction, and for
-// what a tile costs besides.
+// what a tile costs besides.  Measured at 8,192 x 6,144 x 2,048 and its gradients.
 struct TileCost {
   int tm, tn;
   double stage, fixed;
 };
-const TileCost kShapes[] = {{256, 256, 1.31, 5.0}, {256, 128, 0.8, 4.0}, {128, 128, 0.52, 3.0}, {64, 128, 0.38, 2.5}, {64, 64, 0.30, 2.0}};
+const TileCost kShapes[] = {{256, 256, 1.31, 6.0}, {256, 128, 1.04, 4.0}, {128, 128, 0.58, 3.0}, {64, 128, 0.40, 2.5}, {64, 64, 0.32, 2.0}};
+// few_kernel's tiles in 16s, wavefronts, workgroups resident on a CU, us for a step of 64 of the contraction a wavefront
+struct FewCost {
+  int mt, nb, waves, resident;
+  double step;
+};
+const FewCost kFews[] = {{1, 1, 8, 1, 0.36}, {1, 1, 4, 2, 0.34}, {1, 2, 4, 2, 0.46}, {2, 2, 4, 2, 0.42}, {4, 2, 4, 1, 0.65}, {4, 4, 4, 1, 0.85}};
+constexpr double kLaunch = 3.5;    // us until the first products of a launch, and for its end
+constexpr double kMemory = 4.8e6;  // bytes a us
 
 // op: the product; rows: pairs
 Plan plan(int op, int64_t pairs, int64_t n, int64_t k, int64_t groups) {
@@ -403,55 +442,72 @@ Plan plan(int op, int64_t pairs, int64_t n, int64_t k, int64_t groups) {
   auto tiles = [&](int64_t tm, int64_t tn) { return (op == kDw ? groups * ceil_div(n, tm) : row_tiles(tm)) * ceil_div(J, tn); };
   p.any = tiles(128, 128) >= 512 ? 128 : 64;
   p.splits = 1;
-  const int64_t rows = pairs / used;   // of a group, on average
-  if (op == kFwd && k % 8 == 0 && rows <= 64) {
-    p.kind = kFew;
-    p.mt = rows <= 16 ? 1 : (rows <= 32 ? 2 : 4);
-    p.tiles = row_tiles(16 * p.mt);
-    const int64_t blocks = used * ceil_div(n, 16);
-    p.nb = p.mt == 1 ? (blocks > 2048 ? 2 : 1) : (p.mt == 2 || blocks < 1024 ? 2 : 4);
-    return p;
-  }
   const double c = op == kFwd ? (double)k : (op == kDx ? (double)n : (double)pairs / (double)groups);
-  if (n % 8 || k % 8) {
+  const bool tiled = n % 8 == 0 && k % 8 == 0, few = op == kDx ? tiled && groups == 1 : op == kFwd && k % 8 == 0 && (groups == 1 || pairs <= 6 * used);
+  if (!tiled && !few) {
     p.tiles = tiles(p.any, p.any);
     p.splits = splits_of(p.tiles, (int64_t)c);
     return p;
   }
-  p.kind = kTiles;
-  // The cheapest shape and number of parts: whole rounds of tiles over the CUs, no faster than the operands come
-  // from memory, and the parts' way through memory.
+  // The cheapest kernel, tile and number of parts: whole rounds of tiles over the CUs (of groups of unknown sizes, as
+  // many tiles as equal ones and half a tile of each group), no faster than the operands come from memory, the
+  // parts' way through memory, and for groups half a tile's time until the last is done.
   const int64_t cu = cus();
-  const double out = (double)(op == kDw ? groups * n * k : pairs * J);
+  const double rows = (double)pairs / used, out = (double)(op == kDw ? groups * n * k : pairs * J);
   const double bytes = 2.0 * (op == kDw ? (double)pairs * (n + k) + out : (double)pairs * (n + k) + (double)used * n * k);
-  double least = 0;
-  for (int i = 0; i < 5; ++i) {
-    const TileCost& t = kShapes[i];
-    const double mt = op == kDw ? (double)(groups * ceil_div(n, t.tm)) : (groups > 1 ? (double)pairs / t.tm + 0.5 * used : (double)ceil_div(pairs, t.tm));
-    for (int64_t parts = 1; parts <= 16; parts *= 2) {
-      if (parts > 1 && c / parts < 256) break;
-      const double items = mt * ceil_div(J, t.tn) * parts, rounds = std::ceil(items / cu);
-      double cost = rounds * (std::ceil(c / 64 / parts) * t.stage + t.fixed);
-      cost = std::max(cost, bytes / 4.5e6 + 1.0);
-      if (parts > 1) cost += 4.0 + out * (8.0 * parts + 2.0) / 4.5e6;
-      if ((i == 0 && parts == 1) || cost < least) {
+  auto m_tiles = [&](int tm) {
+    if (op == kDw) return (double)(groups * ceil_div(n, tm));
+    return groups > 1 ? used * std::max(1.0, rows / tm + 0.5) : (double)ceil_div(pairs, tm);
+  };
+  auto time = [&](double items, double slots, double item) {
+    const double rounds = groups > 1 ? std::max(1.0, items / slots) : std::ceil(items / slots);
+    return kLaunch + std::max(rounds * item, bytes / kMemory) + (groups > 1 ? 0.5 * item : 0.0);
+  };
+  double least = 1e30;
+  if (few)
+    for (const FewCost& f : kFews) {
+      // kDx loads w by pieces of its rows, and of groups tiles of 32 x 32 were the fastest
+      if ((op == kDx && f.mt != f.nb) || (op == kDx && f.mt == 1) || (groups > 1 && f.mt != 2)) continue;
+      const double items = m_tiles(16 * f.mt) * ceil_div(J, 16 * f.nb);
+      if (f.nb == 1 && (f.waves == 8) != (row_tiles(16) * ceil_div(J, 16) <= cu)) continue;   // as few_launch has it
+      const double step = f.step * (op == kDx && f.nb == 2 ? 1.5 : 1.0);
+      const double cost = time(items, (double)cu * f.resident, (1.0 + std::ceil(c / (64 * f.waves)) * step) * (groups > 1 ? 1.5 : 1.0));
+      if (cost < least) {
         least = cost;
-        p.shape = i;
-        p.splits = parts;
+        p.kind = kFew;
+        p.mt = f.mt;
+        p.nb = f.nb;
       }
     }
-  }
-  p.tiles = tiles(kShapes[p.shape].tm, kShapes[p.shape].tn);
+  if (tiled)
+    for (int i = 0; i < 5; ++i) {
+      const TileCost& t = kShapes[i];
+      for (int64_t parts = 1; parts <= 16; parts *= 2) {
+        if (parts > 1 && c / parts < 256) break;
+        // (groups' small tiles share less of the operands in L2)
+        const double stage = t.stage * (groups > 1 && t.tm == 64 ? 1.4 : 1.0);
+        double cost = time(m_tiles(t.tm) * ceil_div(J, t.tn) * parts, (double)cu, std::ceil(c / 64 / parts) * stage + t.fixed);
+        if (parts > 1) cost += 4.0 + out * (8.0 * parts + 2.0) / kMemory;
+        if (cost < least) {
+          least = cost;
+          p.kind = kTiles;
+          p.shape = i;
+          p.splits = parts;
+        }
+      }
+    }
+  p.tiles = p.kind == kFew ? row_tiles(16 * p.mt) : tiles(kShapes[p.shape].tm, kShapes[p.shape].tn);
   return p;
 }
 
 bool even(const void* q, int64_t stride) { return (uintptr_t)q % 16 == 0 && stride % 8 == 0; }
 
 // Whether few_kernel can read the operands: rows at multiples of 16 bytes, offsets that 32 bits hold.
-bool few_fits(const Args& a, int64_t k) {
+bool few_fits(int op, const Args& a) {
   const int64_t most = ((int64_t)1 << 31) - (1 << 20);
-  return k % 8 == 0 && even(a.a, a.lda) && even(a.b, a.ldb) && a.b_group % 8 == 0 && a.ldb <= most / 128 && a.lda <= most / 128 &&
-         k <= most / 4 && (!a.rows || (a.x_rows >= 1 && a.x_rows * a.lda <= most));
+  return a.C % 8 == 0 && (op == kFwd || a.J % 8 == 0) && even(a.a, a.lda) && even(a.b, a.ldb) && a.b_group % 8 == 0 &&
+         a.ldb <= most / 128 && a.lda <= most / 128 && a.C <= most / 4 && (op == kFwd || (a.C + 128) * a.ldb <= most) &&
+         (!a.rows || (a.x_rows >= 1 && a.x_rows * a.lda <= most));
 }
 
 // Whether the tiled kernels can read and write the operands: rows at multiples of 16 bytes, offsets that 32
@@ -473,9 +529,12 @@ int64_t part_bytes(int op, const Plan& p, int64_t pairs, int64_t n, int64_t k, i
   return p.splits * out * 4;
 }
 
-int64_t slope_splits(int64_t pairs, int64_t n, int64_t groups) {
-  const int64_t items = ceil_div(n, 256) * std::max<int64_t>(groups, 1);
-  return std::max<int64_t>(1, std::min<int64_t>({ceil_div(1024, items), ceil_div(pairs / std::max<int64_t>(groups, 1), 64), 64}));
+// Parts of a group's rows for slope_kernel, 1: all rows by one workgroup, 32 side by side.  Up to 512 rows of a
+// group on average one launch without parts is faster: 300 rows of 2,816 took 15 + 4 us with parts of 60 rows, and
+// take 10 without.  Above, a part for each 128 rows of the average, 64 at most.
+int64_t slope_splits(int64_t pairs, int64_t groups) {
+  const int64_t rows = pairs / groups;
+  return rows <= 512 ? 1 : std::min<int64_t>(ceil_div(rows, 128), 64);
 }
 
 template <typename T, int MODE>
@@ -483,8 +542,8 @@ int run_typed(const Args& a, const Plan& p, int64_t n, int64_t k, hipStream_t s)
   static const char* const names[] = {"linear_fwd", "linear_dx", "linear_dw"};
   // (tile256 loads the row numbers of a tile one tile ahead, which takes a contraction of more than two stages)
   const int shape = p.shape == 0 && MODE == kFwd && a.rows && ceil_div(ceil_div(k, a.splits), 64) * 64 <= 128 ? 1 : p.shape;
-  if (p.kind == kFew && few_fits(a, k)) {
-    few_launch(T::kType, p.mt, p.nb, a, p.tiles, cus(), s);
+  if (p.kind == kFew && few_fits(MODE, a)) {
+    few_launch(MODE, T::kType, p.mt, p.nb, a, p.tiles, cus(), s);
   } else if (p.kind == kTiles && tiles_fit(MODE, a, a.pairs, n, k)) {
     if (shape == 0)
       tile_launch(MODE, T::kType, names[MODE], a, p.tiles * p.splits, cus(), s);
@@ -547,7 +606,7 @@ extern "C" int64_t ferry_linear_workspace_bytes(int32_t op, int64_t pairs, int64
   if (pairs < 0 || pairs >= kMost || n < 1 || n >= kMost || k < 1 || k >= kMost || groups < 1 || groups > kMaxGroups)
     return -1;
   if (op == FERRY_LINEAR_GRAD_Z) {
-    const int64_t s = slope_splits(pairs, n, groups);
+    const int64_t s = slope_splits(pairs, groups);
     return s > 1 ? s * groups * n * 4 : 0;
   }
   if (op < kFwd || op > kDw) return -1;
@@ -594,7 +653,7 @@ extern "C" int ferry_linear_grad_z(const void* grad, int32_t dtype, int64_t pair
   if (activation == kNone && !db) return 0;
   FERRY_CHECK_ARG(pairs == 0 || grad, "null pointer argument");
   SlopeArgs a = {};
-  a.splits = (int32_t)slope_splits(pairs, n, groups);
+  a.splits = (int32_t)slope_splits(pairs, groups);
   const int64_t need = db && a.splits > 1 ? a.splits * groups * n * 4 : 0;
   FERRY_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need), "workspace too small (%lld < %lld bytes)",
                   (long long)workspace_bytes, (long long)need);
@@ -603,11 +662,13 @@ extern "C" int ferry_linear_grad_z(const void* grad, int32_t dtype, int64_t pair
   a.part = (float*)workspace, a.ldy = grad_stride, a.pairs = pairs, a.N = n;
   a.starts = starts, a.groups = (int32_t)groups, a.act = activation;
   hipStream_t s = (hipStream_t)stream;
-  const dim3 grid((unsigned)std::min<int64_t>(ceil_div(n, 256) * groups * a.splits, kMaxGrid));
+  auto go = [&](auto kernel, int cols) {
+    launch("linear_slope", kernel, dim3((unsigned)std::min<int64_t>(ceil_div(n, cols) * groups * a.splits, kMaxGrid)), dim3(256), 0, s, a);
+  };
   if (dtype == FERRY_BF16)
-    launch("linear_slope", slope_kernel<Bf16>, grid, dim3(256), 0, s, a);
+    a.splits > 1 ? go(slope_kernel<Bf16, 8>, 256) : go(slope_kernel<Bf16, 32>, 64);
   else
-    launch("linear_slope", slope_kernel<F16>, grid, dim3(256), 0, s, a);
+    a.splits > 1 ? go(slope_kernel<F16, 8>, 256) : go(slope_kernel<F16, 32>, 64);
   FERRY_LAUNCHED("linear_slope");
   if (need) {
     const dim3 g2((unsigned)std::min<int64_t>(ceil_div(groups * n, 256), 65536));

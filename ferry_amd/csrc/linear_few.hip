@@ -16,9 +16,10 @@ namespace {
 // that are not there cost nothing (they read as 0 without a transaction), the others come from L2.
 // Workgroups stay and take items in turn (column blocks fastest), since a workgroup that finds no rows costs
 // as much as its dispatch, and of 128 experts a decode step uses 40.
-template <typename T, bool GATHER, int MT, int NB, int WK, int R>
+template <typename T, int MODE, bool GATHER, int MT, int NB, int WK, int R>
 __global__ __launch_bounds__(64 * WK) void few_kernel(Args a) {
-  constexpr int LW = 2 * NB, LX = 2 * MT, L = LW + LX;   // loads of a chunk
+  constexpr bool XB = MODE == kDx;   // w staged by rows of the contraction
+  constexpr int LW = 2 * NB, LX = 2 * MT, L = LW + LX, TN = 16 * NB;   // loads of a chunk; columns
   constexpr int kSlot = 16 * (NB + MT) * 128;
   static_assert(MT * NB * 1024 <= R * kSlot, "the sums of a wavefront fit its ring");
   __shared__ Table tt;
@@ -52,21 +53,28 @@ __global__ __launch_bounds__(64 * WK) void few_kernel(Args a) {
       load_lds4(rows, lane * 8, lds_at(row_s[wave][0]));
       load_lds4(rows, lane * 8 + 4, lds_at(row_s[wave][1]));
     }
-    const u32x4 bw = buffer_at(a.b + g * a.b_group + (int64_t)j0 * a.ldb, ((vj - 1) * a.ldb + C) * 2);
+    const u32x4 bw = XB ? buffer_at(a.b + g * a.b_group + j0, ((C - 1) * a.ldb + vj) * 2)
+                        : buffer_at(a.b + g * a.b_group + (int64_t)j0 * a.ldb, ((vj - 1) * a.ldb + C) * 2);
     const u32x4 bx = GATHER ? buffer_at(a.a, ((a.x_rows - 1) * a.lda + C) * 2)
                             : buffer_at(a.a + (int64_t)(start + m0) * a.lda, ((vr - 1) * a.lda + C) * 2);
     uint32_t xo[LX];
     // chunk of place lane % 8 in the rows 8 q + lane / 8, and whether it lies in the contraction at step i
-    auto chunk = [&](int q) { return (lane & 7) ^ swz_direct(8 * (q & 1) + r8); };
-    auto load_w = [&](int i, int slot) {
+    auto chunk = [&](int q) __attribute__((always_inline)) { return (lane & 7) ^ swz_direct(8 * (q & 1) + r8); };
+    auto load_w = [&](int i, int slot) __attribute__((always_inline)) {
       const int c = (i * WK + wave) * 64;
       const uint32_t dst = ring + slot * kSlot;
 #pragma unroll
-      for (int q = 0; q < LW; ++q)
-        load_lds(bw, c + chunk(q) * 8 < C ? (uint32_t)(8 * q + r8) * ldb2 + chunk(q) * 16 : kNowhere, c < C ? c * 2 : 0,
-                 dst + 1024 * q);
+      for (int q = 0; q < LW; ++q) {
+        if constexpr (XB) {
+          const int r = 512 / TN * q + lane / (TN / 8), k = (lane % (TN / 8)) ^ swz_across<TN>(r);
+          load_lds(bw, c < C ? (uint32_t)r * ldb2 + k * 16 : kNowhere, c < C ? c * ldb2 : 0, dst + 1024 * q);
+        } else {
+          load_lds(bw, c + chunk(q) * 8 < C ? (uint32_t)(8 * q + r8) * ldb2 + chunk(q) * 16 : kNowhere, c < C ? c * 2 : 0,
+                   dst + 1024 * q);
+        }
+      }
     };
-    auto load_x = [&](int i, int slot) {
+    auto load_x = [&](int i, int slot) __attribute__((always_inline)) {
       const int c = (i * WK + wave) * 64;
       const uint32_t dst = ring + slot * kSlot + LW * 1024;
 #pragma unroll
@@ -95,13 +103,18 @@ __global__ __launch_bounds__(64 * WK) void few_kernel(Args a) {
 #pragma unroll
       for (int b = 0; b < NB; ++b) acc[i][b] = f32x4{0, 0, 0, 0};
     const int more = steps > R ? steps - R : 0;   // chunks that the loop loads
-    auto step = [&](int i, int slot) {
+    auto step = [&](int i, int slot) __attribute__((always_inline)) {
       const uint32_t st = ring + slot * kSlot;
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
         s16x8 fw[NB], fx[MT];
 #pragma unroll
-        for (int b = 0; b < NB; ++b) fw[b] = read_direct(st + frag_direct(16 * b, ks));
+        for (int b = 0; b < NB; ++b) {
+          if constexpr (XB)
+            fw[b] = read_across(st + frag_across<TN>(16 * b, ks, 0), st + frag_across<TN>(16 * b, ks, 1));
+          else
+            fw[b] = read_direct(st + frag_direct(16 * b, ks));
+        }
 #pragma unroll
         for (int m = 0; m < MT; ++m) fx[m] = read_direct(st + LW * 1024 + frag_direct(16 * m, ks));
 #pragma unroll
@@ -117,7 +130,7 @@ __global__ __launch_bounds__(64 * WK) void few_kernel(Args a) {
     };
     // chunk i has landed when at most what was loaded after it is outstanding: of the first R, the rows of x
     // of the others and one chunk for each step so far; then the R - 1 chunks before it, or those left
-    static_for<0, R>([&](auto ii) {
+    static_for<0, R>([&](auto ii) __attribute__((always_inline)) {
       constexpr int I = decltype(ii)::value;
       if (I < steps) {
         if (I <= more)
@@ -154,33 +167,34 @@ __global__ __launch_bounds__(64 * WK) void few_kernel(Args a) {
   }
 }
 
-template <typename T, bool GATHER>
+template <typename T, int MODE, bool GATHER>
 void few_typed(int mt, int nb, const Args& a, int64_t tiles, int64_t cus, hipStream_t s) {
   const int64_t items = tiles * ceil_div(a.J, 16 * nb);
   auto go = [&](auto kernel, int threads, int resident) {
     launch("linear_few", kernel, dim3((unsigned)std::min(items, cus * resident)), dim3(threads), 0, s, a);
   };
-  if (mt == 1 && nb == 1 && items <= cus)
-    go(few_kernel<T, GATHER, 1, 1, 8, 4>, 512, 1);
-  else if (mt == 1 && nb == 1)
-    go(few_kernel<T, GATHER, 1, 1, 4, 4>, 256, 2);
-  else if (mt == 1)
-    go(few_kernel<T, GATHER, 1, 2, 4, 3>, 256, 2);
-  else if (mt == 2)
-    go(few_kernel<T, GATHER, 2, 2, 4, 2>, 256, 2);
+  if constexpr (MODE == kFwd) {
+    if (nb == 1 && items <= cus) return go(few_kernel<T, MODE, GATHER, 1, 1, 8, 4>, 512, 1);
+    if (nb == 1) return go(few_kernel<T, MODE, GATHER, 1, 1, 4, 4>, 256, 2);
+    if (mt == 1) return go(few_kernel<T, MODE, GATHER, 1, 2, 4, 3>, 256, 2);
+  }
+  if (mt == 2)
+    go(few_kernel<T, MODE, GATHER, 2, 2, 4, 2>, 256, 2);
   else if (nb == 2)
-    go(few_kernel<T, GATHER, 4, 2, 4, 2>, 256, 1);
+    go(few_kernel<T, MODE, GATHER, 4, 2, 4, 2>, 256, 1);
   else
-    go(few_kernel<T, GATHER, 4, 4, 4, 2>, 256, 1);
+    go(few_kernel<T, MODE, GATHER, 4, 4, 4, 2>, 256, 1);
+}
+template <typename T>
+void few_mode(int mode, int mt, int nb, const Args& a, int64_t tiles, int64_t cus, hipStream_t s) {
+  if (mode == kDx) return few_typed<T, kDx, false>(mt, nb, a, tiles, cus, s);
+  a.rows ? few_typed<T, kFwd, true>(mt, nb, a, tiles, cus, s) : few_typed<T, kFwd, false>(mt, nb, a, tiles, cus, s);
 }
 
 }  // namespace
 
-void few_launch(int32_t dtype, int mt, int nb, const Args& a, int64_t tiles, int64_t cus, hipStream_t s) {
-  if (dtype == FERRY_BF16)
-    a.rows ? few_typed<Bf16, true>(mt, nb, a, tiles, cus, s) : few_typed<Bf16, false>(mt, nb, a, tiles, cus, s);
-  else
-    a.rows ? few_typed<F16, true>(mt, nb, a, tiles, cus, s) : few_typed<F16, false>(mt, nb, a, tiles, cus, s);
+void few_launch(int mode, int32_t dtype, int mt, int nb, const Args& a, int64_t tiles, int64_t cus, hipStream_t s) {
+  dtype == FERRY_BF16 ? few_mode<Bf16>(mode, mt, nb, a, tiles, cus, s) : few_mode<F16>(mode, mt, nb, a, tiles, cus, s);
 }
 
 }  // namespace lin

@@ -19,6 +19,11 @@ __device__ __forceinline__ u32x4 buffer_at(const void* p, int64_t bytes) {
 }
 constexpr uint32_t kNowhere = 0xfffffff0u;   // an offset behind the end of every buffer
 
+// (descriptors are wave-uniform, but the compiler may keep them in vector registers)
+__device__ __forceinline__ u32x4 scalar(const u32x4& r) {
+  return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)r[0]), (uint32_t)__builtin_amdgcn_readfirstlane((int)r[1]),
+               (uint32_t)__builtin_amdgcn_readfirstlane((int)r[2]), 0x00020000u};
+}
 // 16 bytes of each lane from offset soff + voff of the buffer to LDS address lds + 16 * lane; 0 from behind the
 // buffer's end (soff itself must lie in it, or be 0: the hardware compares voff with size - soff).  Inline asm,
 // so that no wait is added: their completion is awaited with wait_cnt.  m0 holds the LDS base; one wait state
@@ -29,7 +34,7 @@ __device__ __forceinline__ void load_lds(u32x4 r, uint32_t voff, uint32_t soff, 
       "s_nop 0\n\t"
       "buffer_load_dwordx4 %0, %1, %3 offen lds"
       :
-      : "v"(voff), "s"(r), "s"(__builtin_amdgcn_readfirstlane((int)lds)), "s"(__builtin_amdgcn_readfirstlane((int)soff))
+      : "v"(voff), "s"(scalar(r)), "s"(__builtin_amdgcn_readfirstlane((int)lds)), "s"(__builtin_amdgcn_readfirstlane((int)soff))
       : "memory");
 }
 // 4 bytes of each lane, as above
@@ -39,7 +44,7 @@ __device__ __forceinline__ void load_lds4(u32x4 r, uint32_t voff, uint32_t lds) 
       "s_nop 0\n\t"
       "buffer_load_dword %0, %1, 0 offen lds"
       :
-      : "v"(voff), "s"(r), "s"(lds)
+      : "v"(voff), "s"(scalar(r)), "s"(__builtin_amdgcn_readfirstlane((int)lds))
       : "memory");
 }
 template <int VM>

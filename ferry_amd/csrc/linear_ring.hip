@@ -38,15 +38,15 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM
   if (RAG && a.zero_rest) zero_rest(a, tt.first, tt.last);
   const int mtiles = __builtin_amdgcn_readfirstlane(tt.total);
   const int total = mtiles * ntj * a.splits;
-  const int per_xcd = gridDim.x % 8 == 0 ? (int)gridDim.x / 8 : 0;   // as in tile256
-  const int first = per_xcd ? (int)(blockIdx.x % 8) * per_xcd + (int)(blockIdx.x / 8) : (int)blockIdx.x;
+  const Rounds rounds(total, !RAG);
+  const int first = rounds.at(0);
   if (first >= total) return;
   const int wm = wave / WN, wn = wave % WN;
   const int j16 = lane & 15, g4 = lane >> 4;
   const uint32_t smem0 = lds_at(smem);
   const uint32_t lda2 = (uint32_t)a.lda * 2, ldb2 = (uint32_t)a.ldb * 2;
   const uint32_t a_step = XA ? 64 * lda2 : 128, b_step = XB ? (GB ? 0 : 64 * ldb2) : 128;
-  auto locate = [&](int item) { return locate_tile<MODE, GATHER, TM, TN>(a, tt, item, mtiles, nti, ntj); };
+  auto locate = [&](int item) __attribute__((always_inline)) { return locate_tile<MODE, GATHER, TM, TN>(a, tt, item, mtiles, nti, ntj); };
 
   // fragment reads: tile i of A 16 WM i + 16 wm + [0, 16), of B 16 NI wn + 16 c (staged by index: pairs interleaved)
   uint32_t a_addr[XA ? MI : 2], b_addr[XB ? NI : 2];
@@ -70,34 +70,34 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM
   // -- the stream of loads --
   u32x4 ra, rb;
   uint32_t sa = 0, sb = 0, avo[LA], bvo[LB];
-  int left = 0, sk = 0, skt = 0, sitem = first, set = 0;   // set: GA the tile's, GB 2 + set its first
+  int left = 0, sk = 0, skt = 0, sround = 0, set = 0;   // set: GA the tile's, GB 2 + set its first
   const int64_t* idx = nullptr;
   // row r of the wavefront's load q of an operand, and the chunk of the row that the lane loads
-  auto row_a = [&](int q) {
+  auto row_a = [&](int q) __attribute__((always_inline)) {
     return XA ? 512 / TM * (LA * wave + q) + lane / (TM / 8) : 8 * (LA * wave + q) + (lane >> 3);
   };
-  auto row_b = [&](int q) {
+  auto row_b = [&](int q) __attribute__((always_inline)) {
     return XB ? 512 / TN * (LB * wave + q) + lane / (TN / 8) : 8 * (LB * wave + q) + (lane >> 3);
   };
-  auto chunk_a = [&](int q) {
+  auto chunk_a = [&](int q) __attribute__((always_inline)) {
     return XA ? (lane % (TM / 8)) ^ swz_across<TM>(row_a(q)) : (lane & 7) ^ swz_direct(row_a(q));
   };
-  auto chunk_b = [&](int q) {
+  auto chunk_b = [&](int q) __attribute__((always_inline)) {
     return XB ? (lane % (TN / 8)) ^ swz_across<TN>(row_b(q)) : (lane & 7) ^ swz_pair(row_b(q));
   };
-  auto tile_rows = [&](const Tile& t, int p) {   // GA: of the wavefront's rows
+  auto tile_rows = [&](const Tile& t, int p) __attribute__((always_inline)) {   // GA: of the wavefront's rows
     const u32x4 r = buffer_at(t.idx, (int64_t)(t.rows < TM ? t.rows : TM) * 8);
     const uint32_t o = lane < 8 * LA ? (uint32_t)(8 * LA * wave + lane) * 8 : kNowhere;
     load_lds4(r, o, lds_at(row_s[p][0]) + 256 * wave);
     load_lds4(r, o == kNowhere ? o : o + 4, lds_at(row_s[p][1]) + 256 * wave);
   };
-  auto stage_rows = [&](const int64_t* at, int n, int p) {   // GB: of the wavefront's rows of BS stages
+  auto stage_rows = [&](const int64_t* at, int n, int p) __attribute__((always_inline)) {   // GB: of the wavefront's rows of BS stages
     const u32x4 r = buffer_at(at, (int64_t)n * 8);
     const uint32_t o = (uint32_t)(lane / RPW * 64 + RPW * wave + lane % RPW) * 8;
     load_lds4(r, o, lds_at(row_s[p][0]) + 256 * wave);
     load_lds4(r, o + 4, lds_at(row_s[p][1]) + 256 * wave);
   };
-  auto begin_tile = [&](const Tile& t) {
+  auto begin_tile = [&](const Tile& t) __attribute__((always_inline)) {
     ra = t.a, rb = t.b, sa = sb = 0, left = t.nc, idx = t.idx, sk = 0;
     skt = t.nc > 64 ? (t.nc + 63) / 64 : 1;
 #pragma unroll
@@ -115,13 +115,13 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM
       for (int q = 0; q < LB; ++q) bvo[q] = (uint32_t)row_b(q) * ldb2 + chunk_b(q) * 16;
     }
     if constexpr (GATHER) {   // the row numbers of the tile after this one
-      const int after = sitem + (int)gridDim.x < total ? sitem + (int)gridDim.x : sitem;
-      const Tile n = locate(after);
+      const int after = rounds.at(sround + 1);
+      const Tile n = locate(after < total ? after : rounds.at(sround));
       if constexpr (GA) tile_rows(n, set ^ 1);
       if constexpr (GB) stage_rows(n.idx, n.nc, 2 + (set ^ 1));
     }
   };
-  auto begin_stage = [&]() {   // before a stage is loaded
+  auto begin_stage = [&]() __attribute__((always_inline)) {   // before a stage is loaded
     if (left <= 0) {   // not there: zeros
       ra[2] = rb[2] = 0;
       sa = sb = 0;
@@ -150,7 +150,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM
       }
     }
   };
-  auto load = [&](auto qq, int slot) {
+  auto load = [&](auto qq, int slot) __attribute__((always_inline)) {
     constexpr int q = decltype(qq)::value;
     const uint32_t dst = smem0 + (uint32_t)(slot * kStage);
     if constexpr (q < LA)
@@ -158,17 +158,17 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM
     else
       load_lds(rb, bvo[q - LA], sb, dst + TM * 128 + 1024 * (LB * wave + q - LA));
   };
-  auto end_stage = [&]() {
+  auto end_stage = [&]() __attribute__((always_inline)) {
     left -= 64;
     sa += a_step;
     sb += b_step;
     if (++sk < skt) return;
     const int kt = skt;
-    sitem += gridDim.x;
-    if (sitem < total) {
+    const int after = rounds.at(++sround);
+    if (after < total) {
       if (GATHER && kt < SST) wait_cnt<0>();   // its row numbers were loaded kt stages ago
       set ^= 1;
-      begin_tile(locate(sitem));
+      begin_tile(locate(after));
     } else {
       left = 0;
       sk = 1;
@@ -177,7 +177,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM
   };
 
   s16x8 t0[MI], w0[NI], t1[MI], w1[NI];
-  auto read = [&](int slot, auto kk, s16x8 (&ft)[MI], s16x8 (&fw)[NI]) {
+  auto read = [&](int slot, auto kk, s16x8 (&ft)[MI], s16x8 (&fw)[NI]) __attribute__((always_inline)) {
     constexpr int KS = decltype(kk)::value;
     const uint32_t st = slot * kStage;
 #pragma unroll
@@ -207,7 +207,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM
   }
   for (int k = 0; k < SST; ++k) {
     begin_stage();
-    static_for<0, LPS>([&](auto q) { load(q, k); });
+    static_for<0, LPS>([&](auto q) __attribute__((always_inline)) { load(q, k); });
     end_stage();
   }
   wait_cnt<(SST - 1) * LPS>();
@@ -217,7 +217,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM
   constexpr int kStores = MI * NI / 2;   // of a wavefront and whole tile
   int early = 0;   // stages whose loads are older than the stores of the tile before
   int bs = 0;
-  for (int item = first; item < total; item += gridDim.x, bs ^= 1) {
+  for (int item = first, round = 0; item < total; item = rounds.at(++round), bs ^= 1) {
     const Tile t = locate(item);
     const int kt = t.nc > 64 ? (t.nc + 63) / 64 : 1;
     const int v = t.rows - 16 * wm;   // 16-row tiles of this wavefront that hold rows
@@ -231,7 +231,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM
     for (int i = 0; i < MI; ++i)
 #pragma unroll
       for (int c = 0; c < NI; ++c) acc[i][c] = f32x4{0, 0, 0, 0};
-    auto mma = [&](int i, const s16x8 (&ft)[MI], const s16x8 (&fw)[NI]) {
+    auto mma = [&](int i, const s16x8 (&ft)[MI], const s16x8 (&fw)[NI]) __attribute__((always_inline)) {
       if (i < nf) {
 #pragma unroll
         for (int c = 0; c < NI; ++c) acc[i][c] = T::mma(fw[c], ft[i], acc[i][c]);
@@ -253,9 +253,9 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM
       wg_barrier();
       read(nxt, I0{}, t0, w0);
       begin_stage();
-      static_for<0, MI>([&](auto ii) {
+      static_for<0, MI>([&](auto ii) __attribute__((always_inline)) {
         constexpr int i = decltype(ii)::value;
-        static_for<i * LPS / MI, (i + 1) * LPS / MI>([&](auto q) { load(q, cur); });
+        static_for<i * LPS / MI, (i + 1) * LPS / MI>([&](auto q) __attribute__((always_inline)) { load(q, cur); });
         mma(i, t1, w1);
       });
       end_stage();
@@ -269,7 +269,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM
     early = t.rows >= TM && t.j0 + TN <= a.J ? SST - 1 : 0;
     const int64_t jc = t.j0 + 16 * NI * wn + (XB ? 16 * (g4 & 1) + 8 * (g4 >> 1) : 8 * g4);
     // the residual is read before the first store, as in tile256
-    auto finish = [&](auto with_res) {
+    auto finish = [&](auto with_res) __attribute__((always_inline)) {
       constexpr bool RES = decltype(with_res)::value;
       u32x4 res[NI / 2][MI] = {};
       if constexpr (RES) {

@@ -18,6 +18,23 @@ struct Tile {
   const int64_t* idx;    // row numbers from the tile's first row (kFwd) or c (kDw) on
 };
 
+// The tiles that a workgroup takes: one of each round of gridDim.x.  Workgroup b runs on XCD b % 8; in a round
+// those of one XCD take a contiguous run.  kDw's groups come by descending rows, whose tiles take as long as
+// these are many, so every other round runs backwards: who had the longest tile of one round gets the shortest
+// of the next.  (65,536 rows of 128 experts by a Zipf law of exponent 1.1, 1,536 x 2,048: in the groups' order
+// 757 us.)
+struct Rounds {
+  int slot, round, total;
+  bool snake;
+  __device__ __forceinline__ Rounds(int total, bool snake) : round(0), total(total), snake(snake) {
+    const int per_xcd = gridDim.x % 8 == 0 ? (int)gridDim.x / 8 : 0;
+    slot = per_xcd ? (int)(blockIdx.x % 8) * per_xcd + (int)(blockIdx.x / 8) : (int)blockIdx.x;
+  }
+  __device__ __forceinline__ int at(int r) const {   // the tile of round r, or one that is not there
+    return r * (int)gridDim.x + (snake && (r & 1) ? (int)gridDim.x - 1 - slot : slot);
+  }
+};
+
 // The tile `item`.  Bands of four row tiles, all columns of a band before the next: what runs at one time on
 // an XCD shares few rows of either operand.  mtiles: of all groups; nti: of a group in kDw.
 template <int MODE, bool GATHER, int TM, int TN>
@@ -27,7 +44,7 @@ __device__ __forceinline__ Tile locate_tile(const Args& a, const Table& tt, int 
   t.s = item % a.splits;
   const int q = item / a.splits;
   int mt, jt, i0;
-  auto banded = [&](int k, int rows) {
+  auto banded = [&](int k, int rows) __attribute__((always_inline)) {
     const int band = k / (4 * ntj), r = k - band * 4 * ntj, h = rows - 4 * band < 4 ? rows - 4 * band : 4;
     jt = r / h;
     mt = 4 * band + r - jt * h;
@@ -37,8 +54,9 @@ __device__ __forceinline__ Tile locate_tile(const Args& a, const Table& tt, int 
     t.g = a.starts ? find_group(tt, mt) : 0;
     i0 = (mt - tt.cum[t.g]) * TM;
   } else {
-    t.g = q / (nti * ntj);
-    banded(q - t.g * nti * ntj, nti);
+    const int rank = q / (nti * ntj);
+    banded(q - rank * nti * ntj, nti);
+    t.g = tt.order[rank];
     i0 = mt * TM;
   }
   t.g = __builtin_amdgcn_readfirstlane(t.g);

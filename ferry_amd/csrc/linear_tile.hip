@@ -83,7 +83,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 
   const uint32_t lda2 = (uint32_t)a.lda * 2, ldb2 = (uint32_t)a.ldb * 2;
   const uint32_t a_step = XA ? 64 * lda2 : 128, b_step = XB ? (GB ? 0 : 64 * ldb2) : 128;
-  auto locate = [&](int item) { return locate_tile<MODE, GATHER, 256, 256>(a, tt, item, mtiles, nti, ntj); };
+  auto locate = [&](int item) __attribute__((always_inline)) { return locate_tile<MODE, GATHER, 256, 256>(a, tt, item, mtiles, nti, ntj); };
 
   // The load stream: the tile whose stages are being loaded.  Staged by index: a wavefront's rows 16 wave +
   // 8 q + lane / 8 of a half, place lane % 8.  By c: its rows 8 wave + 4 q + lane / 16, place lane % 16.
@@ -93,16 +93,16 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   int left = 0;                  // of the contraction, from the stage on
   const int64_t* idx = nullptr;  // GB: row numbers from the stage on
   uint32_t avo[GA ? 2 : 1][2], bvo[2];
-  auto chunk_a = [&](int q) {
+  auto chunk_a = [&](int q) __attribute__((always_inline)) {
     return XA ? (lane & 15) ^ swz_across<128>(8 * wave + 4 * q + (lane >> 4))
               : (lane & 7) ^ swz_direct(16 * wave + 8 * q + (lane >> 3));
   };
-  auto chunk_b = [&](int q) {
+  auto chunk_b = [&](int q) __attribute__((always_inline)) {
     return XB ? (lane & 15) ^ swz_across<128>(8 * wave + 4 * q + (lane >> 4))
               : (lane & 7) ^ swz_pair(16 * wave + 8 * q + (lane >> 3));
   };
   // GA: the row numbers of a tile's `n` rows into set p
-  auto tile_rows = [&](const int64_t* at, int n, int p) {
+  auto tile_rows = [&](const int64_t* at, int n, int p) __attribute__((always_inline)) {
     if (wave < 4) {
       const u32x4 r = buffer_at(at, (int64_t)(n < 256 ? n : 256) * 8);
       const uint32_t o = (uint32_t)(64 * wave + lane) * 8;
@@ -111,14 +111,14 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
   };
   // GB: those of 8 stages, `n` c from `at` on, into set p
-  auto stage8_rows = [&](const int64_t* at, int n, int p) {
+  auto stage8_rows = [&](const int64_t* at, int n, int p) __attribute__((always_inline)) {
     const u32x4 r = buffer_at(at, (int64_t)n * 8);
     const uint32_t o = (uint32_t)((lane >> 3) * 64 + 8 * wave + (lane & 7)) * 8;
     load_lds4(r, o, lds_at(row_s[p][0]) + 256 * wave);
     load_lds4(r, o + 4, lds_at(row_s[p][1]) + 256 * wave);
   };
   // the stream goes on with the tile t; GA: p its set of row numbers
-  auto begin_tile = [&](const Tile& t, int p) {
+  auto begin_tile = [&](const Tile& t, int p) __attribute__((always_inline)) {
     ra = t.a, rb = t.b, sa = sb = 0, left = t.nc, idx = t.idx;
     // a half without rows or columns loads the other's: what it gives is not stored
     a_half = XA ? 256 : (t.rows > 128 ? 128 * lda2 : 0);
@@ -141,7 +141,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
   };
   // before the stage k of the stream's tile is loaded; GB: p the tile's first set is 2 + p
-  auto begin_stage = [&](int k, int p) {
+  auto begin_stage = [&](int k, int p) __attribute__((always_inline)) {
     if (left <= 0) {   // not there: zeros
       ra[2] = rb[2] = 0;
       sa = sb = 0;
@@ -170,24 +170,24 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       }
     }
   };
-  auto end_stage = [&]() {
+  auto end_stage = [&]() __attribute__((always_inline)) {
     left -= 64;
     sa += a_step;
     sb += b_step;
   };
-  auto load_a = [&](int h, int slot) {
+  auto load_a = [&](int h, int slot) __attribute__((always_inline)) {
     const uint32_t dst = smem0 + (uint32_t)((2 * h + slot) * kHalf + 2048 * wave);
 #pragma unroll
     for (int q = 0; q < 2; ++q) load_lds(ra, avo[GA ? h : 0][q], GA || h == 0 ? sa : sa + (left > 0 ? a_half : 0), dst + 1024 * q);
   };
-  auto load_b = [&](int h, int slot) {
+  auto load_b = [&](int h, int slot) __attribute__((always_inline)) {
     const uint32_t dst = smem0 + (uint32_t)((4 + 2 * h + slot) * kHalf + 2048 * wave);
 #pragma unroll
     for (int q = 0; q < 2; ++q) load_lds(rb, bvo[q], h == 0 ? sb : sb + (left > 0 ? b_half : 0), dst + 1024 * q);
   };
 
   s16x8 ft[4][2], fw[2][2][2];
-  auto read_a = [&](auto hh, auto ss) {
+  auto read_a = [&](auto hh, auto ss) __attribute__((always_inline)) {
     constexpr int off = (2 * decltype(hh)::value + decltype(ss)::value) * kHalf;
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks)
@@ -199,7 +199,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
           ft[i][ks] = read_direct(a_addr[ks] + (off + i * 32 * 128));
       }
   };
-  auto read_b = [&](auto hh, auto ss) {
+  auto read_b = [&](auto hh, auto ss) __attribute__((always_inline)) {
     constexpr int H = decltype(hh)::value, off = (2 * H + decltype(ss)::value) * kHalf;
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks)
@@ -212,10 +212,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       }
   };
 
-  // XCD-aware order: workgroup b runs on XCD b % 8; in each round of gridDim tiles those of one XCD take a
-  // contiguous run
-  const int per_xcd = gridDim.x % 8 == 0 ? (int)gridDim.x / 8 : 0;
-  const int first = per_xcd ? (int)(blockIdx.x % 8) * per_xcd + (int)(blockIdx.x / 8) : (int)blockIdx.x;
+  const Rounds rounds(total, !RAG);
+  const int first = rounds.at(0);
   if (first >= total) return;
   typedef std::integral_constant<int, 0> I0;
   typedef std::integral_constant<int, 1> I1;
@@ -247,9 +245,11 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   wg_barrier();
   if (wm == 1) wg_barrier();   // the second group runs one segment behind the first
   int stores = 0;   // at least so many stores of the tile before may be outstanding, behind the loads in flight: 0 or 16
-  for (int item = first; item < total; item += gridDim.x, set ^= 1) {
+  int after;
+  for (int item = first, round = 0;; item = after, ++round, set ^= 1) {
     // the tile after this one; after the last its own first stages are loaded again
-    const int after = item + (int)gridDim.x < total ? item + (int)gridDim.x : item;
+    const bool last = rounds.at(round + 1) >= total;
+    after = last ? item : rounds.at(round + 1);
     if constexpr (GATHER) {
       const Tile t = locate(after);
       if constexpr (GA) tile_rows(t.idx, t.rows, set ^ 1);
@@ -273,7 +273,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
     if (GB && pairs <= 1) wait_cnt<0>();   // the next tile's row numbers are needed at once
 
-    auto pipeline = [&](auto part) {
+    auto pipeline = [&](auto part) __attribute__((always_inline)) {
       constexpr bool PARTIAL = decltype(part)::value;
       f32x4 acc[2][2][4][2];   // [A half][B half][16-row tile][16-column tile]
 #pragma unroll
@@ -284,9 +284,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
           for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int c = 0; c < 2; ++c) acc[ha][hb][i][c] = f32x4{0, 0, 0, 0};
-      auto mma = [&](auto ha, auto hb) {
+      auto mma = [&](auto ha, auto hb) __attribute__((always_inline)) {
         constexpr int A = decltype(ha)::value, B = decltype(hb)::value;
-        auto tile_row = [&](int i, int ks) {
+        auto tile_row = [&](int i, int ks) __attribute__((always_inline)) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) acc[A][B][i][c] = T::mma(fw[B][c][ks], ft[i][ks], acc[A][B][i][c]);
         };
@@ -313,7 +313,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       // The next segment's half has landed, this one's fragments are read.  The first seven halves of a tile
       // were loaded before the stores of the tile before: those may be outstanding too.
       int early = stores ? 7 : 0;
-      auto mem_end = [&]() {
+      auto mem_end = [&]() __attribute__((always_inline)) {
         if (early > 0) {
           --early;
           wait_cnt<28>();
@@ -323,7 +323,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         wg_barrier();
       };
       // a stage in slot S, loading the stage k of the stream into it
-      auto stage = [&](int k, int p, auto ss) {
+      auto stage = [&](int k, int p, auto ss) __attribute__((always_inline)) {
         constexpr int S = decltype(ss)::value;
         typedef std::integral_constant<int, S> IS;
         typedef std::integral_constant<int, 1 - S> IO;
@@ -361,7 +361,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       const int64_t jc = cur.j0 + 32 * wn + (XB ? 16 * (g4 & 1) + 8 * (g4 >> 1) : 8 * g4);
       stores = cur.rows >= 256 && cur.j0 + 256 <= a.J ? 16 : 0;
       // a B half's residual is read before its first store: a wait for it behind that would wait for the store too
-      auto finish = [&](auto with_res) {
+      auto finish = [&](auto with_res) __attribute__((always_inline)) {
         constexpr bool RES = decltype(with_res)::value;
 #pragma unroll
         for (int hb = 0; hb < 2; ++hb) {
@@ -402,6 +402,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       pipeline(std::false_type{});
     else
       pipeline(std::true_type{});
+    if (last) break;
   }
   if (wm == 0) wg_barrier();
   wait_cnt<0>();   // no load may write this workgroup's LDS after its end

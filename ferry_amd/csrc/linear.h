@@ -154,18 +154,19 @@ __device__ __forceinline__ int group_start(const Args& a, int g) { return in_pai
 
 struct Table {
   __attribute__((aligned(16))) int32_t cum[kMaxGroups];   // tiles before the group, 0x7fffffff behind the last
-  int32_t start[kMaxGroups], rows[kMaxGroups];
-  int32_t total, first, last;   // tiles; rows of the grouped order before the first and behind the last group
+  int32_t rows[kMaxGroups];
   uint16_t order[kMaxGroups];   // not RAGGED_I: the groups by descending rows
+  int32_t total, first, last;   // tiles; rows of the grouped order before the first and behind the last group
 };
 
-// The groups' starts, rows and tiles: `rows` rows a tile with RAGGED_I, else `rows` tiles for each group.  By
-// wavefront 0, all loads at once; all others wait.
+// The groups' rows and tiles: `rows` rows a tile with RAGGED_I, else `rows` tiles for each group, whose order is by
+// descending rows.  start (nullable): the groups' first rows.  Loads and sums by wavefront 0, all loads at once.
 template <bool RAGGED_I>
-__device__ __forceinline__ void build_table(const Args& a, Table& t, int rows) {
+__device__ __forceinline__ void build_table(const Args& a, Table& t, int rows, int32_t* start = nullptr) {
   constexpr int Q = kMaxGroups / 64;
+  const int G = a.groups;
   if (threadIdx.x < 64) {
-    const int lane = threadIdx.x, G = a.groups;
+    const int lane = threadIdx.x;
     int64_t lo[Q] = {}, hi[Q] = {};
     int64_t end = a.pairs, begin = 0;
     if (a.starts) {
@@ -181,16 +182,13 @@ __device__ __forceinline__ void build_table(const Args& a, Table& t, int rows) {
     } else {
       hi[0] = a.pairs;
     }
-    int s[Q], n[Q];
-#pragma unroll
-    for (int q = 0; q < Q; ++q) s[q] = in_pairs(a, lo[q]), n[q] = in_pairs(a, hi[q]);
     int sum = 0;
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
       const int g = q * 64 + lane;
       if (q * 64 < G) {
-        n[q] = n[q] > s[q] ? n[q] - s[q] : 0;
-        const int c = g < G ? (RAGGED_I ? (int)(((uint32_t)n[q] + rows - 1) / (uint32_t)rows) : rows) : 0;
+        const int s = in_pairs(a, lo[q]), e = in_pairs(a, hi[q]), n = e > s && g < G ? e - s : 0;
+        const int c = g < G ? (RAGGED_I ? (int)(((uint32_t)n + rows - 1) / (uint32_t)rows) : rows) : 0;
         int incl = c;
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) {
@@ -198,8 +196,8 @@ __device__ __forceinline__ void build_table(const Args& a, Table& t, int rows) {
           if (lane >= off) incl += v;
         }
         t.cum[g] = g < G ? sum + incl - c : 0x7fffffff;
-        t.start[g] = s[q];
-        t.rows[g] = n[q];
+        if (start) start[g] = s;
+        t.rows[g] = n;
         sum += __shfl(incl, 63, 64);
       } else {
         t.cum[g] = 0x7fffffff;
@@ -213,17 +211,17 @@ __device__ __forceinline__ void build_table(const Args& a, Table& t, int rows) {
   }
   __syncthreads();
   if constexpr (!RAGGED_I) {
-    for (int g = threadIdx.x; g < a.groups; g += blockDim.x) {
+    for (int g = threadIdx.x; g < G; g += blockDim.x) {
       const int n = t.rows[g];
       int rank = 0;
-      for (int h = 0; h < a.groups; ++h) rank += t.rows[h] > n || (t.rows[h] == n && h < g);
+      for (int h = 0; h < G; ++h) rank += t.rows[h] > n || (t.rows[h] == n && h < g);
       t.order[rank] = (uint16_t)g;
     }
     __syncthreads();
   }
 }
 
-// the group of tile m: the last g with cum[g] <= m (groups without tiles share their successor's cum)
+// the group of tile m: the last g with cum[g] <= m (groups without tiles share their successor's)
 __device__ __forceinline__ int find_group(const Table& t, int m) {
   const int lane = threadIdx.x & 63;
   int le = 0;

@@ -40,10 +40,11 @@ __global__ __launch_bounds__(256) void any_kernel(Args a) {
   constexpr bool kAcrossA = MODE == kDw, kAcrossB = MODE != kFwd, kRaggedI = MODE != kDw;
   constexpr int kStage = (TI + TJ) * 128, MI = TI / 32, NJ = TJ / 32;
   __shared__ Table tt;
+  __shared__ int32_t first_s[kMaxGroups];
   __shared__ __attribute__((aligned(1024))) char smem[2 * kStage];
   const int ntj = (int)ceil_div(a.J, TJ);
   const int nti = kRaggedI ? 0 : (int)ceil_div(a.I, TI);
-  build_table<kRaggedI>(a, tt, kRaggedI ? TI : nti);
+  build_table<kRaggedI>(a, tt, kRaggedI ? TI : nti, first_s);
   if (a.zero_rest) zero_rest(a, tt.first, tt.last);
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -55,7 +56,7 @@ __global__ __launch_bounds__(256) void any_kernel(Args a) {
     const int64_t t = item / a.splits;
     const int jt = (int)(t % ntj), mt = (int)(t / ntj);
     const int g = a.starts ? find_group(tt, mt) : 0;
-    const int64_t start = tt.start[g], n = tt.rows[g];
+    const int64_t start = first_s[g], n = tt.rows[g];
     const int64_t i0 = (int64_t)(mt - tt.cum[g]) * TI, j0 = (int64_t)jt * TJ;
     const int64_t I = kRaggedI ? n : a.I, C = kRaggedI ? a.C : n;
     const int64_t per = ceil_div(ceil_div(C, a.splits), 64) * 64;
@@ -519,7 +520,7 @@ bool tiles_fit(int op, const Args& a, int64_t pairs, int64_t n, int64_t k) {
     return false;
   const int64_t most = ((int64_t)1 << 31) - (1 << 20);   // elements, with room for a stage behind the end
   const int64_t ia = op == kDw ? pairs : (a.rows ? a.x_rows : 512), ib = op == kFwd ? 512 : (op == kDx ? n : (a.rows ? a.x_rows : pairs));
-  if (a.lda > most / 512 || a.ldb > most / 512 || ia * a.lda > most || ib * a.ldb > most || a.C > most / 4) return false;
+  if (a.J > most / 1024 || a.lda > most / 512 || a.ldb > most / 512 || a.ldo > most / 512 || a.ldr > most / 512 || ia * a.lda > most || ib * a.ldb > most || a.C > most / 4) return false;
   return true;
 }
 

@@ -23,10 +23,11 @@ __global__ __launch_bounds__(64 * WK) void few_kernel(Args a) {
   constexpr int kSlot = 16 * (NB + MT) * 128;
   static_assert(MT * NB * 1024 <= R * kSlot, "the sums of a wavefront fit its ring");
   __shared__ Table tt;
+  __shared__ int32_t first_s[kMaxGroups];
   __shared__ __attribute__((aligned(1024))) char smem[WK * R * kSlot];
   __shared__ __attribute__((aligned(256))) uint32_t row_s[GATHER ? WK : 1][2][GATHER ? 64 : 1];
   if (a.starts) {
-    build_table<true>(a, tt, 16 * MT);
+    build_table<true>(a, tt, 16 * MT, first_s);
     if (a.zero_rest) zero_rest(a, tt.first, tt.last);
   }
   const int ntj = (int)ceil_div(a.J, 16 * NB);
@@ -42,9 +43,9 @@ __global__ __launch_bounds__(64 * WK) void few_kernel(Args a) {
     int g = 0, start = 0, n = (int)a.pairs, m0 = mt * 16 * MT;
     if (a.starts) {
       g = find_group(tt, mt);
-      start = __builtin_amdgcn_readfirstlane(tt.start[g]);
-      n = __builtin_amdgcn_readfirstlane(tt.rows[g]);
       m0 = (mt - __builtin_amdgcn_readfirstlane(tt.cum[g])) * 16 * MT;
+      start = __builtin_amdgcn_readfirstlane(first_s[g]);
+      n = __builtin_amdgcn_readfirstlane(tt.rows[g]);
     }
     const int vr = n - m0 < 16 * MT ? n - m0 : 16 * MT;   // rows, > 0
     const int64_t vj = a.J - j0 < 16 * NB ? a.J - j0 : 16 * NB;

@@ -26,6 +26,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM
   // GB: rows of x of a wavefront and stage, stages whose row numbers 64 lanes load at once
   constexpr int RPW = LB * 512 / TN, BS = 64 / RPW;
   __shared__ Table tt;
+  __shared__ typename Tiles<MODE, GATHER, TM, TN>::Store places;
   __shared__ __attribute__((aligned(1024))) char smem[SST * kStage];
   // row numbers (low and high words), each wavefront its own.  GA: of a tile, two in turn.  GB: of BS stages,
   // sets 0 and 1 in turn, 2 and 3 for the first ones of a tile.
@@ -33,20 +34,16 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM
   __shared__ __attribute__((aligned(256))) uint32_t bias_s[MODE == kFwd ? 2 : 1][MODE == kFwd ? 64 : 1];   // as in tile256
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int ntj = (int)ceil_div(a.J, TN), nti = RAG ? 0 : (int)ceil_div(a.I, TM);
-  build_table<RAG>(a, tt, RAG ? TM : nti);
+  build_table<RAG>(a, tt, RAG ? TM : (int)ceil_div(a.I, TM));
   if (RAG && a.zero_rest) zero_rest(a, tt.first, tt.last);
-  const int mtiles = __builtin_amdgcn_readfirstlane(tt.total);
-  const int total = mtiles * ntj * a.splits;
-  const Rounds rounds(total, !RAG);
-  const int first = rounds.at(0);
-  if (first >= total) return;
+  Tiles<MODE, GATHER, TM, TN> tiles(a, tt, places);   // of the products
+  if (!tiles.next()) return;
+  Tiles<MODE, GATHER, TM, TN> ahead = tiles;          // of the stream of loads
   const int wm = wave / WN, wn = wave % WN;
   const int j16 = lane & 15, g4 = lane >> 4;
   const uint32_t smem0 = lds_at(smem);
   const uint32_t lda2 = (uint32_t)a.lda * 2, ldb2 = (uint32_t)a.ldb * 2;
   const uint32_t a_step = XA ? 64 * lda2 : 128, b_step = XB ? (GB ? 0 : 64 * ldb2) : 128;
-  auto locate = [&](int item) __attribute__((always_inline)) { return locate_tile<MODE, GATHER, TM, TN>(a, tt, item, mtiles, nti, ntj); };
 
   // fragment reads: tile i of A 16 WM i + 16 wm + [0, 16), of B 16 NI wn + 16 c (staged by index: pairs interleaved)
   uint32_t a_addr[XA ? MI : 2], b_addr[XB ? NI : 2];
@@ -70,7 +67,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM
   // -- the stream of loads --
   u32x4 ra, rb;
   uint32_t sa = 0, sb = 0, avo[LA], bvo[LB];
-  int left = 0, sk = 0, skt = 0, sround = 0, set = 0;   // set: GA the tile's, GB 2 + set its first
+  int left = 0, sk = 0, skt = 0, set = 0;   // set: GA the tile's, GB 2 + set its first
   const int64_t* idx = nullptr;
   // row r of the wavefront's load q of an operand, and the chunk of the row that the lane loads
   auto row_a = [&](int q) __attribute__((always_inline)) {
@@ -86,7 +83,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM
     return XB ? (lane % (TN / 8)) ^ swz_across<TN>(row_b(q)) : (lane & 7) ^ swz_pair(row_b(q));
   };
   auto tile_rows = [&](const Tile& t, int p) __attribute__((always_inline)) {   // GA: of the wavefront's rows
-    const u32x4 r = buffer_at(t.idx, (int64_t)(t.rows < TM ? t.rows : TM) * 8);
+    const u32x4 r = buffer_at(a.rows + t.p0, (int64_t)(t.rows < TM ? t.rows : TM) * 8);
     const uint32_t o = lane < 8 * LA ? (uint32_t)(8 * LA * wave + lane) * 8 : kNowhere;
     load_lds4(r, o, lds_at(row_s[p][0]) + 256 * wave);
     load_lds4(r, o == kNowhere ? o : o + 4, lds_at(row_s[p][1]) + 256 * wave);
@@ -98,7 +95,8 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM
     load_lds4(r, o + 4, lds_at(row_s[p][1]) + 256 * wave);
   };
   auto begin_tile = [&](const Tile& t) __attribute__((always_inline)) {
-    ra = t.a, rb = t.b, sa = sb = 0, left = t.nc, idx = t.idx, sk = 0;
+    ra = t.a, rb = t.b, sa = sb = 0, left = t.nc, sk = 0;
+    if constexpr (GB) idx = a.rows + t.p0;
     skt = t.nc > 64 ? (t.nc + 63) / 64 : 1;
 #pragma unroll
     for (int q = 0; q < LA; ++q) {
@@ -115,10 +113,10 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM
       for (int q = 0; q < LB; ++q) bvo[q] = (uint32_t)row_b(q) * ldb2 + chunk_b(q) * 16;
     }
     if constexpr (GATHER) {   // the row numbers of the tile after this one
-      const int after = rounds.at(sround + 1);
-      const Tile n = locate(after < total ? after : rounds.at(sround));
+      Tiles<MODE, GATHER, TM, TN> next = ahead;
+      const Tile n = next.next() ? next.tile() : t;
       if constexpr (GA) tile_rows(n, set ^ 1);
-      if constexpr (GB) stage_rows(n.idx, n.nc, 2 + (set ^ 1));
+      if constexpr (GB) stage_rows(a.rows + n.p0, n.nc, 2 + (set ^ 1));
     }
   };
   auto begin_stage = [&]() __attribute__((always_inline)) {   // before a stage is loaded
@@ -164,11 +162,10 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM
     sb += b_step;
     if (++sk < skt) return;
     const int kt = skt;
-    const int after = rounds.at(++sround);
-    if (after < total) {
+    if (ahead.next()) {
       if (GATHER && kt < SST) wait_cnt<0>();   // its row numbers were loaded kt stages ago
       set ^= 1;
-      begin_tile(locate(after));
+      begin_tile(ahead.tile());
     } else {
       left = 0;
       sk = 1;
@@ -199,9 +196,9 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM
   typedef std::integral_constant<int, 1> I1;
 
   {
-    const Tile t = locate(first);
+    const Tile t = tiles.tile();
     if constexpr (GA) tile_rows(t, 0);
-    if constexpr (GB) stage_rows(t.idx, t.nc, 2);
+    if constexpr (GB) stage_rows(a.rows + t.p0, t.nc, 2);
     if (GATHER) wait_cnt<0>();
     begin_tile(t);
   }
@@ -217,8 +214,8 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM
   constexpr int kStores = MI * NI / 2;   // of a wavefront and whole tile
   int early = 0;   // stages whose loads are older than the stores of the tile before
   int bs = 0;
-  for (int item = first, round = 0; item < total; item = rounds.at(++round), bs ^= 1) {
-    const Tile t = locate(item);
+  for (bool more = true; more; more = tiles.next(), bs ^= 1) {
+    const Tile t = tiles.tile();
     const int kt = t.nc > 64 ? (t.nc + 63) / 64 : 1;
     const int v = t.rows - 16 * wm;   // 16-row tiles of this wavefront that hold rows
     const int nf = __builtin_amdgcn_readfirstlane(v <= 0 ? 0 : ((v + 16 * WM - 1) / (16 * WM) < MI ? (v + 16 * WM - 1) / (16 * WM) : MI));
@@ -265,9 +262,9 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM
       wait_cnt<0>();
       wg_barrier();
     }
-    uint16_t* const out = a.out + (MODE == kDw ? t.g * a.o_group : 0);
-    early = t.rows >= TM && t.j0 + TN <= a.J ? SST - 1 : 0;
-    const int64_t jc = t.j0 + 16 * NI * wn + (XB ? 16 * (g4 & 1) + 8 * (g4 >> 1) : 8 * g4);
+    const Output<T, MODE, TM, TN> o(a, t);
+    early = SST - 1;
+    const int cols = (int)a.J - t.j0, ecol = 16 * NI * wn + (XB ? 16 * (g4 & 1) + 8 * (g4 >> 1) : 8 * g4);
     // the residual is read before the first store, as in tile256
     auto finish = [&](auto with_res) __attribute__((always_inline)) {
       constexpr bool RES = decltype(with_res)::value;
@@ -276,26 +273,22 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM
 #pragma unroll
         for (int cc = 0; cc < NI / 2; ++cc)
 #pragma unroll
-          for (int i = 0; i < MI; ++i) {
-            const int r = 16 * WM * i + 16 * wm + j16;
-            if (r < t.rows && jc + 32 * cc < a.J)
-              res[cc][i] = *reinterpret_cast<const u32x4*>(a.residual + (t.row0 + r) * a.ldr + jc + 32 * cc);
-          }
+          for (int i = 0; i < MI; ++i)
+            res[cc][i] = o.residual(ecol + 32 * cc < cols ? (16 * WM * i + 16 * wm + j16) * o.ldr + (ecol + 32 * cc) * 2 : kNowhere);
         wait_loads();
       }
 #pragma unroll
       for (int cc = 0; cc < NI / 2; ++cc) {
-        const int64_t j = jc + 32 * cc;
-        const int rows_in = j < a.J ? t.rows : 0;   // (all lanes take part in the exchange below)
+        const int j = ecol + 32 * cc;
         u32x4 bias = {0, 0, 0, 0};
         if constexpr (MODE == kFwd)
-          bias = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(bias_s[bs]) + (j - t.j0) * 2);
+          bias = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(bias_s[bs]) + j * 2);
 #pragma unroll
         for (int i = 0; i < MI; ++i) {
-          const int r = 16 * WM * i + 16 * wm + j16;
+          const uint32_t r = (uint32_t)(16 * WM * i + 16 * wm + j16);
           float v8[8];
           columns8<XB>(acc[i][2 * cc], acc[i][2 * cc + 1], v8);
-          if (r < rows_in) store8<T, MODE, MODE == kFwd && !GATHER ? -1 : (int)kNone>(a, t, out, r, j, v8, bias, res[cc][i]);
+          o.template store<MODE == kFwd && !GATHER ? -1 : (int)kNone>(r * o.ldo, r * o.ldp, j, j < cols, v8, bias, res[cc][i]);
         }
       }
     };

@@ -44,6 +44,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   constexpr bool XA = MODE == kDw, XB = MODE != kFwd, RAG = MODE != kDw;
   constexpr bool GA = GATHER && MODE == kFwd, GB = GATHER && MODE == kDw;
   __shared__ Table tt;
+  __shared__ typename Tiles<MODE, GATHER, 256, 256>::Store places;
   __shared__ __attribute__((aligned(1024))) char smem[8 * kHalf];
   // GA: the rows of x of a tile's rows, two tiles in turn.  GB: those of 8 stages, each wavefront its own 8
   // rows of a stage: sets 0 and 1 in turn, 2 and 3 for the first 8 stages of a tile.  Low and high words.
@@ -51,11 +52,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   __shared__ __attribute__((aligned(256))) uint32_t bias_s[MODE == kFwd ? 2 : 1][MODE == kFwd ? 128 : 1];   // of the tile's columns, in turn
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int ntj = (int)ceil_div(a.J, 256), nti = RAG ? 0 : (int)ceil_div(a.I, 256);
-  build_table<RAG>(a, tt, RAG ? 256 : nti);
+  build_table<RAG>(a, tt, RAG ? 256 : (int)ceil_div(a.I, 256));
   if (RAG && a.zero_rest) zero_rest(a, tt.first, tt.last);
-  const int mtiles = __builtin_amdgcn_readfirstlane(tt.total);
-  const int total = mtiles * ntj * a.splits;
+  Tiles<MODE, GATHER, 256, 256> tiles(a, tt, places);
+  if (!tiles.next()) return;
   const int wm = wave >> 2, wn = wave & 3;
   const int j16 = lane & 15, g4 = lane >> 4;
   const uint32_t smem0 = lds_at(smem);
@@ -83,7 +83,6 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 
   const uint32_t lda2 = (uint32_t)a.lda * 2, ldb2 = (uint32_t)a.ldb * 2;
   const uint32_t a_step = XA ? 64 * lda2 : 128, b_step = XB ? (GB ? 0 : 64 * ldb2) : 128;
-  auto locate = [&](int item) __attribute__((always_inline)) { return locate_tile<MODE, GATHER, 256, 256>(a, tt, item, mtiles, nti, ntj); };
 
   // The load stream: the tile whose stages are being loaded.  Staged by index: a wavefront's rows 16 wave +
   // 8 q + lane / 8 of a half, place lane % 8.  By c: its rows 8 wave + 4 q + lane / 16, place lane % 16.
@@ -119,7 +118,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   };
   // the stream goes on with the tile t; GA: p its set of row numbers
   auto begin_tile = [&](const Tile& t, int p) __attribute__((always_inline)) {
-    ra = t.a, rb = t.b, sa = sb = 0, left = t.nc, idx = t.idx;
+    ra = t.a, rb = t.b, sa = sb = 0, left = t.nc;
+    if constexpr (GB) idx = a.rows + t.p0;
     // a half without rows or columns loads the other's: what it gives is not stored
     a_half = XA ? 256 : (t.rows > 128 ? 128 * lda2 : 0);
     b_half = XB ? 256 : (a.J - t.j0 > 128 ? 128 * ldb2 : 0);
@@ -212,17 +212,14 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       }
   };
 
-  const Rounds rounds(total, !RAG);
-  const int first = rounds.at(0);
-  if (first >= total) return;
   typedef std::integral_constant<int, 0> I0;
   typedef std::integral_constant<int, 1> I1;
 
   int set = 0;   // GA: the set of the tile's row numbers; GB: its first set is 2 + set
   {
-    const Tile t = locate(first);
-    if constexpr (GA) tile_rows(t.idx, t.rows, 0);
-    if constexpr (GB) stage8_rows(t.idx, t.nc, 2);
+    const Tile t = tiles.tile();
+    if constexpr (GA) tile_rows(a.rows + t.p0, t.rows, 0);
+    if constexpr (GB) stage8_rows(a.rows + t.p0, t.nc, 2);
     if (GATHER) {
       wait_cnt<0>();
       wg_barrier();
@@ -244,20 +241,11 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   wait_cnt<12>();   // every wavefront has read B half 0 of stage 0 before stage 2's replaces it
   wg_barrier();
   if (wm == 1) wg_barrier();   // the second group runs one segment behind the first
-  int stores = 0;   // at least so many stores of the tile before may be outstanding, behind the loads in flight: 0 or 16
-  int after;
-  for (int item = first, round = 0;; item = after, ++round, set ^= 1) {
-    // the tile after this one; after the last its own first stages are loaded again
-    const bool last = rounds.at(round + 1) >= total;
-    after = last ? item : rounds.at(round + 1);
-    if constexpr (GATHER) {
-      const Tile t = locate(after);
-      if constexpr (GA) tile_rows(t.idx, t.rows, set ^ 1);
-      if constexpr (GB) stage8_rows(t.idx, t.nc, 2 + (set ^ 1));
-    }
+  int stores = 0;   // so many stores of the tile before, or more, lie behind the loads in flight: 0 or 16
+  for (;; set ^= 1) {
     int nf[2], pairs, rows;
     {
-      const Tile t = locate(item);
+      const Tile t = tiles.tile();
       rows = t.rows;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {   // 16-row tiles of each A half that hold rows
@@ -270,6 +258,15 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         const u32x4 r = buffer_at(a.bias + t.g * a.bias_group + j, a.bias && a.splits == 1 && j < a.J ? (a.J - j) * 2 : 0);
         load_lds4(r, lane * 4, lds_at(bias_s[set]) + 256 * wave);
       }
+    }
+    // the tile after this one; after the last its own first stages are loaded again
+    const int here = tiles.at;
+    const bool last = !tiles.next();
+    if (last) tiles.at = here;
+    if constexpr (GATHER) {
+      const Tile t = tiles.tile();
+      if constexpr (GA) tile_rows(a.rows + t.p0, t.rows, set ^ 1);
+      if constexpr (GB) stage8_rows(a.rows + t.p0, t.nc, 2 + (set ^ 1));
     }
     if (GB && pairs <= 1) wait_cnt<0>();   // the next tile's row numbers are needed at once
 
@@ -350,46 +347,45 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         stage(2 * k, set, I0{});
         stage(2 * k + 1, set, I1{});
       }
-      begin_tile(locate(after), set ^ 1);   // the last two stages load the next tile's first two
+      begin_tile(tiles.tile(), set ^ 1);   // the last two stages load the next tile's first two
       stage(0, set ^ 1, I0{});
       stage(1, set ^ 1, I1{});
 
-      const Tile cur = locate(item);
-      int erow = 16 * wm + j16;
-      asm volatile("" : "+v"(erow));   // the stores' addresses are computed here, not kept through the loop
-      uint16_t* const out = a.out + (MODE == kDw ? cur.g * a.o_group : 0);
-      const int64_t jc = cur.j0 + 32 * wn + (XB ? 16 * (g4 & 1) + 8 * (g4 >> 1) : 8 * g4);
-      stores = cur.rows >= 256 && cur.j0 + 256 <= a.J ? 16 : 0;
+      const int then = tiles.at;
+      tiles.at = here;
+      const Tile cur = tiles.tile();
+      tiles.at = then;
+      const Output<T, MODE, 256, 256> o(a, cur);
+      stores = 16;
+      int erow = 16 * wm + j16, ecol = 32 * wn + (XB ? 16 * (g4 & 1) + 8 * (g4 >> 1) : 8 * g4);
+      asm volatile("" : "+v"(erow), "+v"(ecol));   // the stores' offsets are computed here, not kept through the loop
+      const int cols = (int)a.J - cur.j0;
       // a B half's residual is read before its first store: a wait for it behind that would wait for the store too
       auto finish = [&](auto with_res) __attribute__((always_inline)) {
         constexpr bool RES = decltype(with_res)::value;
 #pragma unroll
         for (int hb = 0; hb < 2; ++hb) {
-          const int64_t j = jc + 128 * hb;
-          const int rows_in = j < a.J ? cur.rows : 0;   // (all lanes take part in the exchange below)
+          const int j = ecol + 128 * hb;
           u32x4 res[2][4] = {};
           if constexpr (RES) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int r = 128 * h + 32 * i + erow;
-                if (r < rows_in) res[h][i] = *reinterpret_cast<const u32x4*>(a.residual + (cur.row0 + r) * a.ldr + j);
-              }
+              for (int i = 0; i < 4; ++i) res[h][i] = o.residual(j < cols ? (erow + 128 * h + 32 * i) * o.ldr + j * 2 : kNowhere);
             wait_loads();
           }
           u32x4 bias = {0, 0, 0, 0};
           if constexpr (MODE == kFwd)
-            bias = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(bias_s[set]) + (j - cur.j0) * 2);
+            bias = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(bias_s[set]) + j * 2);
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               __builtin_amdgcn_sched_barrier(0);   // one row at a time: registers
-              const int r = 128 * h + 32 * i + erow;
+              const uint32_t r = (uint32_t)(erow + 128 * h + 32 * i);
               float v[8];
               columns8<XB>(acc[h][hb][i][0], acc[h][hb][i][1], v);
-              if (r < rows_in) store8<T, MODE, ACT>(a, cur, out, r, j, v, bias, res[h][i]);
+              o.template store<ACT>(r * o.ldo, r * o.ldp, j, j < cols, v, bias, res[h][i]);
             }
         }
       };

@@ -31,8 +31,8 @@ __device__ __forceinline__ u32x4 load8(const uint16_t* p, int n) {
   return v;
 }
 
-// TI x TJ outputs per workgroup of four wavefronts, 64 of the contraction a step through registers into
-// one of two LDS buffers, the loads of a step issued before the products of the one before.  Loads are
+// TI x TJ outputs per workgroup of four wavefronts, 64 of the contraction a step through registers into one of two
+// LDS buffers, the loads of a step issued two steps before its products: bound by their latency.  Loads are
 // 16 bytes at any alignment; what lies outside the matrices, the group or the contraction is 0 in LDS, so
 // that nothing a neighbouring row holds, a NaN included, enters a sum.
 template <typename T, int MODE, int TI, int TJ>
@@ -85,22 +85,26 @@ __global__ __launch_bounds__(256) void any_kernel(Args a) {
         pb[q] = j < a.J ? bw + j * a.ldb + (tid & 7) * 8 : nullptr;
       }
     }
-    u32x4 va[MI], vb[NJ];
-    auto load = [&](int64_t c) {
+    // registers of two steps in turn: a step's loads have two steps of products to arrive
+    struct Regs {
+      u32x4 a[MI], b[NJ];
+    };
+    Regs r0, r1;
+    auto load = [&](int64_t c, Regs& v) __attribute__((always_inline)) {
 #pragma unroll
       for (int q = 0; q < MI; ++q) {
         if constexpr (!kAcrossA) {
-          va[q] = load8(pa[q] + c, pa[q] ? (int)(c1 - c < 64 ? c1 - c : 64) - (tid & 7) * 8 : 0);
+          v.a[q] = load8(pa[q] + c, pa[q] ? (int)(c1 - c < 64 ? c1 - c : 64) - (tid & 7) * 8 : 0);
         } else {
           constexpr int per_row = TI / 8;
           const int64_t cc = c + tid / per_row + (256 / per_row) * q, i = i0 + (tid % per_row) * 8;
-          va[q] = load8(a.a + (start + cc) * a.lda + i, cc < c1 ? (int)(I - i < 8 ? I - i : 8) : 0);
+          v.a[q] = load8(a.a + (start + cc) * a.lda + i, cc < c1 ? (int)(I - i < 8 ? I - i : 8) : 0);
         }
       }
 #pragma unroll
       for (int q = 0; q < NJ; ++q) {
         if constexpr (!kAcrossB) {
-          vb[q] = load8(pb[q] + c, pb[q] ? (int)(c1 - c < 64 ? c1 - c : 64) - (tid & 7) * 8 : 0);
+          v.b[q] = load8(pb[q] + c, pb[q] ? (int)(c1 - c < 64 ? c1 - c : 64) - (tid & 7) * 8 : 0);
         } else {
           constexpr int per_row = TJ / 8;
           const int64_t cc = c + tid / per_row + (256 / per_row) * q, j = j0 + (tid % per_row) * 8;
@@ -113,25 +117,25 @@ __global__ __launch_bounds__(256) void any_kernel(Args a) {
               ok = (uint64_t)r < (uint64_t)a.x_rows;
             }
           }
-          vb[q] = load8(bw + (ok ? r * a.ldb : 0) + j, ok ? (int)(a.J - j < 8 ? a.J - j : 8) : 0);
+          v.b[q] = load8(bw + (ok ? r * a.ldb : 0) + j, ok ? (int)(a.J - j < 8 ? a.J - j : 8) : 0);
         }
       }
     };
-    auto store = [&](int buf) {
+    auto store = [&](int buf, const Regs& v) __attribute__((always_inline)) {
       char* const st = smem + buf * kStage;
 #pragma unroll
       for (int q = 0; q < MI; ++q) {
         constexpr int per_row = kAcrossA ? TI / 8 : 8;
         const int r = tid / per_row + (256 / per_row) * q, k = tid % per_row;
         const int at = kAcrossA ? r * TI * 2 + ((k ^ swz_across<TI>(r)) << 4) : r * 128 + ((k ^ swz_direct(r)) << 4);
-        *reinterpret_cast<u32x4*>(st + at) = va[q];
+        *reinterpret_cast<u32x4*>(st + at) = v.a[q];
       }
 #pragma unroll
       for (int q = 0; q < NJ; ++q) {
         constexpr int per_row = kAcrossB ? TJ / 8 : 8;
         const int r = tid / per_row + (256 / per_row) * q, k = tid % per_row;
         const int at = kAcrossB ? r * TJ * 2 + ((k ^ swz_across<TJ>(r)) << 4) : r * 128 + ((k ^ swz_direct(r)) << 4);
-        *reinterpret_cast<u32x4*>(st + TI * 128 + at) = vb[q];
+        *reinterpret_cast<u32x4*>(st + TI * 128 + at) = v.b[q];
       }
     };
     f32x4 acc[MI][NJ];
@@ -140,13 +144,7 @@ __global__ __launch_bounds__(256) void any_kernel(Args a) {
 #pragma unroll
       for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
     __syncthreads();   // the tile before has read its last buffer
-    load(c0);
-    store(0);
-    int buf = 0;
-    for (int64_t c = c0; c < c1; c += 64, buf ^= 1) {
-      const bool more = c + 64 < c1;
-      if (more) load(c + 64);
-      __syncthreads();
+    auto products = [&](int buf) __attribute__((always_inline)) {
       const uint32_t la = lds0 + buf * kStage, lb = la + TI * 128;
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
@@ -164,7 +162,20 @@ __global__ __launch_bounds__(256) void any_kernel(Args a) {
 #pragma unroll
           for (int j = 0; j < NJ; ++j) acc[i][j] = T::mma(fb[j], fa[i], acc[i][j]);
       }
-      if (more) store(buf ^ 1);
+    };
+    // the step of c, which lies in buffer buf; v: free, w: the next step's
+    auto step = [&](int64_t c, int buf, Regs& v, const Regs& w) __attribute__((always_inline)) {
+      if (c + 128 < c1) load(c + 128, v);
+      __syncthreads();
+      products(buf);
+      if (c + 64 < c1) store(buf ^ 1, w);
+    };
+    load(c0, r0);
+    if (c0 + 64 < c1) load(c0 + 64, r1);
+    store(0, r0);
+    for (int64_t c = c0; c < c1; c += 128) {
+      step(c, 0, r0, r1);
+      if (c + 64 < c1) step(c + 64, 1, r1, r0);
     }
     // lane l holds columns 4 (l / 16) + [0, 4) of row l % 16 of each 16 x 16 tile
 #pragma unroll
@@ -436,7 +447,7 @@ constexpr double kLaunch = 3.5;    // us until the first products of a launch, a
 constexpr double kMemory = 4.8e6;  // bytes a us
 
 // op: the product; rows: pairs
-Plan plan(int op, int64_t pairs, int64_t n, int64_t k, int64_t groups) {
+Plan make_plan(int op, int64_t pairs, int64_t n, int64_t k, int64_t groups, int64_t cu) {
   Plan p = {};
   const int64_t J = op == kFwd ? n : k, used = std::min(groups, std::max<int64_t>(pairs, 1));
   auto row_tiles = [&](int64_t t) { return ceil_div(pairs, t) + (groups > 1 ? used : 0); };
@@ -453,7 +464,6 @@ Plan plan(int op, int64_t pairs, int64_t n, int64_t k, int64_t groups) {
   // The cheapest kernel, tile and number of parts: whole rounds of tiles over the CUs (of groups of unknown sizes, as
   // many tiles as equal ones and half a tile of each group), no faster than the operands come from memory, the
   // parts' way through memory, and for groups half a tile's time until the last is done.
-  const int64_t cu = cus();
   const double rows = (double)pairs / used, out = (double)(op == kDw ? groups * n * k : pairs * J);
   const double bytes = 2.0 * (op == kDw ? (double)pairs * (n + k) + out : (double)pairs * (n + k) + (double)used * n * k);
   auto m_tiles = [&](int tm) {
@@ -499,6 +509,24 @@ Plan plan(int op, int64_t pairs, int64_t n, int64_t k, int64_t groups) {
     }
   p.tiles = p.kind == kFew ? row_tiles(16 * p.mt) : tiles(kShapes[p.shape].tm, kShapes[p.shape].tn);
   return p;
+}
+
+// make_plan for the current device; a thread keeps its latest plans, by the sizes they depend on
+Plan plan(int op, int64_t pairs, int64_t n, int64_t k, int64_t groups) {
+  struct Kept {
+    int64_t key[6];
+    Plan plan;
+  };
+  static thread_local Kept kept[16];
+  const int64_t key[6] = {op + 1, pairs, n, k, groups, cus()};
+  uint64_t h = 0;
+  for (int64_t v : key) h = (h ^ (uint64_t)v) * 0x9e3779b97f4a7c15ull;
+  Kept& e = kept[h >> 60];
+  if (!std::equal(key, key + 6, e.key)) {
+    e.plan = make_plan(op, pairs, n, k, groups, key[5]);
+    std::copy(key, key + 6, e.key);
+  }
+  return e.plan;
 }
 
 bool even(const void* q, int64_t stride) { return (uintptr_t)q % 16 == 0 && stride % 8 == 0; }

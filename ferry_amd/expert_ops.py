@@ -7,6 +7,7 @@ so that call sites written against the reference work unchanged; the fused hot-p
 points (router_topk, layout, expert_ffn, combine, history_update) are exposed next to them.
 All tensors are CUDA (HIP) tensors; every op runs on the current stream.
 """
+import functools
 import math
 from operator import add, attrgetter
 
@@ -508,6 +509,9 @@ _HALF = {torch.bfloat16: 0, torch.float16: 2}                                 # 
 
 def _half_rows(t, name, device=None, dtype=None):
     """(address, row stride) of the rows of a bf16 or fp16 tensor, on ``device`` and of ``dtype`` if given."""
+    if (dtype is not None and isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == device
+            and t.is_contiguous() and t.dim()):   # the usual case (the checks below take 1 us longer)
+        return t.data_ptr(), t.shape[-1]
     stride = _row_stride(t, name)
     if dtype is None:
         if t.dtype not in _HALF:
@@ -532,9 +536,15 @@ def _weight_groups(w, name, device, dtype):
     return w.data_ptr(), row if n > 1 else k, group
 
 
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(product, pairs, n, k, groups, device):
+    with torch.cuda.device(device):
+        return lib().ferry_linear_workspace_bytes(product, pairs, n, k, groups)
+
+
 def _workspace(product, pairs, n, k, groups, device):
     """(tensor or None, address, bytes) of a linear product's scratch memory."""
-    need = lib().ferry_linear_workspace_bytes(product, pairs, n, k, groups)
+    need = _workspace_bytes(product, pairs, n, k, groups, device)
     if need <= 0:
         return None, None, 0
     ws = torch.empty(need, dtype=torch.uint8, device=device)

@@ -656,7 +656,7 @@ extern "C" int ferry_expert_linear(const void* x, int32_t dtype, int64_t x_rows,
                       bias_stride >= 0 && (!residual || residual_stride >= 0),
                   "strides must reach over their rows");
   if (pairs == 0) return 0;
-  FERRY_CHECK_ARG(x && w && out, "null pointer argument");
+  FERRY_CHECK_ARG((x || x_rows == 0) && w && out, "null pointer argument");
   Args a = {};
   a.a = (const uint16_t*)x, a.lda = x_stride;
   a.b = (const uint16_t*)w, a.ldb = w_stride, a.b_group = w_group_stride;
@@ -736,7 +736,7 @@ extern "C" int ferry_expert_linear_grad_w(const void* dz, int32_t dtype, int64_t
   if (int rc = check_sizes(dtype, pairs, n, k, groups, starts)) return rc;
   FERRY_CHECK_ARG(x_rows >= 0 && (rows || x_rows >= pairs), "x must have a row for every row of the gradient");
   FERRY_CHECK_ARG((dz_stride >= n || pairs <= 1) && (x_stride >= k || x_rows <= 1), "strides must reach over their rows");
-  FERRY_CHECK_ARG(dw && (pairs == 0 || (dz && x)), "null pointer argument");
+  FERRY_CHECK_ARG(dw && (pairs == 0 || (dz && (x || x_rows == 0))), "null pointer argument");
   Args a = {};
   a.a = (const uint16_t*)dz, a.lda = dz_stride;
   a.b = (const uint16_t*)x, a.ldb = x_stride;

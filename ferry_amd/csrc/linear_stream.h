@@ -183,8 +183,8 @@ __device__ __forceinline__ void columns8(const f32x4& t0, const f32x4& t1, float
 }
 
 // dw is stored past the caches (non-temporal), whose lines the operands keep: a training step of 3,000 rows of 64
-// experts, 2,048 x 1,408, 318 -> 300 us, of 65,536 rows of 128 experts and of one dense layer the same time.  y and dx,
-// whose readers come at once, are not: 65,536 rows of 128 experts then took 1,755 us instead of 1,610.
+// experts, 2,048 x 1,408, 318 -> 300 us; of 65,536 rows of 128 experts and of one dense layer the same time.  y and dx,
+// whose readers come at once, are not: they gain or lose 1 %.
 constexpr int kPast = 2;
 
 // The epilogue of a tile: eight consecutive columns of a row at a time, through buffers that begin at the tile's

@@ -584,6 +584,8 @@ def _linear(x, weight, bias, activation, residual, out, keep):
         raise RuntimeError('weight must be [n, k] for x [..., k]')
     w, ws = _half_rows(weight, 'weight', dev, dtype)
     n, k = weight.shape
+    if not n or not k:
+        raise RuntimeError('n and k must be at least 1')
     *lead, _ = x.shape
     m = math.prod(lead)
     shape = (*lead, n)
@@ -617,7 +619,7 @@ def linear(x, weight, bias=None, activation=None, residual=None, out=None, retur
     ``x`` [..., k], ``weight`` [n, k] (a matrix may have a row stride), ``bias`` [n] and ``residual``
     [..., n] are bf16 or fp16, all the same; sums are fp32.  ``activation`` is None, 'relu', 'silu', 'gelu'
     (the normal distribution's) or 'gelu_tanh'.  ``out`` (optional) receives the result and may be
-    ``residual`` itself.  ``return_pre=True`` returns (result, the activation's rounded argument [rows, n],
+    ``residual`` itself, but share no memory with the other arguments.  ``return_pre=True`` returns (result, the activation's rounded argument [rows, n],
     or None without an activation), what ``linear_grad`` needs.  Rows that start at multiples of 16 bytes
     are fastest; any other alignment is taken.
 
@@ -671,6 +673,8 @@ def linear_grad(grad, x, weight, pre=None, activation=None, need_x=True, need_we
         raise RuntimeError('weight must be [n, k] for x [..., k]')
     w, ws = _half_rows(weight, 'weight', dev, dtype)
     n, k = weight.shape
+    if not n or not k:
+        raise RuntimeError('n and k must be at least 1')
     *lead, _ = x.shape
     m = math.prod(lead)
     _, gs = _half_rows(grad, 'grad', dev, dtype)
@@ -725,6 +729,8 @@ def _expert_args(x, weight, starts, rows):
     dtype, dev = x.dtype, x.get_device()
     if x.dim() != 2 or not isinstance(weight, torch.Tensor) or weight.dim() != 3 or weight.shape[2] != x.shape[1]:
         raise RuntimeError('x must be [rows, k] and weight [experts, n, k]')
+    if not weight.shape[0] or not weight.shape[1] or not weight.shape[2]:
+        raise RuntimeError('experts, n and k must be at least 1')
     w, ws, wg = _weight_groups(weight, 'weight', dev, dtype)
     first = _at(starts, 'starts', torch.int64, dev)
     if starts.shape != (weight.shape[0] + 1,):

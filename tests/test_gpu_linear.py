@@ -441,6 +441,95 @@ def test_starts_and_rows_out_of_range():
                        ops().expert_linear_grad(dy, zeroed, w, tame)[1])
 
 
+@pytest.mark.parametrize('counts,n,k', [([40, 3], 512, 320), ([300, 0, 513, 40], 1032, 264), ([700, 400, 900], 2048, 200),
+                                        ([2, 1, 0, 5], 72, 1000), ([600, 500], 35, 141)])
+def test_bad_rows_in_every_kernel(counts, n, k):
+    """Entries of rows that name no row of x, their high words set among them, read as zeros, at the sizes of each
+    kernel; NaN in the row they would name otherwise."""
+    P = sum(counts)
+    starts = groups_of(counts)
+    x, w, dy = normal(P, k, seed=1), normal(len(counts), n, k, seed=2, scale=k ** -0.5), normal(P, n, seed=3)
+    rows = torch.randperm(P, device='cuda')
+    bad = rows.clone()
+    at = [0, P // 2, P - 1]
+    bad[at] = torch.tensor([-1, P, (1 << 32) + 1], device='cuda')
+    zeroed = x[rows]
+    zeroed[at] = 0
+    want = expert_reference(zeroed, w, starts, dy=dy)
+    close(ops().expert_linear(x, w, starts, rows=bad), *want['y'], 'y')
+    close(ops().expert_linear_grad(dy, x, w, starts, rows=bad)[1], *want['dw'], 'dw')
+
+
+@pytest.mark.parametrize('n,k', [(512, 256), (40, 72), (33, 65)])
+def test_experts_without_rows(n, k):
+    """No expert has a row, or x has none: zeros, and nothing of what is there."""
+    x, w = torch.full((300, k), math.nan, dtype=BF16, device='cuda'), normal(5, n, k, seed=1)
+    starts = torch.zeros(6, dtype=torch.int64, device='cuda')
+    assert not ops().expert_linear(x, w, starts).any()
+    dy = torch.full((300, n), math.inf, dtype=BF16, device='cuda')
+    for g in ops().expert_linear_grad(dy, x, w, starts):
+        assert not g.any()
+    y = ops().expert_linear(x[:0], w, starts)
+    assert y.shape == (0, n)
+    dx, dw, db = ops().expert_linear_grad(y, x[:0], w, starts)
+    assert dx.shape == (0, k) and not dw.any() and not db.any()
+    rows = torch.zeros(7, dtype=torch.int64, device='cuda')   # rows of an x without any
+    spread = torch.tensor([0, 7, 7, 7, 7, 7], device='cuda')
+    assert not ops().expert_linear(x[:0], w, spread, rows=rows).any()
+    assert not ops().expert_linear_grad(normal(7, n, seed=2), x[:0], w, spread, rows=rows)[1].any()
+
+
+@pytest.mark.parametrize('m', [3, 300, 2100])
+def test_unaligned_bias_residual_and_pre(m):
+    """A bias, a residual and an output that start at any element, on operands that do not."""
+    n, k = 520, 264
+    x, w = normal(m, k, seed=1), normal(n, k, seed=2, scale=k ** -0.5)
+    bias, res = normal(n + 1, seed=3)[1:], normal(m * n + 3, seed=4)[3:].view(m, n)
+    y, b, _, _ = layer(x, w, bias, 'gelu', res)
+    close(ops().linear(x, w, bias, 'gelu', res), y, b, 'y')
+    close(ops().linear(x, w, bias, 'gelu', res.clone(), out=res), y, b, 'out')
+
+
+def test_one_row_of_any_stride_and_single_columns():
+    x, w = normal(1, 64, seed=1), normal(48, 64, seed=2)
+    assert torch.equal(ops().linear(x.as_strided((1, 64), (7, 1)), w), ops().linear(x, w))
+    y, b, z, zb = layer(x[:, :1], w[:, :1])
+    close(ops().linear(x[:, :1], w[:, :1]), y, b, 'k = 1')
+    y, b, _, _ = layer(normal(50, 64, seed=3), w[:1])
+    close(ops().linear(normal(50, 64, seed=3), w[:1]), y, b, 'n = 1')
+    for bad in ((x[:, :0], w[:, :0]), (x, w[:0])):
+        with pytest.raises(RuntimeError, match='at least 1'):
+            ops().linear(*bad)
+    with pytest.raises(RuntimeError, match='at least 1'):
+        ops().expert_linear(x, w[None, :0], groups_of([1]))
+
+
+def test_refusals_on_the_device():
+    x, w = normal(6, 64, seed=1), normal(48, 64, seed=2)
+    starts = groups_of([6])
+    cases = [
+        (lambda: ops().linear(x.float(), w.float()), 'bf16 or fp16'), (lambda: ops().linear(x, w.half()), 'weight must be'),
+        (lambda: ops().linear(x, w[:, :32]), 'weight must be'), (lambda: ops().linear(x.t(), w[:, :6]), 'contiguous'),
+        (lambda: ops().linear(x, w, bias=w[0]), 'bias must be'), (lambda: ops().linear(x, w, residual=x), 'residual must be'),
+        (lambda: ops().linear(x, w, out=x), 'out must be'),
+        (lambda: ops().linear(x, w, out=torch.empty(48, 6, dtype=BF16, device='cuda').t()), 'contiguous'),
+        (lambda: ops().linear(x, w, bias=w[:, 0]), 'contiguous'), (lambda: ops().linear(x, w.cpu()), 'CUDA'),
+        (lambda: ops().linear(x.clone().requires_grad_(), w, out=torch.empty(6, 48, dtype=BF16, device='cuda')), 'no gradients'),
+        (lambda: ops().linear(x.clone().requires_grad_(), w, return_pre=True), 'no gradients'),
+        (lambda: ops().linear_grad(x, x, w), 'grad must be'), (lambda: ops().linear_grad(x @ w.t(), x, w, None, 'silu'), 'pre must be'),
+        (lambda: ops().expert_linear(x, w, starts), 'experts, n, k'), (lambda: ops().expert_linear(x, w[None], starts[:1]), 'starts must'),
+        (lambda: ops().expert_linear(x, w[None], starts.int()), 'starts must'),
+        (lambda: ops().expert_linear(x, w[None].transpose(1, 2).contiguous().transpose(1, 2), starts), 'rows of weight'),
+        (lambda: ops().expert_linear(x, w[None], starts, bias=w[:1]), 'bias must be'),
+        (lambda: ops().expert_linear(x, w[None], starts, rows=starts.int()), 'rows must'),
+        (lambda: ops().expert_linear(x.clone().requires_grad_(), w[None], starts, rows=torch.arange(6, device='cuda')), 'pair_pos'),
+        (lambda: ops().expert_linear(x, w[None].expand(513, 48, 64), torch.zeros(514, dtype=torch.int64, device='cuda')), 'groups must'),
+        (lambda: ops().sum_pairs(x, torch.zeros(7, dtype=torch.int32, device='cuda'), 3), 'pair_pos must')]
+    for call, word in cases:
+        with pytest.raises(RuntimeError, match=word):
+            call()
+
+
 @pytest.mark.parametrize('dtype', [BF16, F16])
 @pytest.mark.parametrize('tokens,topk,k', [(1, 1, 8), (5, 3, 7), (70, 6, 2048), (300, 8, 1001)])
 def test_sum_pairs(tokens, topk, k, dtype):

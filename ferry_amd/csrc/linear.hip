@@ -276,12 +276,12 @@ __device__ __forceinline__ void slope8(int act, float (&f)[8]) {
 // dz = dy f'(pre) rounded, and db = the sum of the unrounded dz over each group's rows.  A workgroup takes
 // 2048 / RL columns (8 a thread) of one part of a group's rows, RL rows side by side and four of those at a
 // time, whose loads are issued together.  Large calls are bound by memory (dy and pre in, dz out) and take RL = 8
-// and parts, which a second launch adds; small ones by the chain of loads of a column's rows, which RL = 32
-// shortens without parts.
+// and parts, which a second launch adds; small ones by the chain of loads of a column's rows, which RL = 32 and, where
+// columns are few, 128 shorten without parts (300 rows of 2,816: 15 + 4 us with parts, 11 with RL = 32).
 template <typename T, int RL>
 __global__ __launch_bounds__(256) void slope_kernel(SlopeArgs a) {
   constexpr int CL = 256 / RL, COLS = CL * 8, U = 4;
-  __shared__ float sum[RL][COLS + 8];
+  __shared__ float sum[4][COLS];
   const int tid = threadIdx.x, rl = tid / CL, cl = (tid % CL) * 8;
   const int64_t jb = ceil_div(a.N, COLS), items = jb * a.groups * a.splits;
   for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
@@ -338,15 +338,20 @@ __global__ __launch_bounds__(256) void slope_kernel(SlopeArgs a) {
         }
       }
     if (!a.db) continue;
-    __syncthreads();
+    // the lanes of a wavefront that hold the same columns, then the wavefronts
 #pragma unroll
-    for (int q = 0; q < 8; ++q) sum[rl][cl + q] = acc[q];
+    for (int off = CL; off < 64; off <<= 1)
+#pragma unroll
+      for (int q = 0; q < 8; ++q) acc[q] += __shfl_xor(acc[q], off, 64);
+    __syncthreads();
+    if ((tid & 63) < CL) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) sum[tid >> 6][cl + q] = acc[q];
+    }
     __syncthreads();
     const int64_t jj = (it % jb) * COLS + tid;
     if (tid < COLS && jj < a.N) {
-      float t = 0;
-#pragma unroll
-      for (int q = 0; q < RL; ++q) t += sum[q][tid];
+      const float t = (sum[0][tid] + sum[1][tid]) + (sum[2][tid] + sum[3][tid]);
       if (a.splits > 1)
         a.part[((int64_t)s * a.groups + g) * a.N + jj] = t;
       else
@@ -355,13 +360,21 @@ __global__ __launch_bounds__(256) void slope_kernel(SlopeArgs a) {
   }
 }
 
+// The parts' sums: 64 columns a workgroup, each wavefront every fourth part, eight loads at a time.
 template <typename T>
 __global__ __launch_bounds__(256) void slope_join_kernel(const float* __restrict__ part, int64_t n, int splits,
                                                          uint16_t* __restrict__ db) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+  __shared__ float sum[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int64_t i0 = (int64_t)blockIdx.x * 64; i0 < n; i0 += (int64_t)gridDim.x * 64) {
+    const int64_t i = i0 + lane < n ? i0 + lane : n - 1;
     float t = 0;
-    for (int s = 0; s < splits; ++s) t += part[s * n + i];
-    db[i] = T::round(t);
+#pragma unroll 8
+    for (int s = wave; s < splits; s += 4) t += part[s * n + i];
+    sum[wave][lane] = t;
+    __syncthreads();
+    if (wave == 0 && i0 + lane < n) db[i] = T::round((sum[0][lane] + sum[1][lane]) + (sum[2][lane] + sum[3][lane]));
+    __syncthreads();
   }
 }
 
@@ -694,13 +707,14 @@ extern "C" int ferry_linear_grad_z(const void* grad, int32_t dtype, int64_t pair
   auto go = [&](auto kernel, int cols) {
     launch("linear_slope", kernel, dim3((unsigned)std::min<int64_t>(ceil_div(n, cols) * groups * a.splits, kMaxGrid)), dim3(256), 0, s, a);
   };
+  const bool few = ceil_div(n, 64) * groups < 128;
   if (dtype == FERRY_BF16)
-    a.splits > 1 ? go(slope_kernel<Bf16, 8>, 256) : go(slope_kernel<Bf16, 32>, 64);
+    a.splits > 1 ? go(slope_kernel<Bf16, 8>, 256) : (few ? go(slope_kernel<Bf16, 128>, 16) : go(slope_kernel<Bf16, 32>, 64));
   else
-    a.splits > 1 ? go(slope_kernel<F16, 8>, 256) : go(slope_kernel<F16, 32>, 64);
+    a.splits > 1 ? go(slope_kernel<F16, 8>, 256) : (few ? go(slope_kernel<F16, 128>, 16) : go(slope_kernel<F16, 32>, 64));
   FERRY_LAUNCHED("linear_slope");
   if (need) {
-    const dim3 g2((unsigned)std::min<int64_t>(ceil_div(groups * n, 256), 65536));
+    const dim3 g2((unsigned)std::min<int64_t>(ceil_div(groups * n, 64), 65536));
     if (dtype == FERRY_BF16)
       launch("linear_slope_join", slope_join_kernel<Bf16>, g2, dim3(256), 0, s, (const float*)a.part, groups * n, (int)a.splits, a.db);
     else

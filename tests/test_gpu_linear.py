@@ -591,7 +591,7 @@ def test_moe_layer_trains():
     # seven roundings of u = 2^-8 in a chain (h, silu, the product, y, its sum, z, dz and their gradients) in
     # norm: at most 14 u with those of the way back
     for a, b in zip((out, *got), (out64, *want)):
-        assert float((a.detach().double() - b).norm()) <= 14 * 2.0 ** -8 * float(b.norm())
+        assert float((a.detach().double() - b).norm()) <= 14 * 2.0 ** -8 * float(b.detach().norm())
     # the gradient of the tokens is the sum of its pairs' rows
     h_dy = normal(T * k, 2 * I, seed=8)
     dxp = ops().expert_linear_grad(h_dy, x, up, lay.starts, lay.rows)[0]

@@ -32,7 +32,8 @@ __device__ __forceinline__ u32x4 load8(const uint16_t* p, int n) {
 }
 
 // TI x TJ outputs per workgroup of four wavefronts, 64 of the contraction a step through registers into one of two
-// LDS buffers, the loads of a step issued two steps before its products: bound by their latency.  Loads are
+// LDS buffers, the loads of a step issued before the products of the one before.  (Loads two steps ahead took 300
+// registers, one wavefront a SIMD: dx of 8,192 x 6,143 x 2,047 in 1,007 us instead of 614.)  Loads are
 // 16 bytes at any alignment; what lies outside the matrices, the group or the contraction is 0 in LDS, so
 // that nothing a neighbouring row holds, a NaN included, enters a sum.
 template <typename T, int MODE, int TI, int TJ>
@@ -85,26 +86,22 @@ __global__ __launch_bounds__(256) void any_kernel(Args a) {
         pb[q] = j < a.J ? bw + j * a.ldb + (tid & 7) * 8 : nullptr;
       }
     }
-    // registers of two steps in turn: a step's loads have two steps of products to arrive
-    struct Regs {
-      u32x4 a[MI], b[NJ];
-    };
-    Regs r0, r1;
-    auto load = [&](int64_t c, Regs& v) __attribute__((always_inline)) {
+    u32x4 va[MI], vb[NJ];
+    auto load = [&](int64_t c) __attribute__((always_inline)) {
 #pragma unroll
       for (int q = 0; q < MI; ++q) {
         if constexpr (!kAcrossA) {
-          v.a[q] = load8(pa[q] + c, pa[q] ? (int)(c1 - c < 64 ? c1 - c : 64) - (tid & 7) * 8 : 0);
+          va[q] = load8(pa[q] + c, pa[q] ? (int)(c1 - c < 64 ? c1 - c : 64) - (tid & 7) * 8 : 0);
         } else {
           constexpr int per_row = TI / 8;
           const int64_t cc = c + tid / per_row + (256 / per_row) * q, i = i0 + (tid % per_row) * 8;
-          v.a[q] = load8(a.a + (start + cc) * a.lda + i, cc < c1 ? (int)(I - i < 8 ? I - i : 8) : 0);
+          va[q] = load8(a.a + (start + cc) * a.lda + i, cc < c1 ? (int)(I - i < 8 ? I - i : 8) : 0);
         }
       }
 #pragma unroll
       for (int q = 0; q < NJ; ++q) {
         if constexpr (!kAcrossB) {
-          v.b[q] = load8(pb[q] + c, pb[q] ? (int)(c1 - c < 64 ? c1 - c : 64) - (tid & 7) * 8 : 0);
+          vb[q] = load8(pb[q] + c, pb[q] ? (int)(c1 - c < 64 ? c1 - c : 64) - (tid & 7) * 8 : 0);
         } else {
           constexpr int per_row = TJ / 8;
           const int64_t cc = c + tid / per_row + (256 / per_row) * q, j = j0 + (tid % per_row) * 8;
@@ -117,25 +114,25 @@ __global__ __launch_bounds__(256) void any_kernel(Args a) {
               ok = (uint64_t)r < (uint64_t)a.x_rows;
             }
           }
-          v.b[q] = load8(bw + (ok ? r * a.ldb : 0) + j, ok ? (int)(a.J - j < 8 ? a.J - j : 8) : 0);
+          vb[q] = load8(bw + (ok ? r * a.ldb : 0) + j, ok ? (int)(a.J - j < 8 ? a.J - j : 8) : 0);
         }
       }
     };
-    auto store = [&](int buf, const Regs& v) __attribute__((always_inline)) {
+    auto store = [&](int buf) __attribute__((always_inline)) {
       char* const st = smem + buf * kStage;
 #pragma unroll
       for (int q = 0; q < MI; ++q) {
         constexpr int per_row = kAcrossA ? TI / 8 : 8;
         const int r = tid / per_row + (256 / per_row) * q, k = tid % per_row;
         const int at = kAcrossA ? r * TI * 2 + ((k ^ swz_across<TI>(r)) << 4) : r * 128 + ((k ^ swz_direct(r)) << 4);
-        *reinterpret_cast<u32x4*>(st + at) = v.a[q];
+        *reinterpret_cast<u32x4*>(st + at) = va[q];
       }
 #pragma unroll
       for (int q = 0; q < NJ; ++q) {
         constexpr int per_row = kAcrossB ? TJ / 8 : 8;
         const int r = tid / per_row + (256 / per_row) * q, k = tid % per_row;
         const int at = kAcrossB ? r * TJ * 2 + ((k ^ swz_across<TJ>(r)) << 4) : r * 128 + ((k ^ swz_direct(r)) << 4);
-        *reinterpret_cast<u32x4*>(st + TI * 128 + at) = v.b[q];
+        *reinterpret_cast<u32x4*>(st + TI * 128 + at) = vb[q];
       }
     };
     f32x4 acc[MI][NJ];
@@ -163,19 +160,15 @@ __global__ __launch_bounds__(256) void any_kernel(Args a) {
           for (int j = 0; j < NJ; ++j) acc[i][j] = T::mma(fb[j], fa[i], acc[i][j]);
       }
     };
-    // the step of c, which lies in buffer buf; v: free, w: the next step's
-    auto step = [&](int64_t c, int buf, Regs& v, const Regs& w) __attribute__((always_inline)) {
-      if (c + 128 < c1) load(c + 128, v);
+    load(c0);
+    store(0);
+    int buf = 0;
+    for (int64_t c = c0; c < c1; c += 64, buf ^= 1) {
+      const bool more = c + 64 < c1;
+      if (more) load(c + 64);
       __syncthreads();
       products(buf);
-      if (c + 64 < c1) store(buf ^ 1, w);
-    };
-    load(c0, r0);
-    if (c0 + 64 < c1) load(c0 + 64, r1);
-    store(0, r0);
-    for (int64_t c = c0; c < c1; c += 128) {
-      step(c, 0, r0, r1);
-      if (c + 64 < c1) step(c + 64, 1, r1, r0);
+      if (more) store(buf ^ 1);
     }
     // lane l holds columns 4 (l / 16) + [0, 4) of row l % 16 of each 16 x 16 tile
 #pragma unroll
@@ -256,7 +249,7 @@ struct SlopeArgs {
   float* part;           // [splits][groups][N], with splits > 1
   int64_t ldy, pairs, N;
   const int64_t* starts;
-  int32_t groups, splits, act, zero_rest, vec;
+  int32_t groups, splits, act;
 };
 
 // f[q] = f'(f[q]), the choice of the activation once for eight
@@ -277,7 +270,7 @@ __device__ __forceinline__ void slope8(int act, float (&f)[8]) {
 // 2048 / RL columns (8 a thread) of one part of a group's rows, RL rows side by side and four of those at a
 // time, whose loads are issued together.  Large calls are bound by memory (dy and pre in, dz out) and take RL = 8
 // and parts, which a second launch adds; small ones by the chain of loads of a column's rows, which RL = 32 and, where
-// columns are few, 128 shorten without parts (300 rows of 2,816: 15 + 4 us with parts, 11 with RL = 32).
+// columns are few, 128 shorten without parts (300 rows of 2,816: 15 + 4 us with parts, 7 with RL = 128).
 template <typename T, int RL>
 __global__ __launch_bounds__(256) void slope_kernel(SlopeArgs a) {
   constexpr int CL = 256 / RL, COLS = CL * 8, U = 4;
@@ -561,8 +554,8 @@ bool tiles_fit(int op, const Args& a, int64_t pairs, int64_t n, int64_t k) {
     return false;
   const int64_t most = ((int64_t)1 << 31) - (1 << 20);   // elements, with room for a stage behind the end
   const int64_t ia = op == kDw ? pairs : (a.rows ? a.x_rows : 512), ib = op == kFwd ? 512 : (op == kDx ? n : (a.rows ? a.x_rows : pairs));
-  if (a.J > most / 1024 || a.lda > most / 512 || a.ldb > most / 512 || a.ldo > most / 512 || a.ldr > most / 512 || ia * a.lda > most || ib * a.ldb > most || a.C > most / 4) return false;
-  return true;
+  return a.J <= most / 1024 && a.lda <= most / 512 && a.ldb <= most / 512 && a.ldo <= most / 512 && a.ldr <= most / 512 && ia * a.lda <= most &&
+         ib * a.ldb <= most && a.C <= most / 4;
 }
 
 int64_t part_bytes(int op, const Plan& p, int64_t pairs, int64_t n, int64_t k, int64_t groups) {
@@ -571,12 +564,13 @@ int64_t part_bytes(int op, const Plan& p, int64_t pairs, int64_t n, int64_t k, i
   return p.splits * out * 4;
 }
 
-// Parts of a group's rows for slope_kernel, 1: all rows by one workgroup, 32 side by side.  Up to 512 rows of a
-// group on average one launch without parts is faster: 300 rows of 2,816 took 15 + 4 us with parts of 60 rows, and
-// take 10 without.  Above, a part for each 128 rows of the average, 64 at most.
+// Parts of a group's rows for slope_kernel, 1: all rows by one workgroup, 32 or 128 side by side.  Few rows take one
+// launch without parts (300 rows of 2,816: 15 + 4 us with parts of 60 rows, 7 without).  Otherwise a part for each 128
+// rows of a group on average, and for each 8,192 of the call, since one group may hold most of them; 64 at most (65,536
+// rows of 1,536 in 128 equal groups: 38 us, 33 without; all of them in one group: 254, 449 without).
 int64_t slope_splits(int64_t pairs, int64_t groups) {
   const int64_t rows = pairs / groups;
-  return rows <= 512 ? 1 : std::min<int64_t>(ceil_div(rows, 128), 64);
+  return rows <= 512 && pairs <= 8192 ? 1 : std::min<int64_t>(std::max(ceil_div(rows, 128), ceil_div(pairs, 8192)), 64);
 }
 
 template <typename T, int MODE>

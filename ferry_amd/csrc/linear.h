@@ -123,12 +123,14 @@ __device__ __forceinline__ float activate(int act, float z) {
   }
 }
 
-// f'(z).  Beyond |z| = 30 those of gelu are 0 or 1 to all bits; the clamp keeps z^3 finite.
+// f'(z).  Beyond |z| = 30 those of gelu are 0 or 1 to all bits; the clamp keeps z^3 finite.  That of silu is beyond 200, and
+// an infinite z, which a finite argument above fp16's largest is rounded to, would make 0 times infinity of it.
 __device__ __forceinline__ float slope(int act, float z) {
   if (z != z) return z;
   switch (act) {
     case kRelu: return z <= 0.f ? 0.f : 1.f;
     case kSilu: {
+      z = fminf(fmaxf(z, -200.f), 200.f);
       const float s = sigmoid(z);
       return s * (1.0f + z * (1.0f - s));
     }

@@ -551,6 +551,12 @@ def _workspace(product, pairs, n, k, groups, device):
     return ws, ws.data_ptr(), need
 
 
+def _written(out):
+    """Tells autograd that ``out`` gets other values: a backward pass that saved the old ones refuses them."""
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)
+
+
 def _watched(what, *tensors):
     """Whether autograd takes part in a call on these tensors (None among them)."""
     if (getattr(forward_ad, '_current_level', 0) >= 0
@@ -606,6 +612,7 @@ def _linear(x, weight, bias, activation, residual, out, keep):
         at, stride = _half_rows(out, 'out', dev, dtype)
         if out.shape != shape:
             raise RuntimeError(f'out must be {list(shape)}')
+        _written(out)
     pre = _matrix(m, n, dtype, x.device) if keep and act else None
     if m:
         _product(x, xs, k, None, m, None, 1, w, ws, 0, n, b, 0, act, r, rs,
@@ -619,9 +626,9 @@ def linear(x, weight, bias=None, activation=None, residual=None, out=None, retur
     ``x`` [..., k], ``weight`` [n, k] (a matrix may have a row stride), ``bias`` [n] and ``residual``
     [..., n] are bf16 or fp16, all the same; sums are fp32.  ``activation`` is None, 'relu', 'silu', 'gelu'
     (the normal distribution's) or 'gelu_tanh'.  ``out`` (optional) receives the result and may be
-    ``residual`` itself, but share no memory with the other arguments.  ``return_pre=True`` returns (result, the activation's rounded argument [rows, n],
-    or None without an activation), what ``linear_grad`` needs.  Rows that start at multiples of 16 bytes
-    are fastest; any other alignment is taken.
+    ``residual`` itself, but share no memory with the other arguments.  ``return_pre=True`` returns (result,
+    the activation's rounded argument [rows, n], or None without an activation), what ``linear_grad`` needs.
+    Rows that start at multiples of 16 bytes are fastest; any other alignment is taken.
 
     The result carries the gradients of x, weight, bias and residual, except with ``out`` or ``return_pre``
     and inside a captured graph (there ``linear`` and ``linear_grad`` are called under torch.no_grad()).
@@ -757,6 +764,7 @@ def _expert_linear(x, weight, starts, bias, rows, out):
         at, stride = _half_rows(out, 'out', x.get_device(), x.dtype)
         if out.shape != (pairs, n):
             raise RuntimeError(f'out must be [{pairs}, {n}]')
+        _written(out)
     if pairs:
         _product(x, xs, k, rows_at, pairs, first, E, w, ws, wg, n, b, bs, 0, None, 0, None, at, stride, int(zero))
     return out
@@ -770,8 +778,8 @@ def expert_linear(x, weight, starts, bias=None, rows=None, pair_pos=None, out=No
     part of cache rows are) and ``bias`` [experts, n] are bf16 or fp16, all the same; sums are fp32, a result
     is rounded once.  ``starts``, ``rows`` and ``pair_pos`` are ``layout``'s, on the device; without ``rows``
     ``x`` is in grouped order already.  An entry of ``rows`` that names no row of x reads as zeros.  Rows
-    before ``starts[0]`` and from ``starts[experts]`` on are 0; in an ``out`` that is passed they stay as
-    they were.
+    before ``starts[0]`` and from ``starts[experts]`` on are 0; in an ``out`` that is passed, which shares no
+    memory with the other arguments, they stay as they were.
 
     The result carries the gradients of x, weight and bias (x's, with ``rows``, needs ``pair_pos`` [tokens *
     topk], the places of each row of x), except with ``out`` and inside a captured graph (there

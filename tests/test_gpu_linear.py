@@ -708,3 +708,30 @@ def test_offsets_past_32_bits(k):
     wide = buf.as_strided((2, 16, k), (stride, k, 1), 0)   # experts' weights far apart
     wide.copy_(ew)
     close(ops().expert_linear(xc, wide, starts, rows=rows), *expert_reference(xc, ew, starts, rows=rows)['y'], 'w')
+
+
+@pytest.mark.parametrize('activation', ['relu', 'silu', 'gelu', 'gelu_tanh'])
+def test_activation_argument_beyond_fp16(activation):
+    """z = -+90,000 is finite in the sums and infinite where it is kept in fp16: f' there is still 0 or 1."""
+    x = torch.tensor([[300.0], [-300.0]], dtype=torch.float16, device='cuda')
+    w = torch.full((9, 1), 300.0, dtype=torch.float16, device='cuda')
+    y, pre = ops().linear(x, w, None, activation, return_pre=True)
+    assert bool(torch.isinf(pre).all()) and bool((y[1] == 0).all())
+    dy = torch.ones(2, 9, dtype=torch.float16, device='cuda')
+    dx, dw, db = ops().linear_grad(dy, x, w, pre, activation)
+    assert dx.flatten().tolist() == [2700, 0]      # 9 * 1 * 300, exact in fp16 (a multiple of 2 below 4,096)
+    assert bool((dw == 300).all()) and bool((db == 1).all())
+
+
+def test_out_is_seen_by_autograd():
+    x, w = normal(8, 16), normal(24, 16, seed=1)
+    starts = torch.tensor([0, 8], device='cuda')
+    out = torch.zeros(8, 24, dtype=BF16, device='cuda')
+    for write in (lambda: ops().linear(x, w, out=out), lambda: ops().expert_linear(x, w[None], starts, out=out)):
+        scale = torch.ones(8, 24, dtype=BF16, device='cuda', requires_grad=True)
+        product = scale * out
+        write()
+        with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+            product.sum().backward()
+    with torch.inference_mode():
+        assert torch.equal(ops().linear(x, w, out=torch.empty(8, 24, dtype=BF16, device='cuda')), ops().linear(x, w))

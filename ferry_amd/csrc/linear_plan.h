@@ -1,0 +1,18 @@
+// Arithmetic of the linear products' launches and pipelines that needs no device: also built by itself, for tests.
+#pragma once
+
+#include <cstdint>
+
+namespace ferry {
+namespace lin {
+
+// ring_kernel's stages of 64 of the contraction: as many as 144 KiB hold, 128 KiB beside the row numbers of a gathered dW
+constexpr int ring_stages(int tm, int tn, bool gathered_dw) { return (gathered_dw ? 131072 : 147456) / ((tm + tn) * 128); }
+
+// Whether ring_kernel's loads are awaited where the stream goes on behind a tile of kt stages: the next tile's row
+// numbers were loaded where this one began.  In the loop each stage waits until the loads of ring - 2 stages at most are
+// outstanding, so kt >= ring - 1 stages suffice; the stages that fill the ring wait for nothing.
+constexpr bool ring_rows_wait(int kt, int ring, bool filling) { return kt < ring + (filling ? 1 : 0); }
+
+}  // namespace lin
+}  // namespace ferry

@@ -1,4 +1,5 @@
 // The linear products on tiles smaller than 256 x 256: where few rows, columns or tiles leave CUs idle with those.
+#include "linear_plan.h"
 #include "linear_stream.h"
 #include "linear_tile.h"
 
@@ -21,7 +22,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM
   constexpr bool XA = MODE == kDw, XB = MODE != kFwd, RAG = MODE != kDw;
   constexpr bool GA = GATHER && MODE == kFwd, GB = GATHER && MODE == kDw;
   constexpr int W = WM * WN, TM = 16 * WM * MI, TN = 16 * WN * NI;
-  constexpr int kStage = (TM + TN) * 128, SST = (GB ? 131072 : 147456) / kStage;
+  constexpr int kStage = (TM + TN) * 128, SST = ring_stages(TM, TN, GB);
   constexpr int LA = TM / (8 * W), LB = TN / (8 * W), LPS = LA + LB;   // loads of a wavefront and stage
   // GB: rows of x of a wavefront and stage, stages whose row numbers 64 lanes load at once
   constexpr int RPW = LB * 512 / TN, BS = 64 / RPW;
@@ -156,14 +157,14 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM
     else
       load_lds(rb, bvo[q - LA], sb, dst + TM * 128 + 1024 * (LB * wave + q - LA));
   };
-  auto end_stage = [&]() __attribute__((always_inline)) {
+  auto end_stage = [&](bool filling) __attribute__((always_inline)) {
     left -= 64;
     sa += a_step;
     sb += b_step;
     if (++sk < skt) return;
     const int kt = skt;
     if (ahead.next()) {
-      if (GATHER && kt < SST) wait_cnt<0>();   // its row numbers were loaded kt stages ago
+      if (GATHER && ring_rows_wait(kt, SST, filling)) wait_cnt<0>();   // its row numbers were loaded kt stages ago
       set ^= 1;
       begin_tile(ahead.tile());
     } else {
@@ -205,7 +206,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM
   for (int k = 0; k < SST; ++k) {
     begin_stage();
     static_for<0, LPS>([&](auto q) __attribute__((always_inline)) { load(q, k); });
-    end_stage();
+    end_stage(true);
   }
   wait_cnt<(SST - 1) * LPS>();
   wg_barrier();
@@ -255,7 +256,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(WM
         static_for<i * LPS / MI, (i + 1) * LPS / MI>([&](auto q) __attribute__((always_inline)) { load(q, cur); });
         mma(i, t1, w1);
       });
-      end_stage();
+      end_stage(false);
       cur = nxt;
     }
     if (MODE == kFwd && kt < SST) {   // the bias was loaded at the tile's start

@@ -1,0 +1,39 @@
+"""The linear products' pipelines where tiles meet: contractions as long as a kernel's ring of stages, one stage less
+and one more, with several tiles to a workgroup.  Formulas and bounds are test_gpu_linear's."""
+import pytest
+import torch
+from test_gpu_linear import BF16, F16, close, expert_reference, groups_of, normal, ops
+
+pytestmark = pytest.mark.gpu
+
+# experts, rows of each, n, k: forward products in 256 x 128, 128 x 128, 64 x 128 and 64 x 64 tiles, whose rings hold 3, 4,
+# 6 and 9 stages of 64 of k
+FORWARD = [(128, 522, 32, 128), (32, 2067, 32, 192), (128, 528, 32, 256), (128, 258, 32, 192), (16, 2101, 32, 256),
+           (64, 521, 32, 320), (32, 8, 1032, 320), (64, 8, 520, 384), (16, 8, 2128, 448), (64, 8, 264, 512),
+           (64, 8, 272, 576), (3, 8, 5752, 640)]
+# gradients of the weights in 128 x 128, 64 x 128 and 64 x 64 tiles, whose rings hold 4, 5 and 8 stages of 64 rows
+WEIGHTS = [(128, 145, 408, 32), (128, 205, 392, 32), (128, 275, 408, 32), (32, 196, 1072, 32), (32, 261, 1072, 32),
+           (16, 196, 32, 2120), (8, 260, 32, 4232), (64, 331, 32, 520), (16, 390, 1032, 32), (32, 467, 32, 520),
+           (32, 530, 520, 32)]
+
+
+def gathered(E, per, n, k, dtype):
+    P = E * per
+    g = torch.Generator(device='cuda').manual_seed(P)
+    R = P // 2
+    rows = torch.randint(0, R, (P,), generator=g, device='cuda')
+    x, w = normal(R, k, dtype=dtype, seed=1), normal(E, n, k, dtype=dtype, seed=2, scale=k ** -0.5)
+    return x, w, groups_of([per] * E), rows, normal(P, n, dtype=dtype, seed=3)
+
+
+@pytest.mark.parametrize('case', FORWARD)
+def test_rows_of_the_next_tile(case):
+    x, w, starts, rows, _ = gathered(*case, BF16 if case[3] % 128 else F16)
+    close(ops().expert_linear(x, w, starts, rows=rows), *expert_reference(x, w, starts, rows=rows)['y'], 'y')
+
+
+@pytest.mark.parametrize('case', WEIGHTS)
+def test_rows_of_the_next_weights(case):
+    x, w, starts, rows, dy = gathered(*case, BF16 if case[1] % 2 else F16)
+    close(ops().expert_linear_grad(dy, x, w, starts, rows, need_x=False, need_bias=False)[1],
+          *expert_reference(x, w, starts, rows=rows, dy=dy)['dw'], 'dw')

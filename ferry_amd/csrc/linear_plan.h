@@ -14,5 +14,11 @@ constexpr int ring_stages(int tm, int tn, bool gathered_dw) { return (gathered_d
 // outstanding, so kt >= ring - 1 stages suffice; the stages that fill the ring wait for nothing.
 constexpr bool ring_rows_wait(int kt, int ring, bool filling) { return kt < ring + (filling ? 1 : 0); }
 
+// tile256's phases behind the stores of the tile before in which these may be outstanding as well.  The phase's wait is for
+// the half that the next phase reads.  Eight halves were loaded before the stores; the first was awaited there, the
+// second too, with the products' last phase, and the other six are awaited by the first six phases.  What the seventh
+// awaits was loaded behind the stores.
+constexpr int kTile256Early = 6;
+
 }  // namespace lin
 }  // namespace ferry

@@ -1,4 +1,5 @@
 // The linear products on whole tiles: rows at multiples of 16 bytes, sizes of multiples of 8.
+#include "linear_plan.h"
 #include "linear_stream.h"
 #include "linear_tile.h"
 
@@ -307,9 +308,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         __builtin_amdgcn_s_setprio(0);
         wg_barrier();
       };
-      // The next segment's half has landed, this one's fragments are read.  The first seven halves of a tile
+      // The next segment's half has landed, this one's fragments are read.  The halves that the first segments wait for
       // were loaded before the stores of the tile before: those may be outstanding too.
-      int early = stores ? 7 : 0;
+      int early = stores ? kTile256Early : 0;
       auto mem_end = [&]() __attribute__((always_inline)) {
         if (early > 0) {
           --early;

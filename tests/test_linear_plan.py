@@ -16,6 +16,7 @@ SOURCE = '''
 using namespace ferry::lin;
 extern "C" int stages(int tm, int tn, int gathered_dw) { return ring_stages(tm, tn, gathered_dw); }
 extern "C" int rows_wait(int kt, int ring, int filling) { return ring_rows_wait(kt, ring, filling); }
+extern "C" int early() { return kTile256Early; }
 '''
 
 
@@ -45,26 +46,28 @@ class Memory:
         assert self.last[name] <= self.landed, f'{name} is read before its loads have landed'
 
 
-def ring(plan, kts, tm, tn, waves, stores, gathered_dw):
-    """ring_kernel with gathered rows on tiles of kts stages, as its first wavefront runs it."""
-    m, S = Memory(), plan.stages(tm, tn, gathered_dw)
+def ring(plan, kts, tm, tn, waves, stores, gathered):
+    """ring_kernel on tiles of kts stages, rows gathered for 'x' (forward), 'dw' or not at all, as its first wavefront runs
+    it."""
+    m, S = Memory(), plan.stages(tm, tn, gathered == 'dw')
     la, lb = tm // (8 * waves), tn // (8 * waves)
     per_stage, batch = la + lb, 64 // (lb * 512 // tn)   # batch: stages whose row numbers are loaded at once
     at = dict(tile=0, stage=0)
 
     def rows(tile):
-        m.issue(('rows', tile, 0), 2)
+        if gathered:
+            m.issue(('rows', tile, 0), 2)
 
     def begin_tile(tile):
         at.update(tile=tile, stage=0)
-        if not gathered_dw:
+        if gathered == 'x':
             m.read(('rows', tile, 0))
         rows(tile + 1)
 
     def load_stage(filling):
         tile, k = at['tile'], at['stage']
         if tile < len(kts):
-            if gathered_dw:
+            if gathered == 'dw':
                 if k % batch == 0:
                     if batch < S and k:
                         m.wait(batch * per_stage)
@@ -75,14 +78,15 @@ def ring(plan, kts, tm, tn, waves, stores, gathered_dw):
         at['stage'] += 1
         if tile < len(kts) and at['stage'] == kts[tile]:
             if tile + 1 < len(kts):
-                if plan.rows_wait(kts[tile], S, filling):
+                if gathered and plan.rows_wait(kts[tile], S, filling):
                     m.wait(0)
                 begin_tile(tile + 1)
             else:
                 at.update(tile=len(kts), stage=0)   # stages of zeros
 
     rows(0)
-    m.wait(0)
+    if gathered:
+        m.wait(0)
     begin_tile(0)
     for _ in range(S):
         load_stage(True)
@@ -91,7 +95,7 @@ def ring(plan, kts, tm, tn, waves, stores, gathered_dw):
     order = [(t, k) for t, kt in enumerate(kts) for k in range(kt)] + [(len(kts), 0)]
     early = done = 0
     for t, kt in enumerate(kts):
-        if not gathered_dw:
+        if gathered != 'dw':
             m.issue(('bias', t), 1)
         for _ in range(kt):
             m.wait((S - 2) * per_stage + (stores if early else 0))
@@ -99,7 +103,7 @@ def ring(plan, kts, tm, tn, waves, stores, gathered_dw):
             done += 1
             m.read(('stage', *order[done]))
             load_stage(False)
-        if not gathered_dw:
+        if gathered != 'dw':
             if kt < S:
                 m.wait(0)
             m.read(('bias', t))
@@ -110,15 +114,122 @@ def ring(plan, kts, tm, tn, waves, stores, gathered_dw):
 RINGS = [(256, 128, 8, 8), (128, 128, 8, 4), (64, 128, 8, 2), (64, 64, 4, 2)]   # tile, wavefronts, stores of one
 
 
-@pytest.mark.parametrize('gathered_dw', [False, True])
+@pytest.mark.parametrize('gathered', [None, 'x', 'dw'])
 @pytest.mark.parametrize('shape', RINGS)
-def test_row_numbers_have_landed(plan, shape, gathered_dw):
+def test_stages_have_landed(plan, shape, gathered):
     """Tiles as long as the ring, shorter and longer ones, in every order of three."""
-    if gathered_dw and shape[0] == 256:
+    if gathered == 'dw' and shape[0] == 256:
         return   # that kernel has no such form
-    S = plan.stages(*shape[:2], gathered_dw)
+    S = plan.stages(*shape[:2], gathered == 'dw')
     lengths = sorted({1, 2, S - 2, S - 1, S, S + 1, S + 2, 2 * S, 2 * S + 3} - {0})
     for kts in itertools.product(lengths, repeat=3):
-        ring(plan, kts, *shape, gathered_dw)
+        ring(plan, kts, *shape, gathered)
     for kt in range(1, 30):
-        ring(plan, [kt] * 6, *shape, gathered_dw)
+        ring(plan, [kt] * 6, *shape, gathered)
+
+
+def few(steps, mt, nb, ring, gathered):
+    """A wavefront of few_kernel over its chunks of the contraction, of which the ring holds `ring`."""
+    m, lw, lx = Memory(), 2 * nb, 2 * mt
+    if gathered:
+        m.issue('rows', 2)
+    for i in range(ring):
+        m.issue(('w', i), lw)
+    if gathered:
+        m.wait(ring * lw)
+        m.read('rows')
+    for i in range(ring):
+        m.issue(('x', i), lx)
+    more = max(steps - ring, 0)
+    for i in range(steps):
+        if i >= ring:
+            m.wait(min(steps - 1 - i, ring - 1) * (lw + lx))
+        else:
+            m.wait((ring - 1 - i) * lx + (i * (lw + lx) if i <= more else 0))
+        m.read(('w', i))
+        m.read(('x', i))
+        if i < more:
+            m.issue(('w', i + ring), lw)
+            m.issue(('x', i + ring), lx)
+
+
+def test_chunks_have_landed():
+    for mt, nb, ring_depth in ((1, 1, 4), (1, 2, 3), (2, 2, 2), (4, 2, 2), (4, 4, 2)):
+        for steps in range(1, 20):
+            few(steps, mt, nb, ring_depth, False)
+            few(steps, mt, nb, ring_depth, True)
+
+
+def tile256(plan, lengths, gathered):
+    """tile256 on tiles whose contractions have these lengths, rows gathered for 'x' (forward), 'dw' or not at all, as its
+    first wavefront runs it: four phases a stage, each of which reads one half of an operand and loads another."""
+    m = Memory()
+    kts = [-(-n // 64) for n in lengths]
+    stream = dict(tile=0, stage=0)
+
+    def begin_tile(tile):
+        stream.update(tile=tile, stage=0)
+        if gathered == 'x' and tile < len(kts):
+            m.read(('rows', tile, 0))
+
+    def begin_stage():
+        tile, k = stream['tile'], stream['stage']
+        if gathered == 'dw' and tile < len(kts):
+            if k % 8 == 0 and kts[tile] - k > 8:
+                m.issue(('rows', tile, k // 8 + 1), 2)
+            if k < kts[tile]:
+                m.read(('rows', tile, k // 8))
+
+    def load(half):
+        m.issue((half, stream['tile'], stream['stage']), 2)
+
+    if gathered:
+        m.issue(('rows', 0, 0), 2)
+        m.wait(0)
+    begin_tile(0)
+    for _ in range(2):
+        begin_stage()
+        for half in ('B0', 'A0', 'B1', 'A1'):
+            load(half)
+        stream['stage'] += 1
+    m.wait(12)
+    m.read(('B0', 0, 0))
+    m.wait(12)
+    stores = False
+    for t, n in enumerate(lengths):
+        pairs = (n + 127) // 128
+        early = plan.early() if stores else 0
+        if gathered == 'x':
+            m.issue(('bias', t), 1)
+        if gathered:
+            m.issue(('rows', t + 1, 0), 2)
+        if gathered == 'dw' and pairs <= 1:
+            m.wait(0)
+        stages = max(2 * pairs, 2)
+        for k in range(stages):
+            if k == stages - 2:
+                begin_tile(t + 1)   # the last two stages load the next tile's first two
+            after = (t, k + 1) if k + 1 < stages else (t + 1, 0)
+            begin_stage()
+            for reads, loads in ((('A0', t, k), 'B0'), (('B1', t, k), 'A0'), (('A1', t, k), 'B1'), (('B0', *after), 'A1')):
+                m.read(reads)
+                load(loads)
+                m.wait(28 if early > 0 else 12)
+                early -= 1
+            stream['stage'] += 1
+        if gathered == 'x':
+            m.read(('bias', t))
+        m.issue(('stores', t), 16)
+        stores = True
+
+
+LENGTHS = [1, 64, 65, 128, 129, 192, 256, 500, 512, 513, 640, 1030, 1600]
+
+
+@pytest.mark.parametrize('gathered', [None, 'x', 'dw'])
+def test_halves_have_landed(plan, gathered):
+    """Tiles of any contractions follow each other (gathered forward ones of more than 128)."""
+    for lengths in itertools.product([n for n in LENGTHS if gathered != 'x' or n > 128], repeat=3):
+        tile256(plan, lengths, gathered)
+    if gathered != 'x':
+        tile256(plan, [0, 0, 300, 0], gathered)

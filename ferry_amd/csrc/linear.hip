@@ -2,6 +2,7 @@
 // every size and alignment, and the entry points.  No counterpart in the reference, whose experts are
 // SwiGLU blocks of bf16 matrices without biases or gradients.
 #include "linear.h"
+#include "linear_plan.h"
 #include "linear_tile.h"
 
 #include <algorithm>
@@ -576,8 +577,7 @@ int64_t slope_splits(int64_t pairs, int64_t groups) {
 template <typename T, int MODE>
 int run_typed(const Args& a, const Plan& p, int64_t n, int64_t k, hipStream_t s) {
   static const char* const names[] = {"linear_fwd", "linear_dx", "linear_dw"};
-  // (tile256 loads the row numbers of a tile one tile ahead, which takes a contraction of more than two stages)
-  const int shape = p.shape == 0 && MODE == kFwd && a.rows && ceil_div(ceil_div(k, a.splits), 64) * 64 <= 128 ? 1 : p.shape;
+  const int shape = p.shape == 0 && MODE == kFwd && a.rows && !tile256_gathers(k, a.splits) ? 1 : p.shape;
   if (p.kind == kFew && few_fits(MODE, a)) {
     few_launch(MODE, T::kType, p.mt, p.nb, a, p.tiles, cus(), s);
   } else if (p.kind == kTiles && tiles_fit(MODE, a, a.pairs, n, k)) {

@@ -20,5 +20,15 @@ constexpr bool ring_rows_wait(int kt, int ring, bool filling) { return kt < ring
 // awaits was loaded behind the stores.
 constexpr int kTile256Early = 6;
 
+// A contraction of c in parts: each but the last has part_length, the last what is left, which may be little or nothing.
+constexpr int64_t part_length(int64_t c, int64_t parts) { return ((c + parts - 1) / parts + 63) / 64 * 64; }
+constexpr int64_t last_part(int64_t c, int64_t parts) {
+  return c > (parts - 1) * part_length(c, parts) ? c - (parts - 1) * part_length(c, parts) : 0;
+}
+
+// Whether tile256 takes a gathered x whose contraction is cut into these parts: it loads the row numbers of a tile where the
+// tile before begins and awaits them with that tile's stages, all but the last two, so every part needs more than two.
+constexpr bool tile256_gathers(int64_t c, int64_t parts) { return last_part(c, parts) > 128; }
+
 }  // namespace lin
 }  // namespace ferry

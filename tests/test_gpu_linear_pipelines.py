@@ -37,3 +37,14 @@ def test_rows_of_the_next_weights(case):
     x, w, starts, rows, dy = gathered(*case, BF16 if case[1] % 2 else F16)
     close(ops().expert_linear_grad(dy, x, w, starts, rows, need_x=False, need_bias=False)[1],
           *expert_reference(x, w, starts, rows=rows, dy=dy)['dw'], 'dw')
+
+
+@pytest.mark.parametrize('counts,n,k', [([2146, 2146], 160, 14464), ([888, 1, 1776, 887], 136, 12312), ([3900, 33], 152, 14400)])
+def test_rows_of_parts(counts, n, k):
+    """256 x 256 tiles of a contraction in 16 parts of which the last is short (64) or empty, with more of these
+    than workgroups."""
+    P = sum(counts)
+    rows = torch.randint(0, P, (P,), generator=torch.Generator(device='cuda').manual_seed(k), device='cuda')
+    x, w = normal(P, k, seed=1), normal(len(counts), n, k, seed=2, scale=k ** -0.5)
+    starts = groups_of(counts)
+    close(ops().expert_linear(x, w, starts, rows=rows), *expert_reference(x, w, starts, rows=rows)['y'], 'y')

@@ -17,6 +17,8 @@ using namespace ferry::lin;
 extern "C" int stages(int tm, int tn, int gathered_dw) { return ring_stages(tm, tn, gathered_dw); }
 extern "C" int rows_wait(int kt, int ring, int filling) { return ring_rows_wait(kt, ring, filling); }
 extern "C" int early() { return kTile256Early; }
+extern "C" int gathers(long c, long parts) { return tile256_gathers(c, parts); }
+extern "C" long part(long c, long parts) { return part_length(c, parts); }
 '''
 
 
@@ -26,7 +28,10 @@ def plan(tmp_path_factory):
     (where / 'plan.cpp').write_text(SOURCE)
     subprocess.run(['g++', '-std=c++17', '-O1', '-shared', '-fPIC', f'-I{CSRC}', '-o', str(where / 'plan.so'),
                     str(where / 'plan.cpp')], check=True)
-    return ctypes.CDLL(str(where / 'plan.so'))
+    so = ctypes.CDLL(str(where / 'plan.so'))
+    so.part.restype = ctypes.c_long
+    so.gathers.argtypes = so.part.argtypes = [ctypes.c_long, ctypes.c_long]
+    return so
 
 
 class Memory:
@@ -233,3 +238,19 @@ def test_halves_have_landed(plan, gathered):
         tile256(plan, lengths, gathered)
     if gathered != 'x':
         tile256(plan, [0, 0, 300, 0], gathered)
+
+
+@pytest.mark.parametrize('parts', [1, 2, 4, 8, 16])
+def test_row_numbers_of_parts_have_landed(plan, parts):
+    """A gathered forward product in parts, the last of which may be short or empty: tile256's tiles of one workgroup are
+    of any parts, so each is followed by each."""
+    taken = 0
+    for k in [*range(128 * parts, 1100 * parts, 8 * parts + 8), 14464, 14400, 20000, 65544]:
+        if plan.gathers(k, parts):
+            per = plan.part(k, parts)
+            lengths = [max(0, min(per, k - s * per)) for s in range(parts)]
+            assert sum(lengths) == k
+            for pair in itertools.product(sorted(set(lengths)), repeat=2):
+                tile256(plan, [*pair, per], 'x')
+            taken += 1
+    assert taken > 10

@@ -30,5 +30,11 @@ constexpr int64_t last_part(int64_t c, int64_t parts) {
 // tile before begins and awaits them with that tile's stages, all but the last two, so every part needs more than two.
 constexpr bool tile256_gathers(int64_t c, int64_t parts) { return last_part(c, parts) > 128; }
 
+// Bytes from tile256's first half of an operand (128 indices) to its second, for an operand of `there` indices from the tile's
+// first on, staged across (by the contraction) or directly (by rows of ld2 bytes).  A second half without indices loads
+// the first again: its offset would lie behind the end of a buffer whose last row is short, where the hardware's
+// comparison with size - offset wraps and keeps no lane inside.
+constexpr uint32_t half_offset(bool across, int64_t there, uint32_t ld2) { return there > 128 ? (across ? 256 : 128 * ld2) : 0; }
+
 }  // namespace lin
 }  // namespace ferry

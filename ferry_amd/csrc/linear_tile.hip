@@ -122,8 +122,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     ra = t.a, rb = t.b, sa = sb = 0, left = t.nc;
     if constexpr (GB) idx = a.rows + t.p0;
     // a half without rows or columns loads the other's: what it gives is not stored
-    a_half = XA ? 256 : (t.rows > 128 ? 128 * lda2 : 0);
-    b_half = XB ? 256 : (a.J - t.j0 > 128 ? 128 * ldb2 : 0);
+    a_half = half_offset(XA, t.rows, lda2);
+    b_half = half_offset(XB, a.J - t.j0, ldb2);
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       const uint32_t ca = (uint32_t)chunk_a(q) * 16, cb = (uint32_t)chunk_b(q) * 16;

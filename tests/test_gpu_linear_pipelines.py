@@ -48,3 +48,23 @@ def test_rows_of_parts(counts, n, k):
     x, w = normal(P, k, seed=1), normal(len(counts), n, k, seed=2, scale=k ** -0.5)
     starts = groups_of(counts)
     close(ops().expert_linear(x, w, starts, rows=rows), *expert_reference(x, w, starts, rows=rows)['y'], 'y')
+
+
+@pytest.mark.parametrize('m,n,k', [(4097, 2120, 2048), (8193, 1344, 1032), (4097, 2048, 2104), (2049, 4104, 2056)])
+def test_one_row_left_and_few_columns(m, n, k):
+    """dW in 256 x 256 tiles whose contraction ends with one row and whose last tiles have fewer than 128 columns."""
+    x, dy = normal(m, k, seed=1), normal(m, n, seed=2)
+    _, dw, _ = ops().linear_grad(dy, x, normal(n, k, seed=3), need_x=False, need_bias=False)
+    starts = groups_of([m])
+    close(dw, *[t[0] for t in expert_reference(x, torch.zeros(1, n, k, dtype=BF16, device='cuda'), starts, dy=dy)['dw']], 'dw')
+
+
+@pytest.mark.parametrize('gather', [False, True])
+@pytest.mark.parametrize('counts,n,k', [([2049, 4097, 65], 2168, 2056), ([129] * 16, 1288, 2104), ([1, 0, 2113, 65], 4104, 2168)])
+def test_one_row_left_of_groups(counts, n, k, gather):
+    P = sum(counts)
+    rows = torch.randint(0, 3, (P,), generator=torch.Generator(device='cuda').manual_seed(k), device='cuda') if gather else None
+    x, dy = normal(3 if gather else P, k, seed=1), normal(P, n, seed=2)
+    w, starts = torch.zeros(len(counts), n, k, dtype=BF16, device='cuda'), groups_of(counts)
+    dw = ops().expert_linear_grad(dy, x, w, starts, rows, need_x=False, need_bias=False)[1]
+    close(dw, *expert_reference(x, w, starts, rows=rows, dy=dy)['dw'], 'dw')

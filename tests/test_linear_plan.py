@@ -17,6 +17,7 @@ using namespace ferry::lin;
 extern "C" int stages(int tm, int tn, int gathered_dw) { return ring_stages(tm, tn, gathered_dw); }
 extern "C" int rows_wait(int kt, int ring, int filling) { return ring_rows_wait(kt, ring, filling); }
 extern "C" int early() { return kTile256Early; }
+extern "C" unsigned half(int across, long there, unsigned ld2) { return half_offset(across, there, ld2); }
 extern "C" int gathers(long c, long parts) { return tile256_gathers(c, parts); }
 extern "C" long part(long c, long parts) { return part_length(c, parts); }
 '''
@@ -30,6 +31,7 @@ def plan(tmp_path_factory):
                     str(where / 'plan.cpp')], check=True)
     so = ctypes.CDLL(str(where / 'plan.so'))
     so.part.restype = ctypes.c_long
+    so.half.argtypes = [ctypes.c_int, ctypes.c_long, ctypes.c_uint]
     so.gathers.argtypes = so.part.argtypes = [ctypes.c_long, ctypes.c_long]
     return so
 
@@ -254,3 +256,29 @@ def test_row_numbers_of_parts_have_landed(plan, parts):
                 tile256(plan, [*pair, per], 'x')
             taken += 1
     assert taken > 10
+
+
+@pytest.mark.parametrize('across', [False, True])
+def test_offsets_lie_in_their_buffers(plan, across):
+    """An operand's buffer ends with the last element of the tile's last row.  The offset of every stage and half that
+    tile256 loads has to lie in it: lanes are compared with what is left behind the offset, unsigned."""
+    for there, c, spare in itertools.product((1, 8, 64, 120, 127, 128, 129, 136, 248, 256, 300), (1, 7, 8, 64, 65, 128, 129, 193, 8193),
+                                             (0, 8, 1000)):
+        inside = min(there, 256)
+        # across: c rows of the indices; direct: a row of the contraction for every index
+        rows, last = (c, inside) if across else (inside, c)
+        ld = last + spare
+        size = ((rows - 1) * ld + last) * 2
+        half = plan.half(across, there, 2 * ld)
+        for stage in range((c + 63) // 64):
+            at = stage * 64 * (ld if across else 1) * 2
+            assert at < size and at + half < size
+            if there > 128:   # the half that is there: its first element
+                assert half == 128 * 2 * (1 if across else ld)
+
+
+def test_offsets_of_gathered_rows(plan):
+    """Rows of x by their numbers, of which there may be one alone."""
+    for there, x_rows in itertools.product((1, 8, 128, 129, 256), (1, 2, 100)):
+        size = ((x_rows - 1) * there + min(there, 256)) * 2
+        assert plan.half(True, there, 2 * there) < size

@@ -547,9 +547,10 @@ bool few_fits(int op, const Args& a) {
 }
 
 // Whether the tiled kernels can read and write the operands: rows at multiples of 16 bytes, offsets that 32
-// bits hold (a tile's, or all of an operand whose rows are gathered or follow the contraction).
+// bits hold (a tile's, or all of an operand whose rows are gathered or follow the contraction).  Their forms for
+// gathered rows add a bias and no more: expert_linear asks for nothing else, and any_kernel takes the C entry's other calls.
 bool tiles_fit(int op, const Args& a, int64_t pairs, int64_t n, int64_t k) {
-  if (a.rows && a.x_rows < 1) return false;
+  if (a.rows && (a.x_rows < 1 || a.act != kNone || a.residual || a.pre)) return false;
   if (n % 8 || k % 8 || !even(a.a, a.lda) || !even(a.b, a.ldb) || a.b_group % 8 || !even(a.out, a.ldo) || a.o_group % 8 ||
       (a.bias && !even(a.bias, a.bias_group)) || (a.residual && !even(a.residual, a.ldr)) || (a.pre && !even(a.pre, 0)))
     return false;

@@ -1,0 +1,71 @@
+"""ferry_expert_linear and the gradients' C entries in the forms that the Python functions do not use.  Formulas and bounds are
+test_gpu_linear's."""
+import pytest
+import torch
+from test_gpu_linear import BF16, F16, close, groups_of, layer, normal, product, rounding
+
+from ferry_amd._lib import last_error, lib
+
+pytestmark = pytest.mark.gpu
+NUMBERS = {None: 0, 'relu': 1, 'silu': 2, 'gelu': 3, 'gelu_tanh': 4}
+
+
+def at(t):
+    return None if t is None else t.data_ptr()
+
+
+def scratch(op, pairs, n, k, groups):
+    size = lib().ferry_linear_workspace_bytes(op, pairs, n, k, groups)
+    return torch.empty(max(size, 16), dtype=torch.uint8, device='cuda'), size
+
+
+def forward(x, w, starts=None, rows=None, bias=None, act=None, residual=None, pre=None, out=None, strides=()):
+    """ferry_expert_linear of x [rows, k] and w [groups, n, k]; strides: those of x, w, residual and out that are not
+    their tensors'."""
+    E, n, k = w.shape
+    pairs = x.shape[0] if rows is None else rows.numel()
+    s = dict(x=x.stride(0), w=w.stride(1), residual=n, out=out.stride(0), **{})
+    s.update(strides)
+    ws, size = scratch(0, pairs, n, k, E)
+    status = lib().ferry_expert_linear(
+        at(x), 0 if x.dtype is BF16 else 2, x.shape[0], k, s['x'], at(rows), pairs, at(starts), E, at(w), n, s['w'], n * k,
+        at(bias), n, NUMBERS[act], at(residual), s['residual'], at(pre), at(out), s['out'], 0, at(ws), size,
+        torch.cuda.current_stream().cuda_stream)
+    assert status == 0, last_error()
+    torch.cuda.synchronize()
+    return out
+
+
+SIZES = [([20], 264, 512), ([3, 0, 17], 256, 256), ([300, 200], 512, 320), ([2100, 1996], 2048, 2048), ([4096], 2048, 512),
+         ([4000, 3000, 1192], 6144, 256), ([60, 77], 35, 131), ([2146, 2146], 160, 14464)]
+
+
+@pytest.mark.parametrize('case', range(len(SIZES)))
+def test_gathered_rows_with_an_epilogue(case):
+    """Rows by their numbers together with an activation, its kept argument and a residual, at each kernel's sizes."""
+    counts, n, k = SIZES[case]
+    dtype, act = (F16 if case % 2 else BF16), ['silu', 'gelu', 'relu', 'gelu_tanh'][case % 4]
+    P, E = sum(counts), len(counts)
+    R = max(1, P // 2)
+    rows = torch.randint(0, R, (P,), generator=torch.Generator(device='cuda').manual_seed(case), device='cuda')
+    x, w = normal(R, k, dtype=dtype, seed=1), normal(E, n, k, dtype=dtype, seed=2, scale=k ** -0.5)
+    bias, res, starts = normal(E, n, dtype=dtype, seed=3), normal(P, n, dtype=dtype, seed=4), groups_of(counts)
+    new = lambda: torch.full((P, n), 7.5, dtype=dtype, device='cuda')
+    all_three, pre = new(), new()
+    forward(x, w, starts, rows, bias, act, res, pre, all_three)
+    only_act, only_res, only_pre, kept = (new() for _ in range(4))
+    forward(x, w, starts, rows, act=act, out=only_act)
+    forward(x, w, starts, rows, residual=res, out=only_res)
+    forward(x, w, starts, rows, pre=kept, out=only_pre)
+    ends = starts.tolist()
+    for e in range(E):
+        g = slice(ends[e], ends[e + 1])
+        xe = x[rows[g]]
+        y, b, z, zb = layer(xe, w[e], bias[e], act, res[g])
+        close(all_three[g], y, b, 'all')
+        close(pre[g], z, zb + rounding(z, dtype), 'pre')
+        close(only_act[g], *layer(xe, w[e], None, act)[:2], 'activation')
+        close(only_res[g], *layer(xe, w[e], None, None, res[g])[:2], 'residual')
+        z, zb = product(xe.double(), w[e].double().t())
+        close(only_pre[g], z, zb + rounding(z, dtype), 'no activation')
+        close(kept[g], z, zb + rounding(z, dtype), 'pre without an activation')

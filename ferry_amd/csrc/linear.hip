@@ -578,7 +578,9 @@ int64_t slope_splits(int64_t pairs, int64_t groups) {
 template <typename T, int MODE>
 int run_typed(const Args& a, const Plan& p, int64_t n, int64_t k, hipStream_t s) {
   static const char* const names[] = {"linear_fwd", "linear_dx", "linear_dw"};
-  const int shape = p.shape == 0 && MODE == kFwd && a.rows && !tile256_gathers(k, a.splits) ? 1 : p.shape;
+  // (tile256 keeps pre beside an activation only)
+  const bool ring = MODE == kFwd && (a.rows ? !tile256_gathers(k, a.splits) : a.pre && a.act == kNone);
+  const int shape = p.shape == 0 && ring ? 1 : p.shape;
   if (p.kind == kFew && few_fits(MODE, a)) {
     few_launch(MODE, T::kType, p.mt, p.nb, a, p.tiles, cus(), s);
   } else if (p.kind == kTiles && tiles_fit(MODE, a, a.pairs, n, k)) {

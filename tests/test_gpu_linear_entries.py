@@ -69,3 +69,19 @@ def test_gathered_rows_with_an_epilogue(case):
         z, zb = product(xe.double(), w[e].double().t())
         close(only_pre[g], z, zb + rounding(z, dtype), 'no activation')
         close(kept[g], z, zb + rounding(z, dtype), 'pre without an activation')
+
+
+@pytest.mark.parametrize('groups', [1, 2])
+@pytest.mark.parametrize('m,n,k', [(5, 264, 512), (300, 512, 320), (2100, 2048, 128), (4104, 4096, 512), (77, 35, 131)])
+def test_pre_without_an_activation(m, n, k, groups):
+    """pre is the rounded argument of any activation, none among them: the product and its bias."""
+    x, w, bias, res = normal(m, k, seed=1), normal(groups, n, k, seed=2, scale=k ** -0.5), normal(groups, n, seed=3), normal(m, n, seed=4)
+    starts = groups_of([m]) if groups == 1 else groups_of([m // 2, m - m // 2])
+    out, pre = (torch.full((m, n), 7.5, dtype=BF16, device='cuda') for _ in range(2))
+    forward(x, w, starts, None, bias, None, res, pre, out)
+    ends = starts.tolist()
+    for e in range(groups):
+        g = slice(ends[e], ends[e + 1])
+        y, b, z, zb = layer(x[g], w[e], bias[e], None, res[g])
+        close(out[g], y, b, 'out')
+        close(pre[g], z, zb + rounding(z, BF16), 'pre')

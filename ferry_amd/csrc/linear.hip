@@ -622,6 +622,10 @@ int run(Args& a, int32_t dtype, int64_t pairs, int64_t n, int64_t k, void* works
   return dtype == FERRY_BF16 ? run_typed<Bf16, MODE>(a, p, n, k, s) : run_typed<F16, MODE>(a, p, n, k, s);
 }
 
+// The distance of rows whose stride a call with one of them need not name: the tiled kernels tell rows that are not there by
+// offsets behind the end of the last one.
+int64_t row_stride(int64_t stride, int64_t rows, int64_t width) { return rows > 1 ? stride : std::max(stride, width); }
+
 constexpr int64_t kMost = (int64_t)1 << 30;   // rows, columns, pairs: tile numbers are counted in 32 bits
 
 int check_sizes(int32_t dtype, int64_t pairs, int64_t n, int64_t k, int64_t groups, const int64_t* starts) {
@@ -668,14 +672,14 @@ extern "C" int ferry_expert_linear(const void* x, int32_t dtype, int64_t x_rows,
   if (pairs == 0) return 0;
   FERRY_CHECK_ARG((x || x_rows == 0) && w && out, "null pointer argument");
   Args a = {};
-  a.a = (const uint16_t*)x, a.lda = x_stride;
-  a.b = (const uint16_t*)w, a.ldb = w_stride, a.b_group = w_group_stride;
-  a.out = (uint16_t*)out, a.ldo = out_stride;
+  a.a = (const uint16_t*)x, a.lda = row_stride(x_stride, x_rows, k);
+  a.b = (const uint16_t*)w, a.ldb = row_stride(w_stride, n, k), a.b_group = w_group_stride;
+  a.out = (uint16_t*)out, a.ldo = row_stride(out_stride, pairs, n);
   a.starts = starts, a.rows = rows, a.x_rows = x_rows;
   a.J = n, a.C = k, a.groups = (int32_t)groups;
   a.act = activation, a.zero_rest = starts && zero_rest;
   a.bias = (const uint16_t*)bias, a.bias_group = bias_stride;
-  a.residual = (const uint16_t*)residual, a.ldr = residual_stride;
+  a.residual = (const uint16_t*)residual, a.ldr = row_stride(residual_stride, pairs, n);
   a.pre = (uint16_t*)pre;
   return run<kFwd>(a, dtype, pairs, n, k, workspace, workspace_bytes, (hipStream_t)stream);
 }
@@ -732,8 +736,8 @@ extern "C" int ferry_expert_linear_grad_x(const void* dz, int32_t dtype, int64_t
   if (pairs == 0) return 0;
   FERRY_CHECK_ARG(dz && w && out, "null pointer argument");
   Args a = {};
-  a.a = (const uint16_t*)dz, a.lda = dz_stride;
-  a.b = (const uint16_t*)w, a.ldb = w_stride, a.b_group = w_group_stride;
+  a.a = (const uint16_t*)dz, a.lda = row_stride(dz_stride, pairs, n);
+  a.b = (const uint16_t*)w, a.ldb = row_stride(w_stride, n, k), a.b_group = w_group_stride;
   a.out = (uint16_t*)out, a.ldo = k;
   a.starts = starts, a.J = k, a.C = n, a.groups = (int32_t)groups, a.zero_rest = starts && zero_rest;
   return run<kDx>(a, dtype, pairs, n, k, workspace, workspace_bytes, (hipStream_t)stream);
@@ -749,8 +753,8 @@ extern "C" int ferry_expert_linear_grad_w(const void* dz, int32_t dtype, int64_t
   FERRY_CHECK_ARG((dz_stride >= n || pairs <= 1) && (x_stride >= k || x_rows <= 1), "strides must reach over their rows");
   FERRY_CHECK_ARG(dw && (pairs == 0 || (dz && (x || x_rows == 0))), "null pointer argument");
   Args a = {};
-  a.a = (const uint16_t*)dz, a.lda = dz_stride;
-  a.b = (const uint16_t*)x, a.ldb = x_stride;
+  a.a = (const uint16_t*)dz, a.lda = row_stride(dz_stride, pairs, n);
+  a.b = (const uint16_t*)x, a.ldb = row_stride(x_stride, x_rows, k);
   a.out = (uint16_t*)dw, a.ldo = k, a.o_group = n * k;
   a.starts = starts, a.rows = rows, a.x_rows = x_rows;
   a.I = n, a.J = k, a.groups = (int32_t)groups;

@@ -85,3 +85,34 @@ def test_pre_without_an_activation(m, n, k, groups):
         y, b, z, zb = layer(x[g], w[e], bias[e], None, res[g])
         close(out[g], y, b, 'out')
         close(pre[g], z, zb + rounding(z, BF16), 'pre')
+
+
+@pytest.mark.parametrize('stride', [0, 8, -8, 1 << 40])
+@pytest.mark.parametrize('groups,n,k', [(1, 264, 512), (64, 27136, 8), (3, 35, 131), (1, 1528, 46616)])
+def test_one_row_of_any_stride(groups, n, k, stride):
+    """One row's strides are not used: x, residual, out and, in the gradients, dz and x."""
+    x, w, res = normal(1, k, seed=1), normal(groups, n, k, seed=2, scale=k ** -0.5), normal(1, n, seed=3)
+    g = groups // 2
+    starts = torch.tensor([0] * (g + 1) + [1] * (groups - g), dtype=torch.int64, device='cuda')
+    beyond = torch.full((n + 64,), 7.5, dtype=BF16, device='cuda')
+    forward(x, w, starts, None, None, 'gelu', res, None, beyond.view(1, -1),
+            dict(x=stride, out=stride, residual=max(stride, 0)))
+    close(beyond[:n][None], *layer(x, w[g], None, 'gelu', res)[:2], 'out')
+    assert bool((beyond[n:] == 7.5).all())
+    if groups * n * k > 1 << 25:
+        return
+    dz = normal(1, n, seed=4)
+    stream = torch.cuda.current_stream().cuda_stream
+    ws, size = scratch(2, 1, n, k, groups)
+    dw = torch.empty(groups, n, k, dtype=BF16, device='cuda')
+    assert lib().ferry_expert_linear_grad_w(at(dz), 0, 1, n, stride, at(x), 1, k, stride, None, at(starts), groups, at(dw),
+                                            at(ws), size, stream) == 0, last_error()
+    want, bound = product(dz.double().t(), x.double())
+    close(dw[g], want, bound + rounding(want, BF16), 'dw')
+    assert not dw[:g].any() and not dw[g + 1:].any()
+    ws, size = scratch(1, 1, n, k, groups)
+    dx = torch.empty(1, k, dtype=BF16, device='cuda')
+    assert lib().ferry_expert_linear_grad_x(at(dz), 0, 1, n, stride, at(starts), groups, at(w), k, k, n * k, at(dx), 0, at(ws),
+                                            size, stream) == 0, last_error()
+    want, bound = product(dz.double(), w[g].double())
+    close(dx, want, bound + rounding(want, BF16), 'dx')

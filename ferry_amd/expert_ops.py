@@ -557,8 +557,15 @@ def _written(out):
         torch.autograd.graph.increment_version(out)
 
 
+def _no_trace(what):
+    """Refuses a call that torch.jit.trace records: the trace would hold the result's allocation and no launch."""
+    if torch.jit.is_tracing():
+        raise RuntimeError(f'{what} cannot be traced')
+
+
 def _watched(what, *tensors):
     """Whether autograd takes part in a call on these tensors (None among them)."""
+    _no_trace(what)
     if (getattr(forward_ad, '_current_level', 0) >= 0
             and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)):
         raise RuntimeError(f'{what} has no forward-mode derivative')
@@ -632,7 +639,7 @@ def linear(x, weight, bias=None, activation=None, residual=None, out=None, retur
 
     The result carries the gradients of x, weight, bias and residual, except with ``out`` or ``return_pre``
     and inside a captured graph (there ``linear`` and ``linear_grad`` are called under torch.no_grad()).
-    No counterpart in the reference."""
+    A torch.jit.trace is refused.  No counterpart in the reference."""
     if _watched('linear', x, weight, bias, residual):
         if out is not None or return_pre:
             raise RuntimeError('linear: out and return_pre carry no gradients; call it under torch.no_grad()')
@@ -671,6 +678,7 @@ def linear_grad(grad, x, weight, pre=None, activation=None, need_x=True, need_we
 
     dz = grad * f'(pre) is rounded to the inputs' type before the products; the bias's gradient sums it
     unrounded.  Makes no use of autograd, so it can be captured into a graph."""
+    _no_trace('linear_grad')
     act = _ACTIVATIONS.get(activation, -1)
     if act < 0:
         raise ValueError("activation must be None, 'relu', 'silu', 'gelu' or 'gelu_tanh'")
@@ -783,8 +791,8 @@ def expert_linear(x, weight, starts, bias=None, rows=None, pair_pos=None, out=No
 
     The result carries the gradients of x, weight and bias (x's, with ``rows``, needs ``pair_pos`` [tokens *
     topk], the places of each row of x), except with ``out`` and inside a captured graph (there
-    ``expert_linear`` and ``expert_linear_grad`` are called under torch.no_grad()).  No counterpart in the
-    reference."""
+    ``expert_linear`` and ``expert_linear_grad`` are called under torch.no_grad()).  A torch.jit.trace is
+    refused.  No counterpart in the reference."""
     if _watched('expert_linear', x, weight, bias):
         if out is not None:
             raise RuntimeError('expert_linear: out carries no gradients; call it under torch.no_grad()')
@@ -801,6 +809,7 @@ def expert_linear_grad(grad, x, weight, starts, rows=None, pair_pos=None, need_x
     gradients of the grouped rows ``pair_pos[t, j]``; without ``pair_pos`` it is those, [pairs, k], in
     grouped order.  Experts without rows have zero gradients; rows of ``grad`` that belong to no expert are
     not read.  Makes no use of autograd, so it can be captured into a graph."""
+    _no_trace('expert_linear_grad')
     xs, w, ws, wg, first, rows_at, pairs = _expert_args(x, weight, starts, rows)
     E, n, k = weight.shape
     _, gs = _half_rows(grad, 'grad', x.get_device(), x.dtype)
@@ -838,6 +847,7 @@ def sum_pairs(part, pair_pos, tokens):
     """out[t] = the fp32 sum, j ascending, of ``part[pair_pos[t, j]]``, rounded once, [tokens, k]: the gradient of
     rows that were gathered from tokens.  ``part`` is contiguous bf16 or fp16 [pairs, k], ``pair_pos`` int32
     with as many entries for every token, ``layout``'s; entries outside [0, pairs) add nothing."""
+    _no_trace('sum_pairs')
     if not isinstance(part, torch.Tensor) or part.dim() != 2 or part.dtype not in _HALF:
         raise RuntimeError('part must be bf16 or fp16 [pairs, k]')
     at, (pairs, k) = _dev(part, 'part'), part.shape

@@ -82,3 +82,16 @@ def test_host_tensors_are_refused():
 def test_names_of_activations():
     with pytest.raises(ValueError, match='activation'):
         ops.linear(torch.zeros((4, 8)), torch.zeros((2, 8)), activation='tanh')
+
+
+@pytest.mark.parametrize('what', ['linear', 'expert_linear', 'linear_grad', 'expert_linear_grad', 'sum_pairs'])
+def test_traces_are_refused(what):
+    """torch.jit.trace would record the allocation of the result and no launch."""
+    x, w = torch.zeros((4, 8), dtype=torch.bfloat16), torch.zeros((2, 8), dtype=torch.bfloat16)
+    starts = torch.zeros(2, dtype=torch.int64)
+    calls = dict(linear=lambda x: ops.linear(x, w), expert_linear=lambda x: ops.expert_linear(x, w[None], starts),
+                 linear_grad=lambda x: ops.linear_grad(x[:, :2], x, w),
+                 expert_linear_grad=lambda x: ops.expert_linear_grad(x[:, :2], x, w[None], starts),
+                 sum_pairs=lambda x: ops.sum_pairs(x, starts.int(), 2))
+    with pytest.raises(RuntimeError, match='cannot be traced'):
+        torch.jit.trace(calls[what], x)

@@ -640,7 +640,7 @@ def linear(x, weight, bias=None, activation=None, residual=None, out=None, retur
     The result carries the gradients of x, weight, bias and residual, except with ``out`` or ``return_pre``
     and inside a captured graph (there ``linear`` and ``linear_grad`` are called under torch.no_grad()).
     A torch.jit.trace is refused.  No counterpart in the reference."""
-    if _watched('linear', x, weight, bias, residual):
+    if _watched('linear', x, weight, bias, residual, out):
         if out is not None or return_pre:
             raise RuntimeError('linear: out and return_pre carry no gradients; call it under torch.no_grad()')
         return _Linear.apply(x, weight, bias, residual, activation)
@@ -793,7 +793,7 @@ def expert_linear(x, weight, starts, bias=None, rows=None, pair_pos=None, out=No
     topk], the places of each row of x), except with ``out`` and inside a captured graph (there
     ``expert_linear`` and ``expert_linear_grad`` are called under torch.no_grad()).  A torch.jit.trace is
     refused.  No counterpart in the reference."""
-    if _watched('expert_linear', x, weight, bias):
+    if _watched('expert_linear', x, weight, bias, out):
         if out is not None:
             raise RuntimeError('expert_linear: out carries no gradients; call it under torch.no_grad()')
         if rows is not None and pair_pos is None and x.requires_grad:

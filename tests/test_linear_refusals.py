@@ -95,3 +95,18 @@ def test_traces_are_refused(what):
                  sum_pairs=lambda x: ops.sum_pairs(x, starts.int(), 2))
     with pytest.raises(RuntimeError, match='cannot be traced'):
         torch.jit.trace(calls[what], x)
+
+
+@pytest.mark.parametrize('leaf', [True, False])
+def test_an_out_that_carries_gradients_is_refused(leaf, monkeypatch):
+    """Its new values would keep the old ones' gradient."""
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: False)
+    x, w = torch.zeros((4, 8), dtype=torch.bfloat16), torch.zeros((2, 8), dtype=torch.bfloat16)
+    out = torch.zeros((4, 2), dtype=torch.bfloat16, requires_grad=True)
+    out = out if leaf else out * 2
+    starts = torch.zeros(2, dtype=torch.int64)
+    for call in (lambda: ops.linear(x, w, out=out), lambda: ops.expert_linear(x, w[None], starts, out=out)):
+        with pytest.raises(RuntimeError, match='no gradients'):
+            call()
+        with torch.no_grad(), pytest.raises(RuntimeError, match='CUDA'):   # as any other out
+            call()

@@ -81,9 +81,9 @@ struct F16 {
 };
 
 // -- activations ---------------------------------------------------------------------------------
-// fp32, with the hardware's exp2 and reciprocal (relative error about 1e-6: the results are rounded to
-// 8 or 11 bits afterwards).  The tanh form is z / (1 + e^-2u), u = sqrt(2 / pi) (z + 0.044715 z^3): no
-// cancellation for negative z.
+// fp32, with the hardware's exp2 and reciprocal: a relative error of about 1e-6, in the tails, where an exponential
+// multiplies the rounding of its argument, of up to 2e-5 (the results are rounded to 8 or 11 bits afterwards).  The
+// tanh form is z / (1 + e^-2u), u = sqrt(2 / pi) (z + 0.044715 z^3): no cancellation for negative z.
 
 // 1 / (1 + 2^-y): two transcendental instructions, which cost as much as eight others
 __device__ __forceinline__ float sigmoid2(float y) {
@@ -93,10 +93,11 @@ __device__ __forceinline__ float sigmoid(float z) { return sigmoid2(1.44269504f 
 // sigmoid(2 u), u = sqrt(2 / pi) (z + 0.044715 z^3), in powers of 2
 __device__ __forceinline__ float gelu_gate(float z) { return sigmoid2(z * fmaf(0.102943240f, z * z, 2.30220819f)); }
 
-// The normal distribution function, erfc(-z / sqrt 2) / 2, with erfc(x) = t e^(P(t) - x^2), t = 1 / (1 + x / 2),
-// for x >= 0: P is a Chebyshev fit of degree 9 over 0 <= x <= 12 to ln(erfc(x) e^(x^2) / t), relative error
-// 4e-7 in fp32 (and e^(-x^2) is 0 where it ends).  Keeping the tail's relative error is what the library's
-// erfc does too, with several times the instructions, 16 x 8 of which an epilogue unrolls.
+// The normal distribution function, erfc(-z / sqrt 2) / 2, with erfc(x) = t e^(P(t) - x^2), t = 1 / (1 + x / 2), for x >= 0,
+// the form that Press et al., Numerical Recipes, use.  P is a Chebyshev fit of degree 9 over 0 <= x <= 12 of our own to
+// ln(erfc(x) e^(x^2) / t).  The fit's relative error is 6e-8; evaluated in fp32 the result's is 4e-7 for |z| < 1, 4e-6 up to 6
+// and 1.7e-5 up to 12 (x's and x^2's roundings, times e^), where rounding to bf16 costs 4e-3; from about |z| = 13 on the
+// result is 0.  An absolute error of 1e-7 would take fewer instructions, but gelu's tail would be lost.
 __device__ __forceinline__ float normal_cdf(float z) {
   const float x = fabsf(z) * 0.70710678f, t = __builtin_amdgcn_rcpf(fmaf(0.5f, x, 1.0f));
   float p = 0.157751014f;

@@ -302,7 +302,8 @@ int ferry_gate_logits(const void* x, int64_t tokens, int64_t hidden, const void*
  * Linear products, dense and grouped by expert, with their gradients (no counterpart in the reference,
  * whose experts are SwiGLU blocks of bf16 matrices without biases).  All matrices are bf16 or fp16
  * (dtype; every one of a call the same), their rows a stride apart and the elements of a row next to each
- * other, at any alignment: rows whose address and stride are multiples of 16 bytes are read fastest.
+ * other, at any alignment: rows whose address and stride are multiples of 16 bytes are read fastest.  The stride of
+ * a matrix of one row is not used.
  * Sums are fp32 (for a contraction in parts, fp32 sums of those in their order); every output is rounded
  * once.  Results do not depend on the order in which workgroups run.
  *
@@ -316,7 +317,8 @@ int ferry_gate_logits(const void* x, int64_t tokens, int64_t hidden, const void*
  * ferry_expert_linear: out[p] = f(x[rows[p]] w[g]^T + bias[g]) + residual[p], with w[g] an [n, k] matrix
  * at w + g * w_group_stride elements, bias[g] its n values at bias + g * bias_stride (bias and residual
  * nullable) and f the activation: none, relu, silu, gelu (of the normal distribution) or its tanh form.
- * pre (nullable, contiguous [pairs, n]) receives the rounded argument of f.  residual may be out itself.
+ * pre (nullable, contiguous [pairs, n]) receives the rounded argument of f.  residual may be out itself.  rows together with
+ * an activation, a residual or pre are slower at large sizes (they take the kernel for any alignment).
  * ferry_linear_grad_z: dz = grad * f'(pre) (contiguous [pairs, n]; only with an activation, which a call
  * with starts has not) and db[g] (nullable, contiguous [groups, n]) = the sum of grad * f'(pre) over the
  * rows of g.
